@@ -30,7 +30,8 @@ ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-DFP8IMMA_NVTX", "-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-Xcompiler", "-O3",
               "--expt-relaxed-constexpr", "-I" + INCLUDE, "-I" + CSRC]
 
-CU_SOURCES = ["api.cu", "gemv_splitk.cu", "decode.cu", "generic.cu", "fp8wgt.cu", "host_util.cu", "gemm_tc.cu", "noalloc.cu", "peer.cu", "quantize.cu"]
+CU_SOURCES = ["api.cu", "gemv_splitk.cu", "decode.cu", "generic.cu", "fp8wgt.cu", "host_util.cu", "gemm_tc.cu", "noalloc.cu", "peer.cu", "quantize.cu",
+              "kv_cache.cu", "kv_attention.cu", "moe.cu", "logprobs.cu"]
 
 
 def _run(cmd: list[str]) -> None:
@@ -108,7 +109,7 @@ def _torch_ext(name: str, sources: list[str], force: bool = False) -> str:
 def build_all(force: bool = False) -> None:
     build_lib(force=force)
     with cf.ThreadPoolExecutor(max_workers=2) as ex:
-        futs = [ex.submit(_torch_ext, "fp8imma_ext", ["fp8imma_ext.cpp"], force),
+        futs = [ex.submit(_torch_ext, "fp8imma_ext", ["fp8imma_ext.cpp", "serving_ops.cpp"], force),
                 ex.submit(_torch_ext, "fp8wgt_ext", ["fp8wgt_ext.cpp"], force)]
         for f in futs:
             f.result()

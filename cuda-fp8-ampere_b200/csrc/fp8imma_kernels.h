@@ -6,6 +6,8 @@
 #include <cstddef>
 #include <cstdint>
 
+struct fp8imma_kv_cache;
+
 namespace fp8imma_b200 {
 
 enum { A_F16 = 0, A_BF16 = 1, A_S8 = 2 };
@@ -89,7 +91,7 @@ struct ScopedScratch {
   cudaError_t release(cudaStream_t st) { return owned && ptr ? cudaFreeAsync(ptr, st) : cudaSuccess; }
 };
 // Tags of the callers of ScopedScratch
-enum { kScratchTc = 2, kScratchRowScales = 3, kScratchGemvRows = 4, kScratchWgt = 5 };
+enum { kScratchTc = 2, kScratchRowScales = 3, kScratchGemvRows = 4, kScratchWgt = 5, kScratchMoe = 6, kScratchAttn = 7, kScratchLogprobs = 8 };
 
 // TMA descriptor for a 2-D byte tensor [outer][inner] (row pitch row_bytes).
 cudaError_t make_tmap_2d_u8(CUtensorMap* map, const void* base, uint64_t inner, uint64_t outer, uint64_t row_bytes,
@@ -174,5 +176,8 @@ cudaError_t launch_generic_s8(const GemvParams& p, int a_type, int fmt, cudaStre
 // Per-row dynamic activation scales: a_inv_h[m] (fp16 bits), g[m] (fp32).
 cudaError_t launch_row_scales(const void* A, int a_type, int M, int K, uint16_t* a_inv_h,
                               float* g, cudaStream_t stream);
+
+// Checks of a paged KV cache shared by its append and its attention.
+cudaError_t kv_cache_check(const ::fp8imma_kv_cache* cache);
 
 }  // namespace fp8imma_b200

@@ -1,0 +1,272 @@
+// Appending key and value rows to the paged 8-bit KV cache (fp8imma_kv_append).
+//
+// Per page and KV head, over the new rows x of the page:
+//   need = 2^e, the smallest power of two >= 2^-126 with absmax_finite(x) <= fmax * 2^e
+//   s'   = max(s, need) when the page holds earlier tokens, else need
+//   earlier codes c -> rne(c * (s / s')), only when s' > s;  new codes = rne_sat(x / s')
+// An FP8 code carries its own exponent, so a scale finer than a power of two
+// would not make the codes more precise, and with powers of two a growing
+// scale only shifts exponents: codes move exactly until they drop below the
+// format's smallest step. Division by s' is an exact product as well, so each
+// stored value is rounded once.
+//
+// One CTA owns one (page, head, K or V), so scales and codes of a page have
+// one writer and no atomics are needed.
+#include "fp8_mma.cuh"
+#include "fp8imma/fp8imma_ext.h"
+#include "fp8imma_kernels.h"
+#include "nvtx_range.h"
+
+#include <cuda_runtime.h>
+
+namespace fp8imma_b200 {
+namespace {
+
+using namespace fp8imma_dev;
+
+constexpr int kThreads = 128;
+constexpr int kKeep = 8;  // 16-byte vectors of a page that a thread keeps between the two passes
+
+struct AppendParams {
+  fp8imma_kv_cache c;
+  const uint16_t* src[2];
+  int64_t ts[2], hs[2];
+  int vec;         // rows are 16-byte aligned
+  int per_seq;     // > 0: every sequence appends this many tokens
+  int pages_seq;   // then: pages a sequence can touch
+};
+
+template <int AT>
+__device__ __forceinline__ uint4 load_row8(const uint16_t* p, bool vec) {
+  if (vec) return __ldg(reinterpret_cast<const uint4*>(p));
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = (uint32_t)__ldg(p + 2 * i) | ((uint32_t)__ldg(p + 2 * i + 1) << 16);
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+template <int AT>
+__device__ __forceinline__ float absmax8(uint4 v) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  float m = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float a = fabsf(a16_to_f32<AT>((uint16_t)(w[i] & 0xFFFFu))), b = fabsf(a16_to_f32<AT>((uint16_t)(w[i] >> 16)));
+    m = fmaxf(m, a < INFINITY ? a : 0.0f);
+    m = fmaxf(m, b < INFINITY ? b : 0.0f);
+  }
+  return m;
+}
+
+template <int AT, int FMT>
+__device__ __forceinline__ uint2 to_codes(uint4 v, float s, float inv) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  // a page's scale that the caller set to something else than a power of two takes the division
+  const bool pow2 = (__float_as_uint(s) & 0x7FFFFFu) == 0u;
+  uint32_t o[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float a = a16_to_f32<AT>((uint16_t)(w[i] & 0xFFFFu)), b = a16_to_f32<AT>((uint16_t)(w[i] >> 16));
+    o[i] = pow2 ? f32x2_to_f8x2<FMT>(a * inv, b * inv) : f32x2_to_f8x2<FMT>(__fdiv_rn(a, s), __fdiv_rn(b, s));
+  }
+  return make_uint2(o[0] | (o[1] << 16), o[2] | (o[3] << 16));
+}
+
+// sequence b's packed token range, clamped to the packed axis
+__device__ __forceinline__ void token_range(const AppendParams& p, int b, int& t0, int& n) {
+  if (p.per_seq > 0) {
+    t0 = b * p.per_seq;
+    n = p.per_seq;
+  } else {
+    t0 = max(0, __ldg(p.c.cu_new + b));
+    n = max(0, min(__ldg(p.c.cu_new + b + 1), p.c.tokens) - t0);
+  }
+}
+
+// pages that sequence b's new tokens touch: first page index and count
+__device__ __forceinline__ int touched(const AppendParams& p, int b, int& first) {
+  int t0, n;
+  token_range(p, b, t0, n);
+  const int len = __ldg(p.c.seq_lens + b), start = max(0, len - n);
+  first = start / p.c.page_size;
+  return (n > 0 && len > start) ? min((len - 1) / p.c.page_size, p.c.max_pages - 1) - first + 1 : 0;
+}
+
+template <int AT, int FMT>
+__global__ void __launch_bounds__(kThreads) kv_append_kernel(const __grid_constant__ AppendParams p) {
+  __shared__ int s_pick[3];
+  __shared__ int s_scan[kThreads / 32];
+  __shared__ float s_max[kThreads / 32];
+  const int tid = threadIdx.x, h = blockIdx.y, which = blockIdx.z;
+  int b = 0, first = 0, pi = 0;
+  if (p.per_seq > 0) {
+    b = blockIdx.x / p.pages_seq;
+    pi = blockIdx.x % p.pages_seq;
+    if (pi >= touched(p, b, first)) return;
+  } else {
+    // unit blockIdx.x of the sequences' touched pages laid end to end
+    if (tid == 0) s_pick[0] = -1;
+    int base = 0;
+    for (int b0 = 0; b0 < p.c.batch; b0 += kThreads) {
+      int f = 0;
+      const int n = b0 + tid < p.c.batch ? max(0, touched(p, b0 + tid, f)) : 0;
+      int x = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, x, o);
+        if ((tid & 31) >= o) x += y;
+      }
+      __syncthreads();
+      if ((tid & 31) == 31) s_scan[tid >> 5] = x;
+      __syncthreads();
+      int before = base;
+      for (int w = 0; w < kThreads / 32; ++w) {
+        if (w < (tid >> 5)) before += s_scan[w];
+        base += s_scan[w];
+      }
+      const int lo = before + x - n;
+      if ((int)blockIdx.x >= lo && (int)blockIdx.x < lo + n) {
+        s_pick[0] = b0 + tid;
+        s_pick[1] = f;
+        s_pick[2] = (int)blockIdx.x - lo;
+      }
+      if ((int)blockIdx.x < base) break;
+    }
+    __syncthreads();
+    b = s_pick[0];
+    if (b < 0) return;
+    first = s_pick[1];
+    pi = s_pick[2];
+  }
+  const int ps = p.c.page_size, D = p.c.head_dim;
+  pi += first;
+  if (pi >= p.c.max_pages) return;
+  const int page = __ldg(p.c.page_table + (size_t)b * p.c.max_pages + pi);
+  if ((unsigned)page >= (unsigned)p.c.num_pages) return;
+  int t0, n;
+  token_range(p, b, t0, n);
+  const int len = __ldg(p.c.seq_lens + b);
+  const int start = len - n;  // position of token t0 (may be negative: those tokens have no place)
+  const int lo = max(max(start, 0), pi * ps), hi = min(len, (pi + 1) * ps);
+  const int slot0 = lo - pi * ps, rows = hi - lo;
+  if (rows <= 0) return;
+  const uint16_t* src = p.src[which] + (int64_t)(t0 + lo - start) * p.ts[which] + (int64_t)h * p.hs[which];
+  const size_t ph = (size_t)page * p.c.kv_heads + h;
+  uint8_t* dst = static_cast<uint8_t*>(which ? p.c.v : p.c.k) + ph * ps * D;
+  float* scale = (which ? p.c.v_scale : p.c.k_scale) + ph;
+  const float s_old = slot0 > 0 ? *scale : 0.0f;
+
+  const int vr = D >> 3, nv = rows * vr;  // 8-element vectors of a row, of the page's new rows
+  uint4 keep[kKeep];
+  float amax = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kKeep; ++i) {
+    const int v = tid + i * kThreads;
+    if (v < nv) {
+      keep[i] = load_row8<AT>(src + (int64_t)(v / vr) * p.ts[which] + (v % vr) * 8, p.vec);
+      amax = fmaxf(amax, absmax8<AT>(keep[i]));
+    }
+  }
+  for (int v = tid + kKeep * kThreads; v < nv; v += kThreads)
+    amax = fmaxf(amax, absmax8<AT>(load_row8<AT>(src + (int64_t)(v / vr) * p.ts[which] + (v % vr) * 8, p.vec)));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+  if ((tid & 31) == 0) s_max[tid >> 5] = amax;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) amax = fmaxf(amax, s_max[w]);
+
+  // amax = 1.m * 2^e <= 1.75 * 2^(8|15) * 2^k  <=>  k >= e - (8|15), one more when 1.m > 1.75
+  const uint32_t bits = __float_as_uint(amax);
+  const int e = (int)(bits >> 23) - 127 - (FMT == F8_E4M3 ? 8 : 15) + ((bits & 0x7FFFFFu) > 0x600000u ? 1 : 0);
+  const float need = __uint_as_float((uint32_t)(max(e, -126) + 127) << 23);
+  const float s_new = fmaxf(s_old, need);
+  const float inv = __fdiv_rn(1.0f, s_new);
+  if (slot0 > 0 && s_new != s_old) {  // uniform: the page's earlier codes move to the larger scale
+    const float ratio = __fdiv_rn(s_old, s_new);
+    for (int v = tid; v < slot0 * (D >> 4); v += kThreads) {
+      uint4 c = reinterpret_cast<uint4*>(dst)[v];
+      uint32_t w[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint32_t a, bb;
+        f8x4_to_f16x4<FMT>(w[i], a, bb);
+        const float2 fa = __half22float2(*reinterpret_cast<__half2*>(&a)), fb = __half22float2(*reinterpret_cast<__half2*>(&bb));
+        w[i] = (uint32_t)f32x2_to_f8x2<FMT>(fa.x * ratio, fa.y * ratio) |
+               ((uint32_t)f32x2_to_f8x2<FMT>(fb.x * ratio, fb.y * ratio) << 16);
+      }
+      reinterpret_cast<uint4*>(dst)[v] = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  }
+  uint2* out = reinterpret_cast<uint2*>(dst + (size_t)slot0 * D);
+#pragma unroll
+  for (int i = 0; i < kKeep; ++i) {
+    const int v = tid + i * kThreads;
+    if (v < nv) out[v] = to_codes<AT, FMT>(keep[i], s_new, inv);
+  }
+  for (int v = tid + kKeep * kThreads; v < nv; v += kThreads)
+    out[v] = to_codes<AT, FMT>(load_row8<AT>(src + (int64_t)(v / vr) * p.ts[which] + (v % vr) * 8, p.vec), s_new, inv);
+  if (tid == 0) *scale = s_new;
+}
+
+template <int AT>
+cudaError_t launch_append(const AppendParams& p, dim3 grid, cudaStream_t st) {
+  if (p.c.format == FP8IMMA_B_E4M3)
+    kv_append_kernel<AT, F8_E4M3><<<grid, kThreads, 0, st>>>(p);
+  else
+    kv_append_kernel<AT, F8_E5M2><<<grid, kThreads, 0, st>>>(p);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t kv_cache_check(const fp8imma_kv_cache* c) {
+  if (!c) return cudaErrorInvalidValue;
+  if (c->tokens <= 0 || c->batch <= 0 || c->num_pages <= 0 || c->max_pages <= 0 || c->kv_heads <= 0)
+    return cudaErrorInvalidConfiguration;
+  if (!c->k || !c->v || !c->k_scale || !c->v_scale || !c->page_table || !c->seq_lens) return cudaErrorInvalidValue;
+  if ((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v)) & 15u) return cudaErrorInvalidValue;
+  if (c->format < 0 || c->format > 1) return cudaErrorInvalidValue;
+  if (c->page_size != 16 && c->page_size != 32 && c->page_size != 64 && c->page_size != 128) return cudaErrorInvalidValue;
+  if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256) return cudaErrorInvalidValue;
+  if (!c->cu_new && c->tokens % c->batch) return cudaErrorInvalidValue;
+  // row indexes of the cache stay within 31 bits
+  if ((int64_t)c->num_pages * c->kv_heads * c->page_size > 0x7fffffffll) return cudaErrorInvalidValue;
+  if ((int64_t)c->max_pages * c->page_size > 0x7fffffffll) return cudaErrorInvalidValue;
+  return cudaSuccess;
+}
+
+}  // namespace fp8imma_b200
+
+using namespace fp8imma_b200;
+
+extern "C" int fp8imma_kv_append(const fp8imma_kv_cache* c, const fp8imma_kv_append_args* a, void* stream) {
+  FP8IMMA_RANGE("fp8imma_kv_append");
+  const cudaError_t e = kv_cache_check(c);
+  if (e != cudaSuccess) return (int)e;
+  if (!a || !a->k || !a->v || a->a_type < 0 || a->a_type > 1) return (int)cudaErrorInvalidValue;
+  AppendParams p = {};
+  p.c = *c;
+  p.src[0] = static_cast<const uint16_t*>(a->k);
+  p.src[1] = static_cast<const uint16_t*>(a->v);
+  p.ts[0] = a->k_token_stride;
+  p.hs[0] = a->k_head_stride;
+  p.ts[1] = a->v_token_stride;
+  p.hs[1] = a->v_head_stride;
+  const uintptr_t bits = reinterpret_cast<uintptr_t>(a->k) | reinterpret_cast<uintptr_t>(a->v) |
+                         (uintptr_t)((p.ts[0] | p.hs[0] | p.ts[1] | p.hs[1]) * 2);
+  if (bits & 1u) return (int)cudaErrorInvalidValue;
+  p.vec = (bits & 15u) == 0;
+  int64_t units;
+  if (!c->cu_new) {
+    p.per_seq = c->tokens / c->batch;
+    p.pages_seq = (p.per_seq + c->page_size - 2) / c->page_size + 1;
+    units = (int64_t)c->batch * p.pages_seq;
+  } else {
+    units = c->tokens / c->page_size + 2ll * c->batch;  // sum over b of ceil((n_b - 1) / page) + 1 at most
+  }
+  if (units > 0x7fffffffll || c->kv_heads > 65535) return (int)cudaErrorInvalidValue;
+  const dim3 grid((unsigned)units, (unsigned)c->kv_heads, 2);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return (int)(a->a_type == FP8IMMA_A_F16 ? launch_append<0>(p, grid, st) : launch_append<1>(p, grid, st));
+}

@@ -43,6 +43,10 @@ EXT_SYMBOLS = [
     "fp8imma_set_fused_gather",
     "fp8imma_fp8wgt_linear_forward",
     "fp8imma_quantize_weights",
+    "fp8imma_kv_append",
+    "fp8imma_kv_attention",
+    "fp8imma_moe_forward",
+    "fp8imma_token_logprobs",
     "fp8imma_set_splitk",
     "fp8imma_set_stream_k",
     "fp8imma_set_small_m_max",
@@ -70,6 +74,32 @@ class FP8ImmaGemmArgs(ctypes.Structure):
         ("col_scales_f32", ctypes.c_void_p), ("global_scale", ctypes.c_float),
         ("a_inv_scale", ctypes.c_float), ("D", ctypes.c_void_p), ("acc_out", ctypes.c_void_p),
     ]
+
+
+def _struct(name: str, doc: str, **groups):
+    """A ctypes mirror of a C argument structure from (type letter, names) pairs in order."""
+    kinds = {"i": ctypes.c_int, "p": ctypes.c_void_p, "l": ctypes.c_int64, "f": ctypes.c_float}
+    fields = [(n, kinds[key[0]]) for key, names in groups.items() for n in names.split()]
+    return type(name, (ctypes.Structure,), {"__doc__": doc, "_fields_": fields})
+
+
+# Mirrors of the argument structures of the decode-step operators
+# (include/fp8imma/fp8imma_ext.h); the keyword's first letter is the type.
+FP8ImmaKvCache = _struct(
+    "FP8ImmaKvCache", "fp8imma_kv_cache", p0="k v k_scale v_scale page_table seq_lens cu_new",
+    i1="format num_pages kv_heads page_size head_dim batch max_pages tokens")
+FP8ImmaKvAppendArgs = _struct(
+    "FP8ImmaKvAppendArgs", "fp8imma_kv_append_args", i0="a_type", p1="k v",
+    l2="k_token_stride k_head_stride v_token_stride v_head_stride")
+FP8ImmaKvAttentionArgs = _struct(
+    "FP8ImmaKvAttentionArgs", "fp8imma_kv_attention_args", i0="a_type heads window", f1="softmax_scale", p2="q",
+    l3="q_token_stride q_head_stride", p4="out lse")
+FP8ImmaMoeArgs = _struct(
+    "FP8ImmaMoeArgs", "fp8imma_moe_args", i0="a_type format act renormalize tokens experts top_k hidden inter", p1="x",
+    l2="x_token_stride", p3="router w_gate_up s_gate_up w_down s_down out ids weights")
+FP8ImmaLogprobsArgs = _struct(
+    "FP8ImmaLogprobsArgs", "fp8imma_logprobs_args", i0="l_type tokens vocab top", f1="temperature", p2="logits",
+    l3="token_stride vocab_stride", p4="token_ids logprobs entropy top_ids top_logprobs")
 
 
 def lib() -> ctypes.CDLL:
@@ -105,6 +135,14 @@ def lib() -> ctypes.CDLL:
     L.fp8imma_gemm_rowquant_noalloc.argtypes = [ctypes.POINTER(FP8ImmaGemmArgs), P]
     L.fp8imma_quantize_weights.restype = I
     L.fp8imma_quantize_weights.argtypes = [P, I, I, I, I, P, P, P, P]
+    L.fp8imma_kv_append.restype = I
+    L.fp8imma_kv_append.argtypes = [ctypes.POINTER(FP8ImmaKvCache), ctypes.POINTER(FP8ImmaKvAppendArgs), P]
+    L.fp8imma_kv_attention.restype = I
+    L.fp8imma_kv_attention.argtypes = [ctypes.POINTER(FP8ImmaKvCache), ctypes.POINTER(FP8ImmaKvAttentionArgs), P]
+    L.fp8imma_moe_forward.restype = I
+    L.fp8imma_moe_forward.argtypes = [ctypes.POINTER(FP8ImmaMoeArgs), P]
+    L.fp8imma_token_logprobs.restype = I
+    L.fp8imma_token_logprobs.argtypes = [ctypes.POINTER(FP8ImmaLogprobsArgs), P]
     L.fp8imma_fp8wgt_linear_forward.restype = I
     L.fp8imma_fp8wgt_linear_forward.argtypes = [P, P, F, P, I, I, I, P]
     L.fp8imma_set_splitk.restype = I

@@ -206,7 +206,10 @@ int64_t last_path() { return fp8imma_last_path(); }
 int64_t set_splitk(int64_t s) { return fp8imma_set_splitk((int)s); }
 int64_t set_small_m_max(int64_t m) { return fp8imma_set_small_m_max((int)m); }
 
+void register_serving_ops(pybind11::module_& m);  // serving_ops.cpp
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+  register_serving_ops(m);
   m.def("imma_fp8_v4_act", &imma_fp8_v4_act,
         "IMMA FP8-as-storage GEMM (v4 actquant), sm_100a\n"
         "A: [M,K] fp16/bf16 contiguous (row-major)\n"

@@ -157,6 +157,126 @@ int fp8imma_gemm_allgather(const fp8imma_gemm_args* args, void* const* peer_out,
 // calls.
 int fp8imma_set_fused_gather(int enable);
 
+// ------------------------------------------------- decode-step operators ----
+// What a decode step needs around the FP8-weight GEMMs. No reference
+// counterpart. Activations are fp16 or bf16 (a_type: FP8IMMA_A_F16 or
+// FP8IMMA_A_BF16); FP8 bytes are E4M3FN or E5M2 (FP8IMMA_B_E4M3 / _E5M2).
+// Forward only, like the GEMMs. Strides are in elements. Same errors as above:
+// cudaErrorInvalidConfiguration for an empty problem, cudaErrorInvalidValue
+// for a missing pointer or an argument outside its range.
+
+// A paged KV cache in 8 bits with one fp32 scale per (page, KV head) for the
+// keys and one for the values: value = code * scale. Page p holds `page_size`
+// consecutive tokens of one sequence; a sequence's page_table row lists its
+// pages in token order, seq_lens[b] is its number of tokens counting those of
+// the present step, and its step's tokens (packed, sequence after sequence;
+// cu_new[b] .. cu_new[b+1] of the packed axis) are the last ones of it. One
+// page belongs to one sequence while tokens are appended to it; attention may
+// read a page through several tables (shared prefixes). A page id outside
+// [0, num_pages) is a hole: nothing is stored there and attention skips it.
+// Lengths past max_pages * page_size count as that many.
+typedef struct fp8imma_kv_cache {
+  void* k;                    // [num_pages, kv_heads, page_size, head_dim] FP8 bytes, 16-byte aligned
+  void* v;
+  float* k_scale;             // [num_pages, kv_heads]
+  float* v_scale;
+  const int32_t* page_table;  // [batch, max_pages]
+  const int32_t* seq_lens;    // [batch]
+  const int32_t* cu_new;      // [batch + 1], or null: tokens / batch tokens for every sequence
+  int format;                 // fp8imma_b_format
+  int num_pages, kv_heads, page_size, head_dim;  // page_size 16, 32, 64 or 128; head_dim 64, 128 or 256
+  int batch, max_pages;
+  int tokens;                 // packed tokens of this step, all sequences
+} fp8imma_kv_cache;
+
+// Store the step's key and value rows. The scale of a page and head is the
+// smallest power of two (2^-126 at least) that brings its rows within the
+// format's range; when a row outgrows the scale of a page that holds earlier
+// tokens, the page's codes move to the larger scale (an exact shift of the
+// exponent but for codes that fall below the format's smallest step). A page
+// whose first token is stored starts anew. NaN is kept, +-Inf saturates.
+typedef struct fp8imma_kv_append_args {
+  int a_type;
+  const void* k;  // [tokens, kv_heads, head_dim], last dimension contiguous
+  const void* v;
+  int64_t k_token_stride, k_head_stride;
+  int64_t v_token_stride, v_head_stride;
+} fp8imma_kv_append_args;
+int fp8imma_kv_append(const fp8imma_kv_cache* cache, const fp8imma_kv_append_args* args, void* stream);
+
+// Causal attention of the step's queries over the cache (grouped heads: query
+// head h reads KV head h / (heads / kv_heads)):
+//   out[t,h] = sum_j softmax_j(softmax_scale * <q[t,h], K_j>) V_j
+// over keys j <= pos(t), and j > pos(t) - window when window > 0, pos(t) being
+// the token's place in its sequence. A row that no key is left for gives 0
+// and lse = -inf. Statistics and sums are fp32.
+typedef struct fp8imma_kv_attention_args {
+  int a_type;                 // of q and out
+  int heads;                  // query heads, a multiple of kv_heads
+  int window;                 // 0: no window
+  float softmax_scale;
+  const void* q;              // [tokens, heads, head_dim], last dimension contiguous
+  int64_t q_token_stride, q_head_stride;
+  void* out;                  // [tokens, heads, head_dim] contiguous
+  float* lse;                 // optional [tokens, heads]: log of the row's sum of exponentials
+} fp8imma_kv_attention_args;
+int fp8imma_kv_attention(const fp8imma_kv_cache* cache, const fp8imma_kv_attention_args* args, void* stream);
+
+// A mixture-of-experts layer for a few tokens (1 .. FP8IMMA_MOE_MAX_TOKENS):
+//   r = x Wr^T; S = the top_k largest of a row's r (ties: lowest index);
+//   p = softmax of r over S (renormalize), or over all experts;
+//   out = sum_{e in S} p_e (act(x Wg_e^T) * (x Wu_e^T)) Wd_e^T
+// with FP8 expert weights as fp8imma_quantize_weights makes them (one fp32
+// scale per weight row). Sums are fp32; the product act(g) * u is rounded to
+// fp16 within its row's range before the second product.
+#define FP8IMMA_MOE_MAX_TOKENS 64
+#define FP8IMMA_MOE_MAX_TOP_K 16
+#define FP8IMMA_MOE_MAX_EXPERTS 1024
+typedef struct fp8imma_moe_args {
+  int a_type;                 // of x, router and out
+  int format;                 // fp8imma_b_format
+  int act;                    // 2 GELU (tanh form), 3 SiLU
+  int renormalize;
+  int tokens, experts, top_k;
+  int hidden, inter;          // multiples of 16
+  const void* x;              // [tokens, hidden], last dimension contiguous
+  int64_t x_token_stride;
+  const void* router;         // [experts, hidden]
+  const void* w_gate_up;      // [experts, 2 * inter, hidden]: gate rows, then up rows; 16-byte aligned
+  const float* s_gate_up;     // [experts, 2 * inter]
+  const void* w_down;         // [experts, hidden, inter]; 16-byte aligned
+  const float* s_down;        // [experts, hidden]
+  void* out;                  // [tokens, hidden] contiguous
+  int32_t* ids;               // optional [tokens, top_k]
+  float* weights;             // optional [tokens, top_k]
+} fp8imma_moe_args;
+int fp8imma_moe_forward(const fp8imma_moe_args* args, void* stream);
+
+// Scores of logits x [tokens, vocab], z = x / temperature:
+//   logprob[t] = z[t, token[t]] - lse_t, lse_t = log sum_j exp z[t,j]
+//   entropy[t] = - sum_j p_j log p_j, p = softmax z
+//   top_ids / top_logprobs: the `top` largest logits of the row in descending
+//   order (equal logits: lowest index first; NaN counts as the largest)
+// -inf logits take no part (p = 0). A token id outside [0, vocab) gives NaN,
+// and so does a row that holds NaN or +inf or only -inf.
+#define FP8IMMA_LOGPROBS_MAX_TOP 32
+enum fp8imma_l_type { FP8IMMA_L_F16 = 0, FP8IMMA_L_BF16 = 1, FP8IMMA_L_F32 = 2 };
+typedef struct fp8imma_logprobs_args {
+  int l_type;                 // fp8imma_l_type
+  int tokens, vocab;
+  int top;                    // 0 .. FP8IMMA_LOGPROBS_MAX_TOP, at most vocab
+  float temperature;          // > 0
+  const void* logits;
+  int64_t token_stride;       // row-major: vocab_stride 1 (or column-major, as
+  int64_t vocab_stride;       // the GEMM's default output: token_stride 1)
+  const int32_t* token_ids;   // [tokens]
+  float* logprobs;            // [tokens]
+  float* entropy;             // [tokens]
+  int32_t* top_ids;           // [tokens, top] (null when top is 0)
+  float* top_logprobs;        // [tokens, top]
+} fp8imma_logprobs_args;
+int fp8imma_token_logprobs(const fp8imma_logprobs_args* args, void* stream);
+
 // Tuning / introspection (no reference counterpart).
 // Force the K split of the small-M kernel (0 = automatic; 1, 2, 4 or 8).
 int fp8imma_set_splitk(int splits);
