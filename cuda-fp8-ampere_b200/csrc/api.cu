@@ -490,7 +490,7 @@ int fp8imma_set_pdl(int enable) {
 
 unsigned int fp8imma_device_error(int clear) {
   return gemv_device_error(clear != 0) | decode_device_error(clear != 0) | tc_device_error(clear != 0) |
-         peer_device_error(clear != 0);
+         peer_device_error(clear != 0) | attn_device_error(clear != 0) | moe_device_error(clear != 0);
 }
 
 int fp8imma_set_wait_limit_ns(unsigned long long ns) {
@@ -499,6 +499,8 @@ int fp8imma_set_wait_limit_ns(unsigned long long ns) {
   if (e == cudaSuccess) e = decode_set_wait_limit(ns);
   if (e == cudaSuccess) e = tc_set_wait_limit(ns);
   if (e == cudaSuccess) e = peer_set_wait_limit(ns);
+  if (e == cudaSuccess) e = attn_set_wait_limit(ns);
+  if (e == cudaSuccess) e = moe_set_wait_limit(ns);
   return (int)e;
 }
 

@@ -91,7 +91,7 @@ struct ScopedScratch {
   cudaError_t release(cudaStream_t st) { return owned && ptr ? cudaFreeAsync(ptr, st) : cudaSuccess; }
 };
 // Tags of the callers of ScopedScratch
-enum { kScratchTc = 2, kScratchRowScales = 3, kScratchGemvRows = 4, kScratchWgt = 5, kScratchMoe = 6, kScratchAttn = 7, kScratchLogprobs = 8 };
+enum { kScratchTc = 2, kScratchRowScales = 3, kScratchGemvRows = 4, kScratchWgt = 5, kScratchMoe = 6, kScratchAttn = 7, kScratchLogprobs = 8, kScratchAttnParts = 9, kScratchMoeSync = 10, kScratchLogprobsSync = 11 };
 
 // TMA descriptor for a 2-D byte tensor [outer][inner] (row pitch row_bytes).
 cudaError_t make_tmap_2d_u8(CUtensorMap* map, const void* base, uint64_t inner, uint64_t outer, uint64_t row_bytes,
@@ -178,6 +178,10 @@ cudaError_t launch_row_scales(const void* A, int a_type, int M, int K, uint16_t*
                               float* g, cudaStream_t stream);
 
 // Checks of a paged KV cache shared by its append and its attention.
+unsigned int attn_device_error(bool clear);
+unsigned int moe_device_error(bool clear);
+cudaError_t attn_set_wait_limit(unsigned long long ns);
+cudaError_t moe_set_wait_limit(unsigned long long ns);
 cudaError_t kv_cache_check(const ::fp8imma_kv_cache* cache);
 
 }  // namespace fp8imma_b200

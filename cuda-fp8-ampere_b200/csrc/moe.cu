@@ -4,6 +4,7 @@
 #include "fp8imma/fp8imma_ext.h"
 #include "fp8imma_kernels.h"
 #include "nvtx_range.h"
+#include "sm100_async.cuh"
 
 #include <cuda_runtime.h>
 
@@ -131,6 +132,10 @@ cudaError_t run_moe(const fp8imma_moe_args& a, cudaStream_t st) {
 }
 
 }  // namespace
+
+unsigned int moe_device_error(bool clear) { return fp8imma_dev::tu_device_error(clear); }
+cudaError_t moe_set_wait_limit(unsigned long long ns) { return fp8imma_dev::tu_set_wait_limit(ns); }
+
 }  // namespace fp8imma_b200
 
 using namespace fp8imma_b200;

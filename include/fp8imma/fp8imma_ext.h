@@ -174,7 +174,8 @@ int fp8imma_set_fused_gather(int enable);
 // page belongs to one sequence while tokens are appended to it; attention may
 // read a page through several tables (shared prefixes). A page id outside
 // [0, num_pages) is a hole: nothing is stored there and attention skips it.
-// Lengths past max_pages * page_size count as that many.
+// Tokens past max_pages * page_size have no place: they are neither stored nor
+// read. Scales are not negative.
 typedef struct fp8imma_kv_cache {
   void* k;                    // [num_pages, kv_heads, page_size, head_dim] FP8 bytes, 16-byte aligned
   void* v;
