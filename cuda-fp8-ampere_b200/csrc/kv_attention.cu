@@ -54,21 +54,20 @@ struct AttnParams {
   int per_seq;   // > 0: every sequence has this many tokens
   int group;     // query heads per KV head
   int vec_q;     // query rows are 16-byte aligned
-  int min_units; // tiles a CTA takes at least
-  unsigned int* counters;  // per (item, row warp): finished parts; zero between calls
+  unsigned int* counters;  // per item: finished parts; zero between calls
   float* parts;            // per (CTA, first / last segment, row warp): M, L, O of a shared item
 };
 
 // ---------------------------------------------------------------- helpers --
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
   uint32_t r;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
   return r;
 }
 __device__ __forceinline__ float ex2(float x) {
@@ -86,15 +85,10 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
-__device__ __forceinline__ uint4 lds128(uint32_t a) {
-  uint4 r;
-  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(a));
-  return r;
-}
-__device__ __forceinline__ uint2 lds64(uint32_t a) {
-  uint2 r;
-  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(r.x), "=r"(r.y) : "r"(a));
-  return r;
+// two outputs in the activation type
+__device__ __forceinline__ uint32_t out_pair(float lo, float hi, int a_type) {
+  if (a_type == FP8IMMA_A_F16) return pack_f16(lo, hi);
+  return (uint32_t)f32_to_a16<1>(lo) | ((uint32_t)f32_to_a16<1>(hi) << 16);
 }
 
 // NaN or infinite code among the four bytes
@@ -137,33 +131,32 @@ __device__ __forceinline__ Seq load_seq(const AttnParams& p, int b, int rows_per
 struct Segment {
   int b, rt, h;
   int first, count;    // tiles [first, first + count) of the item
-  int64_t item0;       // unit index of the item's first tile
-  int64_t item;        // item index over all sequences
+  int item0;           // unit index of the item's first tile
+  int item;            // item index over all sequences
   int lo, hi;          // keys that some row of the tile sees: [lo, hi)
   int pos_min, pos_max;
 };
 
 // Walks the units [u, end) segment by segment.
 struct Walk {
-  int64_t u, end, base, item_base;  // base: first unit of sequence b, item_base: its first item
+  int u, end, base, item_base;  // base: first unit of sequence b, item_base: its first item
   int b;
   Seq s;
   __device__ __forceinline__ bool next(const AttnParams& p, int rows_per_tile, Segment& g) {
     if (u >= end) return false;
-    int64_t items = (int64_t)s.row_tiles * p.c.kv_heads;
+    int items = s.row_tiles * p.c.kv_heads;
     while (u - base >= items * s.tiles) {  // u < end <= all units: ends at the last sequence
       base += items * s.tiles;
       item_base += items;
       s = load_seq(p, ++b, rows_per_tile);
-      items = (int64_t)s.row_tiles * p.c.kv_heads;
+      items = s.row_tiles * p.c.kv_heads;
     }
-    const int64_t off = u - base;
-    const int64_t it = off / s.tiles;
+    const int off = u - base, it = off / s.tiles;
     g.b = b;
-    g.rt = (int)(it / p.c.kv_heads);
-    g.h = (int)(it % p.c.kv_heads);
-    g.first = (int)(off - it * s.tiles);
-    g.count = (int)min((int64_t)(s.tiles - g.first), end - u);
+    g.rt = it / p.c.kv_heads;
+    g.h = it % p.c.kv_heads;
+    g.first = off - it * s.tiles;
+    g.count = min(s.tiles - g.first, end - u);
     g.item0 = base + it * s.tiles;
     g.item = item_base + it;
     const int r0 = g.rt * rows_per_tile, r1 = min(s.rows, r0 + rows_per_tile) - 1;
@@ -176,13 +169,16 @@ struct Walk {
   }
 };
 
-__device__ __forceinline__ int64_t run_begin(int64_t units, int ctas, int c) { return units * c / ctas; }
-__device__ __forceinline__ int run_of(int64_t units, int ctas, int64_t u) {  // the CTA whose run holds unit u
-  int c = (int)(u * ctas / units);
-  while (run_begin(units, ctas, c + 1) <= u) ++c;
-  while (run_begin(units, ctas, c) > u) --c;
-  return c;
-}
+// CTA c's run of the units: they differ by one in length at most.
+struct Runs {
+  int per, rem;
+  __device__ __forceinline__ Runs(int units, int ctas) : per(units / ctas), rem(units % ctas) {}
+  __device__ __forceinline__ int begin(int c) const { return c * per + min(c, rem); }
+  __device__ __forceinline__ int of(int u) const {  // the CTA whose run holds unit u
+    const int cut = rem * (per + 1);
+    return u < cut ? u / (per + 1) : rem + (u - cut) / per;
+  }
+};
 
 // Shapes of a variant: head_dim D, NT tiles of 8 query rows a warp, RW warps
 // along the rows (8 / RW along the keys).
@@ -190,12 +186,19 @@ template <int D, int NT, int RW>
 struct Shape {
   static constexpr int kRows = 8 * NT * RW;
   static constexpr int kKeyWarps = kConsumers / RW;
+  // A warp takes kNG groups of 16 keys at once, where registers allow two: the
+  // chains of dependent products, not the issue slots, are what a group waits
+  // for. With one row warp, warps then take every other stage.
+  static constexpr int kNG = D == 64 || (D == 128 && NT == 1) ? 2 : 1;
+  static constexpr int kSplit = kKeyWarps * kNG > kKeys / 16 ? kKeyWarps * kNG / (kKeys / 16) : 1;  // stages dealt to warps in turn
+  static constexpr int kPosWarps = kKeyWarps / kSplit;
   static constexpr int kHalves = D == 256 ? 2 : 1;        // 128-byte column halves of a tile
   static constexpr int kTileBytes = kKeys * D;            // K (or V) of a stage
   static constexpr int kStageBytes = 2 * kTileBytes;
   static constexpr int kMT = D / 16;                      // 16-channel tiles of O^T
+  static constexpr int kVecs = kMT * NT * 32;             // float4 of O of a warp
   static constexpr int kPartFloats = (kMT * NT * 4 + NT * 4) * 32;  // O, M and L of a warp, register by register
-  static constexpr int kMergeBytes = kConsumers / 2 * kPartFloats * 4;
+  static constexpr int kMergeBytes = kConsumers * kPartFloats * 4;
   static constexpr int kStages = (227 * 1024 - 2048 - kMergeBytes) / kStageBytes < 6 ? (227 * 1024 - 2048 - kMergeBytes) / kStageBytes : 6;
   static constexpr int kSmem = kStages * kStageBytes + kMergeBytes + 1024;
 };
@@ -205,6 +208,96 @@ struct StageInfo {
   int live[kSlots];  // the page exists
 };
 
+// What the output of an item needs to know.
+struct Item {
+  int t0, rows, rt, h;
+};
+struct Shared {  // an item that several CTAs worked on
+  Item item;
+  int index, item0, c0, c1, last;
+};
+
+// Where the x-th float4 of a part lies: two channels of two rows, as a lane's
+// fragment of O^T holds them, and that lane's M and L.
+template <int D, int NT, int RW>
+struct Frag {
+  using S = Shape<D, NT, RW>;
+  int warp, lane, nt, i, at_o, at_ml;
+  __device__ __forceinline__ explicit Frag(int x) {
+    warp = x / S::kVecs;
+    const int v = x % S::kVecs;
+    lane = v & 31;
+    nt = (v >> 5) % NT;
+    i = (v >> 5) / NT;
+    at_o = v * 4;
+    at_ml = ((S::kMT * NT + nt) * 32 + lane) * 4;
+  }
+};
+
+// Parts of a softmax joined: reference, sum and output of two rows. Eight parts
+// are asked for at a time, so the join waits for memory once per eight.
+struct Joined {
+  float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
+  float4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+  template <class ML, class O>
+  __device__ __forceinline__ void join(int n, ML ml, O part) {
+    constexpr int B = 8;
+#pragma unroll 1
+    for (int k = 0; k < n; k += B) {
+      float4 x[B], y[B];
+#pragma unroll
+      for (int e = 0; e < B; ++e) {
+        x[e] = make_float4(-INFINITY, -INFINITY, 0.0f, 0.0f);
+        y[e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (k + e < n) {
+          x[e] = ml(k + e);
+          y[e] = part(k + e);
+        }
+      }
+      float n0 = m0, n1 = m1;
+#pragma unroll
+      for (int e = 0; e < B; ++e) {
+        n0 = fmaxf(n0, x[e].x);
+        n1 = fmaxf(n1, x[e].y);
+      }
+      const float s0 = n0 == -INFINITY ? 0.0f : n0, s1 = n1 == -INFINITY ? 0.0f : n1;
+      const float g0 = ex2(m0 - s0), g1 = ex2(m1 - s1);
+      m0 = n0;
+      m1 = n1;
+      l0 *= g0;
+      l1 *= g1;
+      o = make_float4(o.x * g0, o.y * g1, o.z * g0, o.w * g1);
+#pragma unroll
+      for (int e = 0; e < B; ++e) {
+        const float f0 = ex2(x[e].x - s0), f1 = ex2(x[e].y - s1);
+        l0 = fmaf(x[e].z, f0, l0);
+        l1 = fmaf(x[e].w, f1, l1);
+        o.x = fmaf(y[e].x, f0, o.x);
+        o.y = fmaf(y[e].y, f1, o.y);
+        o.z = fmaf(y[e].z, f0, o.z);
+        o.w = fmaf(y[e].w, f1, o.w);
+      }
+    }
+  }
+};
+
+template <int D, int NT, int RW>
+__device__ __forceinline__ void store(const AttnParams& p, const Item& it, const Frag<D, NT, RW>& f, const Joined& j) {
+  using S = Shape<D, NT, RW>;
+  constexpr int kHalfTiles = S::kMT / S::kHalves;
+  const int row0 = it.rt * S::kRows + (f.warp * NT + f.nt) * 8 + 2 * (f.lane & 3);
+  const int ch = f.i / kHalfTiles * 128 + (f.lane >> 2) * (2 * kHalfTiles) + 2 * (f.i % kHalfTiles);
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    const int r = row0 + c;
+    if (r >= it.rows) continue;
+    const int64_t row = (int64_t)(it.t0 + r / p.group) * p.a.heads + it.h * p.group + r % p.group;
+    const float L = c ? j.l1 : j.l0, inv = L == 0.0f ? 0.0f : __fdiv_rn(1.0f, L);
+    *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.a.out) + row * D + ch) = out_pair((c ? j.o.y : j.o.x) * inv, (c ? j.o.w : j.o.z) * inv, p.a.a_type);
+    if (p.a.lse && f.i == 0 && f.lane < 4) p.a.lse[row] = L == 0.0f ? -INFINITY : 0.6931471805599453f * ((c ? j.m1 : j.m0) + log2f(L));
+  }
+}
+
 template <int FMT, int D, int NT, int RW>
 __global__ void __launch_bounds__(kThreads, 1)
     kv_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
@@ -213,8 +306,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t s_full[S::kStages], s_empty[S::kStages];
   __shared__ StageInfo s_info[S::kStages];
-  __shared__ int64_t s_scan[kThreads / 32], s_scan_items[kThreads / 32];
-  __shared__ int64_t s_start[3];  // sequence, its first unit, its first item
+  __shared__ int s_scan[2][kThreads / 32];
+  __shared__ Shared s_shared[2];
+  __shared__ int s_start[3];  // sequence, its first unit, its first item
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   float* merge = reinterpret_cast<float*>(smem_raw + (smem_base - smem_u32(smem_raw)) + S::kStages * S::kStageBytes);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -222,81 +316,76 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (tid == 0) {
     for (int i = 0; i < S::kStages; ++i) {
       mbar_init(&s_full[i], 1);
-      mbar_init(&s_empty[i], kConsumers);
+      mbar_init(&s_empty[i], kConsumers / S::kSplit);
     }
     fence_barrier_init();
     prefetch_tensormap(&map_k);
     prefetch_tensormap(&map_v);
   }
 
-  // this CTA's run of units
-  int64_t units = 0;
-  for (int b0 = 0; b0 < p.c.batch; b0 += kThreads) {
-    int64_t n = 0;
+  pdl_launch_dependents();
+  pdl_wait();  // all that follows may have been written by the kernel before
+
+  // this CTA's run of units: scan of the sequences' units and items
+  int units = 0, items = 0, n = 0, ni = 0, at = 0, at_i = 0;
+  auto scan = [&](int b0) {  // of sequences b0 .. b0 + kThreads: this thread's start, the running totals
+    n = ni = 0;
     if (b0 + tid < p.c.batch) {
       const Seq s = load_seq(p, b0 + tid, S::kRows);
-      n = (int64_t)s.row_tiles * p.c.kv_heads * s.tiles;
+      ni = s.row_tiles * p.c.kv_heads;
+      n = ni * s.tiles;
     }
+    int x = n, xi = ni;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, o), yi = __shfl_up_sync(0xffffffffu, xi, o);
+      if (lane >= o) {
+        x += y;
+        xi += yi;
+      }
+    }
     __syncthreads();
-    if (lane == 0) s_scan[warp] = n;
+    if (lane == 31) {
+      s_scan[0][warp] = x;
+      s_scan[1][warp] = xi;
+    }
     __syncthreads();
-    for (int w = 0; w < kThreads / 32; ++w) units += s_scan[w];
-  }
+    at = units + x - n;
+    at_i = items + xi - ni;
+#pragma unroll
+    for (int w = 0; w < kThreads / 32; ++w) {
+      if (w < warp) {
+        at += s_scan[0][w];
+        at_i += s_scan[1][w];
+      }
+      units += s_scan[0][w];
+      items += s_scan[1][w];
+    }
+  };
+  for (int b0 = 0; b0 < p.c.batch; b0 += kThreads) scan(b0);
   if (units == 0) return;
-  const int ctas = (int)min((int64_t)gridDim.x, (units + p.min_units - 1) / p.min_units);
+  const int ctas = min((int)gridDim.x, units);
   if ((int)blockIdx.x >= ctas) return;
+  const Runs runs(units, ctas);
   Walk walk;
-  walk.u = run_begin(units, ctas, blockIdx.x);
-  walk.end = run_begin(units, ctas, blockIdx.x + 1);
-  {
-    int64_t base = 0, base_i = 0;
-    for (int b0 = 0; b0 < p.c.batch; b0 += kThreads) {
-      int64_t n = 0, ni = 0;
-      if (b0 + tid < p.c.batch) {
-        const Seq s = load_seq(p, b0 + tid, S::kRows);
-        ni = (int64_t)s.row_tiles * p.c.kv_heads;
-        n = ni * s.tiles;
-      }
-      int64_t x = n, xi = ni;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int64_t y = __shfl_up_sync(0xffffffffu, x, o), yi = __shfl_up_sync(0xffffffffu, xi, o);
-        if (lane >= o) {
-          x += y;
-          xi += yi;
-        }
-      }
-      __syncthreads();
-      if (lane == 31) {
-        s_scan[warp] = x;
-        s_scan_items[warp] = xi;
-      }
-      __syncthreads();
-      int64_t before = base, before_i = base_i;
-      for (int w = 0; w < kThreads / 32; ++w) {
-        if (w < warp) {
-          before += s_scan[w];
-          before_i += s_scan_items[w];
-        }
-        base += s_scan[w];
-        base_i += s_scan_items[w];
-      }
-      const int64_t at = before + x - n;
-      if (walk.u >= at && walk.u < at + n) {
-        s_start[0] = b0 + tid;
-        s_start[1] = at;
-        s_start[2] = before_i + xi - ni;
-      }
-      if (walk.u < base) break;
+  walk.u = runs.begin(blockIdx.x);
+  walk.end = runs.begin(blockIdx.x + 1);
+  const int all = units;
+  if (p.c.batch > kThreads) units = items = 0;
+  for (int b0 = 0; b0 < p.c.batch; b0 += kThreads) {
+    if (p.c.batch > kThreads) scan(b0);
+    if (walk.u >= at && walk.u < at + n) {
+      s_start[0] = b0 + tid;
+      s_start[1] = at;
+      s_start[2] = at_i;
     }
-    __syncthreads();
-    walk.b = (int)s_start[0];
-    walk.base = s_start[1];
-    walk.item_base = s_start[2];
-    walk.s = load_seq(p, walk.b, S::kRows);
   }
+  units = all;
+  __syncthreads();
+  walk.b = s_start[0];
+  walk.base = s_start[1];
+  walk.item_base = s_start[2];
+  walk.s = load_seq(p, walk.b, S::kRows);
 
   const int ps = p.c.page_size;
   Segment g;
@@ -313,27 +402,35 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int* table = p.c.page_table + (size_t)g.b * p.c.max_pages;
       // tiles with keys that some row sees
       const int from = max(tile_lo, g.lo / kKeys), to = min(tile_hi, (g.hi + kKeys - 1) / kKeys);
-      int ids = -1;
-      auto fetch = [&](int tile) {  // ids of the 32 pages from `tile` on
-        const int pi = tile * per_stage + lane;
-        return pi < p.c.max_pages && pi * ps < g.hi && (pi + 1) * ps > g.lo ? __ldg(table + pi) : -1;
-      };
+      // page ids and scales, a page a lane, a batch of 32 pages ahead of the
+      // copies: the ids of the next batch are asked for when one begins, its
+      // scales one tile later
       const int batch = 32 / per_stage;  // tiles of a batch
-      int next_ids = from < to ? fetch(from) : -1;
+      auto fetch_ids = [&](int tile) {
+        const int pi = tile * per_stage + lane;
+        return tile < to && pi < p.c.max_pages && pi * ps < g.hi && (pi + 1) * ps > g.lo ? __ldg(table + pi) : -1;
+      };
+      int ids = -1, next_ids = from < to ? fetch_ids(from) : -1;
+      float kss = 0.0f, vss = 0.0f, next_ks = 0.0f, next_vs = 0.0f;
+      auto fetch_scales = [&]() {
+        if ((unsigned)next_ids < (unsigned)p.c.num_pages) {
+          const size_t ph = (size_t)next_ids * p.c.kv_heads + g.h;
+          next_ks = __ldg(p.c.k_scale + ph);
+          next_vs = __ldg(p.c.v_scale + ph);
+        }
+      };
+      fetch_scales();
       for (int tile = from; tile < to && ok; ++tile) {
         const int at = (tile - from) % batch * per_stage;
-        float ks = 0.0f, vs = 0.0f;
         if (at == 0) {
           ids = next_ids;
-          next_ids = tile + batch < to ? fetch(tile + batch) : -1;
+          kss = next_ks;
+          vss = next_vs;
+          next_ids = fetch_ids(tile + batch);
         }
-        const int page = __shfl_sync(0xffffffffu, ids, at + (lane < per_stage ? lane : 0));
+        const int src = at + (lane < per_stage ? lane : 0);
+        const int page = __shfl_sync(0xffffffffu, ids, src);
         const bool live = lane < per_stage && (unsigned)page < (unsigned)p.c.num_pages;
-        if (live) {
-          const size_t ph = (size_t)page * p.c.kv_heads + g.h;
-          ks = __ldg(p.c.k_scale + ph);
-          vs = __ldg(p.c.v_scale + ph);
-        }
         const uint32_t n_live = (uint32_t)__popc(__ballot_sync(0xffffffffu, live));
         ok = mbar_wait(&s_empty[stage], phase, ERR_WAIT_EMPTY);
         if (!ok) break;
@@ -353,6 +450,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             tma_load_2d(dst + S::kTileBytes + off, &map_v, &s_full[stage], hf * 128, y);
           }
         }
+        const float ks = __shfl_sync(0xffffffffu, kss, src), vs = __shfl_sync(0xffffffffu, vss, src);
+        if (at == per_stage) fetch_scales();
         if (lane < kSlots) {
           s_info[stage].ks[lane] = ks;
           s_info[stage].vs[lane] = vs;
@@ -386,17 +485,22 @@ __global__ void __launch_bounds__(kThreads, 1)
   // V: keys behind this lane's operand pairs
   const int vkey[4] = {D == 64 ? 4 * t4 : 2 * t4, D == 64 ? 4 * t4 + 1 : 2 * t4 + 1, D == 64 ? 4 * t4 + 2 : 2 * t4 + 8,
                        D == 64 ? 4 * t4 + 3 : 2 * t4 + 9};
-  int stage = 0;
+  const int kpos = kw % S::kPosWarps, turn = kw / S::kPosWarps;
+  uint8_t* const ring = smem_raw + (smem_base - smem_u32(smem_raw));
+  int stage = 0, count = 0;  // count: stages so far
   uint32_t phase = 0;
   bool ok = true;
+  constexpr int NG = S::kNG;
   constexpr int QW = D / 8;  // 32-bit words of Q a lane and row: D / 4 channels
   uint32_t q[NT][QW];
   float cq[NT][2];
   int pos[NT][2];
+  const int walk_begin = walk.u;
+  int n_shared = 0;
   float o[S::kMT][NT][4], m[NT][2], l[NT][2];
 
   while (walk.next(p, S::kRows, g)) {
-    const Seq s = walk.s;
+    const Seq& s = walk.s;
     // queries of this lane: row q4 of each 8-row tile, channels t4 * 32 .. (D = 64: t4 * 16 ..; D = 256: in both halves)
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -466,181 +570,212 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     const int tile_lo = s.tile0 + g.first;
     const int from = max(tile_lo, g.lo / kKeys), to = min(tile_lo + g.count, (g.hi + kKeys - 1) / kKeys);
-    for (int tile = from; tile < to; ++tile) {
-      if (ok) ok = mbar_wait(&s_full[stage], phase, ERR_WAIT_FULL);
-      const uint32_t kb = smem_base + stage * S::kStageBytes, vb = kb + S::kTileBytes;
-      for (int gi = kw; gi < kKeys / 16; gi += S::kKeyWarps) {
-        const int j0 = tile * kKeys + gi * 16, slot = gi * 16 / ps;
-        if (!s_info[stage].live[slot] || j0 >= g.hi || j0 + 15 < g.lo) continue;  // warp-uniform: nothing of it is seen
-        const float ks = s_info[stage].ks[slot], vs0 = s_info[stage].vs[slot];
-        const float vs = vs0 < kTinyScale ? kTinyScale : vs0, lvs = lg2(vs), ivs = __fdividef(1.0f, vs);
-        // some row does not see some key of the group
-        const bool edge = j0 + 15 > g.pos_min || j0 + 15 >= g.hi || (p.a.window > 0 && j0 <= g.pos_max - p.a.window);
-
-        // S^T = K Q^T, two chains of sums
-        float sa[NT][4], sb[NT][4];
+    for (int tile = from; tile < to; ++tile, ++count) {
+      if (S::kSplit == 1 || count % S::kSplit == turn) {
+        if (ok) ok = mbar_wait(&s_full[stage], phase, ERR_WAIT_FULL);
+        const uint8_t* const kt = ring + stage * S::kStageBytes;
+        const uint8_t* const vt = kt + S::kTileBytes;
+#pragma unroll 1
+        for (int g0 = kpos * NG; g0 < kKeys / 16; g0 += S::kPosWarps * NG) {
+          // the warp's groups: which of them any row sees, whether some row does not see some key of them
+          float ks[NG], lvs[NG], ivs[NG];
+          bool seen[NG], any = false, edge = false;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int c = 0; c < 4; ++c) sa[nt][c] = sb[nt][c] = 0.0f;
-        const int r_lo = gi * 16 + key_lo, r_hi = gi * 16 + key_hi;
-#pragma unroll
-        for (int hf = 0; hf < S::kHalves; ++hf) {
-          constexpr int W = D == 64 ? 4 : 8;  // words of K a lane and key (and half)
-          uint32_t ka[W], kc[W];
-#pragma unroll
-          for (int i = 0; i < W; i += 4) {
-            uint32_t xa, xc;
-            if (D == 64) {
-              xa = (uint32_t)((r_lo >> 1) * 128 + (((((r_lo & 1) << 2) + t4) ^ ((r_lo >> 1) & 7)) << 4));
-              xc = (uint32_t)((r_hi >> 1) * 128 + (((((r_hi & 1) << 2) + t4) ^ ((r_hi >> 1) & 7)) << 4));
-            } else {
-              xa = (uint32_t)(hf * (kKeys * 128) + r_lo * 128 + (((2 * t4 + i / 4) ^ (r_lo & 7)) << 4));
-              xc = (uint32_t)(hf * (kKeys * 128) + r_hi * 128 + (((2 * t4 + i / 4) ^ (r_hi & 7)) << 4));
-            }
-            const uint4 a = lds128(kb + xa), c = lds128(kb + xc);
-            ka[i] = a.x, ka[i + 1] = a.y, ka[i + 2] = a.z, ka[i + 3] = a.w;
-            kc[i] = c.x, kc[i + 1] = c.y, kc[i + 2] = c.z, kc[i + 3] = c.w;
+          for (int k = 0; k < NG; ++k) {
+            const int j0 = tile * kKeys + (g0 + k) * 16, slot = (g0 + k) * 16 / ps;
+            seen[k] = s_info[stage].live[slot] && j0 < g.hi && j0 + 15 >= g.lo;
+            ks[k] = s_info[stage].ks[slot];
+            const float vs = s_info[stage].vs[slot] < kTinyScale ? kTinyScale : s_info[stage].vs[slot];
+            lvs[k] = lg2(vs);
+            ivs[k] = __fdividef(1.0f, vs);
+            any |= seen[k];
+            edge |= !seen[k] || j0 + 15 > g.pos_min || j0 + 15 >= g.hi || (p.a.window > 0 && j0 <= g.pos_max - p.a.window);
           }
+          if (!any) continue;
+
+          // S^T = K Q^T, two chains of sums a group
+          float sa[NG][NT][4], sb[NG][NT][4];
 #pragma unroll
-          for (int i = 0; i < W; ++i) {
-            uint32_t a0, a2, a1, a3;
-            f8x4_to_f16x4<FMT>(ka[i], a0, a2);
-            f8x4_to_f16x4<FMT>(kc[i], a1, a3);
+          for (int k = 0; k < NG; ++k)
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
-              mma_f16(i & 1 ? sb[nt] : sa[nt], a0, a1, a2, a3, q[nt][2 * (hf * W + i)], q[nt][2 * (hf * W + i) + 1]);
-          }
-        }
-        bool raise = false;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
+              for (int c = 0; c < 4; ++c) sa[k][nt][c] = sb[k][nt][c] = 0.0f;
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            float x = fmaf(sa[nt][c] + sb[nt][c], cq[nt][c & 1] * ks, lvs);
-            if (edge) {
-              const int j = j0 + (c < 2 ? key_lo : key_hi), pc = pos[nt][c & 1];
-              if (j > pc || j >= g.hi || (p.a.window > 0 && j <= pc - p.a.window)) x = -INFINITY;
-            }
-            sa[nt][c] = x;
-            raise |= x > m[nt][c & 1] + kRaise;
-          }
-        }
-        if (__any_sync(0xffffffffu, raise)) {  // some row's maximum has moved
+          for (int hf = 0; hf < S::kHalves; ++hf) {
+            constexpr int W = D == 64 ? 4 : 8;  // words of K a lane and key (and half)
+            uint32_t ka[NG][W], kc[NG][W];
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
+            for (int k = 0; k < NG; ++k) {
+              const int r_lo = (g0 + k) * 16 + key_lo, r_hi = (g0 + k) * 16 + key_hi;
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              float x = fmaxf(sa[nt][c], sa[nt][c + 2]);
-              x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
-              x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
-              x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-              const float mn = fmaxf(m[nt][c], x);
-              const float f = mn == m[nt][c] ? 1.0f : ex2(m[nt][c] - mn);
-              m[nt][c] = mn;
-              l[nt][c] *= f;
-#pragma unroll
-              for (int i = 0; i < S::kMT; ++i) {
-                o[i][nt][c] *= f;
-                o[i][nt][c + 2] *= f;
-              }
-            }
-        }
-        uint32_t pb[NT][2];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-          for (int c = 0; c < 4; ++c) sa[nt][c] = ex2(sa[nt][c] - (m[nt][c & 1] == -INFINITY ? 0.0f : m[nt][c & 1]));
-          l[nt][0] = fmaf(sa[nt][0] + sa[nt][2], ivs, l[nt][0]);
-          l[nt][1] = fmaf(sa[nt][1] + sa[nt][3], ivs, l[nt][1]);
-          pb[nt][0] = transpose_8x8(pack_f16(sa[nt][0], sa[nt][1]));
-          pb[nt][1] = transpose_8x8(pack_f16(sa[nt][2], sa[nt][3]));
-        }
-
-        // O^T += V^T P^T
-        bool odd_values = false;
-#pragma unroll
-        for (int hf = 0; hf < S::kHalves; ++hf) {
-          constexpr int W = D == 64 ? 2 : 4;  // words of V a lane and key (and half): channels q4 * 4 W ..
-          uint32_t v[4][W];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const int r = gi * 16 + vkey[k];
-            if (D == 64) {
-              const uint2 x = lds64(vb + (r >> 1) * 128 + (((((r & 1) << 2) + (q4 >> 1)) ^ ((r >> 1) & 7)) << 4) + (q4 & 1) * 8);
-              v[k][0] = x.x, v[k][1] = x.y;
-            } else {
-              const uint4 x = lds128(vb + hf * (kKeys * 128) + r * 128 + ((q4 ^ (r & 7)) << 4));
-              v[k][0] = x.x, v[k][1] = x.y, v[k][W - 2] = x.z, v[k][W - 1] = x.w;
-            }
-            if (edge) {
-              // a key that no row sees may hold anything, a key that some row does not see must not reach it by 0 * NaN
-              const int j = j0 + vkey[k];
-              const bool gone = j >= g.hi || j < g.lo;
-#pragma unroll
-              for (int i = 0; i < W; ++i) {
-                if (gone) v[k][i] = 0u;
-                if (nonfinite4<FMT>(v[k][i])) odd_values = true;
-              }
-            }
-          }
-          if (edge && __any_sync(0xffffffffu, odd_values)) {
-            // rare: take the non-finite codes out of the product and add them to the rows that see them
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-#pragma unroll
-              for (int i = 0; i < W; ++i) {
-                const uint32_t mk = FMT == F8_E4M3 ? 0x7F7F7F7Fu : 0x7C7C7C7Cu;
-                v[k][i] &= ~__vcmpeq4(v[k][i] & mk, mk);
-              }
-            for (int k = 0; k < 16; ++k) {
-              const int fr = D == 64 ? ((k >> 2) * 2 + (k & 1) + (k & 2) * 4) : k;  // fragment row of key k
-              float pv[NT][2];
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                  const float lo = __shfl_sync(0xffffffffu, sa[nt][c], (fr & 7) * 4 + t4), hi = __shfl_sync(0xffffffffu, sa[nt][c + 2], (fr & 7) * 4 + t4);
-                  pv[nt][c] = fr < 8 ? lo : hi;
+              for (int i = 0; i < W; i += 4) {
+                int xa, xc;
+                if (D == 64) {
+                  xa = (r_lo >> 1) * 128 + (((((r_lo & 1) << 2) + t4) ^ ((r_lo >> 1) & 7)) << 4);
+                  xc = (r_hi >> 1) * 128 + (((((r_hi & 1) << 2) + t4) ^ ((r_hi >> 1) & 7)) << 4);
+                } else {
+                  xa = hf * (kKeys * 128) + r_lo * 128 + (((2 * t4 + i / 4) ^ (r_lo & 7)) << 4);
+                  xc = hf * (kKeys * 128) + r_hi * 128 + (((2 * t4 + i / 4) ^ (r_hi & 7)) << 4);
                 }
-              const int r = gi * 16 + k, j = j0 + k;
-              if (j >= g.hi || j < g.lo) continue;
+                const uint4 a = *reinterpret_cast<const uint4*>(kt + xa), c = *reinterpret_cast<const uint4*>(kt + xc);
+                ka[k][i] = a.x, ka[k][i + 1] = a.y, ka[k][i + 2] = a.z, ka[k][i + 3] = a.w;
+                kc[k][i] = c.x, kc[k][i + 1] = c.y, kc[k][i + 2] = c.z, kc[k][i + 3] = c.w;
+              }
+            }
 #pragma unroll
-              for (int i = 0; i < 2 * W; ++i)
+            for (int i = 0; i < W; ++i)
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                  const int ch = q4 * 4 * W + 2 * i + e;  // channel within the half
-                  const uint32_t a = D == 64 ? (r >> 1) * 128 + (((((r & 1) << 2) + (ch >> 4)) ^ ((r >> 1) & 7)) << 4) + (ch & 15)
-                                             : hf * (kKeys * 128) + r * 128 + (((ch >> 4) ^ (r & 7)) << 4) + (ch & 15);
-                  uint32_t byte;
-                  asm volatile("ld.shared.u8 %0, [%1];" : "=r"(byte) : "r"(vb + a));
-                  const float val = f8_to_f32<FMT>((uint8_t)byte);
-                  if (!(fabsf(val) < INFINITY)) {
+              for (int k = 0; k < NG; ++k) {
+                uint32_t a0, a2, a1, a3;
+                f8x4_to_f16x4<FMT>(ka[k][i], a0, a2);
+                f8x4_to_f16x4<FMT>(kc[k][i], a1, a3);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+                  mma_f16(i & 1 ? sb[k][nt] : sa[k][nt], a0, a1, a2, a3, q[nt][2 * (hf * W + i)], q[nt][2 * (hf * W + i) + 1]);
+              }
+          }
+          bool raise = false;
+#pragma unroll
+          for (int k = 0; k < NG; ++k)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int c = 0; c < 4; ++c) {
+                float x = fmaf(sa[k][nt][c] + sb[k][nt][c], cq[nt][c & 1] * ks[k], lvs[k]);
+                if (edge) {
+                  const int j = tile * kKeys + (g0 + k) * 16 + (c < 2 ? key_lo : key_hi), pc = pos[nt][c & 1];
+                  if (!seen[k] || j > pc || j >= g.hi || (p.a.window > 0 && j <= pc - p.a.window)) x = -INFINITY;
+                }
+                sa[k][nt][c] = x;
+                raise |= x > m[nt][c & 1] + kRaise;
+              }
+          if (__any_sync(0xffffffffu, raise)) {  // some row's maximum has moved
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int c = 0; c < 2; ++c) {
+                float x = fmaxf(sa[0][nt][c], sa[0][nt][c + 2]);
+#pragma unroll
+                for (int k = 1; k < NG; ++k) x = fmaxf(x, fmaxf(sa[k][nt][c], sa[k][nt][c + 2]));
+                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+                const float mn = fmaxf(m[nt][c], x);
+                const float f = mn == m[nt][c] ? 1.0f : ex2(m[nt][c] - mn);
+                m[nt][c] = mn;
+                l[nt][c] *= f;
+#pragma unroll
+                for (int i = 0; i < S::kMT; ++i) {
+                  o[i][nt][c] *= f;
+                  o[i][nt][c + 2] *= f;
+                }
+              }
+          }
+          uint32_t pb[NG][NT][2];
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            const float m0 = m[nt][0] == -INFINITY ? 0.0f : m[nt][0], m1 = m[nt][1] == -INFINITY ? 0.0f : m[nt][1];
+#pragma unroll
+            for (int k = 0; k < NG; ++k) {
+#pragma unroll
+              for (int c = 0; c < 4; ++c) sa[k][nt][c] = ex2(sa[k][nt][c] - (c & 1 ? m1 : m0));
+              l[nt][0] = fmaf(sa[k][nt][0] + sa[k][nt][2], ivs[k], l[nt][0]);
+              l[nt][1] = fmaf(sa[k][nt][1] + sa[k][nt][3], ivs[k], l[nt][1]);
+              pb[k][nt][0] = transpose_8x8(pack_f16(sa[k][nt][0], sa[k][nt][1]));
+              pb[k][nt][1] = transpose_8x8(pack_f16(sa[k][nt][2], sa[k][nt][3]));
+            }
+          }
+
+          // O^T += V^T P^T
+#pragma unroll
+          for (int k = 0; k < NG; ++k)
+#pragma unroll
+            for (int hf = 0; hf < S::kHalves; ++hf) {
+              constexpr int W = D == 64 ? 2 : 4;  // words of V a lane and key (and half): channels q4 * 4 W ..
+              uint32_t v[4][W];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const int r = (g0 + k) * 16 + vkey[e];
+                if (D == 64) {
+                  const uint2 x = *reinterpret_cast<const uint2*>(vt + (r >> 1) * 128 + (((((r & 1) << 2) + (q4 >> 1)) ^ ((r >> 1) & 7)) << 4) + (q4 & 1) * 8);
+                  v[e][0] = x.x, v[e][1] = x.y;
+                } else {
+                  const uint4 x = *reinterpret_cast<const uint4*>(vt + hf * (kKeys * 128) + r * 128 + ((q4 ^ (r & 7)) << 4));
+                  v[e][0] = x.x, v[e][1] = x.y, v[e][W - 2] = x.z, v[e][W - 1] = x.w;
+                }
+              }
+              if (edge) {
+                // a key that no row sees may hold anything, and a key that some row does not see must not reach it by 0 * NaN
+                bool odd = false;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const int j = tile * kKeys + (g0 + k) * 16 + vkey[e];
+                  const bool gone = !seen[k] || j >= g.hi || j < g.lo;
+#pragma unroll
+                  for (int i = 0; i < W; ++i) {
+                    if (gone) v[e][i] = 0u;
+                    odd |= nonfinite4<FMT>(v[e][i]);
+                  }
+                }
+                if (__any_sync(0xffffffffu, odd)) {
+                  // rare: take the non-finite codes out of the product and add them to the rows that see them
+#pragma unroll
+                  for (int e = 0; e < 4; ++e)
+#pragma unroll
+                    for (int i = 0; i < W; ++i) {
+                      const uint32_t mk = FMT == F8_E4M3 ? 0x7F7F7F7Fu : 0x7C7C7C7Cu;
+                      v[e][i] &= ~__vcmpeq4(v[e][i] & mk, mk);
+                    }
+#pragma unroll 1
+                  for (int e = 0; e < 16; ++e) {
+                    const int fr = D == 64 ? ((e >> 2) * 2 + (e & 1) + (e & 2) * 4) : e;  // fragment row of key e
+                    float pv[NT][2];
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                      for (int c = 0; c < 2; ++c)
-                        if (pv[nt][c] != 0.0f) o[hf * 2 * W + i][nt][c + 2 * e] += pv[nt][c] * val;
+                      for (int c = 0; c < 2; ++c) {
+                        const float lo = __shfl_sync(0xffffffffu, sa[k][nt][c], (fr & 7) * 4 + t4), hi = __shfl_sync(0xffffffffu, sa[k][nt][c + 2], (fr & 7) * 4 + t4);
+                        pv[nt][c] = fr < 8 ? lo : hi;
+                      }
+                    const int r = (g0 + k) * 16 + e, j = tile * kKeys + r;
+                    if (j >= g.hi || j < g.lo) continue;
+#pragma unroll
+                    for (int i = 0; i < 2 * W; ++i)
+#pragma unroll
+                      for (int f = 0; f < 2; ++f) {
+                        const int ch = q4 * 4 * W + 2 * i + f;  // channel within the half
+                        const uint8_t byte = vt[D == 64 ? (r >> 1) * 128 + (((((r & 1) << 2) + (ch >> 4)) ^ ((r >> 1) & 7)) << 4) + (ch & 15)
+                                                        : hf * (kKeys * 128) + r * 128 + (((ch >> 4) ^ (r & 7)) << 4) + (ch & 15)];
+                        const float val = f8_to_f32<FMT>(byte);
+                        if (!(fabsf(val) < INFINITY)) {
+#pragma unroll
+                          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                            for (int c = 0; c < 2; ++c)
+                              if (pv[nt][c] != 0.0f) o[hf * 2 * W + i][nt][c + 2 * f] += pv[nt][c] * val;
+                        }
+                      }
                   }
                 }
+              }
+#pragma unroll
+              for (int i = 0; i < W; ++i) {
+                uint32_t a0, a1, a2, a3;
+                f8x4_to_f16x4<FMT>(__byte_perm(v[0][i], v[1][i], 0x5140), a0, a1);
+                f8x4_to_f16x4<FMT>(__byte_perm(v[2][i], v[3][i], 0x5140), a2, a3);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) mma_f16(o[hf * 2 * W + 2 * i][nt], a0, a1, a2, a3, pb[k][nt][0], pb[k][nt][1]);
+                f8x4_to_f16x4<FMT>(__byte_perm(v[0][i], v[1][i], 0x7362), a0, a1);
+                f8x4_to_f16x4<FMT>(__byte_perm(v[2][i], v[3][i], 0x7362), a2, a3);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) mma_f16(o[hf * 2 * W + 2 * i + 1][nt], a0, a1, a2, a3, pb[k][nt][0], pb[k][nt][1]);
+              }
             }
-          }
-#pragma unroll
-          for (int i = 0; i < W; ++i) {
-            uint32_t a0, a1, a2, a3;
-            f8x4_to_f16x4<FMT>(__byte_perm(v[0][i], v[1][i], 0x5140), a0, a1);
-            f8x4_to_f16x4<FMT>(__byte_perm(v[2][i], v[3][i], 0x5140), a2, a3);
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) mma_f16(o[hf * 2 * W + 2 * i][nt], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
-            f8x4_to_f16x4<FMT>(__byte_perm(v[0][i], v[1][i], 0x7362), a0, a1);
-            f8x4_to_f16x4<FMT>(__byte_perm(v[2][i], v[3][i], 0x7362), a2, a3);
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) mma_f16(o[hf * 2 * W + 2 * i + 1][nt], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
-          }
         }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s_empty[stage]);
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&s_empty[stage]);
       if (++stage == S::kStages) {
         stage = 0;
         phase ^= 1;
@@ -656,103 +791,71 @@ __global__ void __launch_bounds__(kThreads, 1)
         l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], 8);
         l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], 16);
       }
-    // a part: O register by register, then M and L, one value a lane; `f` visits each
-    auto put = [&](float* dst) {
+    float* const mine = merge + (rw * S::kKeyWarps + kw) * S::kPartFloats;
 #pragma unroll
-      for (int i = 0; i < S::kMT; ++i)
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-          *reinterpret_cast<float4*>(dst + ((i * NT + nt) * 32 + lane) * 4) = make_float4(o[i][nt][0], o[i][nt][1], o[i][nt][2], o[i][nt][3]);
+    for (int i = 0; i < S::kMT; ++i)
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
-        *reinterpret_cast<float4*>(dst + ((S::kMT * NT + nt) * 32 + lane) * 4) = make_float4(m[nt][0], m[nt][1], l[nt][0], l[nt][1]);
-    };
-    auto add = [&](const float* src, bool global) {  // joins another part to this one
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        const float4* x = reinterpret_cast<const float4*>(src + ((S::kMT * NT + nt) * 32 + lane) * 4);
-        const float4 ml = global ? __ldcg(x) : *x;
-        const float m0 = fmaxf(m[nt][0], ml.x), m1 = fmaxf(m[nt][1], ml.y);
-        const float a0 = m[nt][0] == m0 ? 1.0f : ex2(m[nt][0] - m0), a1 = m[nt][1] == m1 ? 1.0f : ex2(m[nt][1] - m1);
-        const float b0 = ml.x == m0 ? 1.0f : ex2(ml.x - m0), b1 = ml.y == m1 ? 1.0f : ex2(ml.y - m1);
-        m[nt][0] = m0;
-        m[nt][1] = m1;
-        l[nt][0] = l[nt][0] * a0 + ml.z * b0;
-        l[nt][1] = l[nt][1] * a1 + ml.w * b1;
-#pragma unroll
-        for (int i = 0; i < S::kMT; ++i) {
-          const float4* y = reinterpret_cast<const float4*>(src + ((i * NT + nt) * 32 + lane) * 4);
-          const float4 v = global ? __ldcg(y) : *y;
-          o[i][nt][0] = o[i][nt][0] * a0 + v.x * b0;
-          o[i][nt][1] = o[i][nt][1] * a1 + v.y * b1;
-          o[i][nt][2] = o[i][nt][2] * a0 + v.z * b0;
-          o[i][nt][3] = o[i][nt][3] * a1 + v.w * b1;
-        }
-      }
-    };
-#pragma unroll
-    for (int half = S::kKeyWarps / 2; half > 0; half >>= 1) {
-      if (kw >= half && kw < 2 * half) put(merge + (rw * (S::kKeyWarps / 2) + kw - half) * S::kPartFloats);
-      named_bar_sync(1, kConsumers * 32);
-      if (kw < half) add(merge + (rw * (S::kKeyWarps / 2) + kw) * S::kPartFloats, false);
-      named_bar_sync(1, kConsumers * 32);
-    }
-    if (kw != 0) continue;
-
-    bool write = true;
-    if (g.count != s.tiles) {
-      // the item is shared by CTAs c0 .. c1: each leaves its part, the last to come joins them in order
-      const int c0 = run_of(units, ctas, g.item0), c1 = run_of(units, ctas, g.item0 + s.tiles - 1);
-      auto part = [&](int c) {  // a CTA's first segment lies in slot 0, its last in slot 1
-        return p.parts + ((int64_t)(c * 2 + (g.item0 > run_begin(units, ctas, c) ? 1 : 0)) * RW + rw) * S::kPartFloats;
-      };
-      put(part(blockIdx.x));
-      __threadfence();
-      __syncwarp();
-      unsigned int prev = 0;
-      unsigned int* ctr = p.counters + g.item * RW + rw;
-      if (lane == 0) asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(prev) : "l"(ctr) : "memory");
-      prev = __shfl_sync(0xffffffffu, prev, 0);
-      write = prev == (unsigned)(c1 - c0);
-      if (write) {
-        __threadfence();
-        if (lane == 0) *ctr = 0;  // ready for the next call
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          m[nt][0] = m[nt][1] = -INFINITY;
-          l[nt][0] = l[nt][1] = 0.0f;
-#pragma unroll
-          for (int i = 0; i < S::kMT; ++i) o[i][nt][0] = o[i][nt][1] = o[i][nt][2] = o[i][nt][3] = 0.0f;
-        }
-        for (int c = c0; c <= c1; ++c) add(part(c), true);
-      }
-    }
-    if (!write) continue;
+        *reinterpret_cast<float4*>(mine + ((i * NT + nt) * 32 + lane) * 4) = make_float4(o[i][nt][0], o[i][nt][1], o[i][nt][2], o[i][nt][3]);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const int row = g.rt * S::kRows + (rw * NT + nt) * 8 + 2 * t4 + c;
-        if (row >= s.rows) continue;
-        const int64_t at = (int64_t)(s.t0 + row / p.group) * p.a.heads + g.h * p.group + row % p.group;
-        const float L = l[nt][c], inv = L == 0.0f ? 0.0f : __fdiv_rn(1.0f, L);
-        uint16_t* out = static_cast<uint16_t*>(p.a.out) + at * D;
-        constexpr int W = D == 64 ? 2 : 4;
-#pragma unroll
-        for (int hf = 0; hf < S::kHalves; ++hf)
-#pragma unroll
-          for (int i = 0; i < 2 * W; i += 4) {
-            uint32_t w[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const float x = o[hf * 2 * W + i + k][nt][c] * inv, y = o[hf * 2 * W + i + k][nt][c + 2] * inv;
-              w[k] = p.a.a_type == FP8IMMA_A_F16 ? pack_f16(x, y)
-                                                 : (uint32_t)f32_to_a16<1>(x) | ((uint32_t)f32_to_a16<1>(y) << 16);
-            }
-            *reinterpret_cast<uint4*>(out + hf * 128 + q4 * 4 * W + 2 * i) = make_uint4(w[0], w[1], w[2], w[3]);
-          }
-        if (p.a.lse && q4 == 0) p.a.lse[at] = L == 0.0f ? -INFINITY : 0.6931471805599453f * (m[nt][c] + log2f(L));
+      *reinterpret_cast<float4*>(mine + ((S::kMT * NT + nt) * 32 + lane) * 4) = make_float4(m[nt][0], m[nt][1], l[nt][0], l[nt][1]);
+    named_bar_sync(1, kConsumers * 32);
+    const Item it = {s.t0, s.rows, g.rt, g.h};
+    const bool shared = g.count != s.tiles;
+    float* const part = p.parts + (int64_t)(blockIdx.x * 2 + (g.item0 > walk_begin ? 1 : 0)) * RW * S::kPartFloats;
+    for (int x = tid; x < RW * S::kVecs; x += kConsumers * 32) {
+      const Frag<D, NT, RW> f(x);
+      Joined j;
+      const float* src = merge + f.warp * S::kKeyWarps * S::kPartFloats;
+      j.join(S::kKeyWarps, [&](int k) { return *reinterpret_cast<const float4*>(src + k * S::kPartFloats + f.at_ml); },
+             [&](int k) { return *reinterpret_cast<const float4*>(src + k * S::kPartFloats + f.at_o); });
+      if (shared) {
+        *reinterpret_cast<float4*>(part + f.warp * S::kPartFloats + f.at_o) = j.o;
+        if (f.i == 0) *reinterpret_cast<float4*>(part + f.warp * S::kPartFloats + f.at_ml) = make_float4(j.m0, j.m1, j.l0, j.l1);
+      } else {
+        store<D, NT, RW>(p, it, f, j);
       }
+    }
+    if (shared && tid == 0) {
+      s_shared[n_shared].item = it;
+      s_shared[n_shared].index = g.item;
+      s_shared[n_shared].c0 = runs.of(g.item0);
+      s_shared[n_shared].c1 = runs.of(g.item0 + s.tiles - 1);
+      s_shared[n_shared].item0 = g.item0;
+    }
+    n_shared += shared;
+    named_bar_sync(1, kConsumers * 32);  // the merge buffer is free again
+  }
+
+  // Shared items (the run's first and last at most): the CTA that comes last
+  // to an item joins all its parts, in CTA order.
+  if (n_shared == 0) return;
+  __threadfence();
+  named_bar_sync(1, kConsumers * 32);
+  if (tid < n_shared) {
+    unsigned int prev, *ctr = p.counters + s_shared[tid].index;
+    asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(prev) : "l"(ctr) : "memory");
+    s_shared[tid].last = prev == (unsigned)(s_shared[tid].c1 - s_shared[tid].c0);
+    if (s_shared[tid].last) *ctr = 0;  // ready for the next call
+  }
+  named_bar_sync(1, kConsumers * 32);
+  __threadfence();
+  for (int k = 0; k < n_shared; ++k) {
+    const Shared& sh = s_shared[k];
+    if (!sh.last) continue;
+    for (int x = tid; x < RW * S::kVecs; x += kConsumers * 32) {
+      const Frag<D, NT, RW> f(x);
+      Joined j;
+      // a CTA's part of the item lies in its slot 0 when its run begins within the item
+      auto src = [&](int c) {
+        c += sh.c0;
+        return p.parts + ((int64_t)(c * 2 + (sh.item0 > runs.begin(c) ? 1 : 0)) * RW + f.warp) * S::kPartFloats;
+      };
+      j.join(sh.c1 - sh.c0 + 1, [&](int c) { return __ldcg(reinterpret_cast<const float4*>(src(c) + f.at_ml)); },
+             [&](int c) { return __ldcg(reinterpret_cast<const float4*>(src(c) + f.at_o)); });
+      store<D, NT, RW>(p, sh.item, f, j);
+    }
   }
 }
 
@@ -773,8 +876,9 @@ cudaError_t launch(AttnParams& p, cudaStream_t st) {
   if (e != cudaSuccess) return e;
   const int64_t items = ((int64_t)p.c.tokens * p.group / S::kRows + p.c.batch) * p.c.kv_heads;
   const int64_t tiles = ((int64_t)p.c.max_pages * p.c.page_size + kKeys - 1) / kKeys;
+  if (items * tiles > 0x7fffffffll) return cudaErrorInvalidValue;  // units are counted in 31 bits
   const int grid = (int)std::min<int64_t>(num_sms_current(), std::max<int64_t>(1, items * tiles));
-  const size_t ctr_bytes = (size_t)items * RW * 4, part_bytes = (size_t)grid * 2 * RW * S::kPartFloats * 4;
+  const size_t ctr_bytes = (size_t)items * 4, part_bytes = (size_t)grid * 2 * RW * S::kPartFloats * 4;
   ScopedScratch ctr, part;
   e = ctr.get(ctr_bytes, st, kScratchAttn);
   if (e == cudaSuccess && ctr.owned) e = cudaMemsetAsync(ctr.ptr, 0, ctr_bytes, st);
@@ -782,8 +886,17 @@ cudaError_t launch(AttnParams& p, cudaStream_t st) {
   if (e == cudaSuccess) {
     p.counters = static_cast<unsigned int*>(ctr.ptr);
     p.parts = static_cast<float*>(part.ptr);
-    kern<<<grid, kThreads, S::kSmem, st>>>(mk, mv, p);
-    e = cudaGetLastError();
+    cudaLaunchConfig_t lc = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    lc.gridDim = dim3(grid);
+    lc.blockDim = dim3(kThreads);
+    lc.dynamicSmemBytes = S::kSmem;
+    lc.stream = st;
+    lc.attrs = attr;
+    lc.numAttrs = api_pdl() ? 1 : 0;
+    e = cudaLaunchKernelEx(&lc, kern, mk, mv, p);
   }
   const cudaError_t e1 = ctr.release(st), e2 = part.release(st);
   return e != cudaSuccess ? e : e1 != cudaSuccess ? e1 : e2;
@@ -837,7 +950,6 @@ extern "C" int fp8imma_kv_attention(const fp8imma_kv_cache* c, const fp8imma_kv_
   p.per_seq = c->cu_new ? 0 : c->tokens / c->batch;
   p.group = a->heads / c->kv_heads;
   p.vec_q = ((reinterpret_cast<uintptr_t>(a->q) | (uintptr_t)((a->q_token_stride | a->q_head_stride) * 2)) & 15u) == 0;
-  p.min_units = 2;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return (int)(c->format == FP8IMMA_B_E4M3 ? launch_d<F8_E4M3>(p, st) : launch_d<F8_E5M2>(p, st));
 }

@@ -189,6 +189,34 @@ def test_attention_ignores_what_lies_behind_the_end(ops, dtype):
     check(*run_attend(ops, q, (table, kc, vc, ks, vs), lens, [0, 1, 2, 3], 0, fmt))
 
 
+@pytest.mark.parametrize("fmt", ["e4m3", "e5m2"])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_attention_nan_in_keys_that_some_rows_do_not_see(ops, d, fmt):
+    """A draft token with NaN (and, in E5M2, infinite) keys and values reaches the rows from its own on and no
+    earlier one; a key that has left the window reaches only the rows that still see it."""
+    g = gen(60)
+    lens, n, hq, hk, ps = [150, 40], 6, 14, 2, 32
+    table, kc, vc, ks, vs = make_cache(g, 2, 5, hk, ps, d, fmt)
+    bad = 0x7F if fmt == "e4m3" else 0x7C
+
+    def at(b, pos):
+        return int(table[b, pos // ps]), slice(None), pos % ps
+
+    vc[at(0, 147)][0, 5::16] = bad       # value of a draft token, some channels, head 0
+    kc[at(1, 37)][1, 3] = 0x7F           # key of a draft token, one channel, head 1
+    vc[at(0, 150 - 6 - 20 + 2)][1] = 0x7F  # leaves the window after the second row
+    q = torch.randn(12, hq, d, generator=g, device="cuda").half()
+    cu, window, scale = [0, 6, 12], 20, 1 / math.sqrt(d)
+    out, lse, _ = run_attend(ops, q, (table, kc, vc, ks, vs), lens, cu, window, fmt)
+    o, l, bound = ref_attention(q, kc, vc, ks, vs, table, lens, cu, scale, window, fmt)
+    assert torch.isfinite(o).any() and not torch.isfinite(o).all()
+    assert torch.equal(torch.isnan(out), torch.isnan(o)) and torch.equal(torch.isnan(lse), torch.isnan(l))
+    inf = torch.isinf(o)
+    assert torch.equal(torch.isinf(out), inf) and torch.equal(out[inf].double(), o[inf])
+    fine = torch.isfinite(o)
+    assert ((out.double() - o).abs()[fine] <= bound[fine]).all()
+
+
 def test_attention_skips_holes(ops):
     """Holes at the front, in the middle, everywhere; holes that hide a whole stretch of pages."""
     g = gen(41)
