@@ -4,26 +4,32 @@
 // Mathematics: r = x Wr^T (fp32), S_t the top_k experts of token t, p the
 // softmax; per chosen (token, expert) slot
 //   h = act(sg (x Wg^T)) * (su (x Wu^T)),  out_t = sum_S p sd (h Wd^T).
-// FP8 codes are multiplied as fp16 (exact); x and h enter as fp16 rows that a
-// power of two has brought into fp16's range (exact for fp16 x and for bf16
-// values within 2^22 of the row's largest; h is rounded to 2^-11), sums are
-// fp32, scales and the powers of two are applied to the sums.
+// FP8 codes are multiplied as fp16 (exact); sums are fp32, scales are applied
+// to the sums. x enters as it is when it is fp16; a bf16 row is brought into
+// fp16's range by a power of two (exact within 2^22 of the row's largest). h
+// is rounded to fp16, 2^-11, after a power of two of its slot that keeps it
+// below 2^15: |act(g) u| <= |g| |u|, and a gate or up sum is at most
+// max_i s_i * fmax * sum |x|. Typical h lie some 2^16 below that bound, well
+// inside fp16's normal range, and no largest value has to be agreed on first.
 //
 // Bound: a few tokens use each weight byte a few times, so the layer costs the
 // bytes of the chosen experts. One cooperative grid, one CTA per SM, keeps
 // their stream running through the whole layer:
-//  0. router logits (warps over experts x tokens), x to fp16 in operand order;
-//     grid barrier; every CTA picks the top_k of all tokens for itself
+//  0. router logits (warps over experts x tokens), x to fp16 in operand order,
+//     the experts' largest scales; grid barrier; every CTA picks the top_k of
+//     all tokens for itself
 //  1. gate / up: the chosen experts' row groups are laid end to end and cut
 //     into equal runs; a unit is 8 RU gate rows and the same 8 RU up rows, so
 //     that both factors of h meet in one fragment; grid barrier
 //  2. down: the same over units of 16 RU rows; slot results to scratch; barrier
 //  3. out = sum over a token's slots, in their order
-// A warp takes every eighth 128-byte column block of the flattened (unit,
-// block) sequence and streams its blocks by TMA into a ring of its own, across
-// unit and phase boundaries: the down weights are under way while the grid
-// meets at the barrier before them. The eight warps' partial sums of a unit
-// meet in shared memory in a fixed order; nothing depends on timing.
+// A warp works on units of its own (few units: a team of 2, 4 or 8 warps shares
+// one along the columns). Each lane copies the 16-byte pieces of its own
+// operand rows asynchronously into a queue of its own in shared memory, some
+// 128-byte column blocks ahead, across unit and phase boundaries: no barrier
+// between lanes or warps, and the down weights are under way while the grid
+// meets at the barrier before them. A team's sums meet in shared memory in a
+// fixed order; nothing depends on timing.
 #include "fp8_mma.cuh"
 #include "fp8imma/fp8imma_ext.h"
 #include "fp8imma_kernels.h"
@@ -37,8 +43,6 @@ namespace {
 
 using namespace fp8imma_dev;
 
-constexpr int kWarps = 8;
-constexpr int kThreads = kWarps * 32;
 constexpr int kMaxSlots = FP8IMMA_MOE_MAX_TOKENS * FP8IMMA_MOE_MAX_TOP_K;
 
 struct MoeParams {
@@ -46,11 +50,11 @@ struct MoeParams {
   unsigned int* sync;  // three barrier counters, zero between calls
   float* logits;       // [tokens, experts]
   uint16_t* xf;        // [tokens, hidden padded to 128] fp16, operand order
-  float* xback;        // [tokens] what a row of xf is to be multiplied by
-  unsigned int* hmax;  // [slots] bits of the largest |h|
-  float* h;            // [slots, inter padded to 128] operand order
+  float* xback;        // [tokens, 2] what a row of xf is to be multiplied by, sum |x|
+  float* smax;         // [experts, 2, chunks] largest gate / up scale of 1024 rows
+  uint16_t* h;         // [slots, inter padded to 128] fp16, operand order
   float* part;         // [slots, hidden]
-  int hpad, ipad;
+  int hpad, ipad, chunks;
 };
 
 // ---------------------------------------------------------------- helpers --
@@ -96,14 +100,14 @@ __device__ __forceinline__ bool grid_barrier(unsigned int* ctr) {
   __shared__ int s_ok;
   __syncthreads();
   if (threadIdx.x == 0) {
-    __threadfence();
-    unsigned int v;
-    asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(v) : "l"(ctr) : "memory");
-    ++v;
+    // the CTA's writes are ordered before the release by the barrier above
+    asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(ctr) : "memory");
+    unsigned int v = 0;
     bool ok = true;
     const unsigned long long t0 = globaltimer_ns();
-    while (v < gridDim.x) {
+    for (;;) {
       asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(ctr) : "memory");
+      if (v >= gridDim.x) break;
       const unsigned long long dt = globaltimer_ns() - t0;
       if (dt > kWaitCheckNs && dt > *(volatile unsigned long long*)&g_fp8imma_wait_limit_ns) {
         atomicCAS(&g_fp8imma_device_error, 0u, (unsigned int)ERR_WAIT_PEER);
@@ -111,7 +115,6 @@ __device__ __forceinline__ bool grid_barrier(unsigned int* ctr) {
         break;
       }
     }
-    __threadfence();
     s_ok = ok;
   }
   __syncthreads();
@@ -124,15 +127,20 @@ struct Runs {  // CTA c's run of the units: they differ by one in length at most
   __device__ __forceinline__ int begin(int c) const { return c * per + min(c, rem); }
 };
 
-// NT: 8-token tiles at most; RU: 16-row tiles of a unit.
-template <int NT, int RU>
+// 16 bytes global -> shared, asynchronously; zeros when not `in`
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool in) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
+}
+
+// NT: 8-token tiles of a unit at most; RU: 16-row tiles of a unit; WARPS a CTA;
+// DEPTH: blocks of a lane's queue.
+template <int NT, int RU, int WARPS, int DEPTH>
 struct Shape {
-  static constexpr int kStageBytes = 2048 * RU;
-  static constexpr int kStages = RU == 1 ? 8 : NT == 8 ? 4 : 5;
-  static constexpr int kRing = kStages * kStageBytes;  // of a warp
-  static constexpr int kRedFloats = 16 * RU * 8 * NT;  // of a warp
-  static constexpr int kRedBufs = NT <= 2 ? 2 : 1;
-  static constexpr int kSmem = 1024 + kWarps * (kRing + kRedBufs * kRedFloats * 4);
+  static constexpr int kThreads = WARPS * 32;
+  static constexpr int kPieces = 4 * RU;               // 16-byte pieces of a block a lane
+  static constexpr int kQueue = DEPTH * kPieces * 512; // of a warp
+  static constexpr int kFragFloats = RU * NT * 4 * 32; // a unit's sums of a warp
+  static constexpr int kSmem = WARPS * (kQueue + kFragFloats * 4);
 };
 
 // Router logits of EX experts x TX tokens a warp, and nothing else.
@@ -190,17 +198,32 @@ __device__ __forceinline__ void router(const MoeParams& p, int wid, int nw, int 
   }
 }
 
-// Place of element k of a row in operand order: lane t4 of a fragment reads
-// bytes 32 t4 .. 32 t4 + 31 of a 128-byte weight block, four a product step s.
-// x keeps eight fp16 (two steps) together, h four fp32 (one step).
-__device__ __forceinline__ int x_place(int k) { return (k & ~127) + (((k & 31) >> 3) << 5) + (((k >> 5) & 3) << 3) + (k & 7); }
-__device__ __forceinline__ int h_place(int k) { return (k & ~127) + (((k & 31) >> 2) << 4) + (((k >> 5) & 3) << 2) + (k & 3); }
+// Place of element k of a row in operand order: lane t4 of a fragment holds
+// bytes 16 t4 .. 16 t4 + 15 of both halves of a 128-byte weight block, four
+// bytes a product step; eight fp16, two steps, lie together.
+__device__ __forceinline__ int place(int k) { return (k & ~127) + (((k >> 5) & 2) + ((k >> 3) & 1)) * 32 + (((k >> 4) & 3) << 3) + (k & 7); }
+
+// Largest gate / up scales by chunks of 1024 rows.
+__device__ __forceinline__ void scale_maxima(const MoeParams& p, int wid, int nw, int lane) {
+#pragma unroll 1
+  for (int u = wid; u < p.a.experts * 2 * p.chunks; u += nw) {
+    const int c = u % p.chunks, row = u / p.chunks;  // row: expert * 2 + (gate, up)
+    const float* s = p.a.s_gate_up + (size_t)row * p.a.inter;
+    const int hi = min(p.a.inter, c * 1024 + 1024);
+    float m = 0.0f;
+#pragma unroll 8
+    for (int i = c * 1024 + lane; i < hi; i += 32) m = fmaxf(m, fabsf(__ldg(s + i)));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if (lane == 0) p.smax[u] = m;
+  }
+}
 
 // A token's row as fp16 in operand order; one warp.
 template <int AT>
 __device__ __forceinline__ void convert_row(const MoeParams& p, int t, int lane, bool vec) {
   const uint16_t* x = static_cast<const uint16_t*>(p.a.x) + t * p.a.x_token_stride;
-  float f = 1.0f, back = 1.0f;
+  float f = 1.0f, back = 1.0f, sum = 0.0f;
   auto load8 = [&](int k) {
     if (vec) return __ldg(reinterpret_cast<const uint4*>(x + k));
     uint32_t w[4];
@@ -226,116 +249,104 @@ __device__ __forceinline__ void convert_row(const MoeParams& p, int t, int lane,
     uint4 v = make_uint4(0, 0, 0, 0);
     if (k < p.a.hidden) {
       v = load8(k);
+      uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sum += fabsf(a16_to_f32<AT>((uint16_t)(w[i] & 0xFFFFu))) + fabsf(a16_to_f32<AT>((uint16_t)(w[i] >> 16)));
       if (AT == 1) {
-        uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) w[i] = pack_f16(__uint_as_float(w[i] << 16) * f, __uint_as_float(w[i] & 0xFFFF0000u) * f);
         v = make_uint4(w[0], w[1], w[2], w[3]);
       }
     }
-    *reinterpret_cast<uint4*>(p.xf + (size_t)t * p.hpad + x_place(k)) = v;
+    *reinterpret_cast<uint4*>(p.xf + (size_t)t * p.hpad + place(k)) = v;
   }
-  if (lane == 0) p.xback[t] = back;
+  sum = warp_sum(sum);
+  if (lane == 0) {
+    p.xback[2 * t] = back;
+    p.xback[2 * t + 1] = sum;
+  }
 }
 
+// An entry is up to 8 NT tokens of a chosen expert.
+constexpr int kMaxEntries = FP8IMMA_MOE_MAX_EXPERTS + kMaxSlots / 8;
 struct Lists {
   unsigned long long tokens[FP8IMMA_MOE_MAX_EXPERTS];  // tokens that chose the expert
-  short expert[FP8IMMA_MOE_MAX_EXPERTS];               // chosen experts, ascending
-  short start[FP8IMMA_MOE_MAX_EXPERTS + 1];            // their first entry in `slot`
+  short first[FP8IMMA_MOE_MAX_EXPERTS];                // an expert's first place in `slot`
+  short expert[kMaxEntries];                           // of an entry, ascending
+  short start[kMaxEntries + 1];                        // its first place in `slot`
   short slot[kMaxSlots];                               // slots by expert, tokens ascending
+  short token[kMaxSlots];                              // and their tokens
   short id[kMaxSlots];                                 // expert of a slot
   float weight[kMaxSlots];                             // p of a slot
-  float scale[kMaxSlots];                              // phase 1: largest |h| bits; phase 2: factor that brings h into fp16's range
-  int active;
-  int scan[kWarps];
+  float scale[kMaxSlots];                              // factor that brings a slot's h into fp16's range
+  float xback[FP8IMMA_MOE_MAX_TOKENS];
+  int entries;
+  int scan[16];
 };
 
-// Two tokens' top_k at once by one warp (their chains of reductions overlap).
-__device__ __forceinline__ void pick(const MoeParams& p, Lists& L, int t0, int lane) {
+// A token's top_k by one warp: rounds of the largest logit not yet taken.
+__device__ __forceinline__ void pick(const MoeParams& p, Lists& L, int t, int lane) {
   const int E = p.a.experts, K = p.a.top_k;
-  unsigned taken[2] = {0u, 0u};
-  float first[2] = {0.0f, 0.0f}, sum[2] = {0.0f, 0.0f};
-  const float* r[2] = {p.logits + (size_t)t0 * E, p.logits + (size_t)min(t0 + 1, p.a.tokens - 1) * E};
-  float keep[2][4];  // the first 128 experts stay in registers
+  const float* r = p.logits + (size_t)t * E;
+  unsigned taken = 0u;  // expert lane + 32 * bit
+  float keep[4], first = 0.0f, sum = 0.0f;  // the first 128 experts stay in registers
 #pragma unroll
-  for (int q = 0; q < 2; ++q)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) keep[q][i] = lane + 32 * i < E ? __ldcg(r[q] + lane + 32 * i) : 0.0f;
+  for (int i = 0; i < 4; ++i) keep[i] = lane + 32 * i < E ? __ldcg(r + lane + 32 * i) : 0.0f;
+#pragma unroll 1
   for (int s = 0; s < K; ++s) {
-    int best[2], at[2];
-    float val[2];
-#pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      best[q] = (int)0x80000000;
-      at[q] = 0x7fffffff;
-      val[q] = 0.0f;
-      bool any = false;
-      auto look = [&](int i, float v) {
-        const int key = order_key(v);
-        if (!((taken[q] >> i) & 1u) && (!any || key > best[q])) {
-          best[q] = key;
-          at[q] = lane + 32 * i;
-          val[q] = v;
-          any = true;
-        }
-      };
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (lane + 32 * i < E) look(i, keep[q][i]);
-      for (int i = 4; lane + 32 * i < E; ++i) look(i, __ldcg(r[q] + lane + 32 * i));
-    }
-#pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      const int top = __reduce_max_sync(0xffffffffu, best[q]);
-      const int e = __reduce_min_sync(0xffffffffu, best[q] == top ? at[q] : 0x7fffffff);
-      val[q] = __shfl_sync(0xffffffffu, val[q], e & 31);
-      if ((e & 31) == lane) taken[q] |= 1u << (e >> 5);
-      if (s == 0) first[q] = val[q];
-      const float w = __expf(val[q] - first[q]);
-      sum[q] += w;
-      if (lane == 0 && t0 + q < p.a.tokens) {
-        L.id[(t0 + q) * K + s] = (short)e;
-        L.weight[(t0 + q) * K + s] = w;
+    int best = (int)0x80000000, at = 0x7fffffff;
+    float val = 0.0f;
+    auto look = [&](int i, float v) {
+      const int key = order_key(v);
+      if (!((taken >> i) & 1u) && (at == 0x7fffffff || key > best)) {
+        best = key;
+        at = lane + 32 * i;
+        val = v;
       }
+    };
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (lane + 32 * i < E) look(i, keep[i]);
+#pragma unroll 1
+    for (int i = 4; lane + 32 * i < E; ++i) look(i, __ldcg(r + lane + 32 * i));
+    const int top = __reduce_max_sync(0xffffffffu, best);
+    const int e = __reduce_min_sync(0xffffffffu, best == top ? at : 0x7fffffff);
+    val = __shfl_sync(0xffffffffu, val, e & 31);
+    if ((e & 31) == lane) taken |= 1u << (e >> 5);
+    if (s == 0) first = val;
+    const float w = __expf(val - first);
+    sum += w;
+    if (lane == 0) {
+      L.id[t * K + s] = (short)e;
+      L.weight[t * K + s] = w;
     }
   }
   if (!p.a.renormalize) {
-#pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      float z = 0.0f;
-      for (int i = lane; i < E; i += 32) z += __expf(__ldcg(r[q] + i) - first[q]);
-      sum[q] = warp_sum(z);
-    }
+    float z = 0.0f;
+    for (int i = lane; i < E; i += 32) z += __expf(__ldcg(r + i) - first);
+    sum = warp_sum(z);
   }
   __syncwarp();
-#pragma unroll
-  for (int q = 0; q < 2; ++q)
-    if (t0 + q < p.a.tokens && lane < K) L.weight[(t0 + q) * K + lane] = __fdiv_rn(L.weight[(t0 + q) * K + lane], sum[q]);
+  if (lane < K) L.weight[t * K + lane] = __fdiv_rn(L.weight[t * K + lane], sum);
 }
 
-template <int FMT, int NT, int RU>
-__global__ void __launch_bounds__(kThreads, 1)
-    moe_kernel(const __grid_constant__ CUtensorMap map_up, const __grid_constant__ CUtensorMap map_down, const __grid_constant__ MoeParams p) {
-  using S = Shape<NT, RU>;
-  extern __shared__ uint8_t smem_raw[];
+template <int FMT, int NT, int RU, int WARPS, int DEPTH>
+__global__ void __launch_bounds__(WARPS * 32, 1) moe_kernel(const __grid_constant__ MoeParams p) {
+  using S = Shape<NT, RU, WARPS, DEPTH>;
+  constexpr int kThreads = S::kThreads;
+  constexpr int CH = NT * RU <= 2 ? 2 : 1;  // chains of dependent products a tile
+  extern __shared__ __align__(16) uint8_t smem_raw[];
   __shared__ Lists L;
-  __shared__ uint64_t s_full[kWarps][S::kStages];
-  const uint32_t off = ((smem_u32(smem_raw) + 1023u) & ~1023u) - smem_u32(smem_raw);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, q4 = lane >> 2, t4 = lane & 3;
-  uint8_t* const ring = smem_raw + off + warp * S::kRing;
-  float* const red = reinterpret_cast<float*>(smem_raw + off + kWarps * S::kRing);
+  const uint4* const queue = reinterpret_cast<const uint4*>(smem_raw + warp * S::kQueue) + lane;  // pieces 32 apart
+  const uint32_t queue_at = smem_u32(queue);
+  float* const frags = reinterpret_cast<float*>(smem_raw + WARPS * S::kQueue);
   const int T = p.a.tokens, E = p.a.experts, K = p.a.top_k, H = p.a.hidden, I = p.a.inter;
-
-  if (lane == 0) {
-    for (int i = 0; i < S::kStages; ++i) mbar_init(&s_full[warp][i], 1);
-    fence_barrier_init();
-    prefetch_tensormap(warp & 1 ? &map_down : &map_up);
-  }
 
   // ------------------------------------------------- 0: router, x to fp16 --
   {
     // warps of the grid, CTA by CTA, so that few units spread over many SMs
-    const int wid = warp * gridDim.x + blockIdx.x, nw = kWarps * gridDim.x;
+    const int wid = warp * gridDim.x + blockIdx.x, nw = WARPS * gridDim.x;
     const bool vec = ((reinterpret_cast<uintptr_t>(p.a.x) | reinterpret_cast<uintptr_t>(p.a.router) | (uintptr_t)(p.a.x_token_stride * 2)) & 15u) == 0;
     const bool bf = p.a.a_type == FP8IMMA_A_BF16;
     for (int t = nw - 1 - wid; t < T; t += nw) {  // from the last warp on: the first have router units
@@ -354,16 +365,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (bf) router<1, 4, 4>(p, wid, nw, lane, vec);
       else router<0, 4, 4>(p, wid, nw, lane, vec);
     }
-    if (blockIdx.x == 0)
-      for (int s = tid; s < T * K; s += kThreads) p.hmax[s] = 0u;
+    scale_maxima(p, nw - 1 - wid, nw, lane);
   }
-  if (!grid_barrier(p.sync)) return;  // no copies are under way yet
+  for (int e = tid; e < E; e += kThreads) L.tokens[e] = 0ull;
+  if (!grid_barrier(p.sync)) return;
   if (blockIdx.x == 0 && tid == 0) p.sync[2] = 0u;  // all CTAs of the call before have left its last barrier
 
   // -------------------------------------------------------- choice, lists --
-  for (int e = tid; e < E; e += kThreads) L.tokens[e] = 0ull;
-  for (int s = tid; s < T * K; s += kThreads) L.scale[s] = 0.0f;
-  for (int t = warp * 2; t < T; t += kWarps * 2) pick(p, L, t, lane);
+  if (tid < T) L.xback[tid] = __ldcg(p.xback + 2 * tid);
+#pragma unroll 1
+  for (int t = warp; t < T; t += WARPS) pick(p, L, t, lane);
   __syncthreads();
   for (int s = tid; s < T * K; s += kThreads) {
     atomicOr(&L.tokens[L.id[s]], 1ull << (s / K));
@@ -371,14 +382,29 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (p.a.ids) p.a.ids[s] = L.id[s];
       if (p.a.weights) p.a.weights[s] = L.weight[s];
     }
+    // the slot's power of two: gate sums are below 2^(eg + 1), up sums below 2^(eu + 1)
+    const float l1 = __ldcg(p.xback + 2 * (s / K) + 1), *m = p.smax + (size_t)L.id[s] * 2 * p.chunks;
+    float mg = 0.0f, mu = 0.0f;
+#pragma unroll 4
+    for (int c = 0; c < p.chunks; ++c) {
+      mg = fmaxf(mg, __ldcg(m + c));
+      mu = fmaxf(mu, __ldcg(m + p.chunks + c));
+    }
+    const float fmax_v = FMT == F8_E4M3 ? 448.0f : 57344.0f;
+    const int eg = (int)(__float_as_uint(mg * fmax_v * l1) >> 23) - 127, eu = (int)(__float_as_uint(mu * fmax_v * l1) >> 23) - 127;
+    const int k = max(-126, min(126, eg + eu - 13));
+    L.scale[s] = __uint_as_float((uint32_t)(127 - k) << 23);
+    L.weight[s] *= __uint_as_float((uint32_t)(127 + k) << 23);  // a slot's result is multiplied by its weight and by what undoes the factor
   }
   __syncthreads();
   {
-    int active = 0, slots = 0;
+    int entries = 0, slots = 0;
+#pragma unroll 1
     for (int e0 = 0; e0 < E; e0 += kThreads) {
       const int e = e0 + tid;
-      const int n = e < E ? __popcll(L.tokens[e]) : 0;
-      int x = n | ((n > 0) << 16);  // slots and experts so far
+      const unsigned long long m = e < E ? L.tokens[e] : 0ull;
+      const int n = __popcll(m), ne = (n + 8 * NT - 1) / (8 * NT);
+      int x = n | (ne << 16);  // slots and entries so far
       const int own = x;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -388,294 +414,281 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncthreads();
       if (lane == 31) L.scan[warp] = x;
       __syncthreads();
-      int before = slots | (active << 16), total = 0;
-      for (int w = 0; w < kWarps; ++w) {
+      int before = slots | (entries << 16), total = 0;
+#pragma unroll 1
+      for (int w = 0; w < WARPS; ++w) {
         if (w < warp) before += L.scan[w];
         total += L.scan[w];
       }
       before += x - own;
-      if (n > 0) {
-        L.expert[before >> 16] = (short)e;
-        L.start[before >> 16] = (short)(before & 0xFFFF);
+      for (int k = 0; k < ne; ++k) {
+        L.expert[(before >> 16) + k] = (short)e;
+        L.start[(before >> 16) + k] = (short)((before & 0xFFFF) + k * 8 * NT);
       }
+      if (e < E) L.first[e] = (short)(before & 0xFFFF);
       slots += total & 0xFFFF;
-      active += total >> 16;
+      entries += total >> 16;
     }
     if (tid == 0) {
-      L.active = active;
-      L.start[active] = (short)slots;
+      L.entries = entries;
+      L.start[entries] = (short)slots;
     }
   }
   __syncthreads();
-  const int active = L.active;
-  for (int a = warp; a < active; a += kWarps) {  // slots of each chosen expert, tokens ascending
-    const unsigned long long m = L.tokens[L.expert[a]];
-    for (int t = lane; t < T; t += 32)
-      if ((m >> t) & 1ull) {
-        int s = t * K;
-        while (L.id[s] != L.expert[a]) ++s;
-        L.slot[L.start[a] + __popcll(m & ((1ull << t) - 1ull))] = (short)s;
-      }
+  for (int s = tid; s < T * K; s += kThreads) {  // slots by expert, tokens ascending
+    const int t = s / K, at = L.first[L.id[s]] + __popcll(L.tokens[L.id[s]] & ((1ull << t) - 1ull));
+    L.slot[at] = (short)s;
+    L.token[at] = (short)t;
   }
   __syncthreads();
 
   // --------------------------------------------------- the weights' stream --
-  // Units per expert, column blocks per unit of the two phases; this CTA's runs.
+  // Units of the two phases, this CTA's runs of them, the teams that share one.
+  const int entries = L.entries;
   const int per1 = (I + 8 * RU - 1) / (8 * RU), per2 = (H + 16 * RU - 1) / (16 * RU);
   const int nb1 = p.hpad >> 7, nb2 = p.ipad >> 7;
-  const Runs runs1(active * per1, gridDim.x), runs2(active * per2, gridDim.x);
+  const Runs runs1(entries * per1, gridDim.x), runs2(entries * per2, gridDim.x);
   const int u1 = runs1.begin(blockIdx.x), n1 = runs1.begin(blockIdx.x + 1) - u1;
   const int u2 = runs2.begin(blockIdx.x), n2 = runs2.begin(blockIdx.x + 1) - u2;
+  auto team_of = [](int longest) {  // warps that share a unit: more than one only where each team has one unit
+    int ks = 1;
+    while (ks < 8 && longest * ks * 2 <= WARPS) ks *= 2;
+    return ks;
+  };
+  const int ks1 = team_of(runs1.per + (runs1.rem > 0)), ks2 = team_of(runs2.per + (runs2.rem > 0));
 
-  // loading side of this warp: next block to ask for
-  int lp = 1, lu = 0, lb = warp, issued = 0, used = 0, lost = 0;
-  bool ok = true;
+  // loading side of this warp: the next block to ask for. A lane copies its
+  // rows' pieces itself: rows r * 8 + q4 of the gate (first) and up (second)
+  // box, bytes 16 t4 of both halves of the block.
+  int lp = 1, lu = warp / ks1, lb = warp % ks1, put = 0, got = 0;
+  const uint8_t* lrow = nullptr;  // the lane's first row of the unit
+  auto unit_row = [&]() {
+    const bool up = lp == 1;
+    const int per = up ? per1 : per2, u = (up ? u1 : u2) + lu, a = u / per;
+    const int row = (u - a * per) * (up ? 8 * RU : 16 * RU) + q4;
+    lrow = static_cast<const uint8_t*>(up ? p.a.w_gate_up : p.a.w_down) + ((size_t)L.expert[a] * (up ? 2 * I : H) + row) * (up ? H : I) + t4 * 16;
+  };
   auto issue = [&]() {
-    if (!ok) return;
-    // one block further down the flattened sequence, over the phases' ends
-    if (lp == 1) {
-      while (lb >= nb1) lb -= nb1, ++lu;
-      if (lu >= n1) lp = 2, lu = 0, lb = warp;
+    bool fresh = put == 0;
+    if (lp == 1 && lb >= nb1) lb = warp % ks1, lu += WARPS / ks1, fresh = true;
+    if (lp == 1 && (lu >= n1 || lb >= nb1)) lp = 2, lu = warp / ks2, lb = warp % ks2, fresh = true;
+    if (lp == 2 && lb >= nb2) lb = warp % ks2, lu += WARPS / ks2, fresh = true;
+    if (lp == 2 && (lu >= n2 || lb >= nb2)) lp = 3;
+    if (lp < 3) {
+      if (fresh) unit_row();
+      const bool up = lp == 1;
+      const int width = up ? H : I;
+      const size_t box = (size_t)(up ? I : 8 * RU) * width;  // from a row of the first box to its row of the second
+      // rows past the last one of the matrix (the end of a unit that is not whole) read its last
+      const int tail = up ? 0x7fffffff : H - 1 - ((u2 + lu) % per2 * (16 * RU) + q4);
+      const uint32_t dst = queue_at + put % DEPTH * (S::kPieces * 512);
+#pragma unroll
+      for (int r = 0; r < RU; ++r)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const int step = r * 8 + (up ? 0 : k * 8 * RU);  // rows down from the lane's first, second box of the down weights included
+          const uint8_t* src = lrow + (up ? (size_t)(r * 8) * width + k * box : (size_t)max(min(step, tail), 0) * width);
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const int at = lb * 128 + j * 64;
+            const bool in = at + t4 * 16 < width;
+            copy16(dst + ((r * 2 + k) * 2 + j) * 512, in ? src + at : static_cast<const uint8_t*>(p.a.w_down), in);
+          }
+        }
+      lb += up ? ks1 : ks2;
+      ++put;
     }
-    if (lp == 2) {
-      while (lb >= nb2) lb -= nb2, ++lu;
-      if (lu >= n2) lp = 3;
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  auto next_block = [&]() {  // the lane's pieces of its next block
+    asm volatile("cp.async.wait_group %0;" ::"n"(DEPTH - 1) : "memory");
+    return queue + got++ % DEPTH * (S::kPieces * 32);
+  };
+#pragma unroll 1
+  for (int i = 0; i < DEPTH; ++i) issue();
+
+  float acc[CH][RU][NT][4];
+  auto clear = [&]() {
+#pragma unroll
+    for (int k = 0; k < CH; ++k)
+#pragma unroll
+      for (int r = 0; r < RU; ++r)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) acc[k][r][nt][c] = 0.0f;
+  };
+  // Sums of the chains, then of the team's warps, in the first warp's
+  // registers; false for the others.
+  auto gather = [&](int ks) {
+    if (CH == 2)
+#pragma unroll
+      for (int r = 0; r < RU; ++r)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) acc[0][r][nt][c] += acc[CH - 1][r][nt][c];
+    if (ks == 1) return true;
+    if (warp % ks) {
+#pragma unroll
+      for (int r = 0; r < RU; ++r)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+          *reinterpret_cast<float4*>(frags + warp * S::kFragFloats + ((r * NT + nt) * 32 + lane) * 4) =
+              make_float4(acc[0][r][nt][0], acc[0][r][nt][1], acc[0][r][nt][2], acc[0][r][nt][3]);
     }
-    if (lp == 3) return;
-    const int st = issued % S::kStages;
-    if (lane == 0) {
-      mbar_arrive_expect_tx(&s_full[warp][st], S::kStageBytes);
-      uint8_t* dst = ring + st * S::kStageBytes;
-      if (lp == 1) {
-        const int u = u1 + lu, e = L.expert[u / per1], row = e * 2 * I + u % per1 * (8 * RU);
-        tma_load_2d(dst, &map_up, &s_full[warp][st], lb * 128, row);
-        tma_load_2d(dst + 1024 * RU, &map_up, &s_full[warp][st], lb * 128, row + I);
-      } else {
-        const int u = u2 + lu, e = L.expert[u / per2], row = e * H + u % per2 * (16 * RU);
-        tma_load_2d(dst, &map_down, &s_full[warp][st], lb * 128, row);
-        tma_load_2d(dst + 1024 * RU, &map_down, &s_full[warp][st], lb * 128, row + 8 * RU);
+    named_bar_sync(1 + warp / ks, ks * 32);
+    if (warp % ks) return false;
+#pragma unroll 1
+    for (int w = warp + 1; w < warp + ks; ++w)
+#pragma unroll
+      for (int r = 0; r < RU; ++r)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          const float4 v = *reinterpret_cast<const float4*>(frags + w * S::kFragFloats + ((r * NT + nt) * 32 + lane) * 4);
+          acc[0][r][nt][0] += v.x;
+          acc[0][r][nt][1] += v.y;
+          acc[0][r][nt][2] += v.z;
+          acc[0][r][nt][3] += v.w;
+        }
+    return true;
+  };
+  // One block's products: fp16 rows xr (8 NT of them, operand order) times the queue's next block.
+  const uint16_t* xr[NT];
+  auto multiply = [&](int kb, int tiles) {
+    uint4 x[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) x[nt][i] = xr[nt] ? *reinterpret_cast<const uint4*>(xr[nt] + kb * 128 + i * 32) : make_uint4(0, 0, 0, 0);
+    const uint4* w = next_block();
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      uint4 g[RU], b[RU], y[NT][2];
+#pragma unroll
+      for (int r = 0; r < RU; ++r) {
+        g[r] = w[((r * 2) * 2 + j) * 32];
+        b[r] = w[((r * 2 + 1) * 2 + j) * 32];
+      }
+      if (j == 0) {  // the second half's operands, while the first half is multiplied
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) y[nt][i] = xr[nt] ? *reinterpret_cast<const uint4*>(xr[nt] + kb * 128 + (2 + i) * 32) : make_uint4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint32_t A[RU][4];
+#pragma unroll
+        for (int r = 0; r < RU; ++r) {
+          f8x4_to_f16x4<FMT>(i == 0 ? g[r].x : i == 1 ? g[r].y : i == 2 ? g[r].z : g[r].w, A[r][0], A[r][2]);
+          f8x4_to_f16x4<FMT>(i == 0 ? b[r].x : i == 1 ? b[r].y : i == 2 ? b[r].z : b[r].w, A[r][1], A[r][3]);
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          if (nt > 0 && nt >= tiles) break;
+          const uint4 v = x[nt][i / 2];
+#pragma unroll
+          for (int r = 0; r < RU; ++r) mma_f16(acc[i % CH][r][nt], A[r][0], A[r][1], A[r][2], A[r][3], i & 1 ? v.z : v.x, i & 1 ? v.w : v.y);
+        }
+      }
+      if (j == 0) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) x[nt][i] = y[nt][i];
       }
     }
-    lb += kWarps;
-    ++issued;
+    issue();  // the lane has read its pieces: their place takes the next block
   };
-  auto wait = [&]() {  // for the next block; after a wait that ran out the rest is passed over
-    const int st = used % S::kStages;
-    if (ok) {
-      ok = mbar_wait(&s_full[warp][st], (uint32_t)((used / S::kStages) & 1), ERR_WAIT_FULL);
-      if (!ok) lost = used;
-    }
-    return ring + st * S::kStageBytes;
-  };
-  auto drain = [&]() {  // before an early end: the copies under way land first
-    for (int k = ok ? used : lost; k < issued; ++k) mbar_wait(&s_full[warp][k % S::kStages], (uint32_t)((k / S::kStages) & 1), ERR_WAIT_FULL);
-  };
-  for (int i = 0; i < S::kStages; ++i) issue();
 
   // ------------------------------------------------ 1: gate, up, activation --
-  int flip = 0, cb = warp;  // reduction buffer; this warp's next block of the unit
-  for (int u = 0; u < n1; ++u) {
-    const int a = (u1 + u) / per1, i0 = (u1 + u) % per1 * (8 * RU), e = L.expert[a];
-    const int s0 = L.start[a], cnt = L.start[a + 1] - s0;
-    const int tiles = (cnt + 7) >> 3;
-    const uint16_t* xr[NT];
+#pragma unroll 1
+  for (int u = warp / ks1; u < n1; u += WARPS / ks1) {
+    const int a = (u1 + u) / per1, i0 = (u1 + u - a * per1) * (8 * RU);
+    const int s0 = L.start[a], cnt = min(L.start[a + 1] - s0, 8 * NT), tiles = (cnt + 7) >> 3;
+    float sg[RU], su[RU];  // scales of the lane's rows
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) xr[nt] = nt * 8 + q4 < cnt ? p.xf + (size_t)(L.slot[s0 + nt * 8 + q4] / K) * p.hpad + t4 * 8 : nullptr;
-    float acc[RU][NT][4];
-#pragma unroll
-    for (int r = 0; r < RU; ++r)
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) acc[r][nt][c] = 0.0f;
-    for (; cb < nb1; cb += kWarps) {
-      uint4 x0[4];  // the first tile's operands are asked for before the wait
-#pragma unroll
-      for (int i = 0; i < 4; ++i) x0[i] = xr[0] ? *reinterpret_cast<const uint4*>(xr[0] + cb * 128 + i * 32) : make_uint4(0, 0, 0, 0);
-      const uint8_t* w = wait();
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {  // halves of the lane's 32 bytes a row
-        uint32_t g[RU][4], b[RU][4];
-#pragma unroll
-        for (int r = 0; r < RU; ++r) {
-          const int at = (r * 8 + q4) * 128 + (((2 * t4 + j) ^ q4) << 4);
-          const uint4 v = *reinterpret_cast<const uint4*>(w + at), z = *reinterpret_cast<const uint4*>(w + 1024 * RU + at);
-          g[r][0] = v.x, g[r][1] = v.y, g[r][2] = v.z, g[r][3] = v.w;
-          b[r][0] = z.x, b[r][1] = z.y, b[r][2] = z.z, b[r][3] = z.w;
-        }
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          uint32_t A[RU][2][4];
-#pragma unroll
-          for (int r = 0; r < RU; ++r)
-#pragma unroll
-            for (int s = 0; s < 2; ++s) {
-              f8x4_to_f16x4<FMT>(g[r][2 * i + s], A[r][s][0], A[r][s][2]);
-              f8x4_to_f16x4<FMT>(b[r][2 * i + s], A[r][s][1], A[r][s][3]);
-            }
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            if (nt > 0 && nt >= tiles) break;
-            const uint4 x = nt == 0 ? x0[2 * j + i] : xr[nt] ? *reinterpret_cast<const uint4*>(xr[nt] + cb * 128 + (2 * j + i) * 32) : make_uint4(0, 0, 0, 0);
-#pragma unroll
-            for (int r = 0; r < RU; ++r) {
-              mma_f16(acc[r][nt], A[r][0][0], A[r][0][1], A[r][0][2], A[r][0][3], x.x, x.y);
-              mma_f16(acc[r][nt], A[r][1][0], A[r][1][1], A[r][1][2], A[r][1][3], x.z, x.w);
-            }
-          }
-        }
-      }
-      ++used;
-      __syncwarp();
-      issue();
+    for (int r = 0; r < RU; ++r) {
+      const int i = min(i0 + r * 8 + q4, I - 1);
+      const float* sc = p.a.s_gate_up + (size_t)L.expert[a] * 2 * I + i;
+      sg[r] = __ldg(sc);
+      su[r] = __ldg(sc + I);
     }
-    cb -= nb1;
-    // the warps' sums meet: rows 16 r + 0..7 gate, + 8..15 up
-    float* mine = red + flip * (kWarps * S::kRedFloats) + warp * S::kRedFloats;
 #pragma unroll
-    for (int r = 0; r < RU; ++r)
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        if (nt >= tiles) break;
-        *reinterpret_cast<float2*>(mine + (r * 16 + q4) * (8 * NT) + nt * 8 + 2 * t4) = make_float2(acc[r][nt][0], acc[r][nt][1]);
-        *reinterpret_cast<float2*>(mine + (r * 16 + 8 + q4) * (8 * NT) + nt * 8 + 2 * t4) = make_float2(acc[r][nt][2], acc[r][nt][3]);
-      }
-    __syncthreads();
-    for (int x = tid; x < ((cnt * 8 * RU + 31) & ~31); x += kThreads) {
-      const int n = x / (8 * RU), i = x % (8 * RU);
-      float hv = 0.0f;
-      if (n < cnt && i0 + i < I) {
-        const float* src = red + flip * (kWarps * S::kRedFloats) + ((i >> 3) * 16 + (i & 7)) * (8 * NT) + n;
-        float gs = 0.0f, us = 0.0f;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-          gs += src[w * S::kRedFloats];
-          us += src[w * S::kRedFloats + 8 * (8 * NT)];
-        }
-        const int s = L.slot[s0 + n];
-        const float xb = __ldcg(p.xback + s / K);
-        const float* sc = p.a.s_gate_up + (size_t)e * 2 * I + i0 + i;
-        hv = gate_act(gs * xb * __ldg(sc), p.a.act) * (us * xb * __ldg(sc + I));
-        p.h[(size_t)s * p.ipad + h_place(i0 + i)] = hv;
-      }
-      // largest |h| of the slot so far (as bits, NaN above all)
-      unsigned m = __float_as_uint(hv) & 0x7FFFFFFFu;
-#pragma unroll
-      for (int o = 1; o < 8; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-      if ((lane & 7) == 0 && n < cnt) atomicMax(reinterpret_cast<unsigned int*>(&L.scale[L.slot[s0 + n]]), m);
-    }
-    if (S::kRedBufs == 2) flip ^= 1;
-    else __syncthreads();
-  }
-  __syncthreads();
-  for (int s = tid; s < T * K; s += kThreads) {
-    const unsigned m = __float_as_uint(L.scale[s]);
-    if (m) atomicMax(p.hmax + s, m);
-  }
-  if (!grid_barrier(p.sync + 1)) {
-    drain();
-    return;
-  }
-  if (blockIdx.x == 0 && tid == 0) p.sync[0] = 0u;
-  for (int s = tid; s < T * K; s += kThreads) {
-    float f, back;
-    row_factor(__uint_as_float(__ldcg(p.hmax + s)), f, back);
-    L.scale[s] = f;
-    // a slot's result is multiplied by its weight and by what undoes the factor
-    L.weight[s] = L.weight[s] * back;
-  }
-  __syncthreads();
-
-  // -------------------------------------------------------------- 2: down --
-  cb = warp;
-  for (int u = 0; u < n2; ++u) {
-    const int a = (u2 + u) / per2, r0 = (u2 + u) % per2 * (16 * RU), e = L.expert[a];
-    const int s0 = L.start[a], cnt = L.start[a + 1] - s0;
-    const int tiles = (cnt + 7) >> 3;
-    const float* hr[NT];
-    float hf[NT];
+    for (int nt = 0; nt < NT; ++nt) xr[nt] = nt * 8 + q4 < cnt ? p.xf + (size_t)L.token[s0 + nt * 8 + q4] * p.hpad + t4 * 8 : nullptr;
+    clear();
+#pragma unroll 1
+    for (int kb = warp % ks1; kb < nb1; kb += ks1) multiply(kb, tiles);
+    if (!gather(ks1)) continue;
+    // gate and up of a row lie in one lane
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const bool in = nt * 8 + q4 < cnt;
-      const int s = in ? L.slot[s0 + nt * 8 + q4] : 0;
-      hr[nt] = in ? p.h + (size_t)s * p.ipad + t4 * 4 : nullptr;
-      hf[nt] = in ? L.scale[s] : 0.0f;
-    }
-    float acc[RU][NT][4];
+      if (nt >= tiles) break;
 #pragma unroll
-    for (int r = 0; r < RU; ++r)
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) acc[r][nt][c] = 0.0f;
-    for (; cb < nb2; cb += kWarps) {
-      float4 x0[8];
-      const int left = I - cb * 128 - t4 * 32;  // the lane's valid channels of the block
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x0[i] = hr[0] && 4 * i < left ? *reinterpret_cast<const float4*>(hr[0] + cb * 128 + i * 16) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      const uint8_t* w = wait();
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        uint32_t g[RU][4], b[RU][4];
+      for (int c = 0; c < 2; ++c) {
+        const int n = nt * 8 + 2 * t4 + c;
+        const bool in = n < cnt;
+        const int s = in ? L.slot[s0 + n] : 0;
+        if (!in) continue;
+        const float xb = L.xback[L.token[s0 + n]], f = L.scale[s];
 #pragma unroll
         for (int r = 0; r < RU; ++r) {
-          const int at = (r * 8 + q4) * 128 + (((2 * t4 + j) ^ q4) << 4);
-          const uint4 v = *reinterpret_cast<const uint4*>(w + at), z = *reinterpret_cast<const uint4*>(w + 1024 * RU + at);
-          g[r][0] = v.x, g[r][1] = v.y, g[r][2] = v.z, g[r][3] = v.w;
-          b[r][0] = z.x, b[r][1] = z.y, b[r][2] = z.z, b[r][3] = z.w;
+          const int i = i0 + r * 8 + q4;
+          const float hv = gate_act(acc[0][r][nt][c] * xb * sg[r], p.a.act) * (acc[0][r][nt][c + 2] * xb * su[r]);
+          if (i < I) p.h[(size_t)s * p.ipad + place(i)] = __half_as_ushort(__float2half_rn(hv * f));
         }
+      }
+    }
+  }
+  // the columns from inter to the padded width are zero
+  if (p.ipad > I)
+    for (int x = blockIdx.x * kThreads + tid; x < T * K * (p.ipad - I); x += gridDim.x * kThreads)
+      p.h[(size_t)(x / (p.ipad - I)) * p.ipad + place(I + x % (p.ipad - I))] = 0;
+  const bool met = grid_barrier(p.sync + 1);
+  if (met && blockIdx.x == 0 && tid == 0) p.sync[0] = 0u;
+  if (!met) {
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    return;
+  }
+
+  // -------------------------------------------------------------- 2: down --
+#pragma unroll 1
+  for (int u = warp / ks2; u < n2; u += WARPS / ks2) {
+    const int a = (u2 + u) / per2, r0 = (u2 + u - a * per2) * (16 * RU);
+    const int s0 = L.start[a], cnt = min(L.start[a + 1] - s0, 8 * NT), tiles = (cnt + 7) >> 3;
+    float sd[2][RU];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          uint32_t A[RU][4];
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int r = 0; r < RU; ++r) sd[k][r] = __ldg(p.a.s_down + (size_t)L.expert[a] * H + min(r0 + k * 8 * RU + r * 8 + q4, H - 1));
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) xr[nt] = nt * 8 + q4 < cnt ? p.h + (size_t)L.slot[s0 + nt * 8 + q4] * p.ipad + t4 * 8 : nullptr;
+    clear();
+#pragma unroll 1
+    for (int kb = warp % ks2; kb < nb2; kb += ks2) multiply(kb, tiles);
+    if (!gather(ks2)) continue;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      if (nt >= tiles) break;
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int n = nt * 8 + 2 * t4 + c;
+        if (n >= cnt) continue;
+        const int s = L.slot[s0 + n];
+        const float wt = L.weight[s];
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
 #pragma unroll
           for (int r = 0; r < RU; ++r) {
-            f8x4_to_f16x4<FMT>(g[r][i], A[r][0], A[r][2]);
-            f8x4_to_f16x4<FMT>(b[r][i], A[r][1], A[r][3]);
+            const int row = r0 + k * 8 * RU + r * 8 + q4;
+            if (row < H) p.part[(size_t)s * H + row] = acc[0][r][nt][c + 2 * k] * sd[k][r] * wt;
           }
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            if (nt > 0 && nt >= tiles) break;
-            const float4 x = nt == 0 ? x0[4 * j + i]
-                             : hr[nt] && 4 * (4 * j + i) < left ? *reinterpret_cast<const float4*>(hr[nt] + cb * 128 + (4 * j + i) * 16)
-                                                                : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            const uint32_t b0 = pack_f16(x.x * hf[nt], x.y * hf[nt]), b1 = pack_f16(x.z * hf[nt], x.w * hf[nt]);
-#pragma unroll
-            for (int r = 0; r < RU; ++r) mma_f16(acc[r][nt], A[r][0], A[r][1], A[r][2], A[r][3], b0, b1);
-          }
-        }
       }
-      ++used;
-      __syncwarp();
-      issue();
     }
-    cb -= nb2;
-    // rows 16 r + 0..7: first box, + 8..15: second box (8 RU rows further on)
-    float* mine = red + flip * (kWarps * S::kRedFloats) + warp * S::kRedFloats;
-#pragma unroll
-    for (int r = 0; r < RU; ++r)
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        if (nt >= tiles) break;
-        *reinterpret_cast<float2*>(mine + (r * 16 + q4) * (8 * NT) + nt * 8 + 2 * t4) = make_float2(acc[r][nt][0], acc[r][nt][1]);
-        *reinterpret_cast<float2*>(mine + (r * 16 + 8 + q4) * (8 * NT) + nt * 8 + 2 * t4) = make_float2(acc[r][nt][2], acc[r][nt][3]);
-      }
-    __syncthreads();
-    for (int x = tid; x < cnt * 16 * RU; x += kThreads) {
-      const int n = x / (16 * RU), i = x % (16 * RU);  // i: row of the unit
-      if (r0 + i >= H) continue;
-      const int box = i / (8 * RU), ri = i % (8 * RU);
-      const float* src = red + flip * (kWarps * S::kRedFloats) + ((ri >> 3) * 16 + box * 8 + (ri & 7)) * (8 * NT) + n;
-      float y = 0.0f;
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) y += src[w * S::kRedFloats];
-      const int s = L.slot[s0 + n];
-      p.part[(size_t)s * H + r0 + i] = y * __ldg(p.a.s_down + (size_t)e * H + r0 + i) * L.weight[s];
-    }
-    if (S::kRedBufs == 2) flip ^= 1;
-    else __syncthreads();
   }
-  if (!ok) drain();
-  if (!grid_barrier(p.sync + 2)) return;  // every copy has been waited for
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  if (!grid_barrier(p.sync + 2)) return;
   if (blockIdx.x == 0 && tid == 0) p.sync[1] = 0u;
 
   // --------------------------------------------------- 3: a token's slots --
@@ -697,20 +710,17 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-template <int FMT, int NT, int RU>
+template <int FMT, int NT, int RU, int WARPS, int DEPTH>
 cudaError_t launch(const fp8imma_moe_args& a, cudaStream_t st) {
-  using S = Shape<NT, RU>;
-  const auto kern = moe_kernel<FMT, NT, RU>;
+  using S = Shape<NT, RU, WARPS, DEPTH>;
+  const auto kern = moe_kernel<FMT, NT, RU, WARPS, DEPTH>;
   cudaError_t e = ensure_smem_attr(reinterpret_cast<const void*>(kern), S::kSmem);
   if (e != cudaSuccess) return e;
   MoeParams p = {};
   p.a = a;
   p.hpad = (a.hidden + 127) & ~127;
   p.ipad = (a.inter + 127) & ~127;
-  CUtensorMap up, down;
-  e = make_tmap_2d_u8(&up, a.w_gate_up, (uint64_t)a.hidden, (uint64_t)a.experts * 2 * a.inter, (uint64_t)a.hidden, 128, 8 * RU, true);
-  if (e == cudaSuccess) e = make_tmap_2d_u8(&down, a.w_down, (uint64_t)a.inter, (uint64_t)a.experts * a.hidden, (uint64_t)a.inter, 128, 8 * RU, true);
-  if (e != cudaSuccess) return e;
+  p.chunks = (a.inter + 1023) / 1024;
   const size_t slots = (size_t)a.tokens * a.top_k;
   size_t at = 0;
   auto take = [&](size_t bytes) {
@@ -718,8 +728,8 @@ cudaError_t launch(const fp8imma_moe_args& a, cudaStream_t st) {
     at += (bytes + 255) & ~size_t(255);
     return was;
   };
-  const size_t o_logits = take((size_t)a.tokens * a.experts * 4), o_xf = take((size_t)a.tokens * p.hpad * 2), o_back = take((size_t)a.tokens * 4),
-               o_max = take(slots * 4), o_h = take(slots * p.ipad * 4), o_part = take(slots * a.hidden * 4);
+  const size_t o_logits = take((size_t)a.tokens * a.experts * 4), o_xf = take((size_t)a.tokens * p.hpad * 2), o_back = take((size_t)a.tokens * 8),
+               o_max = take((size_t)a.experts * 2 * p.chunks * 4), o_h = take(slots * p.ipad * 2), o_part = take(slots * a.hidden * 4);
   ScopedScratch sync, work;
   e = sync.get(256, st, kScratchMoeSync);
   if (e == cudaSuccess && sync.owned) e = cudaMemsetAsync(sync.ptr, 0, 256, st);
@@ -730,34 +740,34 @@ cudaError_t launch(const fp8imma_moe_args& a, cudaStream_t st) {
     p.logits = reinterpret_cast<float*>(base + o_logits);
     p.xf = reinterpret_cast<uint16_t*>(base + o_xf);
     p.xback = reinterpret_cast<float*>(base + o_back);
-    p.hmax = reinterpret_cast<unsigned int*>(base + o_max);
-    p.h = reinterpret_cast<float*>(base + o_h);
+    p.smax = reinterpret_cast<float*>(base + o_max);
+    p.h = reinterpret_cast<uint16_t*>(base + o_h);
     p.part = reinterpret_cast<float*>(base + o_part);
     cudaLaunchConfig_t lc = {};
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeCooperative;  // the CTAs wait for one another: all of them have to be resident
     attr[0].val.cooperative = 1;
     lc.gridDim = dim3(num_sms_current());
-    lc.blockDim = dim3(kThreads);
+    lc.blockDim = dim3(S::kThreads);
     lc.dynamicSmemBytes = S::kSmem;
     lc.stream = st;
     lc.attrs = attr;
     lc.numAttrs = 1;
-    e = cudaLaunchKernelEx(&lc, kern, up, down, p);
+    e = cudaLaunchKernelEx(&lc, kern, p);
   }
   const cudaError_t e1 = sync.release(st), e2 = work.release(st);
   return e != cudaSuccess ? e : e1 != cudaSuccess ? e1 : e2;
 }
 
-// Token tiles by the number of tokens (an expert can be chosen by all of
-// them); with more tokens a unit gets more rows, so that a token's operands,
-// read again for each unit, cost less than the weights.
+// Token tiles by the number of tokens, which an expert may all be given; with
+// many tokens a unit has more rows, so that the tokens' operands, read again
+// for each unit, cost less beside the weights.
 template <int FMT>
 cudaError_t launch_nt(const fp8imma_moe_args& a, cudaStream_t st) {
-  if (a.tokens <= 8) return launch<FMT, 1, 1>(a, st);
-  if (a.tokens <= 16) return launch<FMT, 2, 2>(a, st);
-  if (a.tokens <= 32) return launch<FMT, 4, 2>(a, st);
-  return launch<FMT, 8, 2>(a, st);
+  if (a.tokens <= 2) return launch<FMT, 1, 1, 16, 4>(a, st);
+  if (a.tokens <= 8) return launch<FMT, 1, 2, 16, 2>(a, st);
+  if (a.tokens <= 16) return launch<FMT, 2, 2, 16, 2>(a, st);
+  return launch<FMT, 4, 2, 8, 4>(a, st);
 }
 
 }  // namespace

@@ -112,8 +112,9 @@ def ref_moe(x, router, wu, su, wd, sd, top_k, renorm, act, fmt):
     """(out, ids, weights, bound) in 64 bits.
 
     The bound: gate and up sums to 2^-18 of the sum of their terms' magnitudes (fp32 sums of exact products, and the
-    activation's own rounding), the inner product rounded to fp16 (2^-11, and 2^-24 of its row's largest where it
-    falls below that range), the down sum to 2^-18, the result rounded once to its type."""
+    activation's own rounding), the inner product rounded to fp16 (2^-11, or 2^-25 where it falls below fp16's normal
+    range, the row having been scaled by a power of two for which the bound on |gate| |up|, the largest scales times
+    fmax times sum |x|, lies between 2^13 and 2^15), the down sum to 2^-18, the result rounded once to its type."""
     t, hdim = x.shape
     inter = wd.shape[2]
     r = x.double() @ router.double().T
@@ -133,7 +134,8 @@ def ref_moe(x, router, wu, su, wd, sd, top_k, renorm, act, fmt):
             a = act64(g, act)
             h = a * u
             dh = 1.2 * 2.0 ** -18 * (mag[:inter] * u.abs() + a.abs() * mag[inter:] + mag[:inter] * mag[inter:] * 2.0 ** -18)
-            dh = dh + h.abs() * (2.0 ** -11 + 2.0 ** -18) + 2.0 ** -24 * h.abs().max()
+            most = su[e].double().view(2, -1).amax(1).prod() * (FMAX[fmt] * xi.abs().sum()) ** 2
+            dh = dh + h.abs() * (2.0 ** -11 + 2.0 ** -18) + 2.0 ** -25 * 2.0 ** -13 * most
             out[i] += w[i, s] * (dn @ h)
             bound[i] += w[i, s] * (dn.abs() @ dh + 2.0 ** -18 * (dn.abs() @ h.abs()))
     bound += out.abs() * (UNIT[x.dtype] + 2.0 ** -18) + 2.0 ** -25
