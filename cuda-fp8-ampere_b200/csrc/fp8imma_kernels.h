@@ -97,6 +97,10 @@ enum { kScratchTc = 2, kScratchRowScales = 3, kScratchGemvRows = 4, kScratchWgt 
 cudaError_t make_tmap_2d_u8(CUtensorMap* map, const void* base, uint64_t inner, uint64_t outer, uint64_t row_bytes,
                             uint32_t box_inner, uint32_t box_outer, bool swizzle128);
 
+// TMA descriptor for a 3-D byte tensor [n2][n1][n0], packed, 128-byte swizzle.
+cudaError_t make_tmap_3d_u8(CUtensorMap* map, const void* base, uint64_t n0, uint64_t n1, uint64_t n2, uint32_t box0,
+                            uint32_t box1, uint32_t box2);
+
 // Device error words of the kernel files that wait on barriers (0 = none),
 // and their wait limits (current device).
 unsigned int gemv_device_error(bool clear);

@@ -1,113 +1,106 @@
 // Log probabilities of given tokens, entropy and top alternatives of logits
 // (fp8imma_token_logprobs).
+//
+// Mathematics, z = x / temperature, in base 2 (u = z log2 e), one pass with a
+// running reference M per lane:
+//   l = sum 2^(u - M),  s = sum 2^(u - M) (u - M)
+//   lse = ln2 (M + log2 l),  entropy = ln2 (log2 l - s / l),  lp(t) = z_t - lse
+// and parts join as l = sum l_i 2^(M_i - M), s = sum 2^(M_i - M) (s_i + (M_i - M) l_i).
+// The top logits are a warp's list of 32, one a lane in descending order; a
+// logit enters it only when it exceeds the list's last, which after the first
+// few hundred logits is rare, so the pass pays one comparison for it. Order is
+// by the logit's bits (order-preserving), then by the lower index, so lists
+// and their joins do not depend on which part is read first.
+//
+// Bound: the logits are read once. A row is cut into as many parts as fill the
+// GPU (one row of 32000 bf16 logits: latency; thousands of rows: bandwidth);
+// the last CTA to finish a row joins its parts in order.
 #include "fp8_mma.cuh"
 #include "fp8imma/fp8imma_ext.h"
 #include "fp8imma_kernels.h"
 #include "nvtx_range.h"
+#include "sm100_async.cuh"
 
-#include <cuda_runtime.h>
+#include <algorithm>
 
 namespace fp8imma_b200 {
 namespace {
 
 using namespace fp8imma_dev;
 
-constexpr int kThreads = 256;
+constexpr int kWarps = 8;
+constexpr int kThreads = kWarps * 32;
+constexpr unsigned long long kNoKey = 0ull;  // below the key of every logit
+
+struct LpParams {
+  fp8imma_logprobs_args a;
+  float to_log2;          // log2(e) / temperature
+  float inv_temp;
+  int parts;              // CTAs a row (row-major) or a group of rows (column-major)
+  int per_part;           // logits of a part
+  int groups;             // column-major: 32-row groups
+  unsigned int* counters; // per row (group): finished parts; zero between calls
+  float* sums;            // [parts, tokens, 4]: M, l, s, -
+  unsigned long long* lists;  // [parts, tokens, 32]
+};
 
 template <int LT>
-__device__ __forceinline__ float load_logit(const void* p, int64_t i) {
-  if (LT == FP8IMMA_L_F32) return static_cast<const float*>(p)[i];
-  return a16_to_f32<LT>(static_cast<const uint16_t*>(p)[i]);
+__device__ __forceinline__ float to_f32(uint32_t bits) {
+  if (LT == FP8IMMA_L_F32) return __uint_as_float(bits);
+  return a16_to_f32<LT>((uint16_t)bits);
 }
 
-// order-preserving integer of a logit: -0 = +0, NaN above everything
-__device__ __forceinline__ int order_key(float v) {
+// Descending order of logits: NaN, +inf .. -inf (-0 = +0), then the lower index.
+__device__ __forceinline__ unsigned long long make_key(float v, int j) {
   const int k = __float_as_int(v);
-  if (isnan(v)) return 0x7fffffff;
-  return k < 0 ? (int)(0x80000000u - (unsigned)k) : k;
+  unsigned o = isnan(v) ? 0xffffffffu : k < 0 ? 0x80000000u - (unsigned)(k & 0x7fffffff) : 0x80000000u + (unsigned)k;
+  return ((unsigned long long)o << 32) | (unsigned)(0x7fffffff - j);
+}
+__device__ __forceinline__ float key_value(unsigned long long key) {
+  const unsigned o = (unsigned)(key >> 32);
+  if (o == 0xffffffffu) return NAN;
+  return o >= 0x80000000u ? __uint_as_float(o - 0x80000000u) : -__uint_as_float(0x80000000u - o);
+}
+__device__ __forceinline__ int key_index(unsigned long long key) { return 0x7fffffff - (int)(unsigned)key; }
+
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
 }
 
-template <class T, class F>
-__device__ __forceinline__ T block_reduce(T v, T* red, F f) {
+// Running sums of one lane (or of a joined part).
+struct Sums {
+  float m = -INFINITY, l = 0.0f, s = 0.0f;
+  bool bad = false;  // NaN or +inf was seen
+  __device__ __forceinline__ void join(float m2, float l2, float s2) {
+    const float mn = fmaxf(m, m2);
+    if (mn == -INFINITY) return;
+    const float a = m == -INFINITY ? 0.0f : ex2(m - mn), b = m2 == -INFINITY ? 0.0f : ex2(m2 - mn);
+    const float da = m == -INFINITY ? 0.0f : m - mn, db = m2 == -INFINITY ? 0.0f : m2 - mn;
+    s = a * (s + da * l) + b * (s2 + db * l2);
+    l = a * l + b * l2;
+    m = mn;
+  }
+};
+
+// A warp's list: lane i holds the i-th largest key. Insert one key (uniform).
+__device__ __forceinline__ void insert(unsigned long long& mine, unsigned long long key, int lane) {
+  const unsigned below = __ballot_sync(0xffffffffu, mine < key);  // a suffix of the lanes: they move down by one
+  const unsigned long long up = __shfl_up_sync(0xffffffffu, mine, 1);
+  if ((below >> lane) & 1u) mine = lane > 0 && ((below >> (lane - 1)) & 1u) ? up : key;
+}
+
+// Two descending lists (one a lane) -> the 32 largest, descending.
+__device__ __forceinline__ unsigned long long merge(unsigned long long a, unsigned long long b, int lane) {
+  const unsigned long long r = __shfl_sync(0xffffffffu, b, 31 - lane);
+  unsigned long long v = a > r ? a : r;  // the 32 largest, bitonic
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = f(v, __shfl_xor_sync(0xffffffffu, v, o));
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = red[0];
-  for (int i = 1; i < kThreads / 32; ++i) v = f(v, red[i]);
+  for (int o = 16; o > 0; o >>= 1) {
+    const unsigned long long w = __shfl_xor_sync(0xffffffffu, v, o);
+    v = (lane & o) ? (w < v ? w : v) : (w > v ? w : v);
+  }
   return v;
 }
-
-// one CTA per row, several passes
-template <int LT>
-__global__ void __launch_bounds__(kThreads) logprobs_kernel(fp8imma_logprobs_args a) {
-  __shared__ float redf[kThreads / 32];
-  __shared__ long long redl[kThreads / 32];
-  const int t = blockIdx.x;
-  const int64_t base = (int64_t)t * a.token_stride;
-  const float it = 1.0f / a.temperature;
-  auto z = [&](int j) { return load_logit<LT>(a.logits, base + (int64_t)j * a.vocab_stride) * it; };
-  float m = -INFINITY;
-  bool nan = false;
-  for (int j = threadIdx.x; j < a.vocab; j += kThreads) {
-    const float v = z(j);
-    nan |= isnan(v);
-    m = fmaxf(m, v);
-  }
-  m = block_reduce(m, redf, [](float x, float y) { return fmaxf(x, y); });
-  nan = __syncthreads_or(nan);
-  float l = 0.0f, s = 0.0f;
-  for (int j = threadIdx.x; j < a.vocab; j += kThreads) {
-    const float d = z(j) - m, e = expf(d);
-    l += e;
-    if (d > -INFINITY) s += e * d;
-  }
-  l = block_reduce(l, redf, [](float x, float y) { return x + y; });
-  s = block_reduce(s, redf, [](float x, float y) { return x + y; });
-  const bool bad = nan || !(fabsf(m) < INFINITY);
-  const float lse = bad ? NAN : m + logf(l);
-  if (threadIdx.x == 0) {
-    const int id = a.token_ids[t];
-    a.logprobs[t] = (unsigned)id < (unsigned)a.vocab ? z(id) - lse : NAN;
-    a.entropy[t] = bad ? NAN : logf(l) - s / l;
-  }
-  long long last = 0x7fffffffffffffffll;
-  for (int k = 0; k < a.top; ++k) {
-    long long best = -0x7fffffffffffffffll - 1;
-    for (int j = threadIdx.x; j < a.vocab; j += kThreads) {
-      const long long key = ((long long)order_key(load_logit<LT>(a.logits, base + (int64_t)j * a.vocab_stride)) << 32) - j;
-      if (key < last && key > best) best = key;
-    }
-    best = block_reduce(best, redl, [](long long x, long long y) { return x > y ? x : y; });
-    last = best;
-    const int id = (int)(-(best & 0xffffffffll) & 0x7fffffff);
-    if (threadIdx.x == 0) {
-      a.top_ids[(int64_t)t * a.top + k] = id;
-      a.top_logprobs[(int64_t)t * a.top + k] = z(id) - lse;
-    }
-  }
-}
-
 }  // namespace
 }  // namespace fp8imma_b200
-
-using namespace fp8imma_b200;
-
-extern "C" int fp8imma_token_logprobs(const fp8imma_logprobs_args* a, void* stream) {
-  FP8IMMA_RANGE("fp8imma_token_logprobs");
-  if (!a) return (int)cudaErrorInvalidValue;
-  if (a->tokens <= 0 || a->vocab <= 0) return (int)cudaErrorInvalidConfiguration;
-  if (!a->logits || !a->token_ids || !a->logprobs || !a->entropy) return (int)cudaErrorInvalidValue;
-  if (a->top < 0 || a->top > FP8IMMA_LOGPROBS_MAX_TOP || a->top > a->vocab) return (int)cudaErrorInvalidValue;
-  if (a->top > 0 && (!a->top_ids || !a->top_logprobs)) return (int)cudaErrorInvalidValue;
-  if (a->l_type < 0 || a->l_type > 2 || !(a->temperature > 0.0f) || !(a->temperature < INFINITY))
-    return (int)cudaErrorInvalidValue;
-  if (a->vocab_stride != 1 && a->token_stride != 1) return (int)cudaErrorInvalidValue;
-  if (reinterpret_cast<uintptr_t>(a->logits) & (a->l_type == FP8IMMA_L_F32 ? 3u : 1u)) return (int)cudaErrorInvalidValue;
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (a->l_type == FP8IMMA_L_F16) logprobs_kernel<FP8IMMA_L_F16><<<a->tokens, kThreads, 0, st>>>(*a);
-  else if (a->l_type == FP8IMMA_L_BF16) logprobs_kernel<FP8IMMA_L_BF16><<<a->tokens, kThreads, 0, st>>>(*a);
-  else logprobs_kernel<FP8IMMA_L_F32><<<a->tokens, kThreads, 0, st>>>(*a);
-  return (int)cudaGetLastError();
-}

@@ -23,12 +23,14 @@
 //     that both factors of h meet in one fragment; grid barrier
 //  2. down: the same over units of 16 RU rows; slot results to scratch; barrier
 //  3. out = sum over a token's slots, in their order
-// A warp works on units of its own (few units: a team of 2, 4 or 8 warps shares
-// one along the columns). Each lane copies the 16-byte pieces of its own
-// operand rows asynchronously into a queue of its own in shared memory, some
-// 128-byte column blocks ahead, across unit and phase boundaries: no barrier
-// between lanes or warps, and the down weights are under way while the grid
-// meets at the barrier before them. A team's sums meet in shared memory in a
+// A warp works on units of its own, or a team of 2, 4 or 8 warps shares one
+// along the columns. Each warp streams the 128-byte column blocks of its units
+// by TMA, one box of 16 RU rows a block, into a ring of its own, across unit
+// and phase boundaries: no barrier between warps, and the down weights are
+// under way while the grid meets at the barrier before them. A box covers the
+// gate and the up rows (a 3-D map over [columns, inter, experts x 2]): copies
+// of 4 KB reach 6.6 TB/s, copies of 2 KB 3.8 TB/s, 16-byte asynchronous copies
+// of 64-byte row pieces 5.6 TB/s. A team's sums meet in shared memory in a
 // fixed order; nothing depends on timing.
 #include "fp8_mma.cuh"
 #include "fp8imma/fp8imma_ext.h"
@@ -43,18 +45,23 @@ namespace {
 
 using namespace fp8imma_dev;
 
+constexpr int kRouterDone = 64, kScaleMax = 128, kSyncWords = kScaleMax + 2 * FP8IMMA_MOE_MAX_EXPERTS;
 constexpr int kMaxSlots = FP8IMMA_MOE_MAX_TOKENS * FP8IMMA_MOE_MAX_TOP_K;
 
 struct MoeParams {
   fp8imma_moe_args a;
-  unsigned int* sync;  // three barrier counters, zero between calls
+  // kept zero between calls: three barrier counters, finished router units of
+  // each group of tokens (from kRouterDone on), the experts' largest gate / up
+  // scales as bits (from kScaleMax on, [experts, 2])
+  unsigned int* sync;
   float* logits;       // [tokens, experts]
   uint16_t* xf;        // [tokens, hidden padded to 128] fp16, operand order
   float* xback;        // [tokens, 2] what a row of xf is to be multiplied by, sum |x|
-  float* smax;         // [experts, 2, chunks] largest gate / up scale of 1024 rows
+  int* ids;            // [slots] the choice
+  float* weights;      // [slots]
   uint16_t* h;         // [slots, inter padded to 128] fp16, operand order
   float* part;         // [slots, hidden]
-  int hpad, ipad, chunks;
+  int hpad, ipad;
 };
 
 // ---------------------------------------------------------------- helpers --
@@ -127,23 +134,76 @@ struct Runs {  // CTA c's run of the units: they differ by one in length at most
   __device__ __forceinline__ int begin(int c) const { return c * per + min(c, rem); }
 };
 
-// 16 bytes global -> shared, asynchronously; zeros when not `in`
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool in) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
+// 3-D tiled TMA load (no multicast) into this CTA's shared memory
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
+          smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
+      : "memory");
 }
 
 // NT: 8-token tiles of a unit at most; RU: 16-row tiles of a unit; WARPS a CTA;
-// DEPTH: blocks of a lane's queue.
+// DEPTH: blocks of a warp's ring.
 template <int NT, int RU, int WARPS, int DEPTH>
 struct Shape {
   static constexpr int kThreads = WARPS * 32;
-  static constexpr int kPieces = 4 * RU;               // 16-byte pieces of a block a lane
-  static constexpr int kQueue = DEPTH * kPieces * 512; // of a warp
+  static constexpr int kBlockBytes = 2048 * RU;
+  static constexpr int kRing = DEPTH * kBlockBytes;    // of a warp
   static constexpr int kFragFloats = RU * NT * 4 * 32; // a unit's sums of a warp
-  static constexpr int kSmem = WARPS * (kQueue + kFragFloats * 4);
+  static constexpr int kSmem = 1024 + WARPS * (kRing + kFragFloats * 4);
 };
 
-// Router logits of EX experts x TX tokens a warp, and nothing else.
+// A token's top_k by one warp: rounds of the largest logit not yet taken, the
+// lowest index among equal ones. A lane keeps the keys of experts lane + 32 i.
+template <int NK>
+__device__ __noinline__ void pick(const float* r, int E, int K, int renormalize, int* ids, float* weights, int* ids_out, float* weights_out, int lane) {
+  constexpr int kNone = (int)0x80000000;  // below the key of every logit
+  int key[NK];
+  float z = 0.0f;
+#pragma unroll
+  for (int i = 0; i < NK; ++i) key[i] = lane + 32 * i < E ? order_key(__ldcg(r + lane + 32 * i)) : kNone;
+  auto value = [](int k) { return __int_as_float(k < 0 ? (int)(0x80000000u - (unsigned)k) : k); };
+  int mine = 0;  // lane s keeps the s-th choice
+  float first = 0.0f, sum = 0.0f, weight = 0.0f;
+#pragma unroll 1
+  for (int s = 0; s < K; ++s) {
+    int best = key[0];
+#pragma unroll
+    for (int i = 1; i < NK; ++i) best = max(best, key[i]);
+    const int top = __reduce_max_sync(0xffffffffu, best);
+    int at = 0x7fffffff;
+#pragma unroll
+    for (int i = NK - 1; i >= 0; --i) at = key[i] == top ? lane + 32 * i : at;
+    const int e = __reduce_min_sync(0xffffffffu, at);
+    if (s == 0) {
+      first = value(top);
+      if (!renormalize)
+#pragma unroll
+        for (int i = 0; i < NK; ++i) z += key[i] == kNone ? 0.0f : __expf(value(key[i]) - first);
+    }
+#pragma unroll
+    for (int i = 0; i < NK; ++i)
+      if (lane + 32 * i == e) key[i] = kNone;
+    const float w = __expf(value(top) - first);
+    sum += w;
+    if (lane == s) {
+      mine = e;
+      weight = w;
+    }
+  }
+  if (!renormalize) sum = warp_sum(z);
+  if (lane < K) {
+    weight = __fdiv_rn(weight, sum);
+    ids[lane] = mine;
+    weights[lane] = weight;
+    if (ids_out) ids_out[lane] = mine;
+    if (weights_out) weights_out[lane] = weight;
+  }
+}
+
+// Router logits of EX experts x TX tokens a warp; the warp that finishes the
+// last of a group of tokens makes their choice.
 template <int AT, int EX, int TX>
 __device__ __forceinline__ void router(const MoeParams& p, int wid, int nw, int lane, bool vec) {
   const int eu = (p.a.experts + EX - 1) / EX, tu = (p.a.tokens + TX - 1) / TX;
@@ -195,35 +255,53 @@ __device__ __forceinline__ void router(const MoeParams& p, int wid, int nw, int 
         const float v = warp_sum(s[e][t]);
         if (lane == 0 && e0 + e < p.a.experts && t0 + t < p.a.tokens) p.logits[(size_t)(t0 + t) * p.a.experts + e0 + e] = v;
       }
+    unsigned int done = 0, *ctr = p.sync + kRouterDone + u / eu;
+    if (lane == 0) asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(done) : "l"(ctr) : "memory");
+    done = __shfl_sync(0xffffffffu, done, 0);
+    __syncwarp();
+    if (done == (unsigned)(eu - 1)) {
+      if (lane == 0) *ctr = 0u;
+#pragma unroll 1
+      for (int t = t0; t < min(t0 + TX, p.a.tokens); ++t) {
+        const int at = t * p.a.top_k;
+        const float* r = p.logits + (size_t)t * p.a.experts;
+        int* ids_out = p.a.ids ? p.a.ids + at : nullptr;
+        float* w_out = p.a.weights ? p.a.weights + at : nullptr;
+        if (p.a.experts <= 128) pick<4>(r, p.a.experts, p.a.top_k, p.a.renormalize, p.ids + at, p.weights + at, ids_out, w_out, lane);
+        else if (p.a.experts <= 256) pick<8>(r, p.a.experts, p.a.top_k, p.a.renormalize, p.ids + at, p.weights + at, ids_out, w_out, lane);
+        else pick<32>(r, p.a.experts, p.a.top_k, p.a.renormalize, p.ids + at, p.weights + at, ids_out, w_out, lane);
+      }
+    }
   }
 }
 
 // Place of element k of a row in operand order: lane t4 of a fragment holds
-// bytes 16 t4 .. 16 t4 + 15 of both halves of a 128-byte weight block, four
-// bytes a product step; eight fp16, two steps, lie together.
-__device__ __forceinline__ int place(int k) { return (k & ~127) + (((k >> 5) & 2) + ((k >> 3) & 1)) * 32 + (((k >> 4) & 3) << 3) + (k & 7); }
+// bytes 32 t4 .. 32 t4 + 31 of a 128-byte weight block, four bytes a product
+// step; eight fp16, two steps, lie together.
+__device__ __forceinline__ int place(int k) { return (k & ~127) + (((k & 31) >> 3) << 5) + (((k >> 5) & 3) << 3) + (k & 7); }
 
-// Largest gate / up scales by chunks of 1024 rows.
+// Largest gate / up scales of each expert, a warp 1024 of them at a time.
 __device__ __forceinline__ void scale_maxima(const MoeParams& p, int wid, int nw, int lane) {
+  const int chunks = (p.a.inter + 1023) >> 10;
 #pragma unroll 1
-  for (int u = wid; u < p.a.experts * 2 * p.chunks; u += nw) {
-    const int c = u % p.chunks, row = u / p.chunks;  // row: expert * 2 + (gate, up)
+  for (int u = wid; u < p.a.experts * 2 * chunks; u += nw) {
+    const int row = u / chunks, c = u - row * chunks;  // row: expert * 2 + (gate, up)
     const float* s = p.a.s_gate_up + (size_t)row * p.a.inter;
     const int hi = min(p.a.inter, c * 1024 + 1024);
     float m = 0.0f;
 #pragma unroll 8
     for (int i = c * 1024 + lane; i < hi; i += 32) m = fmaxf(m, fabsf(__ldg(s + i)));
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    if (lane == 0) p.smax[u] = m;
+    const unsigned bits = __reduce_max_sync(0xffffffffu, __float_as_uint(m));
+    if (lane == 0) atomicMax(p.sync + kScaleMax + row, bits);
   }
 }
 
-// A token's row as fp16 in operand order; one warp.
-template <int AT>
-__device__ __forceinline__ void convert_row(const MoeParams& p, int t, int lane, bool vec) {
+// A token's row as fp16 in operand order, its factor and sum |x|; one CTA.
+template <int AT, int THREADS>
+__device__ __forceinline__ void convert_row(const MoeParams& p, int t, bool vec) {
+  __shared__ float s_big[THREADS / 32], s_sum[THREADS / 32];
   const uint16_t* x = static_cast<const uint16_t*>(p.a.x) + t * p.a.x_token_stride;
-  float f = 1.0f, back = 1.0f, sum = 0.0f;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   auto load8 = [&](int k) {
     if (vec) return __ldg(reinterpret_cast<const uint4*>(x + k));
     uint32_t w[4];
@@ -231,28 +309,40 @@ __device__ __forceinline__ void convert_row(const MoeParams& p, int t, int lane,
     for (int i = 0; i < 4; ++i) w[i] = (uint32_t)__ldg(x + k + 2 * i) | ((uint32_t)__ldg(x + k + 2 * i + 1) << 16);
     return make_uint4(w[0], w[1], w[2], w[3]);
   };
-  if (AT == 1) {
-    float big = 0.0f;
-#pragma unroll 4
-    for (int k = lane * 8; k < p.a.hidden; k += 256) {
-      const uint4 v = load8(k);
-      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  float big = 0.0f, sum = 0.0f;
+  for (int k = threadIdx.x * 8; k < p.a.hidden; k += THREADS * 8) {
+    const uint4 v = load8(k);
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) big = fmaxf(big, fmaxf(fabsf(__uint_as_float(w[i] << 16)), fabsf(__uint_as_float(w[i] & 0xFFFF0000u))));
+    for (int i = 0; i < 4; ++i) {
+      const float a = fabsf(a16_to_f32<AT>((uint16_t)(w[i] & 0xFFFFu))), b = fabsf(a16_to_f32<AT>((uint16_t)(w[i] >> 16)));
+      big = fmaxf(big, fmaxf(a, b));
+      sum += a + b;
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
-    row_factor(big, f, back);
   }
-#pragma unroll 4
-  for (int k = lane * 8; k < p.hpad; k += 256) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+  sum = warp_sum(sum);
+  __syncthreads();
+  if (lane == 0) {
+    s_big[warp] = big;
+    s_sum[warp] = sum;
+  }
+  __syncthreads();
+  big = sum = 0.0f;
+#pragma unroll
+  for (int w = 0; w < THREADS / 32; ++w) {
+    big = fmaxf(big, s_big[w]);
+    sum += s_sum[w];
+  }
+  float f = 1.0f, back = 1.0f;
+  if (AT == 1) row_factor(big, f, back);
+  for (int k = threadIdx.x * 8; k < p.hpad; k += THREADS * 8) {
     uint4 v = make_uint4(0, 0, 0, 0);
     if (k < p.a.hidden) {
       v = load8(k);
-      uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) sum += fabsf(a16_to_f32<AT>((uint16_t)(w[i] & 0xFFFFu))) + fabsf(a16_to_f32<AT>((uint16_t)(w[i] >> 16)));
       if (AT == 1) {
+        uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) w[i] = pack_f16(__uint_as_float(w[i] << 16) * f, __uint_as_float(w[i] & 0xFFFF0000u) * f);
         v = make_uint4(w[0], w[1], w[2], w[3]);
@@ -260,8 +350,7 @@ __device__ __forceinline__ void convert_row(const MoeParams& p, int t, int lane,
     }
     *reinterpret_cast<uint4*>(p.xf + (size_t)t * p.hpad + place(k)) = v;
   }
-  sum = warp_sum(sum);
-  if (lane == 0) {
+  if (threadIdx.x == 0) {
     p.xback[2 * t] = back;
     p.xback[2 * t + 1] = sum;
   }
@@ -284,64 +373,26 @@ struct Lists {
   int scan[16];
 };
 
-// A token's top_k by one warp: rounds of the largest logit not yet taken.
-__device__ __forceinline__ void pick(const MoeParams& p, Lists& L, int t, int lane) {
-  const int E = p.a.experts, K = p.a.top_k;
-  const float* r = p.logits + (size_t)t * E;
-  unsigned taken = 0u;  // expert lane + 32 * bit
-  float keep[4], first = 0.0f, sum = 0.0f;  // the first 128 experts stay in registers
-#pragma unroll
-  for (int i = 0; i < 4; ++i) keep[i] = lane + 32 * i < E ? __ldcg(r + lane + 32 * i) : 0.0f;
-#pragma unroll 1
-  for (int s = 0; s < K; ++s) {
-    int best = (int)0x80000000, at = 0x7fffffff;
-    float val = 0.0f;
-    auto look = [&](int i, float v) {
-      const int key = order_key(v);
-      if (!((taken >> i) & 1u) && (at == 0x7fffffff || key > best)) {
-        best = key;
-        at = lane + 32 * i;
-        val = v;
-      }
-    };
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (lane + 32 * i < E) look(i, keep[i]);
-#pragma unroll 1
-    for (int i = 4; lane + 32 * i < E; ++i) look(i, __ldcg(r + lane + 32 * i));
-    const int top = __reduce_max_sync(0xffffffffu, best);
-    const int e = __reduce_min_sync(0xffffffffu, best == top ? at : 0x7fffffff);
-    val = __shfl_sync(0xffffffffu, val, e & 31);
-    if ((e & 31) == lane) taken |= 1u << (e >> 5);
-    if (s == 0) first = val;
-    const float w = __expf(val - first);
-    sum += w;
-    if (lane == 0) {
-      L.id[t * K + s] = (short)e;
-      L.weight[t * K + s] = w;
-    }
-  }
-  if (!p.a.renormalize) {
-    float z = 0.0f;
-    for (int i = lane; i < E; i += 32) z += __expf(__ldcg(r + i) - first);
-    sum = warp_sum(z);
-  }
-  __syncwarp();
-  if (lane < K) L.weight[t * K + lane] = __fdiv_rn(L.weight[t * K + lane], sum);
-}
-
 template <int FMT, int NT, int RU, int WARPS, int DEPTH>
-__global__ void __launch_bounds__(WARPS * 32, 1) moe_kernel(const __grid_constant__ MoeParams p) {
+__global__ void __launch_bounds__(WARPS * 32, 1)
+    moe_kernel(const __grid_constant__ CUtensorMap map_up, const __grid_constant__ CUtensorMap map_down, const __grid_constant__ MoeParams p) {
   using S = Shape<NT, RU, WARPS, DEPTH>;
   constexpr int kThreads = S::kThreads;
   constexpr int CH = NT * RU <= 2 ? 2 : 1;  // chains of dependent products a tile
-  extern __shared__ __align__(16) uint8_t smem_raw[];
+  extern __shared__ uint8_t smem_raw[];
   __shared__ Lists L;
+  __shared__ uint64_t s_full[WARPS][DEPTH];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, q4 = lane >> 2, t4 = lane & 3;
-  const uint4* const queue = reinterpret_cast<const uint4*>(smem_raw + warp * S::kQueue) + lane;  // pieces 32 apart
-  const uint32_t queue_at = smem_u32(queue);
-  float* const frags = reinterpret_cast<float*>(smem_raw + WARPS * S::kQueue);
+  uint8_t* const base = smem_raw + (((smem_u32(smem_raw) + 1023u) & ~1023u) - smem_u32(smem_raw));
+  uint8_t* const ring = base + warp * S::kRing;
+  float* const frags = reinterpret_cast<float*>(base + WARPS * S::kRing);
   const int T = p.a.tokens, E = p.a.experts, K = p.a.top_k, H = p.a.hidden, I = p.a.inter;
+
+  if (lane == 0) {
+    for (int i = 0; i < DEPTH; ++i) mbar_init(&s_full[warp][i], 1);
+    fence_barrier_init();
+    prefetch_tensormap(warp & 1 ? &map_down : &map_up);
+  }
 
   // ------------------------------------------------- 0: router, x to fp16 --
   {
@@ -349,52 +400,41 @@ __global__ void __launch_bounds__(WARPS * 32, 1) moe_kernel(const __grid_constan
     const int wid = warp * gridDim.x + blockIdx.x, nw = WARPS * gridDim.x;
     const bool vec = ((reinterpret_cast<uintptr_t>(p.a.x) | reinterpret_cast<uintptr_t>(p.a.router) | (uintptr_t)(p.a.x_token_stride * 2)) & 15u) == 0;
     const bool bf = p.a.a_type == FP8IMMA_A_BF16;
-    for (int t = nw - 1 - wid; t < T; t += nw) {  // from the last warp on: the first have router units
-      if (bf) convert_row<1>(p, t, lane, vec);
-      else convert_row<0>(p, t, lane, vec);
+    for (int t = gridDim.x - 1 - blockIdx.x; t < T; t += gridDim.x) {  // the last CTAs: with few router units they have none
+      if (bf) convert_row<1, kThreads>(p, t, vec);
+      else convert_row<0, kThreads>(p, t, vec);
     }
-    if (NT == 1) {  // 8 tokens at most
-      if (T == 1) {
-        if (bf) router<1, 1, 1>(p, wid, nw, lane, vec);
-        else router<0, 1, 1>(p, wid, nw, lane, vec);
-      } else {
-        if (bf) router<1, 1, 4>(p, wid, nw, lane, vec);
-        else router<0, 1, 4>(p, wid, nw, lane, vec);
-      }
+    // one token and expert a warp while that is one round of the grid's warps; then four experts, then four tokens as well
+    if (E * T <= nw) {
+      if (bf) router<1, 1, 1>(p, wid, nw, lane, vec);
+      else router<0, 1, 1>(p, wid, nw, lane, vec);
+    } else if (((E + 3) >> 2) * T <= nw) {
+      if (bf) router<1, 4, 1>(p, wid, nw, lane, vec);
+      else router<0, 4, 1>(p, wid, nw, lane, vec);
     } else {
       if (bf) router<1, 4, 4>(p, wid, nw, lane, vec);
       else router<0, 4, 4>(p, wid, nw, lane, vec);
     }
-    scale_maxima(p, nw - 1 - wid, nw, lane);
+    scale_maxima(p, ((warp + WARPS / 2) % WARPS) * gridDim.x + blockIdx.x, nw, lane);  // from the middle warps on: the first have router units
   }
   for (int e = tid; e < E; e += kThreads) L.tokens[e] = 0ull;
   if (!grid_barrier(p.sync)) return;
   if (blockIdx.x == 0 && tid == 0) p.sync[2] = 0u;  // all CTAs of the call before have left its last barrier
 
-  // -------------------------------------------------------- choice, lists --
+  // ---------------------------------------------------------------- lists --
   if (tid < T) L.xback[tid] = __ldcg(p.xback + 2 * tid);
-#pragma unroll 1
-  for (int t = warp; t < T; t += WARPS) pick(p, L, t, lane);
-  __syncthreads();
   for (int s = tid; s < T * K; s += kThreads) {
-    atomicOr(&L.tokens[L.id[s]], 1ull << (s / K));
-    if (blockIdx.x == 0) {
-      if (p.a.ids) p.a.ids[s] = L.id[s];
-      if (p.a.weights) p.a.weights[s] = L.weight[s];
-    }
+    const int t = s / K, e = __ldcg(p.ids + s);
+    const float l1 = __ldcg(p.xback + 2 * t + 1), w = __ldcg(p.weights + s);
+    L.id[s] = (short)e;
+    atomicOr(&L.tokens[e], 1ull << t);
     // the slot's power of two: gate sums are below 2^(eg + 1), up sums below 2^(eu + 1)
-    const float l1 = __ldcg(p.xback + 2 * (s / K) + 1), *m = p.smax + (size_t)L.id[s] * 2 * p.chunks;
-    float mg = 0.0f, mu = 0.0f;
-#pragma unroll 4
-    for (int c = 0; c < p.chunks; ++c) {
-      mg = fmaxf(mg, __ldcg(m + c));
-      mu = fmaxf(mu, __ldcg(m + p.chunks + c));
-    }
     const float fmax_v = FMT == F8_E4M3 ? 448.0f : 57344.0f;
-    const int eg = (int)(__float_as_uint(mg * fmax_v * l1) >> 23) - 127, eu = (int)(__float_as_uint(mu * fmax_v * l1) >> 23) - 127;
+    const uint2 m = __ldcg(reinterpret_cast<const uint2*>(p.sync + kScaleMax) + e);
+    const int eg = (int)(__float_as_uint(__uint_as_float(m.x) * fmax_v * l1) >> 23) - 127, eu = (int)(__float_as_uint(__uint_as_float(m.y) * fmax_v * l1) >> 23) - 127;
     const int k = max(-126, min(126, eg + eu - 13));
     L.scale[s] = __uint_as_float((uint32_t)(127 - k) << 23);
-    L.weight[s] *= __uint_as_float((uint32_t)(127 + k) << 23);  // a slot's result is multiplied by its weight and by what undoes the factor
+    L.weight[s] = w * __uint_as_float((uint32_t)(127 + k) << 23);  // a slot's result is multiplied by its weight and by what undoes the factor
   }
   __syncthreads();
   {
@@ -457,52 +497,58 @@ __global__ void __launch_bounds__(WARPS * 32, 1) moe_kernel(const __grid_constan
   };
   const int ks1 = team_of(runs1.per + (runs1.rem > 0)), ks2 = team_of(runs2.per + (runs2.rem > 0));
 
-  // loading side of this warp: the next block to ask for. A lane copies its
-  // rows' pieces itself: rows r * 8 + q4 of the gate (first) and up (second)
-  // box, bytes 16 t4 of both halves of the block.
-  int lp = 1, lu = warp / ks1, lb = warp % ks1, put = 0, got = 0;
-  const uint8_t* lrow = nullptr;  // the lane's first row of the unit
-  auto unit_row = [&]() {
-    const bool up = lp == 1;
-    const int per = up ? per1 : per2, u = (up ? u1 : u2) + lu, a = u / per;
-    const int row = (u - a * per) * (up ? 8 * RU : 16 * RU) + q4;
-    lrow = static_cast<const uint8_t*>(up ? p.a.w_gate_up : p.a.w_down) + ((size_t)L.expert[a] * (up ? 2 * I : H) + row) * (up ? H : I) + t4 * 16;
+  // loading side of this warp: the next block to ask for
+  int lp = 1, lu = warp / ks1, lb = warp % ks1, issued = 0, used = 0, lost = 0, lrow = 0, lexp = 0;
+  bool ok = true;
+  auto unit_at = [&]() {
+    const int per = lp == 1 ? per1 : per2, u = (lp == 1 ? u1 : u2) + lu, a = u / per;
+    lexp = L.expert[a];
+    lrow = (u - a * per) * (lp == 1 ? 8 * RU : 16 * RU);
   };
-  auto issue = [&]() {
-    bool fresh = put == 0;
-    if (lp == 1 && lb >= nb1) lb = warp % ks1, lu += WARPS / ks1, fresh = true;
-    if (lp == 1 && (lu >= n1 || lb >= nb1)) lp = 2, lu = warp / ks2, lb = warp % ks2, fresh = true;
-    if (lp == 2 && lb >= nb2) lb = warp % ks2, lu += WARPS / ks2, fresh = true;
-    if (lp == 2 && (lu >= n2 || lb >= nb2)) lp = 3;
-    if (lp < 3) {
-      if (fresh) unit_row();
-      const bool up = lp == 1;
-      const int width = up ? H : I;
-      const size_t box = (size_t)(up ? I : 8 * RU) * width;  // from a row of the first box to its row of the second
-      // rows past the last one of the matrix (the end of a unit that is not whole) read its last
-      const int tail = up ? 0x7fffffff : H - 1 - ((u2 + lu) % per2 * (16 * RU) + q4);
-      const uint32_t dst = queue_at + put % DEPTH * (S::kPieces * 512);
-#pragma unroll
-      for (int r = 0; r < RU; ++r)
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const int step = r * 8 + (up ? 0 : k * 8 * RU);  // rows down from the lane's first, second box of the down weights included
-          const uint8_t* src = lrow + (up ? (size_t)(r * 8) * width + k * box : (size_t)max(min(step, tail), 0) * width);
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const int at = lb * 128 + j * 64;
-            const bool in = at + t4 * 16 < width;
-            copy16(dst + ((r * 2 + k) * 2 + j) * 512, in ? src + at : static_cast<const uint8_t*>(p.a.w_down), in);
-          }
-        }
-      lb += up ? ks1 : ks2;
-      ++put;
+  auto seek = [&]() {  // to the next block when the unit's are done
+    if (lp == 1 && lb >= nb1) {
+      lb = warp % ks1, lu += WARPS / ks1;
+      if (lu < n1) {
+        unit_at();
+      } else {
+        lp = 2, lu = warp / ks2, lb = warp % ks2;
+        if (lu < n2 && lb < nb2) unit_at();
+        else lp = 3;
+      }
+    } else if (lp == 2 && lb >= nb2) {
+      lb = warp % ks2, lu += WARPS / ks2;
+      if (lu < n2) unit_at();
+      else lp = 3;
     }
-    asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  auto next_block = [&]() {  // the lane's pieces of its next block
-    asm volatile("cp.async.wait_group %0;" ::"n"(DEPTH - 1) : "memory");
-    return queue + got++ % DEPTH * (S::kPieces * 32);
+  if (lu < n1 && lb < nb1) {
+    unit_at();
+  } else {
+    lu = n1, lb = nb1;
+    seek();
+  }
+  auto issue = [&]() {
+    if (lp == 3 || !ok) return;
+    const int st = issued % DEPTH;
+    if (lane == 0) {
+      mbar_arrive_expect_tx(&s_full[warp][st], S::kBlockBytes);
+      tma_load_3d(ring + st * S::kBlockBytes, lp == 1 ? &map_up : &map_down, &s_full[warp][st], lb * 128, lrow, lp == 1 ? 2 * lexp : lexp);
+    }
+    ++issued;
+    lb += lp == 1 ? ks1 : ks2;
+    seek();
+  };
+  auto next_block = [&]() {  // waits for it; after a wait that ran out the rest is passed over
+    const int st = used % DEPTH;
+    if (ok) {
+      ok = mbar_wait(&s_full[warp][st], (uint32_t)((used / DEPTH) & 1), ERR_WAIT_FULL);
+      if (!ok) lost = used;
+    }
+    ++used;
+    return ring + st * S::kBlockBytes;
+  };
+  auto drain = [&]() {  // before an early end: the copies under way land first
+    for (int k = ok ? used : lost; k < issued; ++k) mbar_wait(&s_full[warp][k % DEPTH], (uint32_t)((k / DEPTH) & 1), ERR_WAIT_FULL);
   };
 #pragma unroll 1
   for (int i = 0; i < DEPTH; ++i) issue();
@@ -538,7 +584,10 @@ __global__ void __launch_bounds__(WARPS * 32, 1) moe_kernel(const __grid_constan
               make_float4(acc[0][r][nt][0], acc[0][r][nt][1], acc[0][r][nt][2], acc[0][r][nt][3]);
     }
     named_bar_sync(1 + warp / ks, ks * 32);
-    if (warp % ks) return false;
+    if (warp % ks) {
+      named_bar_sync(1 + warp / ks, ks * 32);  // the first warp has read them
+      return false;
+    }
 #pragma unroll 1
     for (int w = warp + 1; w < warp + ks; ++w)
 #pragma unroll
@@ -551,9 +600,10 @@ __global__ void __launch_bounds__(WARPS * 32, 1) moe_kernel(const __grid_constan
           acc[0][r][nt][2] += v.z;
           acc[0][r][nt][3] += v.w;
         }
+    named_bar_sync(1 + warp / ks, ks * 32);
     return true;
   };
-  // One block's products: fp16 rows xr (8 NT of them, operand order) times the queue's next block.
+  // One block's products: fp16 rows xr (8 NT of them, operand order) times the ring's next block.
   const uint16_t* xr[NT];
   auto multiply = [&](int kb, int tiles) {
     uint4 x[NT][2];
@@ -561,14 +611,15 @@ __global__ void __launch_bounds__(WARPS * 32, 1) moe_kernel(const __grid_constan
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int i = 0; i < 2; ++i) x[nt][i] = xr[nt] ? *reinterpret_cast<const uint4*>(xr[nt] + kb * 128 + i * 32) : make_uint4(0, 0, 0, 0);
-    const uint4* w = next_block();
+    const uint8_t* w = next_block();
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       uint4 g[RU], b[RU], y[NT][2];
 #pragma unroll
       for (int r = 0; r < RU; ++r) {
-        g[r] = w[((r * 2) * 2 + j) * 32];
-        b[r] = w[((r * 2 + 1) * 2 + j) * 32];
+        const int at = (r * 8 + q4) * 128 + (((2 * t4 + j) ^ q4) << 4);
+        g[r] = *reinterpret_cast<const uint4*>(w + at);
+        b[r] = *reinterpret_cast<const uint4*>(w + 1024 * RU + at);
       }
       if (j == 0) {  // the second half's operands, while the first half is multiplied
 #pragma unroll
@@ -599,7 +650,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1) moe_kernel(const __grid_constan
           for (int i = 0; i < 2; ++i) x[nt][i] = y[nt][i];
       }
     }
-    issue();  // the lane has read its pieces: their place takes the next block
+    __syncwarp();
+    issue();  // into the place of the block just read
   };
 
   // ------------------------------------------------ 1: gate, up, activation --
@@ -646,9 +698,12 @@ __global__ void __launch_bounds__(WARPS * 32, 1) moe_kernel(const __grid_constan
     for (int x = blockIdx.x * kThreads + tid; x < T * K * (p.ipad - I); x += gridDim.x * kThreads)
       p.h[(size_t)(x / (p.ipad - I)) * p.ipad + place(I + x % (p.ipad - I))] = 0;
   const bool met = grid_barrier(p.sync + 1);
-  if (met && blockIdx.x == 0 && tid == 0) p.sync[0] = 0u;
+  if (met && blockIdx.x == 0) {  // every CTA has read them
+    if (tid == 0) p.sync[0] = 0u;
+    for (int e = tid; e < 2 * E; e += kThreads) p.sync[kScaleMax + e] = 0u;
+  }
   if (!met) {
-    asm volatile("cp.async.wait_all;" ::: "memory");
+    drain();
     return;
   }
 
@@ -687,7 +742,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) moe_kernel(const __grid_constan
       }
     }
   }
-  asm volatile("cp.async.wait_all;" ::: "memory");
+  if (!ok) drain();
   if (!grid_barrier(p.sync + 2)) return;
   if (blockIdx.x == 0 && tid == 0) p.sync[1] = 0u;
 
@@ -718,9 +773,12 @@ cudaError_t launch(const fp8imma_moe_args& a, cudaStream_t st) {
   if (e != cudaSuccess) return e;
   MoeParams p = {};
   p.a = a;
+  CUtensorMap up, down;
+  e = make_tmap_3d_u8(&up, a.w_gate_up, a.hidden, a.inter, (uint64_t)a.experts * 2, 128, 8 * RU, 2);
+  if (e == cudaSuccess) e = make_tmap_3d_u8(&down, a.w_down, a.inter, a.hidden, a.experts, 128, 16 * RU, 1);
+  if (e != cudaSuccess) return e;
   p.hpad = (a.hidden + 127) & ~127;
   p.ipad = (a.inter + 127) & ~127;
-  p.chunks = (a.inter + 1023) / 1024;
   const size_t slots = (size_t)a.tokens * a.top_k;
   size_t at = 0;
   auto take = [&](size_t bytes) {
@@ -729,10 +787,10 @@ cudaError_t launch(const fp8imma_moe_args& a, cudaStream_t st) {
     return was;
   };
   const size_t o_logits = take((size_t)a.tokens * a.experts * 4), o_xf = take((size_t)a.tokens * p.hpad * 2), o_back = take((size_t)a.tokens * 8),
-               o_max = take((size_t)a.experts * 2 * p.chunks * 4), o_h = take(slots * p.ipad * 2), o_part = take(slots * a.hidden * 4);
+               o_ids = take(slots * 4), o_wts = take(slots * 4), o_h = take(slots * p.ipad * 2), o_part = take(slots * a.hidden * 4);
   ScopedScratch sync, work;
-  e = sync.get(256, st, kScratchMoeSync);
-  if (e == cudaSuccess && sync.owned) e = cudaMemsetAsync(sync.ptr, 0, 256, st);
+  e = sync.get(kSyncWords * 4, st, kScratchMoeSync);
+  if (e == cudaSuccess && sync.owned) e = cudaMemsetAsync(sync.ptr, 0, kSyncWords * 4, st);
   if (e == cudaSuccess) e = work.get(at, st, kScratchMoe);
   if (e == cudaSuccess) {
     char* base = static_cast<char*>(work.ptr);
@@ -740,7 +798,8 @@ cudaError_t launch(const fp8imma_moe_args& a, cudaStream_t st) {
     p.logits = reinterpret_cast<float*>(base + o_logits);
     p.xf = reinterpret_cast<uint16_t*>(base + o_xf);
     p.xback = reinterpret_cast<float*>(base + o_back);
-    p.smax = reinterpret_cast<float*>(base + o_max);
+    p.ids = reinterpret_cast<int*>(base + o_ids);
+    p.weights = reinterpret_cast<float*>(base + o_wts);
     p.h = reinterpret_cast<uint16_t*>(base + o_h);
     p.part = reinterpret_cast<float*>(base + o_part);
     cudaLaunchConfig_t lc = {};
@@ -753,7 +812,7 @@ cudaError_t launch(const fp8imma_moe_args& a, cudaStream_t st) {
     lc.stream = st;
     lc.attrs = attr;
     lc.numAttrs = 1;
-    e = cudaLaunchKernelEx(&lc, kern, p);
+    e = cudaLaunchKernelEx(&lc, kern, up, down, p);
   }
   const cudaError_t e1 = sync.release(st), e2 = work.release(st);
   return e != cudaSuccess ? e : e1 != cudaSuccess ? e1 : e2;
@@ -764,10 +823,9 @@ cudaError_t launch(const fp8imma_moe_args& a, cudaStream_t st) {
 // for each unit, cost less beside the weights.
 template <int FMT>
 cudaError_t launch_nt(const fp8imma_moe_args& a, cudaStream_t st) {
-  if (a.tokens <= 2) return launch<FMT, 1, 1, 16, 4>(a, st);
   if (a.tokens <= 8) return launch<FMT, 1, 2, 16, 2>(a, st);
   if (a.tokens <= 16) return launch<FMT, 2, 2, 16, 2>(a, st);
-  return launch<FMT, 4, 2, 8, 4>(a, st);
+  return launch<FMT, 4, 4, 8, 2>(a, st);
 }
 
 }  // namespace
