@@ -54,6 +54,7 @@ struct AttnParams {
   int per_seq;   // > 0: every sequence has this many tokens
   int group;     // query heads per KV head
   int vec_q;     // query rows are 16-byte aligned
+  int max_items; // items of the step at most (counters)
   unsigned int* counters;  // per item: finished parts; zero between calls
   float* parts;            // per (CTA, first / last segment, row warp): M, L, O of a shared item
 };
@@ -199,7 +200,12 @@ struct Shape {
   static constexpr int kVecs = kMT * NT * 32;             // float4 of O of a warp
   static constexpr int kPartFloats = (kMT * NT * 4 + NT * 4) * 32;  // O, M and L of a warp, register by register
   static constexpr int kMergeBytes = kConsumers * kPartFloats * 4;
-  static constexpr int kStages = (227 * 1024 - 2048 - kMergeBytes) / kStageBytes < 6 ? (227 * 1024 - 2048 - kMergeBytes) / kStageBytes : 6;
+  // As many stages as fit, six at most, and a multiple of kSplit: each stage is
+  // then always read by the same warps, which wait for every one of its phases
+  // in turn. (A warp that skipped a stage's phase would take the parity of the
+  // one before for the one it wants and read, and release, too early.)
+  static constexpr int kFit = (227 * 1024 - 2048 - kMergeBytes) / kStageBytes < 6 ? (227 * 1024 - 2048 - kMergeBytes) / kStageBytes : 6;
+  static constexpr int kStages = kFit / kSplit * kSplit;
   static constexpr int kSmem = kStages * kStageBytes + kMergeBytes + 1024;
 };
 
@@ -364,6 +370,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   };
   for (int b0 = 0; b0 < p.c.batch; b0 += kThreads) scan(b0);
   if (units == 0) return;
+  if (items > p.max_items) {  // offsets that do not ascend: more rows than tokens
+    if (tid == 0) atomicCAS(&g_fp8imma_device_error, 0u, (unsigned int)ERR_BAD_OFFSETS);
+    return;
+  }
   const int ctas = min((int)gridDim.x, units);
   if ((int)blockIdx.x >= ctas) return;
   const Runs runs(units, ctas);
@@ -862,7 +872,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 template <int FMT, int D, int NT, int RW>
 cudaError_t launch(AttnParams& p, cudaStream_t st) {
   using S = Shape<D, NT, RW>;
-  static_assert(S::kStages >= 2, "ring too short");
+  static_assert(S::kStages >= 2 && S::kStages % S::kSplit == 0, "ring too short, or stages change hands");
   const auto kern = kv_attention_kernel<FMT, D, NT, RW>;
   cudaError_t e = ensure_smem_attr(reinterpret_cast<const void*>(kern), S::kSmem);
   if (e != cudaSuccess) return e;
@@ -878,6 +888,7 @@ cudaError_t launch(AttnParams& p, cudaStream_t st) {
   const int64_t tiles = ((int64_t)p.c.max_pages * p.c.page_size + kKeys - 1) / kKeys;
   if (items * tiles > 0x7fffffffll) return cudaErrorInvalidValue;  // units are counted in 31 bits
   const int grid = (int)std::min<int64_t>(num_sms_current(), std::max<int64_t>(1, items * tiles));
+  p.max_items = (int)items;
   const size_t ctr_bytes = (size_t)items * 4, part_bytes = (size_t)grid * 2 * RW * S::kPartFloats * 4;
   ScopedScratch ctr, part;
   e = ctr.get(ctr_bytes, st, kScratchAttn);

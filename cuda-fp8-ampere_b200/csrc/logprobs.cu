@@ -22,6 +22,7 @@
 #include "sm100_async.cuh"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace fp8imma_b200 {
 namespace {
@@ -69,38 +70,463 @@ __device__ __forceinline__ float ex2(float x) {
   return r;
 }
 
-// Running sums of one lane (or of a joined part).
+constexpr float kLowest = -1e38f;  // reference before any logit was seen
+constexpr float kRaise = 8.0f;     // the reference follows the maximum when it lies this far above
+
+// Running sums of a lane or of joined parts.
 struct Sums {
-  float m = -INFINITY, l = 0.0f, s = 0.0f;
-  bool bad = false;  // NaN or +inf was seen
+  float m = kLowest, l = 0.0f, s = 0.0f;
   __device__ __forceinline__ void join(float m2, float l2, float s2) {
-    const float mn = fmaxf(m, m2);
-    if (mn == -INFINITY) return;
-    const float a = m == -INFINITY ? 0.0f : ex2(m - mn), b = m2 == -INFINITY ? 0.0f : ex2(m2 - mn);
-    const float da = m == -INFINITY ? 0.0f : m - mn, db = m2 == -INFINITY ? 0.0f : m2 - mn;
-    s = a * (s + da * l) + b * (s2 + db * l2);
+    const float mn = fmaxf(m, m2), da = m - mn, db = m2 - mn, a = ex2(da), b = ex2(db);
+    s = a * fmaf(da, l, s) + b * fmaf(db, l2, s2);
     l = a * l + b * l2;
     m = mn;
   }
+  __device__ __forceinline__ void raise(float to) {
+    const float d = m - to, f = ex2(d);
+    s = f * fmaf(d, l, s);
+    l *= f;
+    m = to;
+  }
+  __device__ __forceinline__ void add(float x, float c) {
+    const float d = fmaf(x, c, -m), e = ex2(d);
+    l += e;
+    s = fmaf(e, fmaxf(d, -1000.0f), s);  // a logit of -inf: 0 * -1000
+  }
+  __device__ __forceinline__ void warp_join() {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      const float m2 = __shfl_xor_sync(0xffffffffu, m, o), l2 = __shfl_xor_sync(0xffffffffu, l, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
+      join(m2, l2, s2);
+    }
+  }
 };
 
-// A warp's list: lane i holds the i-th largest key. Insert one key (uniform).
+// A warp's list: lane i holds the i-th largest key. Enters one key (the same
+// in all lanes).
 __device__ __forceinline__ void insert(unsigned long long& mine, unsigned long long key, int lane) {
-  const unsigned below = __ballot_sync(0xffffffffu, mine < key);  // a suffix of the lanes: they move down by one
   const unsigned long long up = __shfl_up_sync(0xffffffffu, mine, 1);
-  if ((below >> lane) & 1u) mine = lane > 0 && ((below >> (lane - 1)) & 1u) ? up : key;
+  if (mine < key) mine = lane > 0 && up < key ? up : key;
 }
-
-// Two descending lists (one a lane) -> the 32 largest, descending.
+__device__ __forceinline__ unsigned long long step(unsigned long long v, int o, bool larger) {
+  const unsigned long long w = __shfl_xor_sync(0xffffffffu, v, o);
+  return (w > v) == larger ? w : v;
+}
+// Two descending lists -> the 32 largest, descending.
 __device__ __forceinline__ unsigned long long merge(unsigned long long a, unsigned long long b, int lane) {
   const unsigned long long r = __shfl_sync(0xffffffffu, b, 31 - lane);
-  unsigned long long v = a > r ? a : r;  // the 32 largest, bitonic
+  unsigned long long v = a > r ? a : r;  // bitonic
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const unsigned long long w = __shfl_xor_sync(0xffffffffu, v, o);
-    v = (lane & o) ? (w < v ? w : v) : (w > v ? w : v);
-  }
+  for (int o = 16; o > 0; o >>= 1) v = step(v, o, !(lane & o));
   return v;
 }
+__device__ __noinline__ unsigned long long sort_merge(unsigned long long list, unsigned long long key, int lane) {
+#pragma unroll
+  for (int k = 2; k <= 32; k <<= 1)
+#pragma unroll
+    for (int o = k >> 1; o > 0; o >>= 1) key = step(key, o, !(lane & o) == !(lane & k));
+  return merge(list, key, lane);
+}
+
+// The warp's list and the value below which nothing can enter it.
+struct Top {
+  unsigned long long mine = kNoKey, last = kNoKey;
+  float bar = NAN;  // NaN: everything may enter
+  __device__ __forceinline__ void enter(unsigned long long key, int top, int lane) {  // one key a lane (kNoKey: none)
+    unsigned who = __ballot_sync(0xffffffffu, key > last);
+    if (!who) return;
+    if (__popc(who) > 6) {
+      mine = sort_merge(mine, key, lane);
+    } else {
+      do {
+        const int src = __ffs(who) - 1;
+        insert(mine, __shfl_sync(0xffffffffu, key, src), lane);
+        who &= who - 1;
+      } while (who);
+    }
+    last = __shfl_sync(0xffffffffu, mine, top - 1);
+    bar = last == kNoKey ? NAN : key_value(last);
+  }
+};
+
+// What a row's sums give: lp(x) = (x - at) * inv - ln_l.
+struct Norm {
+  float at, inv, ln_l, entropy;
+  unsigned long long mine;  // the lane's entry of the list
+};
+
+// Rows that the pass cannot do: no logit within (-1e38, 1e38) log2 units, NaN,
+// infinities. One warp, two passes over the row, differences before scaling.
+template <int LT, class Load>
+__device__ __noinline__ Norm careful(int vocab, int n_top, float to_log2, float inv_temp, Load load, int lane) {
+  float m = -INFINITY;
+  bool bad = false;
+  Top top;
+  for (int j0 = 0; j0 < vocab; j0 += 32) {
+    const bool in = j0 + lane < vocab;
+    const float x = in ? load(j0 + lane) : -INFINITY;
+    bad |= !(x < INFINITY);
+    m = fmaxf(m, x);
+    if (n_top) top.enter(in ? make_key(x, j0 + lane) : kNoKey, n_top, lane);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  bad = __any_sync(0xffffffffu, bad) || m == -INFINITY;
+  float l = 0.0f, s = 0.0f;
+  for (int j = lane; j < vocab && !bad; j += 32) {
+    const float d = (load(j) - m) * to_log2, e = ex2(d);
+    l += e;
+    s = fmaf(e, fmaxf(d, -1000.0f), s);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    l += __shfl_xor_sync(0xffffffffu, l, o);
+    s += __shfl_xor_sync(0xffffffffu, s, o);
+  }
+  Norm n = {m, inv_temp, logf(l), logf(l) - 0.6931471805599453f * (s / l), top.mine};
+  if (bad) n.at = n.entropy = NAN;
+  return n;
+}
+
+// A row's results from its joined sums and list; one warp.
+template <int LT>
+__device__ __forceinline__ void finish(const LpParams& p, int t, const Sums& z, const Top& top, int lane) {
+  const int64_t row = (int64_t)t * p.a.token_stride;
+  const void* logits = p.a.logits;
+  const int64_t stride = p.a.vocab_stride;
+  auto load = [logits, row, stride](int j) {
+    const int64_t at = row + (int64_t)j * stride;
+    return LT == FP8IMMA_L_F32 ? __ldg(static_cast<const float*>(logits) + at) : to_f32<LT>(__ldg(static_cast<const uint16_t*>(logits) + at));
+  };
+  const int id = __ldg(p.a.token_ids + t);
+  const bool known = (unsigned)id < (unsigned)p.a.vocab;
+  const float x = known ? load(id) : NAN;
+  Norm n = {0.0f, p.inv_temp, 0.6931471805599453f * (z.m + log2f(z.l)), 0.6931471805599453f * (log2f(z.l) - z.s / z.l), top.mine};
+  if (!(z.l > 0.0f && z.l < INFINITY && fabsf(z.m) < -kLowest)) n = careful<LT>(p.a.vocab, p.a.top, p.to_log2, p.inv_temp, load, lane);
+  if (lane == 0) {
+    p.a.logprobs[t] = fmaf(x - n.at, n.inv, -n.ln_l);
+    p.a.entropy[t] = n.entropy;
+  }
+  if (lane < p.a.top) {
+    p.a.top_ids[(int64_t)t * p.a.top + lane] = key_index(n.mine);
+    p.a.top_logprobs[(int64_t)t * p.a.top + lane] = fmaf(key_value(n.mine) - n.at, n.inv, -n.ln_l);
+  }
+}
+
+// This CTA came last to `counter` (all of its threads call; its results are in
+// global memory).
+__device__ __forceinline__ bool came_last(unsigned int* counter, int parts) {
+  __shared__ int s_last;
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    unsigned int prev;
+    asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(prev) : "l"(counter) : "memory");
+    s_last = prev == (unsigned)(parts - 1);
+    if (s_last) *counter = 0;  // ready for the next call
+  }
+  __syncthreads();
+  __threadfence();
+  return s_last != 0;
+}
+
+__device__ __forceinline__ void put_part(const LpParams& p, int part, int t, const Sums& z, const Top& top, int lane) {
+  const int64_t at = (int64_t)part * p.a.tokens + t;
+  if (lane == 0) *reinterpret_cast<float4*>(p.sums + at * 4) = make_float4(z.m, z.l, z.s, 0.0f);
+  if (p.a.top) p.lists[at * 32 + lane] = top.mine;
+}
+// Parts first, first + stride, ... of token t joined in this order, the sums of
+// 32 parts at a time.
+__device__ __forceinline__ void get_parts(const LpParams& p, int first, int stride, int t, Sums& z, Top& top, int lane) {
+  for (int k = first + lane * stride; k < p.parts; k += 32 * stride) {
+    const float4 v = __ldcg(reinterpret_cast<const float4*>(p.sums + ((int64_t)k * p.a.tokens + t) * 4));
+    z.join(v.x, v.y, v.z);
+  }
+  z.warp_join();
+  if (p.a.top) {
+#pragma unroll 4
+    for (int k = first; k < p.parts; k += stride) top.mine = merge(top.mine, __ldcg(p.lists + ((int64_t)k * p.a.tokens + t) * 32 + lane), lane);
+  }
+}
+
+// Row-major logits: CTA (part, token); a warp takes every eighth run of 32
+// 16-byte vectors of the part. Rows of any alignment: vectors lie on 16-byte
+// boundaries, the row's first and last may be partial.
+template <int LT>
+__global__ void __launch_bounds__(kThreads, 4) logprobs_row_kernel(const __grid_constant__ LpParams p) {
+  constexpr int kVec = LT == FP8IMMA_L_F32 ? 4 : 8, kSize = LT == FP8IMMA_L_F32 ? 4 : 2, kAhead = 4;
+  __shared__ float s_sums[kWarps][3];
+  __shared__ unsigned long long s_list[kWarps][32];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int part = blockIdx.x, V = p.a.vocab, top = p.a.top;
+  const float c = p.to_log2;
+  for (int t = blockIdx.y; t < p.a.tokens; t += gridDim.y) {
+    const char* row = static_cast<const char*>(p.a.logits) + (int64_t)t * p.a.token_stride * kSize;
+    const int lead = (int)((reinterpret_cast<uintptr_t>(row) & 15u) / kSize);  // logits between a boundary and the row
+    const int vecs = (lead + V + kVec - 1) / kVec;
+    const int v0 = part * p.per_part, v1 = min(vecs, v0 + p.per_part);
+    const char* base = row - lead * kSize;
+    Sums z;
+    Top list;
+    uint4 next[kAhead];
+    auto fetch = [&](int v) {  // vector v of the row; logits outside it are NaN-free filler
+      if (v >= v1) return make_uint4(0, 0, 0, 0);
+      const int j = v * kVec - lead;
+      if (j >= 0 && j + kVec <= V) return __ldg(reinterpret_cast<const uint4*>(base + (size_t)v * 16));
+      uint32_t w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (LT == FP8IMMA_L_F32) {
+          w[i] = j + i >= 0 && j + i < V ? __ldg(reinterpret_cast<const unsigned*>(base + (size_t)v * 16) + i) : 0u;
+        } else {
+          const unsigned short* q = reinterpret_cast<const unsigned short*>(base + (size_t)v * 16) + 2 * i;
+          const uint32_t lo = j + 2 * i >= 0 && j + 2 * i < V ? __ldg(q) : 0u, hi = j + 2 * i + 1 >= 0 && j + 2 * i + 1 < V ? __ldg(q + 1) : 0u;
+          w[i] = lo | (hi << 16);
+        }
+      }
+      return make_uint4(w[0], w[1], w[2], w[3]);
+    };
+    const int first = v0 + warp * 32 + lane;
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) next[k] = fetch(first + k * kThreads);
+    for (int vb = v0 + warp * 32; vb < v1; vb += kThreads * kAhead) {  // warp-uniform
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        if (vb + k * kThreads >= v1) break;
+        const int v = vb + lane + k * kThreads, j = v * kVec - lead;
+        const uint4 q = next[k];
+        next[k] = fetch(v + kAhead * kThreads);
+        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+        float x[kVec];
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) x[i] = LT == FP8IMMA_L_F32 ? __uint_as_float(w[i]) : to_f32<LT>((w[i / 2] >> (i & 1 ? 16 : 0)) & 0xFFFFu);
+        const bool whole = v < v1 && j >= 0 && j + kVec <= V;
+        if (!whole) {
+#pragma unroll
+          for (int i = 0; i < kVec; ++i)
+            if (v >= v1 || j + i < 0 || j + i >= V) x[i] = -INFINITY;
+        }
+        float big = x[0];
+#pragma unroll
+        for (int i = 1; i < kVec; ++i) big = fmaxf(big, x[i]);
+        if (big * c > z.m + kRaise) z.raise(big * c);
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) z.add(x[i], c);
+        if (top && __any_sync(0xffffffffu, !(big <= list.bar))) {
+#pragma unroll 1
+          for (int i = 0; i < kVec; ++i) {
+            float xi = x[0];
+#pragma unroll
+            for (int e = 1; e < kVec; ++e) xi = i == e ? x[e] : xi;
+            const bool in = v < v1 && j + i >= 0 && j + i < V;
+            list.enter(in ? make_key(xi, j + i) : kNoKey, top, lane);
+          }
+        }
+      }
+    }
+    z.warp_join();
+    if (t != (int)blockIdx.y) __syncthreads();  // the row before has been read from shared memory
+    if (lane == 0) {
+      s_sums[warp][0] = z.m;
+      s_sums[warp][1] = z.l;
+      s_sums[warp][2] = z.s;
+    }
+    if (top) s_list[warp][lane] = list.mine;
+    __syncthreads();
+    if (warp == 0) {
+      z = Sums();
+      for (int w = 0; w < kWarps; ++w) z.join(s_sums[w][0], s_sums[w][1], s_sums[w][2]);
+      if (top)
+        for (int w = 1; w < kWarps; ++w) list.mine = merge(list.mine, s_list[w][lane], lane);
+      if (p.parts == 1) finish<LT>(p, t, z, list, lane);
+      else put_part(p, part, t, z, list, lane);
+    }
+    if (p.parts > 1 && came_last(p.counters + t, p.parts)) {
+      // the warps join every eighth part each, the first warp joins theirs
+      Sums all;
+      Top l;
+      get_parts(p, warp, kWarps, t, all, l, lane);
+      if (lane == 0) {
+        s_sums[warp][0] = all.m;
+        s_sums[warp][1] = all.l;
+        s_sums[warp][2] = all.s;
+      }
+      s_list[warp][lane] = l.mine;
+      __syncthreads();
+      if (warp == 0) {
+        for (int w = 1; w < kWarps; ++w) {
+          all.join(s_sums[w][0], s_sums[w][1], s_sums[w][2]);
+          if (top) l.mine = merge(l.mine, s_list[w][lane], lane);
+        }
+        finish<LT>(p, t, all, l, lane);
+      }
+    }
+  }
+}
+
+// Column-major logits (the GEMM's default output): CTA (part, group of up to 32
+// tokens). Tiles of kTile vocabulary rows go through shared memory, whose rows
+// are padded so that a warp then reads a token's column without conflicts; a
+// warp keeps up to four tokens.
+constexpr int kTile = 256;
+template <int LT>
+__global__ void __launch_bounds__(kThreads) logprobs_col_kernel(const __grid_constant__ LpParams p) {
+  using Word = typename std::conditional<LT == FP8IMMA_L_F32, uint32_t, uint16_t>::type;
+  constexpr int kPitch = LT == FP8IMMA_L_F32 ? 33 : 34, kVec = 16 / sizeof(Word);
+  __shared__ __align__(16) Word s_tile[kTile * kPitch];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int part = blockIdx.x, V = p.a.vocab, top = p.a.top;
+  const float c = p.to_log2;
+  for (int group = blockIdx.y; group < p.groups; group += gridDim.y) {
+    const int t0 = group * 32, n = min(32, p.a.tokens - t0);
+    const int j0 = part * p.per_part, j1 = min(V, j0 + p.per_part);
+    const Word* src = static_cast<const Word*>(p.a.logits) + t0;
+    const bool vec = ((reinterpret_cast<uintptr_t>(src) | (uintptr_t)(p.a.vocab_stride * sizeof(Word)) | (uintptr_t)(n * sizeof(Word))) & 15u) == 0;
+    Sums z[4];
+    Top list[4];
+    for (int jt = j0; jt < j1; jt += kTile) {
+      const int rows = min(kTile, j1 - jt);
+      __syncthreads();  // the tile before has been read
+      if (vec) {
+        const int per = n / kVec;
+#pragma unroll 4
+        for (int x = tid; x < rows * per; x += kThreads) {
+          const int r = x / per, q = x - r * per;
+          const uint4 v = __ldg(reinterpret_cast<const uint4*>(src + (int64_t)(jt + r) * p.a.vocab_stride + q * kVec));
+          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+          uint32_t* dst = reinterpret_cast<uint32_t*>(&s_tile[r * kPitch + q * kVec]);  // even pitch for 16-bit words
+#pragma unroll
+          for (int i = 0; i < 4; ++i) dst[i] = w[i];
+        }
+      } else {
+#pragma unroll 4
+        for (int x = tid; x < rows * n; x += kThreads) {
+          const int r = x / n, q = x - r * n;
+          s_tile[r * kPitch + q] = __ldg(src + (int64_t)(jt + r) * p.a.vocab_stride + q);
+        }
+      }
+      __syncthreads();
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int t = warp + k * kWarps;
+        if (t >= n) break;
+#pragma unroll 1
+        for (int r0 = 0; r0 < rows; r0 += 128) {  // four logits a lane at once
+          float x[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[i] = r0 + i * 32 + lane < rows ? to_f32<LT>(s_tile[(r0 + i * 32 + lane) * kPitch + t]) : -INFINITY;
+          const float big = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+          if (big * c > z[k].m + kRaise) z[k].raise(big * c);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) z[k].add(x[i], c);
+          if (top && __any_sync(0xffffffffu, !(big <= list[k].bar))) {
+#pragma unroll 1
+            for (int i = 0; i < 4; ++i) {
+              const float xi = i == 0 ? x[0] : i == 1 ? x[1] : i == 2 ? x[2] : x[3];
+              const int r = r0 + i * 32 + lane;
+              list[k].enter(r < rows ? make_key(xi, jt + r) : kNoKey, top, lane);
+            }
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int t = warp + k * kWarps;
+      if (t >= n) break;
+      z[k].warp_join();
+      if (p.parts == 1) finish<LT>(p, t0 + t, z[k], list[k], lane);
+      else put_part(p, part, t0 + t, z[k], list[k], lane);
+    }
+    if (p.parts > 1 && came_last(p.counters + group, p.parts)) {
+      for (int t = warp; t < n; t += kWarps) {
+        Sums all;
+        Top l;
+        get_parts(p, 0, 1, t0 + t, all, l, lane);
+        finish<LT>(p, t0 + t, all, l, lane);
+      }
+    }
+  }
+}
+
+template <int LT>
+cudaError_t launch(LpParams& p, cudaStream_t st) {
+  const bool rows = p.a.vocab_stride == 1;
+  const int sms = num_sms_current();
+  const int vec = LT == FP8IMMA_L_F32 ? 4 : 8;
+  // Parts: enough CTAs for two (row-major: four resident) on each SM, but no
+  // part below the logits that make joining it worth while.
+  int units, full;  // units: rows or groups; full: pieces of a row that a part is made of
+  if (rows) {
+    units = p.a.tokens;
+    full = (p.a.vocab + 2 * vec - 2) / vec;
+    const int64_t want = (4ll * sms + units - 1) / units, most = (full + kThreads - 1) / kThreads;
+    p.parts = (int)std::max<int64_t>(1, std::min(want, most));
+    if (units >= 2 * sms) p.parts = 1;
+  } else {
+    units = p.groups = (p.a.tokens + 31) / 32;
+    full = p.a.vocab;
+    const int64_t want = (2ll * sms + units - 1) / units, most = (full + kTile - 1) / kTile;
+    p.parts = (int)std::max<int64_t>(1, std::min(want, most));
+  }
+  p.per_part = (full + p.parts - 1) / p.parts;
+  if (rows) p.per_part = (p.per_part + 31) & ~31;
+  p.parts = (full + p.per_part - 1) / p.per_part;
+  ScopedScratch ctr, work;
+  cudaError_t e = cudaSuccess;
+  if (p.parts > 1) {
+    const size_t at = (size_t)p.parts * p.a.tokens;
+    e = ctr.get((size_t)units * 4, st, kScratchLogprobsSync);
+    if (e == cudaSuccess && ctr.owned) e = cudaMemsetAsync(ctr.ptr, 0, (size_t)units * 4, st);
+    if (e == cudaSuccess) e = work.get(at * (16 + 256), st, kScratchLogprobs);
+    p.counters = static_cast<unsigned int*>(ctr.ptr);
+    p.lists = static_cast<unsigned long long*>(work.ptr);
+    p.sums = reinterpret_cast<float*>(static_cast<char*>(work.ptr) + at * 256);
+  }
+  if (e == cudaSuccess) {
+    cudaLaunchConfig_t lc = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    lc.gridDim = dim3(p.parts, std::min(units, 65535));
+    lc.blockDim = dim3(kThreads);
+    lc.stream = st;
+    lc.attrs = attr;
+    lc.numAttrs = api_pdl() ? 1 : 0;
+    e = rows ? cudaLaunchKernelEx(&lc, logprobs_row_kernel<LT>, p) : cudaLaunchKernelEx(&lc, logprobs_col_kernel<LT>, p);
+  }
+  const cudaError_t e1 = ctr.release(st), e2 = work.release(st);
+  return e != cudaSuccess ? e : e1 != cudaSuccess ? e1 : e2;
+}
+
 }  // namespace
 }  // namespace fp8imma_b200
+
+using namespace fp8imma_b200;
+
+extern "C" int fp8imma_token_logprobs(const fp8imma_logprobs_args* a, void* stream) {
+  FP8IMMA_RANGE("fp8imma_token_logprobs");
+  if (!a) return (int)cudaErrorInvalidValue;
+  if (a->tokens <= 0 || a->vocab <= 0) return (int)cudaErrorInvalidConfiguration;
+  if (!a->logits || !a->token_ids || !a->logprobs || !a->entropy) return (int)cudaErrorInvalidValue;
+  if (a->top < 0 || a->top > FP8IMMA_LOGPROBS_MAX_TOP || a->top > a->vocab) return (int)cudaErrorInvalidValue;
+  if (a->top > 0 && (!a->top_ids || !a->top_logprobs)) return (int)cudaErrorInvalidValue;
+  if (a->l_type < 0 || a->l_type > 2 || !(a->temperature > 0.0f) || !(a->temperature < INFINITY))
+    return (int)cudaErrorInvalidValue;
+  if (a->vocab_stride != 1 && a->token_stride != 1) return (int)cudaErrorInvalidValue;
+  if (a->vocab > 0x7fffff00) return (int)cudaErrorInvalidValue;
+  if (reinterpret_cast<uintptr_t>(a->logits) & (a->l_type == FP8IMMA_L_F32 ? 3u : 1u)) return (int)cudaErrorInvalidValue;
+  LpParams p = {};
+  p.a = *a;
+  p.inv_temp = 1.0f / a->temperature;
+  p.to_log2 = 1.4426950408889634f * p.inv_temp;
+  if (!(p.to_log2 < INFINITY)) return (int)cudaErrorInvalidValue;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (a->l_type == FP8IMMA_L_F16) return (int)launch<FP8IMMA_L_F16>(p, st);
+  if (a->l_type == FP8IMMA_L_BF16) return (int)launch<FP8IMMA_L_BF16>(p, st);
+  return (int)launch<FP8IMMA_L_F32>(p, st);
+}

@@ -117,7 +117,7 @@ __device__ __forceinline__ bool grid_barrier(unsigned int* ctr) {
       if (v >= gridDim.x) break;
       const unsigned long long dt = globaltimer_ns() - t0;
       if (dt > kWaitCheckNs && dt > *(volatile unsigned long long*)&g_fp8imma_wait_limit_ns) {
-        atomicCAS(&g_fp8imma_device_error, 0u, (unsigned int)ERR_WAIT_PEER);
+        atomicCAS(&g_fp8imma_device_error, 0u, (unsigned int)ERR_WAIT_GRID);
         ok = false;
         break;
       }

@@ -22,6 +22,8 @@ enum : unsigned int {
   ERR_WAIT_TMEM_FULL = 3u,
   ERR_WAIT_TMEM_EMPTY = 4u,
   ERR_WAIT_PEER = 5u,  // a peer GPU's gather signal did not arrive
+  ERR_WAIT_GRID = 6u,  // a CTA of a cooperative grid did not arrive at its barrier
+  ERR_BAD_OFFSETS = 7u,  // cu_new does not ascend (no work was done)
 };
 
 constexpr unsigned long long kWaitLimitNs = 2000000000ull;  // 2 s: far beyond any healthy wait
