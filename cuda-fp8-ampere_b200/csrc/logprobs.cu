@@ -6,11 +6,12 @@
 //   l = sum 2^(u - M),  s = sum 2^(u - M) (u - M)
 //   lse = ln2 (M + log2 l),  entropy = ln2 (log2 l - s / l),  lp(t) = z_t - lse
 // and parts join as l = sum l_i 2^(M_i - M), s = sum 2^(M_i - M) (s_i + (M_i - M) l_i).
-// The top logits are a warp's list of 32, one a lane in descending order; a
-// logit enters it only when it exceeds the list's last, which after the first
-// few hundred logits is rare, so the pass pays one comparison for it. Order is
-// by the logit's bits (order-preserving), then by the lower index, so lists
-// and their joins do not depend on which part is read first.
+// The top logits are a warp's list of 32, one a lane in descending order. The
+// pass compares a lane's largest of eight logits with what the list would take;
+// those that reach it go to a buffer in shared memory, and 32 of them at a time
+// are sorted and merged into the list. Order is by the logit's bits
+// (order-preserving), then by the lower index, so lists and their joins do not
+// depend on which part is read first.
 //
 // Bound: the logits are read once. A row is cut into as many parts as fill the
 // GPU (one row of 32000 bf16 logits: latency; thousands of rows: bandwidth);
@@ -29,8 +30,7 @@ namespace {
 
 using namespace fp8imma_dev;
 
-constexpr int kWarps = 8;
-constexpr int kThreads = kWarps * 32;
+constexpr int kColWarps = 8;
 constexpr unsigned long long kNoKey = 0ull;  // below the key of every logit
 
 struct LpParams {
@@ -39,7 +39,7 @@ struct LpParams {
   float inv_temp;
   int parts;              // CTAs a row (row-major) or a group of rows (column-major)
   int per_part;           // logits of a part
-  int groups;             // column-major: 32-row groups
+  int group, groups;      // column-major: tokens of a group, groups
   unsigned int* counters; // per row (group): finished parts; zero between calls
   float* sums;            // [parts, tokens, 4]: M, l, s, -
   unsigned long long* lists;  // [parts, tokens, 32]
@@ -56,6 +56,10 @@ __device__ __forceinline__ unsigned long long make_key(float v, int j) {
   const int k = __float_as_int(v);
   unsigned o = isnan(v) ? 0xffffffffu : k < 0 ? 0x80000000u - (unsigned)(k & 0x7fffffff) : 0x80000000u + (unsigned)k;
   return ((unsigned long long)o << 32) | (unsigned)(0x7fffffff - j);
+}
+__device__ __forceinline__ unsigned order_bits(float v) {  // of a number
+  const unsigned k = __float_as_uint(v);
+  return k >> 31 ? 0x80000000u - (k & 0x7fffffffu) : k | 0x80000000u;
 }
 __device__ __forceinline__ float key_value(unsigned long long key) {
   const unsigned o = (unsigned)(key >> 32);
@@ -128,26 +132,61 @@ __device__ __noinline__ unsigned long long sort_merge(unsigned long long list, u
   return merge(list, key, lane);
 }
 
-// The warp's list and the value below which nothing can enter it.
+// A warp's list.
 struct Top {
-  unsigned long long mine = kNoKey, last = kNoKey;
-  float bar = NAN;  // NaN: everything may enter
-  __device__ __forceinline__ void enter(unsigned long long key, int top, int lane) {  // one key a lane (kNoKey: none)
-    unsigned who = __ballot_sync(0xffffffffu, key > last);
-    if (!who) return;
-    if (__popc(who) > 6) {
-      mine = sort_merge(mine, key, lane);
-    } else {
-      do {
-        const int src = __ffs(who) - 1;
-        insert(mine, __shfl_sync(0xffffffffu, key, src), lane);
-        who &= who - 1;
-      } while (who);
-    }
-    last = __shfl_sync(0xffffffffu, mine, top - 1);
-    bar = last == kNoKey ? NAN : key_value(last);
-  }
+  unsigned long long mine = kNoKey, last = kNoKey;  // the lane's entry, the list's top-th
 };
+// Enters one key a lane (kNoKey: none).
+__device__ __forceinline__ void enter(Top& t, unsigned long long key, int top, int lane) {
+  unsigned who = __ballot_sync(0xffffffffu, key > t.last);
+  if (!who) return;
+  if (__popc(who) > 4) {
+    t.mine = sort_merge(t.mine, key, lane);
+  } else {
+    do {
+      insert(t.mine, __shfl_sync(0xffffffffu, key, __ffs(who) - 1), lane);
+      who &= who - 1;
+    } while (who);
+  }
+  t.last = __shfl_sync(0xffffffffu, t.mine, top - 1);
+}
+// Candidates for a warp's list, gathered in shared memory.
+constexpr int kBuffer = 32 + 256;
+struct Buffer {
+  unsigned long long key[kBuffer];
+  unsigned int count;
+};
+// The smallest value that can still enter: `floor` is a value that the row's
+// top-th logit is known to reach (order bits), which an equal one may share.
+__device__ __forceinline__ float enters_at(const Top& t, unsigned floor) {
+  const unsigned own = t.last == kNoKey ? 0u : (unsigned)(t.last >> 32) + 1u;  // later logits come with higher indexes
+  const unsigned o = max(own, floor);
+  return o == 0u ? -INFINITY : key_value((unsigned long long)o << 32);
+}
+// Sorts the gathered keys into the list; leaves fewer than `keep` of them.
+__device__ __noinline__ Top flush(Top t, Buffer* b, unsigned keep, int top, int lane) {
+  __syncwarp();
+  unsigned n = b->count;
+  while (n >= keep && n > 0) {
+    const unsigned take = min(n, 32u);
+    n -= take;
+    t.mine = sort_merge(t.mine, lane < (int)take ? b->key[n + lane] : kNoKey, lane);
+  }
+  __syncwarp();
+  if (lane == 0) b->count = n;
+  __syncwarp();
+  t.last = __shfl_sync(0xffffffffu, t.mine, top - 1);
+  return t;
+}
+// The value that the top-th largest of the lanes' values reaches (-inf: none).
+__device__ __noinline__ float first_bar(float big, int top, int lane) {
+  unsigned long long key = make_key(big, lane);
+#pragma unroll
+  for (int k = 2; k <= 32; k <<= 1)
+#pragma unroll
+    for (int o = k >> 1; o > 0; o >>= 1) key = step(key, o, !(lane & o) == !(lane & k));
+  return key_value(__shfl_sync(0xffffffffu, key, top - 1));
+}
 
 // What a row's sums give: lp(x) = (x - at) * inv - ln_l.
 struct Norm {
@@ -167,7 +206,7 @@ __device__ __noinline__ Norm careful(int vocab, int n_top, float to_log2, float 
     const float x = in ? load(j0 + lane) : -INFINITY;
     bad |= !(x < INFINITY);
     m = fmaxf(m, x);
-    if (n_top) top.enter(in ? make_key(x, j0 + lane) : kNoKey, n_top, lane);
+    if (n_top) enter(top, in ? make_key(x, j0 + lane) : kNoKey, n_top, lane);
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
@@ -249,85 +288,110 @@ __device__ __forceinline__ void get_parts(const LpParams& p, int first, int stri
   }
 }
 
-// Row-major logits: CTA (part, token); a warp takes every eighth run of 32
-// 16-byte vectors of the part. Rows of any alignment: vectors lie on 16-byte
-// boundaries, the row's first and last may be partial.
-template <int LT>
-__global__ void __launch_bounds__(kThreads, 4) logprobs_row_kernel(const __grid_constant__ LpParams p) {
-  constexpr int kVec = LT == FP8IMMA_L_F32 ? 4 : 8, kSize = LT == FP8IMMA_L_F32 ? 4 : 2, kAhead = 4;
+// N logits of a lane into its sums, and those that may enter the list into
+// the buffer; element i has index j + i * stride where bit i of `valid` is set.
+template <int N>
+__device__ __forceinline__ void take(const float (&x)[N], float c, Sums& z, bool top, float bar, Buffer* buf, int j, int stride, unsigned valid, bool& gathered) {
+  float big = x[0];
+#pragma unroll
+  for (int i = 1; i < N; ++i) big = fmaxf(big, x[i]);
+  if (big * c > z.m + kRaise) z.raise(big * c);
+#pragma unroll
+  for (int i = 0; i < N; ++i) z.add(x[i], c);
+  if (top && big >= bar) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (x[i] >= bar && ((valid >> i) & 1u)) {
+        buf->key[atomicAdd(&buf->count, 1u)] = make_key(x[i], j + i * stride);
+        gathered = true;
+      }
+  }
+}
+
+// Row-major logits: CTA (part, token); the warps take runs of 32 16-byte
+// vectors of the part in turn, four at a time. Rows lie at any alignment:
+// vectors start at 16-byte boundaries, what lies before the first and behind
+// the last whole vector is read one logit a lane. The warps share the value
+// that the row's top logits are known to reach, so that one warp's finds spare
+// the others theirs.
+template <int LT, int kWarps>
+__global__ void __launch_bounds__(kWarps * 32, 32 / kWarps) logprobs_row_kernel(const __grid_constant__ LpParams p) {
+  constexpr int kVec = LT == FP8IMMA_L_F32 ? 4 : 8, kSize = LT == FP8IMMA_L_F32 ? 4 : 2, kAhead = 4, kThreads = kWarps * 32;
+  constexpr uint32_t kNone = LT == FP8IMMA_L_F32 ? 0xFF800000u : LT == FP8IMMA_L_BF16 ? 0xFF80FF80u : 0xFC00FC00u;  // -inf
   __shared__ float s_sums[kWarps][3];
   __shared__ unsigned long long s_list[kWarps][32];
+  __shared__ Buffer s_buf[kWarps];
+  __shared__ unsigned int s_floor;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) s_floor = 0u;
+  if (lane == 0) s_buf[warp].count = 0u;
   pdl_launch_dependents();
   pdl_wait();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  __syncthreads();
   const int part = blockIdx.x, V = p.a.vocab, top = p.a.top;
   const float c = p.to_log2;
+  Buffer* const buf = &s_buf[warp];
   for (int t = blockIdx.y; t < p.a.tokens; t += gridDim.y) {
     const char* row = static_cast<const char*>(p.a.logits) + (int64_t)t * p.a.token_stride * kSize;
-    const int lead = (int)((reinterpret_cast<uintptr_t>(row) & 15u) / kSize);  // logits between a boundary and the row
-    const int vecs = (lead + V + kVec - 1) / kVec;
-    const int v0 = part * p.per_part, v1 = min(vecs, v0 + p.per_part);
-    const char* base = row - lead * kSize;
+    const int lead = min(V, (int)((16u - (reinterpret_cast<uintptr_t>(row) & 15u)) & 15u) / kSize);  // logits before the first whole vector
+    const int vecs = (V - lead) / kVec;
+    const int v0 = min(vecs, part * p.per_part), v1 = part == p.parts - 1 ? vecs : min(vecs, v0 + p.per_part);
+    const uint4* base = reinterpret_cast<const uint4*>(row + lead * kSize);
     Sums z;
     Top list;
-    uint4 next[kAhead];
-    auto fetch = [&](int v) {  // vector v of the row; logits outside it are NaN-free filler
-      if (v >= v1) return make_uint4(0, 0, 0, 0);
-      const int j = v * kVec - lead;
-      if (j >= 0 && j + kVec <= V) return __ldg(reinterpret_cast<const uint4*>(base + (size_t)v * 16));
-      uint32_t w[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (LT == FP8IMMA_L_F32) {
-          w[i] = j + i >= 0 && j + i < V ? __ldg(reinterpret_cast<const unsigned*>(base + (size_t)v * 16) + i) : 0u;
-        } else {
-          const unsigned short* q = reinterpret_cast<const unsigned short*>(base + (size_t)v * 16) + 2 * i;
-          const uint32_t lo = j + 2 * i >= 0 && j + 2 * i < V ? __ldg(q) : 0u, hi = j + 2 * i + 1 >= 0 && j + 2 * i + 1 < V ? __ldg(q + 1) : 0u;
-          w[i] = lo | (hi << 16);
-        }
+    float bar = top ? -INFINITY : INFINITY;
+    bool fresh = true;  // no bar yet
+    auto settle = [&](bool gathered) {
+      if (!__any_sync(0xffffffffu, gathered)) return;
+      __syncwarp();
+      if (buf->count >= 32u) {
+        list = flush(list, buf, 32u, top, lane);
+        if (lane == 0) atomicMax(&s_floor, (unsigned)(list.last >> 32));
       }
-      return make_uint4(w[0], w[1], w[2], w[3]);
     };
-    const int first = v0 + warp * 32 + lane;
-#pragma unroll
-    for (int k = 0; k < kAhead; ++k) next[k] = fetch(first + k * kThreads);
+    auto end = [&](int j) {  // one logit a lane from an end of the row (j < 0: none)
+      float x[1] = {-INFINITY};
+      if (j >= 0) x[0] = LT == FP8IMMA_L_F32 ? __ldg(reinterpret_cast<const float*>(row) + j) : to_f32<LT>(__ldg(reinterpret_cast<const unsigned short*>(row) + j));
+      bool gathered = false;
+      take<1>(x, c, z, top > 0, bar, buf, j, 0, j >= 0, gathered);
+    };
+    // the list takes equal logits in the order of their indexes: the head first, the tail last
+    if (warp == 0 && part == 0) end(lane < lead ? lane : -1);
     for (int vb = v0 + warp * 32; vb < v1; vb += kThreads * kAhead) {  // warp-uniform
+      uint4 q[kAhead];
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        const int v = vb + lane + k * kThreads;
+        q[k] = make_uint4(kNone, kNone, kNone, kNone);
+        if (v < v1) q[k] = __ldg(base + v);
+      }
+      if (top) bar = fmaxf(bar, enters_at(list, *(volatile unsigned int*)&s_floor));
 #pragma unroll
       for (int k = 0; k < kAhead; ++k) {
         if (vb + k * kThreads >= v1) break;
-        const int v = vb + lane + k * kThreads, j = v * kVec - lead;
-        const uint4 q = next[k];
-        next[k] = fetch(v + kAhead * kThreads);
-        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+        const int v = vb + lane + k * kThreads;
+        const uint32_t w[4] = {q[k].x, q[k].y, q[k].z, q[k].w};
         float x[kVec];
 #pragma unroll
         for (int i = 0; i < kVec; ++i) x[i] = LT == FP8IMMA_L_F32 ? __uint_as_float(w[i]) : to_f32<LT>((w[i / 2] >> (i & 1 ? 16 : 0)) & 0xFFFFu);
-        const bool whole = v < v1 && j >= 0 && j + kVec <= V;
-        if (!whole) {
+        if (fresh && top) {  // first vector: what the top-th of the lanes' largest reaches
+          float big = x[0];
 #pragma unroll
-          for (int i = 0; i < kVec; ++i)
-            if (v >= v1 || j + i < 0 || j + i >= V) x[i] = -INFINITY;
+          for (int i = 1; i < kVec; ++i) big = fmaxf(big, x[i]);
+          bar = fmaxf(bar, first_bar(big, top, lane));
+          fresh = false;
         }
-        float big = x[0];
-#pragma unroll
-        for (int i = 1; i < kVec; ++i) big = fmaxf(big, x[i]);
-        if (big * c > z.m + kRaise) z.raise(big * c);
-#pragma unroll
-        for (int i = 0; i < kVec; ++i) z.add(x[i], c);
-        if (top && __any_sync(0xffffffffu, !(big <= list.bar))) {
-#pragma unroll 1
-          for (int i = 0; i < kVec; ++i) {
-            float xi = x[0];
-#pragma unroll
-            for (int e = 1; e < kVec; ++e) xi = i == e ? x[e] : xi;
-            const bool in = v < v1 && j + i >= 0 && j + i < V;
-            list.enter(in ? make_key(xi, j + i) : kNoKey, top, lane);
-          }
-        }
+        bool gathered = false;
+        take<kVec>(x, c, z, top > 0, bar, buf, lead + v * kVec, 1, v < v1 ? 0xFFu : 0u, gathered);
+        if (top) settle(gathered);
       }
     }
+    if (warp == 0 && part == p.parts - 1) {
+      const int j = lead + vecs * kVec + lane;
+      end(j < V ? j : -1);
+    }
+    if (top) list = flush(list, buf, 1u, top, lane);
     z.warp_join();
-    if (t != (int)blockIdx.y) __syncthreads();  // the row before has been read from shared memory
     if (lane == 0) {
       s_sums[warp][0] = z.m;
       s_sums[warp][1] = z.l;
@@ -335,6 +399,7 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_row_kernel(const __grid_
     }
     if (top) s_list[warp][lane] = list.mine;
     __syncthreads();
+    if (threadIdx.x == 0) s_floor = 0u;
     if (warp == 0) {
       z = Sums();
       for (int w = 0; w < kWarps; ++w) z.join(s_sums[w][0], s_sums[w][1], s_sums[w][2]);
@@ -344,7 +409,7 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_row_kernel(const __grid_
       else put_part(p, part, t, z, list, lane);
     }
     if (p.parts > 1 && came_last(p.counters + t, p.parts)) {
-      // the warps join every eighth part each, the first warp joins theirs
+      // the warps join every so many parts each, the first warp joins theirs
       Sums all;
       Top l;
       get_parts(p, warp, kWarps, t, all, l, lane);
@@ -363,47 +428,67 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_row_kernel(const __grid_
         finish<LT>(p, t, all, l, lane);
       }
     }
+    __syncthreads();  // shared memory is free for the next row
   }
 }
 
-// Column-major logits (the GEMM's default output): CTA (part, group of up to 32
-// tokens). Tiles of kTile vocabulary rows go through shared memory, whose rows
-// are padded so that a warp then reads a token's column without conflicts; a
-// warp keeps up to four tokens.
-constexpr int kTile = 256;
+// Column-major logits (the GEMM's default output): CTA (part, group of up to
+// p.group tokens). Tiles of kTile vocabulary rows go through shared memory,
+// whose rows are padded so that a warp then reads a token's column without
+// conflicts; the next tile is under way meanwhile. A warp keeps up to four
+// tokens.
+constexpr int kTile = 256;  // 128 of fp32
 template <int LT>
-__global__ void __launch_bounds__(kThreads) logprobs_col_kernel(const __grid_constant__ LpParams p) {
+__global__ void __launch_bounds__(kColWarps * 32) logprobs_col_kernel(const __grid_constant__ LpParams p) {
   using Word = typename std::conditional<LT == FP8IMMA_L_F32, uint32_t, uint16_t>::type;
-  constexpr int kPitch = LT == FP8IMMA_L_F32 ? 33 : 34, kVec = 16 / sizeof(Word);
-  __shared__ __align__(16) Word s_tile[kTile * kPitch];
+  constexpr int kWarps = kColWarps, kThreads = kColWarps * 32, kPitch = LT == FP8IMMA_L_F32 ? 33 : 34, kVec = 16 / sizeof(Word);
+  constexpr int kRows = LT == FP8IMMA_L_F32 ? kTile / 2 : kTile, kEach = kRows / 32;  // rows of a tile, of a lane
+  constexpr int kAhead = kRows * 32 / kVec / kThreads;  // 16-byte pieces of a tile a thread
+  __shared__ __align__(16) Word s_tile[kRows * kPitch];
+  __shared__ Buffer s_buf[kWarps];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (lane == 0) s_buf[warp].count = 0u;
   pdl_launch_dependents();
   pdl_wait();
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int part = blockIdx.x, V = p.a.vocab, top = p.a.top;
   const float c = p.to_log2;
+  Buffer* const buf = &s_buf[warp];
   for (int group = blockIdx.y; group < p.groups; group += gridDim.y) {
-    const int t0 = group * 32, n = min(32, p.a.tokens - t0);
+    const int t0 = group * p.group, n = min(p.group, p.a.tokens - t0);
     const int j0 = part * p.per_part, j1 = min(V, j0 + p.per_part);
     const Word* src = static_cast<const Word*>(p.a.logits) + t0;
     const bool vec = ((reinterpret_cast<uintptr_t>(src) | (uintptr_t)(p.a.vocab_stride * sizeof(Word)) | (uintptr_t)(n * sizeof(Word))) & 15u) == 0;
+    const int per = n / kVec;
     Sums z[4];
     Top list[4];
-    for (int jt = j0; jt < j1; jt += kTile) {
-      const int rows = min(kTile, j1 - jt);
+    uint4 next[kAhead];
+    auto fetch = [&](int jt) {
+      const int rows = min(kRows, j1 - jt);
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        const int x = tid + k * kThreads, r = x / per, q = x - r * per;
+        if (x < rows * per) next[k] = __ldg(reinterpret_cast<const uint4*>(src + (int64_t)(jt + r) * p.a.vocab_stride + q * kVec));
+      }
+    };
+    if (vec && j0 < j1) fetch(j0);
+    for (int jt = j0; jt < j1; jt += kRows) {
+      const int rows = min(kRows, j1 - jt);
       __syncthreads();  // the tile before has been read
       if (vec) {
-        const int per = n / kVec;
-#pragma unroll 4
-        for (int x = tid; x < rows * per; x += kThreads) {
-          const int r = x / per, q = x - r * per;
-          const uint4 v = __ldg(reinterpret_cast<const uint4*>(src + (int64_t)(jt + r) * p.a.vocab_stride + q * kVec));
-          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-          uint32_t* dst = reinterpret_cast<uint32_t*>(&s_tile[r * kPitch + q * kVec]);  // even pitch for 16-bit words
 #pragma unroll
-          for (int i = 0; i < 4; ++i) dst[i] = w[i];
+        for (int k = 0; k < kAhead; ++k) {
+          const int x = tid + k * kThreads, r = x / per, q = x - r * per;
+          if (x < rows * per) {
+            uint32_t* dst = reinterpret_cast<uint32_t*>(&s_tile[r * kPitch + q * kVec]);  // even pitch for 16-bit words
+            dst[0] = next[k].x;
+            dst[1] = next[k].y;
+            dst[2] = next[k].z;
+            dst[3] = next[k].w;
+          }
         }
+        if (jt + kRows < j1) fetch(jt + kRows);
       } else {
-#pragma unroll 4
+#pragma unroll 8
         for (int x = tid; x < rows * n; x += kThreads) {
           const int r = x / n, q = x - r * n;
           s_tile[r * kPitch + q] = __ldg(src + (int64_t)(jt + r) * p.a.vocab_stride + q);
@@ -414,24 +499,25 @@ __global__ void __launch_bounds__(kThreads) logprobs_col_kernel(const __grid_con
       for (int k = 0; k < 4; ++k) {
         const int t = warp + k * kWarps;
         if (t >= n) break;
-#pragma unroll 1
-        for (int r0 = 0; r0 < rows; r0 += 128) {  // four logits a lane at once
-          float x[4];
+        float x[kEach];  // the lane's logits of the tile
 #pragma unroll
-          for (int i = 0; i < 4; ++i) x[i] = r0 + i * 32 + lane < rows ? to_f32<LT>(s_tile[(r0 + i * 32 + lane) * kPitch + t]) : -INFINITY;
-          const float big = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-          if (big * c > z[k].m + kRaise) z[k].raise(big * c);
+        for (int i = 0; i < kEach; ++i) x[i] = i * 32 + lane < rows ? to_f32<LT>(s_tile[(i * 32 + lane) * kPitch + t]) : -INFINITY;
+        float bar = INFINITY;
+        if (top) {
+          bar = enters_at(list[k], 0u);
+          if (jt == j0) {
+            float big = x[0];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) z[k].add(x[i], c);
-          if (top && __any_sync(0xffffffffu, !(big <= list[k].bar))) {
-#pragma unroll 1
-            for (int i = 0; i < 4; ++i) {
-              const float xi = i == 0 ? x[0] : i == 1 ? x[1] : i == 2 ? x[2] : x[3];
-              const int r = r0 + i * 32 + lane;
-              list[k].enter(r < rows ? make_key(xi, jt + r) : kNoKey, top, lane);
-            }
+            for (int i = 1; i < kEach; ++i) big = fmaxf(big, x[i]);
+            bar = fmaxf(bar, first_bar(big, top, lane));
           }
         }
+        unsigned valid = 0u;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) valid |= (unsigned)(i * 32 + lane < rows) << i;
+        bool gathered = false;
+        take<kEach>(x, c, z[k], top > 0, bar, buf, jt + lane, 32, valid, gathered);
+        if (top && __any_sync(0xffffffffu, gathered)) list[k] = flush(list[k], buf, 1u, top, lane);
       }
     }
 #pragma unroll
@@ -460,22 +546,27 @@ cudaError_t launch(LpParams& p, cudaStream_t st) {
   const int vec = LT == FP8IMMA_L_F32 ? 4 : 8;
   // Parts: enough CTAs for two (row-major: four resident) on each SM, but no
   // part below the logits that make joining it worth while.
+  int warps = 8;  // of a row's CTA
   int units, full;  // units: rows or groups; full: pieces of a row that a part is made of
   if (rows) {
     units = p.a.tokens;
-    full = (p.a.vocab + 2 * vec - 2) / vec;
-    const int64_t want = (4ll * sms + units - 1) / units, most = (full + kThreads - 1) / kThreads;
+    full = (p.a.vocab + vec - 1) / vec;
+    const int64_t want = (4ll * sms + units - 1) / units, most = (full + 255) / 256;
     p.parts = (int)std::max<int64_t>(1, std::min(want, most));
     if (units >= 2 * sms) p.parts = 1;
+    if (units >= 8 * sms) warps = 2;
   } else {
-    units = p.groups = (p.a.tokens + 31) / 32;
+    // groups of 8 tokens, one a warp, while that leaves a CTA a fair part of the
+    // columns; of 32 beyond, for whole sectors of the logits
+    p.group = p.a.tokens <= 64 ? 8 : 32;
+    units = p.groups = (p.a.tokens + p.group - 1) / p.group;
     full = p.a.vocab;
     const int64_t want = (2ll * sms + units - 1) / units, most = (full + kTile - 1) / kTile;
-    p.parts = (int)std::max<int64_t>(1, std::min(want, most));
+    p.parts = (int)std::max<int64_t>(1, std::min<int64_t>(std::min(want, most), 74));
   }
   p.per_part = (full + p.parts - 1) / p.parts;
   if (rows) p.per_part = (p.per_part + 31) & ~31;
-  p.parts = (full + p.per_part - 1) / p.per_part;
+  p.parts = (full + p.per_part - 1) / p.per_part;  // the last part of a row takes what is left of it
   ScopedScratch ctr, work;
   cudaError_t e = cudaSuccess;
   if (p.parts > 1) {
@@ -493,11 +584,13 @@ cudaError_t launch(LpParams& p, cudaStream_t st) {
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     lc.gridDim = dim3(p.parts, std::min(units, 65535));
-    lc.blockDim = dim3(kThreads);
+    lc.blockDim = dim3(rows ? 32 * warps : kColWarps * 32);
     lc.stream = st;
     lc.attrs = attr;
     lc.numAttrs = api_pdl() ? 1 : 0;
-    e = rows ? cudaLaunchKernelEx(&lc, logprobs_row_kernel<LT>, p) : cudaLaunchKernelEx(&lc, logprobs_col_kernel<LT>, p);
+    e = !rows        ? cudaLaunchKernelEx(&lc, logprobs_col_kernel<LT>, p)
+        : warps == 8 ? cudaLaunchKernelEx(&lc, logprobs_row_kernel<LT, 8>, p)
+                     : cudaLaunchKernelEx(&lc, logprobs_row_kernel<LT, 2>, p);
   }
   const cudaError_t e1 = ctr.release(st), e2 = work.release(st);
   return e != cudaSuccess ? e : e1 != cudaSuccess ? e1 : e2;
