@@ -37,6 +37,7 @@ struct LpParams {
   fp8imma_logprobs_args a;
   float to_log2;          // log2(e) / temperature
   float inv_temp;
+  int flush_at;           // gathered logits that are worth a sort: with a longer list a sort raises its bar less
   int parts;              // CTAs a row (row-major) or a group of rows (column-major)
   int per_part;           // logits of a part
   int group, groups;      // column-major: tokens of a group, groups
@@ -124,10 +125,11 @@ __device__ __forceinline__ unsigned long long merge(unsigned long long a, unsign
   for (int o = 16; o > 0; o >>= 1) v = step(v, o, !(lane & o));
   return v;
 }
-__device__ __noinline__ unsigned long long sort_merge(unsigned long long list, unsigned long long key, int lane) {
-#pragma unroll
-  for (int k = 2; k <= 32; k <<= 1)
-#pragma unroll
+// n keys of the first lanes (kNoKey in the others) sorted and merged into a list.
+__device__ __noinline__ unsigned long long sort_merge(unsigned long long list, unsigned long long key, int n, int lane) {
+#pragma unroll 1
+  for (int k = 2; k < 2 * n; k <<= 1)
+#pragma unroll 1
     for (int o = k >> 1; o > 0; o >>= 1) key = step(key, o, !(lane & o) == !(lane & k));
   return merge(list, key, lane);
 }
@@ -141,7 +143,7 @@ __device__ __forceinline__ void enter(Top& t, unsigned long long key, int top, i
   unsigned who = __ballot_sync(0xffffffffu, key > t.last);
   if (!who) return;
   if (__popc(who) > 4) {
-    t.mine = sort_merge(t.mine, key, lane);
+    t.mine = sort_merge(t.mine, key, 32, lane);
   } else {
     do {
       insert(t.mine, __shfl_sync(0xffffffffu, key, __ffs(who) - 1), lane);
@@ -150,12 +152,10 @@ __device__ __forceinline__ void enter(Top& t, unsigned long long key, int top, i
   }
   t.last = __shfl_sync(0xffffffffu, t.mine, top - 1);
 }
-// Candidates for a warp's list, gathered in shared memory.
+// Candidates for a warp's list, gathered in shared memory: up to 31 left over
+// and 8 a lane more.
 constexpr int kBuffer = 32 + 256;
-struct Buffer {
-  unsigned long long key[kBuffer];
-  unsigned int count;
-};
+
 // The smallest value that can still enter: `floor` is a value that the row's
 // top-th logit is known to reach (order bits), which an equal one may share.
 __device__ __forceinline__ float enters_at(const Top& t, unsigned floor) {
@@ -163,29 +163,25 @@ __device__ __forceinline__ float enters_at(const Top& t, unsigned floor) {
   const unsigned o = max(own, floor);
   return o == 0u ? -INFINITY : key_value((unsigned long long)o << 32);
 }
-// Sorts the gathered keys into the list; leaves fewer than `keep` of them.
-__device__ __noinline__ Top flush(Top t, Buffer* b, unsigned keep, int top, int lane) {
+// Sorts the n gathered keys into the list.
+__device__ __noinline__ Top flush(Top t, const unsigned long long* buf, int n, int top, int lane) {
   __syncwarp();
-  unsigned n = b->count;
-  while (n >= keep && n > 0) {
-    const unsigned take = min(n, 32u);
-    n -= take;
-    t.mine = sort_merge(t.mine, lane < (int)take ? b->key[n + lane] : kNoKey, lane);
-  }
-  __syncwarp();
-  if (lane == 0) b->count = n;
+  for (; n > 0; n -= 32) t.mine = sort_merge(t.mine, lane < n ? buf[n - 1 - lane] : kNoKey, min(n, 32), lane);
   __syncwarp();
   t.last = __shfl_sync(0xffffffffu, t.mine, top - 1);
   return t;
 }
 // The value that the top-th largest of the lanes' values reaches (-inf: none).
 __device__ __noinline__ float first_bar(float big, int top, int lane) {
-  unsigned long long key = make_key(big, lane);
-#pragma unroll
+  unsigned v = order_bits(big);
+#pragma unroll 1
   for (int k = 2; k <= 32; k <<= 1)
-#pragma unroll
-    for (int o = k >> 1; o > 0; o >>= 1) key = step(key, o, !(lane & o) == !(lane & k));
-  return key_value(__shfl_sync(0xffffffffu, key, top - 1));
+#pragma unroll 1
+    for (int o = k >> 1; o > 0; o >>= 1) {
+      const unsigned w = __shfl_xor_sync(0xffffffffu, v, o);
+      v = !(lane & o) == !(lane & k) ? max(v, w) : min(v, w);
+    }
+  return key_value((unsigned long long)__shfl_sync(0xffffffffu, v, top - 1) << 32);
 }
 
 // What a row's sums give: lp(x) = (x - at) * inv - ln_l.
@@ -227,9 +223,13 @@ __device__ __noinline__ Norm careful(int vocab, int n_top, float to_log2, float 
   return n;
 }
 
-// A row's results from its joined sums and list; one warp.
+// A row's results from its joined sums (those of lane 0) and list; one warp.
 template <int LT>
-__device__ __forceinline__ void finish(const LpParams& p, int t, const Sums& z, const Top& top, int lane) {
+__device__ __forceinline__ void finish(const LpParams& p, int t, Sums z, const Top& top, int lane) {
+  // the same in all lanes: the branch below is taken by the warp as one
+  z.m = __shfl_sync(0xffffffffu, z.m, 0);
+  z.l = __shfl_sync(0xffffffffu, z.l, 0);
+  z.s = __shfl_sync(0xffffffffu, z.s, 0);
   const int64_t row = (int64_t)t * p.a.token_stride;
   const void* logits = p.a.logits;
   const int64_t stride = p.a.vocab_stride;
@@ -288,23 +288,104 @@ __device__ __forceinline__ void get_parts(const LpParams& p, int first, int stri
   }
 }
 
-// N logits of a lane into its sums, and those that may enter the list into
-// the buffer; element i has index j + i * stride where bit i of `valid` is set.
-template <int N>
-__device__ __forceinline__ void take(const float (&x)[N], float c, Sums& z, bool top, float bar, Buffer* buf, int j, int stride, unsigned valid, bool& gathered) {
-  float big = x[0];
+// Largest logit of a 16-byte vector's 32-bit words, packed.
+template <int LT>
+__device__ __forceinline__ uint32_t max_words(uint32_t a, uint32_t b) {
+  if (LT == FP8IMMA_L_F32) return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+  uint32_t r;
+  if (LT == FP8IMMA_L_F16) asm("max.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  else asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+template <int LT>
+__device__ __forceinline__ float max_of_word(uint32_t a) {
+  if (LT == FP8IMMA_L_F32) return __uint_as_float(a);
+  return fmaxf(to_f32<LT>(a & 0xFFFFu), to_f32<LT>(a >> 16));
+}
+template <int LT>
+__device__ __forceinline__ float logit_of(const uint4& q, int i) {  // i: a constant
+  const uint32_t w = LT == FP8IMMA_L_F32 ? (i == 0 ? q.x : i == 1 ? q.y : i == 2 ? q.z : q.w) : (i < 2 ? q.x : i < 4 ? q.y : i < 6 ? q.z : q.w);
+  return LT == FP8IMMA_L_F32 ? __uint_as_float(w) : to_f32<LT>(i & 1 ? w >> 16 : w & 0xFFFFu);
+}
+// One logit a lane into the buffer where it may enter the list (`in`); the
+// buffer's new length, the same in all lanes like the old one.
+__device__ __forceinline__ int put(float x, bool in, unsigned long long* buf, int n, int j, int lane) {
+  const unsigned m = __ballot_sync(0xffffffffu, in);
+  if (m) {
+    if (in) buf[n + __popc(m & ((1u << lane) - 1u))] = make_key(x, j);
+    n += __popc(m);
+  }
+  return n;
+}
+// The same for a vector's logits; the lane's first has index j.
+template <int LT>
+__device__ __noinline__ int gather(uint4 q, float bar, bool in, unsigned long long* buf, int n, int j, int lane) {
 #pragma unroll
-  for (int i = 1; i < N; ++i) big = fmaxf(big, x[i]);
-  if (big * c > z.m + kRaise) z.raise(big * c);
+  for (int i = 0; i < (LT == FP8IMMA_L_F32 ? 4 : 8); ++i) {
+    const float x = logit_of<LT>(q, i);
+    n = put(x, in && x >= bar, buf, n, j + i, lane);
+  }
+  return n;
+}
+template <int LT>
+__device__ __forceinline__ float max_of(const uint4& q) {
+  return max_of_word<LT>(max_words<LT>(max_words<LT>(q.x, q.y), max_words<LT>(q.z, q.w)));
+}
+// The lane's logits of four vectors that may enter the list, into the buffer,
+// as few lanes have one: each finds its place by an atomic count, and what does
+// not fit is counted only (the caller then goes vector by vector).
+struct Quad {
+  uint4 q[4];
+};
+template <int LT>
+__device__ __noinline__ void gather(Quad v, float bar, unsigned long long* buf, unsigned int* count, int j, int stride, int valid) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) z.add(x[i], c);
-  if (top && big >= bar) {
+  for (int k = 0; k < 4; ++k) {
+    if (k >= valid || !(max_of<LT>(v.q[k]) >= bar)) continue;
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (x[i] >= bar && ((valid >> i) & 1u)) {
-        buf->key[atomicAdd(&buf->count, 1u)] = make_key(x[i], j + i * stride);
-        gathered = true;
+    for (int i = 0; i < (LT == FP8IMMA_L_F32 ? 4 : 8); ++i) {
+      const float x = logit_of<LT>(v.q[k], i);
+      if (x >= bar) {
+        const unsigned at = atomicAdd(count, 1u);
+        if (at < kBuffer) buf[at] = make_key(x, j + k * stride + i);
       }
+    }
+  }
+}
+
+// A CTA's sums and lists (one a warp) joined in the first warp, the sums in its
+// lane 0: pairs of warps in a fixed order.
+template <int kWarps>
+__device__ __forceinline__ void join_warps(Sums& z, Top& list, float (*sums)[3], unsigned long long (*lists)[32], bool top, int warp, int lane) {
+  if (lane == 0) {
+    sums[warp][0] = z.m;
+    sums[warp][1] = z.l;
+    sums[warp][2] = z.s;
+  }
+  if (top) lists[warp][lane] = list.mine;
+  __syncthreads();
+  if (top) {
+#pragma unroll 1
+    for (int half = kWarps / 2; half > 0; half >>= 1) {
+      if (warp < half) {
+        list.mine = merge(list.mine, lists[warp + half][lane], lane);
+        if (half > 1) lists[warp][lane] = list.mine;
+      }
+      if (half > 1) __syncthreads();
+    }
+  }
+  if (warp == 0) {
+    z = Sums();
+    if (lane < kWarps) {
+      z.m = sums[lane][0];
+      z.l = sums[lane][1];
+      z.s = sums[lane][2];
+    }
+#pragma unroll
+    for (int o = kWarps / 2; o > 0; o >>= 1) {
+      const float m2 = __shfl_xor_sync(0xffffffffu, z.m, o), l2 = __shfl_xor_sync(0xffffffffu, z.l, o), s2 = __shfl_xor_sync(0xffffffffu, z.s, o);
+      z.join(m2, l2, s2);
+    }
   }
 }
 
@@ -320,17 +401,16 @@ __global__ void __launch_bounds__(kWarps * 32, 32 / kWarps) logprobs_row_kernel(
   constexpr uint32_t kNone = LT == FP8IMMA_L_F32 ? 0xFF800000u : LT == FP8IMMA_L_BF16 ? 0xFF80FF80u : 0xFC00FC00u;  // -inf
   __shared__ float s_sums[kWarps][3];
   __shared__ unsigned long long s_list[kWarps][32];
-  __shared__ Buffer s_buf[kWarps];
-  __shared__ unsigned int s_floor;
+  __shared__ unsigned long long s_buf[kWarps][kBuffer];
+  __shared__ unsigned int s_floor, s_count[kWarps];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) s_floor = 0u;
-  if (lane == 0) s_buf[warp].count = 0u;
   pdl_launch_dependents();
   pdl_wait();
   __syncthreads();
   const int part = blockIdx.x, V = p.a.vocab, top = p.a.top;
   const float c = p.to_log2;
-  Buffer* const buf = &s_buf[warp];
+  unsigned long long* const buf = s_buf[warp];
   for (int t = blockIdx.y; t < p.a.tokens; t += gridDim.y) {
     const char* row = static_cast<const char*>(p.a.logits) + (int64_t)t * p.a.token_stride * kSize;
     const int lead = min(V, (int)((16u - (reinterpret_cast<uintptr_t>(row) & 15u)) & 15u) / kSize);  // logits before the first whole vector
@@ -341,92 +421,89 @@ __global__ void __launch_bounds__(kWarps * 32, 32 / kWarps) logprobs_row_kernel(
     Top list;
     float bar = top ? -INFINITY : INFINITY;
     bool fresh = true;  // no bar yet
-    auto settle = [&](bool gathered) {
-      if (!__any_sync(0xffffffffu, gathered)) return;
-      __syncwarp();
-      if (buf->count >= 32u) {
-        list = flush(list, buf, 32u, top, lane);
-        if (lane == 0) atomicMax(&s_floor, (unsigned)(list.last >> 32));
-      }
-    };
+    int n = 0;          // gathered
     auto end = [&](int j) {  // one logit a lane from an end of the row (j < 0: none)
-      float x[1] = {-INFINITY};
-      if (j >= 0) x[0] = LT == FP8IMMA_L_F32 ? __ldg(reinterpret_cast<const float*>(row) + j) : to_f32<LT>(__ldg(reinterpret_cast<const unsigned short*>(row) + j));
-      bool gathered = false;
-      take<1>(x, c, z, top > 0, bar, buf, j, 0, j >= 0, gathered);
+      float x = -INFINITY;
+      if (j >= 0) x = LT == FP8IMMA_L_F32 ? __ldg(reinterpret_cast<const float*>(row) + j) : to_f32<LT>(__ldg(reinterpret_cast<const unsigned short*>(row) + j));
+      if (x * c > z.m + kRaise) z.raise(x * c);
+      z.add(x, c);
+      if (top) n = put(x, j >= 0 && x >= bar, buf, n, j, lane);
     };
     // the list takes equal logits in the order of their indexes: the head first, the tail last
     if (warp == 0 && part == 0) end(lane < lead ? lane : -1);
+#pragma unroll 1
     for (int vb = v0 + warp * 32; vb < v1; vb += kThreads * kAhead) {  // warp-uniform
-      uint4 q[kAhead];
+      Quad quad;
+      uint4 (&q)[kAhead] = quad.q;
 #pragma unroll
       for (int k = 0; k < kAhead; ++k) {
         const int v = vb + lane + k * kThreads;
         q[k] = make_uint4(kNone, kNone, kNone, kNone);
         if (v < v1) q[k] = __ldg(base + v);
       }
-      if (top) bar = fmaxf(bar, enters_at(list, *(volatile unsigned int*)&s_floor));
+      uint32_t w = kNone;
 #pragma unroll
-      for (int k = 0; k < kAhead; ++k) {
-        if (vb + k * kThreads >= v1) break;
-        const int v = vb + lane + k * kThreads;
-        const uint32_t w[4] = {q[k].x, q[k].y, q[k].z, q[k].w};
-        float x[kVec];
+      for (int k = 0; k < kAhead; ++k) w = max_words<LT>(w, max_words<LT>(max_words<LT>(q[k].x, q[k].y), max_words<LT>(q[k].z, q[k].w)));
+      const float big = max_of_word<LT>(w);
+      if (top) {
+        if (fresh) bar = fmaxf(bar, first_bar(big, top, lane));  // what the top-th of the lanes' largest reaches
+        else if (kWarps > 1) bar = fmaxf(bar, enters_at(Top(), *(volatile unsigned int*)&s_floor));
+        fresh = false;
+      }
+      if (big * c > z.m + kRaise) z.raise(big * c);
 #pragma unroll
-        for (int i = 0; i < kVec; ++i) x[i] = LT == FP8IMMA_L_F32 ? __uint_as_float(w[i]) : to_f32<LT>((w[i / 2] >> (i & 1 ? 16 : 0)) & 0xFFFFu);
-        if (fresh && top) {  // first vector: what the top-th of the lanes' largest reaches
-          float big = x[0];
+      for (int k = 0; k < kAhead; ++k)
+        if (k == 0 || vb + k * kThreads < v1) {
 #pragma unroll
-          for (int i = 1; i < kVec; ++i) big = fmaxf(big, x[i]);
-          bar = fmaxf(bar, first_bar(big, top, lane));
-          fresh = false;
+          for (int i = 0; i < kVec; ++i) z.add(logit_of<LT>(q[k], i), c);
         }
-        bool gathered = false;
-        take<kVec>(x, c, z, top > 0, bar, buf, lead + v * kVec, 1, v < v1 ? 0xFFu : 0u, gathered);
-        if (top) settle(gathered);
+      if (top && __any_sync(0xffffffffu, big >= bar)) {
+        if (lane == 0) s_count[warp] = n;
+        __syncwarp();
+        if (big >= bar) gather<LT>(quad, bar, buf, &s_count[warp], lead + (vb + lane) * kVec, kThreads * kVec, (v1 - vb - lane + kThreads - 1) / kThreads);
+        __syncwarp();
+        const int found = *(volatile unsigned int*)&s_count[warp];
+        bool flushed = false;
+        if (found <= kBuffer) {
+          n = found;
+          flushed = n >= p.flush_at;
+          if (flushed) list = flush(list, buf, n, top, lane);
+        } else {  // equal logits everywhere, or a row that rises
+#pragma unroll 1
+          for (int k = 0; k < kAhead; ++k) {
+            const int v = vb + lane + k * kThreads;
+            const uint4 qk = k == 0 ? q[0] : k == 1 ? q[1] : k == 2 ? q[2] : q[3];
+            n = gather<LT>(qk, bar, v < v1, buf, n, lead + v * kVec, lane);
+            list = flush(list, buf, n, top, lane);
+            n = 0;
+          }
+          flushed = true;
+        }
+        if (flushed) {
+          n = 0;
+          bar = fmaxf(bar, enters_at(list, 0u));
+          if (kWarps > 1 && lane == 0) atomicMax(&s_floor, (unsigned)(list.last >> 32));
+        }
       }
     }
     if (warp == 0 && part == p.parts - 1) {
       const int j = lead + vecs * kVec + lane;
       end(j < V ? j : -1);
     }
-    if (top) list = flush(list, buf, 1u, top, lane);
+    if (top) list = flush(list, buf, n, top, lane);
     z.warp_join();
-    if (lane == 0) {
-      s_sums[warp][0] = z.m;
-      s_sums[warp][1] = z.l;
-      s_sums[warp][2] = z.s;
-    }
-    if (top) s_list[warp][lane] = list.mine;
-    __syncthreads();
+    join_warps<kWarps>(z, list, s_sums, s_list, top > 0, warp, lane);
     if (threadIdx.x == 0) s_floor = 0u;
     if (warp == 0) {
-      z = Sums();
-      for (int w = 0; w < kWarps; ++w) z.join(s_sums[w][0], s_sums[w][1], s_sums[w][2]);
-      if (top)
-        for (int w = 1; w < kWarps; ++w) list.mine = merge(list.mine, s_list[w][lane], lane);
       if (p.parts == 1) finish<LT>(p, t, z, list, lane);
       else put_part(p, part, t, z, list, lane);
     }
-    if (p.parts > 1 && came_last(p.counters + t, p.parts)) {
-      // the warps join every so many parts each, the first warp joins theirs
+    if (p.parts > 1 && came_last(p.counters + t, p.parts)) {  // the warps join every so many parts each, then theirs
       Sums all;
       Top l;
       get_parts(p, warp, kWarps, t, all, l, lane);
-      if (lane == 0) {
-        s_sums[warp][0] = all.m;
-        s_sums[warp][1] = all.l;
-        s_sums[warp][2] = all.s;
-      }
-      s_list[warp][lane] = l.mine;
-      __syncthreads();
-      if (warp == 0) {
-        for (int w = 1; w < kWarps; ++w) {
-          all.join(s_sums[w][0], s_sums[w][1], s_sums[w][2]);
-          if (top) l.mine = merge(l.mine, s_list[w][lane], lane);
-        }
-        finish<LT>(p, t, all, l, lane);
-      }
+      join_warps<kWarps>(all, l, s_sums, s_list, top > 0, warp, lane);
+      if (warp == 0) finish<LT>(p, t, all, l, lane);
     }
     __syncthreads();  // shared memory is free for the next row
   }
@@ -435,32 +512,31 @@ __global__ void __launch_bounds__(kWarps * 32, 32 / kWarps) logprobs_row_kernel(
 // Column-major logits (the GEMM's default output): CTA (part, group of up to
 // p.group tokens). Tiles of kTile vocabulary rows go through shared memory,
 // whose rows are padded so that a warp then reads a token's column without
-// conflicts; the next tile is under way meanwhile. A warp keeps up to four
+// conflicts; the next tile is under way meanwhile. A warp keeps up to two
 // tokens.
 constexpr int kTile = 256;  // 128 of fp32
 template <int LT>
-__global__ void __launch_bounds__(kColWarps * 32) logprobs_col_kernel(const __grid_constant__ LpParams p) {
+__global__ void __launch_bounds__(kColWarps * 32, 4) logprobs_col_kernel(const __grid_constant__ LpParams p) {
   using Word = typename std::conditional<LT == FP8IMMA_L_F32, uint32_t, uint16_t>::type;
-  constexpr int kWarps = kColWarps, kThreads = kColWarps * 32, kPitch = LT == FP8IMMA_L_F32 ? 33 : 34, kVec = 16 / sizeof(Word);
+  constexpr int kWarps = kColWarps, kThreads = kColWarps * 32, kPitch = LT == FP8IMMA_L_F32 ? 9 : 18, kVec = 16 / sizeof(Word);
   constexpr int kRows = LT == FP8IMMA_L_F32 ? kTile / 2 : kTile, kEach = kRows / 32;  // rows of a tile, of a lane
-  constexpr int kAhead = kRows * 32 / kVec / kThreads;  // 16-byte pieces of a tile a thread
+  constexpr int kAhead = kRows * (LT == FP8IMMA_L_F32 ? 8 : 16) / kVec / kThreads;  // 16-byte pieces of a tile a thread
   __shared__ __align__(16) Word s_tile[kRows * kPitch];
-  __shared__ Buffer s_buf[kWarps];
+  __shared__ unsigned long long s_buf[kWarps][kBuffer];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  if (lane == 0) s_buf[warp].count = 0u;
   pdl_launch_dependents();
   pdl_wait();
   const int part = blockIdx.x, V = p.a.vocab, top = p.a.top;
   const float c = p.to_log2;
-  Buffer* const buf = &s_buf[warp];
+  unsigned long long* const buf = s_buf[warp];
   for (int group = blockIdx.y; group < p.groups; group += gridDim.y) {
     const int t0 = group * p.group, n = min(p.group, p.a.tokens - t0);
     const int j0 = part * p.per_part, j1 = min(V, j0 + p.per_part);
     const Word* src = static_cast<const Word*>(p.a.logits) + t0;
     const bool vec = ((reinterpret_cast<uintptr_t>(src) | (uintptr_t)(p.a.vocab_stride * sizeof(Word)) | (uintptr_t)(n * sizeof(Word))) & 15u) == 0;
     const int per = n / kVec;
-    Sums z[4];
-    Top list[4];
+    Sums z[2];
+    Top list[2];
     uint4 next[kAhead];
     auto fetch = [&](int jt) {
       const int rows = min(kRows, j1 - jt);
@@ -496,32 +572,32 @@ __global__ void __launch_bounds__(kColWarps * 32) logprobs_col_kernel(const __gr
       }
       __syncthreads();
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
+      for (int k = 0; k < 2; ++k) {
         const int t = warp + k * kWarps;
         if (t >= n) break;
         float x[kEach];  // the lane's logits of the tile
 #pragma unroll
         for (int i = 0; i < kEach; ++i) x[i] = i * 32 + lane < rows ? to_f32<LT>(s_tile[(i * 32 + lane) * kPitch + t]) : -INFINITY;
-        float bar = INFINITY;
-        if (top) {
-          bar = enters_at(list[k], 0u);
-          if (jt == j0) {
-            float big = x[0];
+        float big = x[0];
 #pragma unroll
-            for (int i = 1; i < kEach; ++i) big = fmaxf(big, x[i]);
-            bar = fmaxf(bar, first_bar(big, top, lane));
+        for (int i = 1; i < kEach; ++i) big = fmaxf(big, x[i]);
+        if (big * c > z[k].m + kRaise) z[k].raise(big * c);
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) z[k].add(x[i], c);
+        if (top) {
+          float bar = enters_at(list[k], 0u);
+          if (jt == j0) bar = fmaxf(bar, first_bar(big, top, lane));
+          if (__any_sync(0xffffffffu, big >= bar)) {
+            int m = 0;
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) m = put(x[i], x[i] >= bar && i * 32 + lane < rows, buf, m, jt + i * 32 + lane, lane);
+            list[k] = flush(list[k], buf, m, top, lane);
           }
         }
-        unsigned valid = 0u;
-#pragma unroll
-        for (int i = 0; i < kEach; ++i) valid |= (unsigned)(i * 32 + lane < rows) << i;
-        bool gathered = false;
-        take<kEach>(x, c, z[k], top > 0, bar, buf, jt + lane, 32, valid, gathered);
-        if (top && __any_sync(0xffffffffu, gathered)) list[k] = flush(list[k], buf, 1u, top, lane);
       }
     }
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
+    for (int k = 0; k < 2; ++k) {
       const int t = warp + k * kWarps;
       if (t >= n) break;
       z[k].warp_join();
@@ -543,6 +619,7 @@ template <int LT>
 cudaError_t launch(LpParams& p, cudaStream_t st) {
   const bool rows = p.a.vocab_stride == 1;
   const int sms = num_sms_current();
+  p.flush_at = p.a.top >= 16 ? 32 : p.a.top >= 8 ? 16 : 8;
   const int vec = LT == FP8IMMA_L_F32 ? 4 : 8;
   // Parts: enough CTAs for two (row-major: four resident) on each SM, but no
   // part below the logits that make joining it worth while.
@@ -554,14 +631,17 @@ cudaError_t launch(LpParams& p, cudaStream_t st) {
     const int64_t want = (4ll * sms + units - 1) / units, most = (full + 255) / 256;
     p.parts = (int)std::max<int64_t>(1, std::min(want, most));
     if (units >= 2 * sms) p.parts = 1;
-    if (units >= 8 * sms) warps = 2;
+    // Each warp keeps a list of its own, so with many rows fewer warps a row
+    // cost less (4096 rows of 32001, 5 alternatives: 1 warp 91 us, 8 warps 136
+    // us), with few rows more warps fill the SMs (700 rows: 48 and 32 us).
+    while (warps > 1 && (int64_t)units * warps > 48ll * sms) warps /= 2;
   } else {
-    // groups of 8 tokens, one a warp, while that leaves a CTA a fair part of the
-    // columns; of 32 beyond, for whole sectors of the logits
-    p.group = p.a.tokens <= 64 ? 8 : 32;
+    // groups of 8 tokens, one a warp; of 16 with 16-bit logits and many tokens,
+    // for whole 32-byte sectors
+    p.group = p.a.tokens <= 64 || LT == FP8IMMA_L_F32 ? 8 : 16;
     units = p.groups = (p.a.tokens + p.group - 1) / p.group;
     full = p.a.vocab;
-    const int64_t want = (2ll * sms + units - 1) / units, most = (full + kTile - 1) / kTile;
+    const int64_t want = std::max<int64_t>(1, 4ll * sms / units), most = (full + kTile - 1) / kTile;
     p.parts = (int)std::max<int64_t>(1, std::min<int64_t>(std::min(want, most), 74));
   }
   p.per_part = (full + p.parts - 1) / p.parts;
@@ -590,7 +670,9 @@ cudaError_t launch(LpParams& p, cudaStream_t st) {
     lc.numAttrs = api_pdl() ? 1 : 0;
     e = !rows        ? cudaLaunchKernelEx(&lc, logprobs_col_kernel<LT>, p)
         : warps == 8 ? cudaLaunchKernelEx(&lc, logprobs_row_kernel<LT, 8>, p)
-                     : cudaLaunchKernelEx(&lc, logprobs_row_kernel<LT, 2>, p);
+        : warps == 4 ? cudaLaunchKernelEx(&lc, logprobs_row_kernel<LT, 4>, p)
+        : warps == 2 ? cudaLaunchKernelEx(&lc, logprobs_row_kernel<LT, 2>, p)
+                     : cudaLaunchKernelEx(&lc, logprobs_row_kernel<LT, 1>, p);
   }
   const cudaError_t e1 = ctr.release(st), e2 = work.release(st);
   return e != cudaSuccess ? e : e1 != cudaSuccess ? e1 : e2;
