@@ -16,8 +16,11 @@
 // rows a KV head the products are far below the tensor rate, so the kernel is
 // built to keep the copies running:
 //  * one CTA per SM; a producer warp streams 128-key stages (one TMA box per
-//    page for K and for V, 128-byte swizzle) through a 3..6 stage ring, page
-//    ids fetched a batch of 32 ahead;
+//    page for K and for V, 128-byte swizzle) through a ring of 2..6 stages, page
+//    ids and scales fetched a batch of 32 ahead. Boxes below 4 KB are slow (2 KB:
+//    3.8 TB/s, 4 KB: 6.6 TB/s), so pages smaller than that are copied 16 bytes a
+//    lane by four producer warps (512 contiguous bytes a warp: 6.6 TB/s) into the
+//    same places;
 //  * the 128-key tiles of all (sequence, row tile, KV head) items are laid end
 //    to end and cut into equal runs, one per CTA, whatever the lengths are
 //    (lengths are read on the device). Items that several CTAs share are joined
@@ -43,7 +46,8 @@ using namespace fp8imma_dev;
 
 constexpr int kKeys = 128;                  // keys of a stage
 constexpr int kConsumers = 8;               // consumer warps
-constexpr int kThreads = (kConsumers + 1) * 32;
+constexpr int kProducers = 4;               // producer warps; TMA takes the first of them only
+constexpr int kThreads = (kConsumers + kProducers) * 32;
 constexpr int kSlots = kKeys / 16;          // pages of a stage at most
 constexpr float kTinyScale = 7.888609e-31f; // 2^-100: value scales below count as this (values below 2^-91)
 constexpr float kRaise = 8.0f;              // M follows the maximum when it lies this far above
@@ -54,6 +58,7 @@ struct AttnParams {
   int per_seq;   // > 0: every sequence has this many tokens
   int group;     // query heads per KV head
   int vec_q;     // query rows are 16-byte aligned
+  int copy;      // pages are copied by lanes instead of TMA
   int max_items; // items of the step at most (counters)
   unsigned int* counters;  // per item: finished parts; zero between calls
   float* parts;            // per (CTA, first / last segment, row warp): M, L, O of a shared item
@@ -85,6 +90,10 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   uint32_t r;
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
+}
+// 16 bytes global -> shared, asynchronously
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 // two outputs in the activation type
 __device__ __forceinline__ uint32_t out_pair(float lo, float hi, int a_type) {
@@ -321,7 +330,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (tid == 0) {
     for (int i = 0; i < S::kStages; ++i) {
-      mbar_init(&s_full[i], 1);
+      mbar_init(&s_full[i], p.copy ? 1 + kProducers * 32 : 1);
       mbar_init(&s_empty[i], kConsumers / S::kSplit);
     }
     fence_barrier_init();
@@ -400,8 +409,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int ps = p.c.page_size;
   Segment g;
 
-  if (warp == kConsumers) {
+  if (warp >= kConsumers) {
     // ---------------------------------------------------------- producer --
+    const int pw = warp - kConsumers;
+    if (pw > 0 && !p.copy) return;
     int stage = 0, issued = 0;
     uint32_t phase = 1;  // the ring starts empty
     bool ok = true;
@@ -444,31 +455,50 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t n_live = (uint32_t)__popc(__ballot_sync(0xffffffffu, live));
         ok = mbar_wait(&s_empty[stage], phase, ERR_WAIT_EMPTY);
         if (!ok) break;
-        if (lane == 0 && n_live) {
-          // one pending arrival stays until the scales are written below
-          asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(&s_full[stage])), "r"(n_live * 2 * page_bytes) : "memory");
-        }
-        __syncwarp();
-        if (live) {
-          uint8_t* dst = smem_raw + (smem_base - smem_u32(smem_raw)) + stage * S::kStageBytes;
-          const int row = (page * p.c.kv_heads + g.h) * ps;  // key row of the whole pool
+        if (p.copy) {
+          // this warp's share of the stage's pages, 512 bytes an instruction
+          const uint32_t dst = smem_base + stage * S::kStageBytes;
+          const unsigned live_pages = __ballot_sync(0xffffffffu, live);
+          for (int sl = pw; sl < per_stage; sl += kProducers) {
+            if (!((live_pages >> sl) & 1u)) continue;
+            const size_t from_byte = (size_t)(__shfl_sync(0xffffffffu, ids, at + sl) * p.c.kv_heads + g.h) * page_bytes;
+            const uint8_t* sk = static_cast<const uint8_t*>(p.c.k) + from_byte;
+            const uint8_t* sv = static_cast<const uint8_t*>(p.c.v) + from_byte;
+            for (int c = lane; c < (int)(page_bytes >> 4); c += 32) {  // 16-byte pieces of the page
+              const int r = c / (8 * S::kHalves), hf = S::kHalves == 2 ? (c >> 3) & 1 : 0;  // 128-byte row and column half
+              const uint32_t to = hf * (kKeys * 128) + sl * (page_bytes / S::kHalves) + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+              copy16(dst + to, sk + c * 16);
+              copy16(dst + S::kTileBytes + to, sv + c * 16);
+            }
+          }
+          asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&s_full[stage])) : "memory");
+        } else {
+          if (lane == 0 && n_live) {
+            // one pending arrival stays until the scales are written below
+            asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(&s_full[stage])), "r"(n_live * 2 * page_bytes) : "memory");
+          }
+          __syncwarp();
+          if (live) {
+            uint8_t* dst = smem_raw + (smem_base - smem_u32(smem_raw)) + stage * S::kStageBytes;
+            const int row = (page * p.c.kv_heads + g.h) * ps;  // key row of the whole pool
 #pragma unroll
-          for (int hf = 0; hf < S::kHalves; ++hf) {
-            const int off = hf * (kKeys * 128) + lane * (int)(page_bytes / S::kHalves);
-            const int y = D == 64 ? row >> 1 : row;
-            tma_load_2d(dst + off, &map_k, &s_full[stage], hf * 128, y);
-            tma_load_2d(dst + S::kTileBytes + off, &map_v, &s_full[stage], hf * 128, y);
+            for (int hf = 0; hf < S::kHalves; ++hf) {
+              const int off = hf * (kKeys * 128) + lane * (int)(page_bytes / S::kHalves);
+              const int y = D == 64 ? row >> 1 : row;
+              tma_load_2d(dst + off, &map_k, &s_full[stage], hf * 128, y);
+              tma_load_2d(dst + S::kTileBytes + off, &map_v, &s_full[stage], hf * 128, y);
+            }
           }
         }
         const float ks = __shfl_sync(0xffffffffu, kss, src), vs = __shfl_sync(0xffffffffu, vss, src);
         if (at == per_stage) fetch_scales();
-        if (lane < kSlots) {
+        if (pw == 0 && lane < kSlots) {
           s_info[stage].ks[lane] = ks;
           s_info[stage].vs[lane] = vs;
           s_info[stage].live[lane] = live;
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(&s_full[stage]);
+        if (pw == 0 && lane == 0) mbar_arrive(&s_full[stage]);
         ++issued;
         if (++stage == S::kStages) {
           stage = 0;
@@ -476,7 +506,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
     }
-    if (!ok) {  // a wait ran out: let the copies in flight land before the CTA ends
+    if (p.copy) asm volatile("cp.async.wait_all;" ::: "memory");
+    if (!ok && !p.copy) {  // a wait ran out: let the copies in flight land before the CTA ends
       for (int i = 0; i < min(issued, S::kStages); ++i) {
         const int k = issued - 1 - i;
         mbar_wait(&s_full[k % S::kStages], (uint32_t)((k / S::kStages) & 1), ERR_WAIT_FULL);
@@ -889,6 +920,7 @@ cudaError_t launch(AttnParams& p, cudaStream_t st) {
   if (items * tiles > 0x7fffffffll) return cudaErrorInvalidValue;  // units are counted in 31 bits
   const int grid = (int)std::min<int64_t>(num_sms_current(), std::max<int64_t>(1, items * tiles));
   p.max_items = (int)items;
+  p.copy = p.c.page_size * (D == 256 ? 128 : D) < 4096;
   const size_t ctr_bytes = (size_t)items * 4, part_bytes = (size_t)grid * 2 * RW * S::kPartFloats * 4;
   ScopedScratch ctr, part;
   e = ctr.get(ctr_bytes, st, kScratchAttn);
