@@ -10,13 +10,17 @@
 // format's smallest step. Division by s' is an exact product as well, so each
 // stored value is rounded once.
 //
-// One CTA owns one (page, head, K or V), so scales and codes of a page have
-// one writer and no atomics are needed.
+// A team of 1 .. 8 warps owns one (page, head, K or V), so scales and codes of
+// a page have one writer and no atomics are needed. A CTA's teams share a page:
+// finding it (a scan of the sequences' lengths) is what a small append spends
+// its time on.
 #include "fp8_mma.cuh"
 #include "fp8imma/fp8imma_ext.h"
 #include "fp8imma_kernels.h"
 #include "nvtx_range.h"
+#include "sm100_async.cuh"
 
+#include <algorithm>
 #include <cuda_runtime.h>
 
 namespace fp8imma_b200 {
@@ -24,7 +28,7 @@ namespace {
 
 using namespace fp8imma_dev;
 
-constexpr int kThreads = 128;
+constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kKeep = 8;  // 16-byte vectors of a page that a thread keeps between the two passes
 
 struct AppendParams {
@@ -34,6 +38,7 @@ struct AppendParams {
   int vec;         // rows are 16-byte aligned
   int per_seq;     // > 0: every sequence appends this many tokens
   int pages_seq;   // then: pages a sequence can touch
+  int team;        // warps of a (page, head, K or V)
 };
 
 template <int AT>
@@ -95,9 +100,11 @@ __device__ __forceinline__ int touched(const AppendParams& p, int b, int& first)
 template <int AT, int FMT>
 __global__ void __launch_bounds__(kThreads) kv_append_kernel(const __grid_constant__ AppendParams p) {
   __shared__ int s_pick[3];
-  __shared__ int s_scan[kThreads / 32];
-  __shared__ float s_max[kThreads / 32];
-  const int tid = threadIdx.x, h = blockIdx.y, which = blockIdx.z;
+  __shared__ int s_scan[kWarps];
+  __shared__ float s_max[kWarps];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  pdl_launch_dependents();
+  pdl_wait();
   int b = 0, first = 0, pi = 0;
   if (p.per_seq > 0) {
     b = blockIdx.x / p.pages_seq;
@@ -105,28 +112,30 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(const __grid_consta
     if (pi >= touched(p, b, first)) return;
   } else {
     // unit blockIdx.x of the sequences' touched pages laid end to end
-    if (tid == 0) s_pick[0] = -1;
+    if (threadIdx.x == 0) s_pick[0] = -1;
     int base = 0;
     for (int b0 = 0; b0 < p.c.batch; b0 += kThreads) {
+      const int mine = b0 + (int)threadIdx.x;
       int f = 0;
-      const int n = b0 + tid < p.c.batch ? max(0, touched(p, b0 + tid, f)) : 0;
+      const int n = mine < p.c.batch ? max(0, touched(p, mine, f)) : 0;
       int x = n;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int y = __shfl_up_sync(0xffffffffu, x, o);
-        if ((tid & 31) >= o) x += y;
+        if (lane >= o) x += y;
       }
       __syncthreads();
-      if ((tid & 31) == 31) s_scan[tid >> 5] = x;
+      if (lane == 31) s_scan[warp] = x;
       __syncthreads();
       int before = base;
-      for (int w = 0; w < kThreads / 32; ++w) {
-        if (w < (tid >> 5)) before += s_scan[w];
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        if (w < warp) before += s_scan[w];
         base += s_scan[w];
       }
       const int lo = before + x - n;
       if ((int)blockIdx.x >= lo && (int)blockIdx.x < lo + n) {
-        s_pick[0] = b0 + tid;
+        s_pick[0] = mine;
         s_pick[1] = f;
         s_pick[2] = (int)blockIdx.x - lo;
       }
@@ -150,31 +159,36 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(const __grid_consta
   const int lo = max(max(start, 0), pi * ps), hi = min(len, (pi + 1) * ps);
   const int slot0 = lo - pi * ps, rows = hi - lo;
   if (rows <= 0) return;
+  // this team's head and tensor; teams past the last one only take part in the barrier
+  const int item = blockIdx.y * (kWarps / p.team) + warp / p.team;
+  const bool on = item < 2 * p.c.kv_heads;
+  const int h = item >> 1, which = item & 1;
+  const int tid = warp % p.team * 32 + lane, step = p.team * 32;
   const uint16_t* src = p.src[which] + (int64_t)(t0 + lo - start) * p.ts[which] + (int64_t)h * p.hs[which];
   const size_t ph = (size_t)page * p.c.kv_heads + h;
   uint8_t* dst = static_cast<uint8_t*>(which ? p.c.v : p.c.k) + ph * ps * D;
   float* scale = (which ? p.c.v_scale : p.c.k_scale) + ph;
-  const float s_old = slot0 > 0 ? *scale : 0.0f;
+  const float s_old = on && slot0 > 0 ? *scale : 0.0f;
 
-  const int vr = D >> 3, nv = rows * vr;  // 8-element vectors of a row, of the page's new rows
+  const int vr = D >> 3, nv = on ? rows * vr : 0;  // 8-element vectors of a row, of the page's new rows
   uint4 keep[kKeep];
   float amax = 0.0f;
 #pragma unroll
   for (int i = 0; i < kKeep; ++i) {
-    const int v = tid + i * kThreads;
-    if (v < nv) {
-      keep[i] = load_row8<AT>(src + (int64_t)(v / vr) * p.ts[which] + (v % vr) * 8, p.vec);
-      amax = fmaxf(amax, absmax8<AT>(keep[i]));
-    }
+    const int v = tid + i * step;
+    if (v < nv) keep[i] = load_row8<AT>(src + (int64_t)(v / vr) * p.ts[which] + (v % vr) * 8, p.vec);
   }
-  for (int v = tid + kKeep * kThreads; v < nv; v += kThreads)
+#pragma unroll
+  for (int i = 0; i < kKeep; ++i)
+    if (tid + i * step < nv) amax = fmaxf(amax, absmax8<AT>(keep[i]));
+  for (int v = tid + kKeep * step; v < nv; v += step)
     amax = fmaxf(amax, absmax8<AT>(load_row8<AT>(src + (int64_t)(v / vr) * p.ts[which] + (v % vr) * 8, p.vec)));
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-  if ((tid & 31) == 0) s_max[tid >> 5] = amax;
+  if (lane == 0) s_max[warp] = amax;
   __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kThreads / 32; ++w) amax = fmaxf(amax, s_max[w]);
+  if (!on) return;
+  for (int w = 0; w < p.team; ++w) amax = fmaxf(amax, s_max[warp / p.team * p.team + w]);
 
   // amax = 1.m * 2^e <= 1.75 * 2^(8|15) * 2^k  <=>  k >= e - (8|15), one more when 1.m > 1.75
   const uint32_t bits = __float_as_uint(amax);
@@ -184,7 +198,7 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(const __grid_consta
   const float inv = __fdiv_rn(1.0f, s_new);
   if (slot0 > 0 && s_new != s_old) {  // uniform: the page's earlier codes move to the larger scale
     const float ratio = __fdiv_rn(s_old, s_new);
-    for (int v = tid; v < slot0 * (D >> 4); v += kThreads) {
+    for (int v = tid; v < slot0 * (D >> 4); v += step) {
       uint4 c = reinterpret_cast<uint4*>(dst)[v];
       uint32_t w[4] = {c.x, c.y, c.z, c.w};
 #pragma unroll
@@ -201,21 +215,27 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(const __grid_consta
   uint2* out = reinterpret_cast<uint2*>(dst + (size_t)slot0 * D);
 #pragma unroll
   for (int i = 0; i < kKeep; ++i) {
-    const int v = tid + i * kThreads;
+    const int v = tid + i * step;
     if (v < nv) out[v] = to_codes<AT, FMT>(keep[i], s_new, inv);
   }
-  for (int v = tid + kKeep * kThreads; v < nv; v += kThreads)
+  for (int v = tid + kKeep * step; v < nv; v += step)
     out[v] = to_codes<AT, FMT>(load_row8<AT>(src + (int64_t)(v / vr) * p.ts[which] + (v % vr) * 8, p.vec), s_new, inv);
   if (tid == 0) *scale = s_new;
 }
 
 template <int AT>
 cudaError_t launch_append(const AppendParams& p, dim3 grid, cudaStream_t st) {
-  if (p.c.format == FP8IMMA_B_E4M3)
-    kv_append_kernel<AT, F8_E4M3><<<grid, kThreads, 0, st>>>(p);
-  else
-    kv_append_kernel<AT, F8_E5M2><<<grid, kThreads, 0, st>>>(p);
-  return cudaGetLastError();
+  cudaLaunchConfig_t lc = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  lc.gridDim = grid;
+  lc.blockDim = dim3(kThreads);
+  lc.stream = st;
+  lc.attrs = attr;
+  lc.numAttrs = api_pdl() ? 1 : 0;
+  return p.c.format == FP8IMMA_B_E4M3 ? cudaLaunchKernelEx(&lc, kv_append_kernel<AT, F8_E4M3>, p)
+                                      : cudaLaunchKernelEx(&lc, kv_append_kernel<AT, F8_E5M2>, p);
 }
 
 }  // namespace
@@ -265,8 +285,13 @@ extern "C" int fp8imma_kv_append(const fp8imma_kv_cache* c, const fp8imma_kv_app
   } else {
     units = c->tokens / c->page_size + 2ll * c->batch;  // sum over b of ceil((n_b - 1) / page) + 1 at most
   }
-  if (units > 0x7fffffffll || c->kv_heads > 65535) return (int)cudaErrorInvalidValue;
-  const dim3 grid((unsigned)units, (unsigned)c->kv_heads, 2);
+  // a team keeps its rows in registers: kKeep vectors a lane
+  const int64_t rows = std::min<int64_t>(c->page_size, ((int64_t)c->tokens + c->batch - 1) / c->batch);
+  p.team = 1;
+  while (p.team < kWarps && rows * (c->head_dim / 8) > (int64_t)p.team * 32 * kKeep) p.team *= 2;
+  const int64_t rows_y = (2ll * c->kv_heads * p.team + kWarps - 1) / kWarps;
+  if (units > 0x7fffffffll || rows_y > 65535) return (int)cudaErrorInvalidValue;
+  const dim3 grid((unsigned)units, (unsigned)rows_y);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return (int)(a->a_type == FP8IMMA_A_F16 ? launch_append<0>(p, grid, st) : launch_append<1>(p, grid, st));
 }
