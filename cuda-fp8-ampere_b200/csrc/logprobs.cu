@@ -274,17 +274,55 @@ __device__ __forceinline__ void put_part(const LpParams& p, int part, int t, con
   if (lane == 0) *reinterpret_cast<float4*>(p.sums + at * 4) = make_float4(z.m, z.l, z.s, 0.0f);
   if (p.a.top) p.lists[at * 32 + lane] = top.mine;
 }
-// Parts first, first + stride, ... of token t joined in this order, the sums of
-// 32 parts at a time.
-__device__ __forceinline__ void get_parts(const LpParams& p, int first, int stride, int t, Sums& z, Top& top, int lane) {
+// Sums of the parts first, first + stride, ... of token t, joined in this order
+// 32 at a time.
+__device__ __forceinline__ Sums get_sums(const LpParams& p, int first, int stride, int t, int lane) {
+  Sums z;
   for (int k = first + lane * stride; k < p.parts; k += 32 * stride) {
     const float4 v = __ldcg(reinterpret_cast<const float4*>(p.sums + ((int64_t)k * p.a.tokens + t) * 4));
     z.join(v.x, v.y, v.z);
   }
   z.warp_join();
-  if (p.a.top) {
-#pragma unroll 4
-    for (int k = first; k < p.parts; k += stride) top.mine = merge(top.mine, __ldcg(p.lists + ((int64_t)k * p.a.tokens + t) * 32 + lane), lane);
+  return z;
+}
+// Their lists merged, the next one under way.
+__device__ __forceinline__ Top get_lists(const LpParams& p, int first, int stride, int t, int lane) {
+  Top l;
+  auto load = [&](int k) { return k < p.parts ? __ldcg(p.lists + ((int64_t)k * p.a.tokens + t) * 32 + lane) : kNoKey; };
+  unsigned long long next = load(first);
+#pragma unroll 1
+  for (int k = first; k < p.parts; k += stride) {
+    const unsigned long long v = next;
+    next = load(k + stride);
+    l.mine = merge(l.mine, v, lane);
+  }
+  return l;
+}
+// The same for all parts by one warp where there are at least `top` of them
+// (and kMostParts at most): no key below the top-th largest of their heads
+// belongs to the row's list, so a lane follows the lists of its parts only as
+// far as that.
+constexpr int kMostParts = 96;
+__device__ __noinline__ Top get_heads(const unsigned long long* lists, int64_t stride, int parts, unsigned long long* buf, int top, int lane) {
+  unsigned long long h[kMostParts / 32];
+#pragma unroll
+  for (int e = 0; e < kMostParts / 32; ++e) h[e] = lane + 32 * e < parts ? __ldcg(lists + (lane + 32 * e) * stride) : kNoKey;
+#pragma unroll
+  for (int e = 0; e < kMostParts / 32; ++e) buf[lane + 32 * e] = h[e];
+  const unsigned long long least = flush(Top(), buf, parts, top, lane).last;
+  Top l;
+  for (int d = 1;; ++d) {
+    int n = 0;
+#pragma unroll
+    for (int e = 0; e < kMostParts / 32; ++e) {
+      const bool in = h[e] != kNoKey && h[e] >= least;
+      const unsigned m = __ballot_sync(0xffffffffu, in);
+      if (in) buf[n + __popc(m & ((1u << lane) - 1u))] = h[e];
+      n += __popc(m);
+      h[e] = in && d < top ? __ldcg(lists + (lane + 32 * e) * stride + d) : kNoKey;
+    }
+    if (n == 0) return l;
+    l = flush(l, buf, n, top, lane);
   }
 }
 
@@ -499,9 +537,9 @@ __global__ void __launch_bounds__(kWarps * 32, 32 / kWarps) logprobs_row_kernel(
       else put_part(p, part, t, z, list, lane);
     }
     if (p.parts > 1 && came_last(p.counters + t, p.parts)) {  // the warps join every so many parts each, then theirs
-      Sums all;
+      Sums all = get_sums(p, warp, kWarps, t, lane);
       Top l;
-      get_parts(p, warp, kWarps, t, all, l, lane);
+      if (top) l = get_lists(p, warp, kWarps, t, lane);
       join_warps<kWarps>(all, l, s_sums, s_list, top > 0, warp, lane);
       if (warp == 0) finish<LT>(p, t, all, l, lane);
     }
@@ -606,9 +644,12 @@ __global__ void __launch_bounds__(kColWarps * 32, 4) logprobs_col_kernel(const _
     }
     if (p.parts > 1 && came_last(p.counters + group, p.parts)) {
       for (int t = warp; t < n; t += kWarps) {
-        Sums all;
+        const Sums all = get_sums(p, 0, 1, t0 + t, lane);
         Top l;
-        get_parts(p, 0, 1, t0 + t, all, l, lane);
+        if (top && p.parts >= top && p.parts <= kMostParts)
+          l = get_heads(p.lists + (int64_t)(t0 + t) * 32, (int64_t)p.a.tokens * 32, p.parts, buf, top, lane);
+        else if (top)
+          l = get_lists(p, 0, 1, t0 + t, lane);
         finish<LT>(p, t0 + t, all, l, lane);
       }
     }
