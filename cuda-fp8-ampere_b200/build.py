@@ -31,7 +31,7 @@ NVCC_FLAGS = ["-DFP8IMMA_NVTX", "-O3", "-std=c++17", "-lineinfo", "-Xcompiler", 
               "--expt-relaxed-constexpr", "-I" + INCLUDE, "-I" + CSRC]
 
 CU_SOURCES = ["api.cu", "gemv_splitk.cu", "decode.cu", "generic.cu", "fp8wgt.cu", "host_util.cu", "gemm_tc.cu", "noalloc.cu", "peer.cu", "quantize.cu",
-              "kv_cache.cu", "kv_attention.cu", "moe.cu", "logprobs.cu"]
+              "kv_cache.cu", "kv_attention.cu", "kv_attention_tc.cu", "moe.cu", "logprobs.cu"]
 
 
 def _run(cmd: list[str]) -> None:

@@ -483,6 +483,12 @@ int fp8imma_set_decode_kernel(int enable) {
   return 0;
 }
 
+int fp8imma_set_attention_tc_rows(int rows) {
+  if (rows < 1) return (int)cudaErrorInvalidValue;
+  attn_set_tc_rows(rows);
+  return 0;
+}
+
 int fp8imma_set_pdl(int enable) {
   g_pdl.store(enable ? 1 : 0);
   return 0;
@@ -490,7 +496,8 @@ int fp8imma_set_pdl(int enable) {
 
 unsigned int fp8imma_device_error(int clear) {
   return gemv_device_error(clear != 0) | decode_device_error(clear != 0) | tc_device_error(clear != 0) |
-         peer_device_error(clear != 0) | attn_device_error(clear != 0) | moe_device_error(clear != 0);
+         peer_device_error(clear != 0) | attn_device_error(clear != 0) |
+         attn_tc_device_error(clear != 0) | moe_device_error(clear != 0);
 }
 
 int fp8imma_set_wait_limit_ns(unsigned long long ns) {
@@ -500,6 +507,7 @@ int fp8imma_set_wait_limit_ns(unsigned long long ns) {
   if (e == cudaSuccess) e = tc_set_wait_limit(ns);
   if (e == cudaSuccess) e = peer_set_wait_limit(ns);
   if (e == cudaSuccess) e = attn_set_wait_limit(ns);
+  if (e == cudaSuccess) e = attn_tc_set_wait_limit(ns);
   if (e == cudaSuccess) e = moe_set_wait_limit(ns);
   return (int)e;
 }

@@ -185,6 +185,10 @@ cudaError_t launch_row_scales(const void* A, int a_type, int M, int K, uint16_t*
 unsigned int attn_device_error(bool clear);
 unsigned int moe_device_error(bool clear);
 cudaError_t attn_set_wait_limit(unsigned long long ns);
+unsigned int attn_tc_device_error(bool clear);
+cudaError_t attn_tc_set_wait_limit(unsigned long long ns);
+// query rows of a sequence and KV head from which the cache attention runs on tcgen05
+void attn_set_tc_rows(int rows);
 cudaError_t moe_set_wait_limit(unsigned long long ns);
 cudaError_t kv_cache_check(const ::fp8imma_kv_cache* cache);
 

@@ -53,6 +53,7 @@ EXT_SYMBOLS = [
     "fp8imma_last_path",
     "fp8imma_set_pdl",
     "fp8imma_set_decode_kernel",
+    "fp8imma_set_attention_tc_rows",
     "fp8imma_set_wait_limit_ns",
     "fp8imma_set_tc_pair",
     "fp8imma_set_tc_splitk",
@@ -161,6 +162,8 @@ def lib() -> ctypes.CDLL:
     L.fp8imma_set_tc_half_tail.argtypes = [I]
     L.fp8imma_set_pdl.restype = I
     L.fp8imma_set_pdl.argtypes = [I]
+    L.fp8imma_set_attention_tc_rows.restype = I
+    L.fp8imma_set_attention_tc_rows.argtypes = [I]
     L.fp8imma_set_decode_kernel.restype = I
     L.fp8imma_set_decode_kernel.argtypes = [I]
     L.fp8imma_set_wait_limit_ns.restype = I

@@ -11,9 +11,14 @@ from serving_ref import F8, FMAX, ref_append, ref_attention
 pytestmark = pytest.mark.gpu
 
 
-@pytest.fixture
-def ops(cuda):
-    return F.ext()
+# rows a KV head from which attention runs on tcgen05: never, from the default on, always
+@pytest.fixture(params=[1 << 20, 24, 1], ids=["mma", "default", "tcgen05"])
+def ops(cuda, request):
+    L = F.lib()
+    assert L.fp8imma_set_attention_tc_rows(request.param) == 0
+    yield F.ext()
+    L.fp8imma_set_attention_tc_rows(24)
+    assert L.fp8imma_device_error(1) == 0
 
 
 def gen(seed):
@@ -351,6 +356,19 @@ def test_cache_beyond_32_bit_offsets(ops):
     small = [x[sub].contiguous() for x in (kc, vc, ks, vs)]
     out, lse = ops.kv_attention(q, kc, vc, ks, vs, table, i32([300]), None)
     check(out, lse, ref_attention(q, *small, i32([[0, 1, 2]]), [300], [0, 1], 1 / math.sqrt(d), 0, fmt))
+
+
+def test_attention_many_empty_sequences(ops):
+    """Runs of sequences without keys between others: each has rows, which see nothing."""
+    g = gen(77)
+    b, w, hk, ps, d, n = 300, 4, 2, 64, 64, 8
+    cache = make_cache(g, b, w, hk, ps, d, "e4m3")
+    lens = [0] * b
+    for i in (0, 5, 6, 150, 299):
+        lens[i] = 8 + 40 * (i % 7)
+    q = torch.randn(b * n, 4 * hk, d, generator=g, device="cuda", dtype=torch.float16)
+    cu = offsets([n] * b)
+    check(*run_attend(ops, q, cache, lens, cu, 0, "e4m3"))
 
 
 def test_empty_step(ops):
