@@ -484,7 +484,7 @@ int fp8imma_set_decode_kernel(int enable) {
 }
 
 int fp8imma_set_attention_tc_rows(int rows) {
-  if (rows < 1) return (int)cudaErrorInvalidValue;
+  if (rows < 0) return (int)cudaErrorInvalidValue;
   attn_set_tc_rows(rows);
   return 0;
 }

@@ -187,7 +187,7 @@ unsigned int moe_device_error(bool clear);
 cudaError_t attn_set_wait_limit(unsigned long long ns);
 unsigned int attn_tc_device_error(bool clear);
 cudaError_t attn_tc_set_wait_limit(unsigned long long ns);
-// query rows of a sequence and KV head from which the cache attention runs on tcgen05
+// query rows of a sequence and KV head from which the cache attention runs on tcgen05 (0: by its own rule)
 void attn_set_tc_rows(int rows);
 cudaError_t moe_set_wait_limit(unsigned long long ns);
 cudaError_t kv_cache_check(const ::fp8imma_kv_cache* cache);

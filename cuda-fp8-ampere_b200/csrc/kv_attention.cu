@@ -639,7 +639,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-std::atomic<int> g_tc_rows{24};
+std::atomic<int> g_tc_rows{0};  // rows from which tcgen05 is used, 0: by tc_pays()
 
 template <int FMT, int D, int NT, int RW>
 cudaError_t launch(AttnParams& p, cudaStream_t st) {
@@ -686,13 +686,34 @@ cudaError_t launch(AttnParams& p, cudaStream_t st) {
   return e != cudaSuccess ? e : e1 != cudaSuccess ? e1 : e2;
 }
 
+// Whether many rows and enough tiles are there for the tcgen05 kernel
+// (kv_attention_tc.cu). A tile costs it about 2 us at head_dim 128, 1.6 at 64,
+// whatever the rows, and a call some 12 us more than here (TMEM, a deeper
+// pipeline); a tile costs this file's kernel 3.2 us with 32 rows of 128 channels,
+// 4.7 with 64, 9 with 128, and half of that at 64 channels, where up to 32 rows
+// stay here. Measured, this kernel against that one, in us: 16 sequences of 8000
+// keys, 64 heads over 8: 32 rows 181/123, 64 rows 263/126, 128 rows 495/136; 24
+// of 6000, 28 heads over 4 of 64: 28 rows 59/69, 35 rows 100/69; few tiles: 8 of
+// 2000, 32 heads over 8, 16 rows 30/39; 4 of 300 18 against 16. Tiles are
+// counted by what the page tables can hold, since lengths lie on the device.
+bool tc_pays(const AttnParams& p, int64_t rows) {
+  if (p.c.head_dim == 256) return false;
+  const int forced = g_tc_rows.load();
+  if (forced > 0) return rows >= forced;
+  if (rows < (p.c.head_dim == 64 ? 33 : 16)) return false;
+  int64_t keys = (int64_t)p.c.max_pages * p.c.page_size;
+  if (p.a.window > 0) keys = std::min<int64_t>(keys, (int64_t)p.a.window + rows / p.group + kKeys);
+  const int64_t tiles = (keys + kKeys - 1) / kKeys * ((rows + 127) / 128) * p.c.batch * p.c.kv_heads;
+  return tiles * std::min<int64_t>(rows, 128) >= 320ll * num_sms_current();
+}
+
 // Query rows a CTA works on at once: the rows of a sequence and KV head
 // (group times its tokens, on average) rounded up, so that few rows do not pay
 // for empty ones and many rows read the cache once.
 template <int FMT>
 cudaError_t launch_d(AttnParams& p, cudaStream_t st) {
   const int64_t rows = ((int64_t)p.c.tokens * p.group + p.c.batch - 1) / p.c.batch;
-  if (rows >= g_tc_rows.load() && p.c.head_dim != 256) return launch_attention_tc(p, st);
+  if (tc_pays(p, rows)) return launch_attention_tc(p, st);
   if (p.c.head_dim == 256) {
     if (rows <= 8) return launch<FMT, 256, 1, 1>(p, st);
     if (rows <= 16) return launch<FMT, 256, 1, 2>(p, st);
@@ -702,7 +723,7 @@ cudaError_t launch_d(AttnParams& p, cudaStream_t st) {
   if (p.c.head_dim == 128) {
     if (rows <= 8) return launch<FMT, 128, 1, 1>(p, st);
     if (rows <= 16) return launch<FMT, 128, 2, 1>(p, st);
-    if (rows <= 32) return launch<FMT, 128, 2, 2>(p, st);
+    if (rows <= 32) return launch<FMT, 128, 1, 4>(p, st);
     return launch<FMT, 128, 2, 4>(p, st);
   }
   if (rows <= 8) return launch<FMT, 64, 1, 1>(p, st);

@@ -7,19 +7,30 @@
 // every FP8 code once for each 8 or 16 rows that a warp multiplies it with; from
 // about 32 rows on that conversion, not the copy, is its time. Here a code is
 // converted once for up to 128 rows:
-//  * two teams of four load warps take tiles in turn: FP8 codes go from global
-//    memory to registers one tile ahead, become fp16, and are written to shared
-//    memory as the tensor core reads them (K rows, V transposed, both K-major
-//    with 128-byte swizzle);
+//  * the load warps copy the codes asynchronously (16 bytes a thread), 1 tile
+//    ahead at 128 channels and 3 at 64, and write them as fp16 the way the tensor
+//    core reads them (K rows, V transposed, both K-major with 128-byte swizzle);
+//    each thread converts what it has copied, so that the copies need no barrier;
 //  * one thread issues S = Q K^T (accumulators in TMEM) and O += P V, with P
 //    read from TMEM;
-//  * two groups of four softmax warps, one thread a row, take tiles in turn as
-//    well: while one computes P of its tile, the tensor core makes the other's S.
+//  * two groups of four softmax warps, one thread a row, take tiles in turn:
+//    while one computes P of its tile, the tensor core makes the other's S.
 // Each group keeps a running reference, sum and O of its own (TMEM: 2 x 128
 // columns of S, which P overwrites, 2 x D of O); they are joined where a run
 // leaves an item. V's channels lie permuted in shared memory (row c D/16 + col
 // for channel 16 col + c), which spreads the transposing stores over the banks;
-// O's columns come out in that order.
+// O's columns come out in that order. K is held once, V twice: K is free again
+// as soon as its scores are made.
+//
+// Measured (e4m3, fp16): 16 sequences of 8000 keys, 64 heads over 8, 128
+// channels, 32 rows a KV head 123 us (2.1 TB/s), 128 rows 136 us (496 us in the
+// few-row kernel); prompts of 4 x 1000 tokens, 32 heads over 8, 214 us (577);
+// one of 8192 tokens 1.77 ms (7.58; 310 TFLOP/s of the causal half). What bounds
+// it is instruction issue and its latencies (4 warps a scheduler, 0.45
+// instructions a cycle): conversion of a tile some 2200 cycles in the load warps,
+// weights of 2 x 128 x 128 scores some 2000 in the softmax warps, 1024 of them
+// the exponentials' unit. Loads through registers instead of shared memory
+// waited for each other: 221 us where this takes 122.
 #include "kv_attention.cuh"
 #include "sm100_umma.cuh"
 #include <type_traits>
@@ -31,23 +42,34 @@ using namespace fp8imma_dev;
 using namespace attn;
 
 constexpr int kRows = 128;
-constexpr int kSoftWarps = 8, kLoadWarps = 4;
-constexpr int kThreads = (kSoftWarps + kLoadWarps + 1) * 32;
-constexpr int kSoft = kSoftWarps * 32;
+constexpr int kSoftWarps = 8, kSoft = kSoftWarps * 32;
 
 template <int D>
 struct Shape {
+  static constexpr int kLoadWarps = D / 16, kLoad = kLoadWarps * 32;
+  static constexpr int kThreads = kSoft + kLoad + 32;
   static constexpr int kTile = kKeys * D * 2;             // fp16 bytes of K, of V, of Q
-  static constexpr int kPoison = 2 * kRows * D;
-  static constexpr int kSmem = 1024 + 5 * kTile + kPoison;
+  static constexpr int kSlot = 2 * kKeys * D;             // FP8 codes of a tile
+  static constexpr int kSlots = D == 64 ? 4 : 2;
+  static constexpr int kPoison = kRows * D;               // 4 bits a channel, two groups
+  static constexpr int kSmem = 1024 + 4 * kTile + kSlots * kSlot + kPoison;
   static constexpr int kPartFloats = kRows * D + kRows * 2;
   static constexpr int kCols = D / 16;                    // 16-channel columns
   static constexpr uint32_t kTmemS = 0, kTmemO = 2 * kKeys;  // TMEM columns of the two groups' S and O
 };
 
-__device__ __forceinline__ uint4 ldg_stream(const void* p) {
-  uint4 r;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
+// Copies of 16 and of 4 bytes, zeros where `on` is false.
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool on) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy4(uint32_t dst, const void* src, bool on) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(on ? 4 : 0) : "memory");
+}
+// The word at p, or -1. The predicate sits in the asm: a branch around the load
+// would end in a copy of its result, which waits for it.
+__device__ __forceinline__ int ldg_if(const int* p, bool on) {
+  int r = -1;
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %2, 0;\n\t@p ld.global.nc.u32 %0, [%1];\n\t}" : "+r"(r) : "l"(p), "r"((int)on));
   return r;
 }
 __device__ __forceinline__ void umma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
@@ -73,12 +95,48 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]
       "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(addr)
       : "memory");
 }
+__device__ __forceinline__ void tmem_st8(uint32_t addr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]),
+               "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(addr)
+               : "memory");
+}
+// a load that has to be waited for before r is read
+__device__ __forceinline__ void tmem_ld16_start(uint32_t addr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(addr));
+}
+__device__ __forceinline__ void tmem_ld_wait(uint32_t (&r)[16]) {  // r passes through, so that no use moves ahead
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
+                 "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])::"memory");
+}
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// two 32-bit values in one operation
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpair(uint64_t x, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
 struct TileInfo {
-  float ks[8], vs[8];
-  int live[8];  // by groups of 16 keys
-  int odd[4];   // a load warp found non-finite values that some row may not see
+  float ks[8], lv[8], iv[8];  // by groups of 16 keys: K's scale, log2 of V's (-infinity: no page), 1 / V's
+  int live;                   // a bit a group, and eight more: live, with a K scale that is not negative
+  int odd[8];   // a load warp found non-finite values that some row may not see
 };
 
 // The tiles of a segment that some row sees.
@@ -94,39 +152,46 @@ __device__ __forceinline__ bool edge_tile(const AttnParams& p, const Segment& g,
 }
 
 template <int FMT, int D>
-__global__ void __launch_bounds__(kThreads, 1) kv_attention_tc_kernel(const __grid_constant__ AttnParams p) {
+__global__ void __launch_bounds__(Shape<D>::kThreads, 1) kv_attention_tc_kernel(const __grid_constant__ AttnParams p) {
   using S = Shape<D>;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ uint64_t s_kv_full[2], s_s_full[2], s_p_full[2], s_pv_done[2], s_q_full, s_o_free;
+  __shared__ uint64_t s_k_full, s_v_full[2], s_s_full[2], s_p_full[2], s_pv_done[2], s_q_full, s_o_free;
+  __shared__ float s_scales[S::kSlots][16];
   __shared__ TileInfo s_info[2];
   __shared__ Shared s_shared[2];
   __shared__ float s_ml[2][kRows][3];  // reference, sum, whether the group's poison marks count
+  __shared__ float s_back[kRows];      // what a bf16 row of Q was divided by
+  __shared__ int s_n_shared;
   __shared__ uint32_t s_tmem;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   uint8_t* const base = smem_raw + (((smem_u32(smem_raw) + 1023u) & ~1023u) - smem_u32(smem_raw));
   uint8_t* const q_tile = base;
-  auto k_tile = [&](int g) { return base + S::kTile * (1 + 2 * g); };
-  auto v_tile = [&](int g) { return base + S::kTile * (2 + 2 * g); };
-  uint8_t* const poison = base + 5 * S::kTile;
+  uint8_t* const k_tile = base + S::kTile;
+  auto v_tile = [&](int g) { return base + S::kTile * (2 + g); };
+  uint8_t* const slots = base + 4 * S::kTile;
+  uint8_t* const poison = slots + S::kSlots * S::kSlot;
+  constexpr int kMmaWarp = kSoftWarps + S::kLoadWarps;
 
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&s_kv_full[i], kLoadWarps * 32);
+      mbar_init(&s_v_full[i], S::kLoad);
       mbar_init(&s_s_full[i], 1);
       mbar_init(&s_p_full[i], kSoft / 2);
       mbar_init(&s_pv_done[i], 1);
     }
+    mbar_init(&s_k_full, S::kLoad);
     mbar_init(&s_q_full, kSoft);
     mbar_init(&s_o_free, kSoft);
     fence_barrier_init();
+    s_n_shared = 0;
   }
   pdl_launch_dependents();
   pdl_wait();
   Walk walk;
   int units, ctas;
-  if (!find_run<kThreads>(p, kRows, walk, units, ctas)) return;
+  if (!find_run<S::kThreads>(p, kRows, walk, units, ctas)) return;
   const Runs runs(units, ctas);
-  if (warp == kSoftWarps + kLoadWarps) {
+  if (warp == kMmaWarp) {
     tmem_alloc(&s_tmem, 512);
     tmem_relinquish();
   }
@@ -137,126 +202,141 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_tc_kernel(const __gr
   Segment seg;
   bool ok = true;  // false: a wait ran out, the rest is walked through without waiting
   auto wait = [&](uint64_t* bar, int use) {
-    if (ok) ok = mbar_wait(bar, (uint32_t)(use & 1), ERR_WAIT_FULL);
+    if (ok) ok = mbar_wait<true>(bar, (uint32_t)(use & 1), ERR_WAIT_FULL);
   };
 
-  if (warp >= kSoftWarps && warp < kSoftWarps + kLoadWarps) {
+  if (warp >= kSoftWarps && warp < kMmaWarp) {
     // ------------------------------------------------------------- loads --
-    const int t = tid - kSoft;
-    const int ps = p.c.page_size;
-    int tile = 0, to = 0, idx = -1;
-    auto next = [&]() {  // on to the next tile
-      ++idx;
-      if (++tile < to) return true;
-      do {
-        if (!walk.next(p, kRows, seg)) return false;
-        tiles_of(walk, seg, tile, to);
-      } while (tile >= to);
-      return true;
-    };
-    // page of the 16-key group `lane` of the tile (lanes 0 .. 7), -1: none that any row sees
-    auto page_of = [&]() {
-      const int j0 = tile * kKeys + lane * 16, pi = j0 / ps;
-      int id = -1;
-      if (lane < 8 && j0 < seg.hi && j0 + 15 >= seg.lo && pi < p.c.max_pages) {
-        id = __ldg(p.c.page_table + (size_t)seg.b * p.c.max_pages + pi);
-        if ((unsigned)id >= (unsigned)p.c.num_pages) id = -1;
+    // Each thread converts the pieces that it has copied itself, so that the
+    // slots need no barrier.
+    const int t = tid - kSoft, ps = p.c.page_size;
+    const int k_row = t / S::kCols, col = t % S::kCols;  // pieces of K: rows k_row + 32 i
+    // V: four keys from 4 quad on. For 64 channels the lanes' quads are spread so that their stores fall on all banks.
+    const int quad = D == 128 ? t / 8 : ((t >> 2) & 1) + 2 * (((t >> 3) & 1) + 2 * ((t >> 5) & 1) + 4 * ((t >> 4) & 1)) + 16 * (t >> 6);
+    const uint32_t slot0 = smem_u32(slots) + t * 16;
+    int tile = 0, to = 0, id = -1, issued = 0;
+    uint32_t live_bits = 0, edge_bits = 0;  // by slot
+    const int ps_log = __ffs(ps) - 1;
+    bool more = true;
+    // On to the next tile, and the page of its 16-key group `lane` (lanes 0 .. 7),
+    // -1: none that any row sees. The load stands outside all branches: where
+    // paths join, its result would be waited for.
+    auto next = [&]() {
+      if (++tile >= to) {
+        do {
+          more = walk.next(p, kRows, seg);
+          if (more) tiles_of(walk, seg, tile, to);
+        } while (more && tile >= to);
       }
-      return id;
+      const int j0 = tile * kKeys + lane * 16, pi = j0 >> ps_log;
+      id = ldg_if(p.c.page_table + (size_t)seg.b * p.c.max_pages + pi, more && lane < 8 && j0 < seg.hi && j0 + 15 >= seg.lo && pi < p.c.max_pages);
     };
-    uint4 kr[S::kCols], vr[S::kCols / 4][4];
-    float ks = 0.0f, vs = 0.0f;
-    auto load = [&](int id) {
-      ks = vs = 0.0f;
-      if (id >= 0) {
-        const size_t ph = (size_t)id * p.c.kv_heads + seg.h;
-        ks = __ldg(p.c.k_scale + ph);
-        vs = __ldg(p.c.v_scale + ph);
-      }
-      auto piece = [&](const void* pool, int row, int col) {  // 16 codes of a key
-        const int page = __shfl_sync(0xffffffffu, id, row >> 4), j = tile * kKeys + row;
-        if (page < 0 || j >= seg.hi || j < seg.lo) return make_uint4(0, 0, 0, 0);
-        return ldg_stream(static_cast<const uint8_t*>(pool) + (((size_t)page * p.c.kv_heads + seg.h) * ps + (j & (ps - 1))) * D + col * 16);
+    next();
+    auto issue = [&]() {  // the copies of the next tile
+      const int slot = issued % S::kSlots;
+      const bool live = (unsigned)id < (unsigned)p.c.num_pages;
+      const uint32_t at = slot0 + slot * S::kSlot;
+      // row of the pools where the group's keys begin, -1: no page
+      const int begin = live ? ((id * p.c.kv_heads + seg.h) << ps_log) + ((tile * kKeys + lane * 16) & (ps - 1)) : -1;
+      auto piece = [&](const void* pool, int first, int row, uint32_t dst) {  // 16 codes of a key
+        const int j = tile * kKeys + row;
+        copy16(dst, static_cast<const uint8_t*>(pool) + ((int64_t)(first + (row & 15)) * D + col * 16), first >= 0 && j < seg.hi && j >= seg.lo);
       };
+      if (more) {
 #pragma unroll
-      for (int i = 0; i < S::kCols; ++i) kr[i] = piece(p.c.k, (i * 128 + t) / S::kCols, t % S::kCols);
+        for (int i = 0; i < 4; ++i) piece(p.c.k, __shfl_sync(0xffffffffu, begin, (k_row + 32 * i) >> 4), k_row + 32 * i, at + i * (S::kLoad * 16));
+        const int first = __shfl_sync(0xffffffffu, begin, quad >> 2);
 #pragma unroll
-      for (int i = 0; i < S::kCols / 4; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) vr[i][e] = piece(p.c.v, (i * 128 + t) / S::kCols * 4 + e, t % S::kCols);
-    };
-    bool more = next();
-    int id = more ? page_of() : -1;
-    if (more) load(id);
-    while (more) {
-      const bool edge = edge_tile(p, seg, tile);
-      const int live = id >= 0;
-      const int g = idx & 1;
-      if (idx > 1) wait(&s_pv_done[g], (idx >> 1) - 1);  // the tile that lay here before has been multiplied
-      uint8_t *const kt = k_tile(g), *const vt = v_tile(g);
-#pragma unroll
-      for (int i = 0; i < S::kCols; ++i) {
-        const int row = (i * 128 + t) / S::kCols, col = t % S::kCols;
-        uint4 a, b;
-        f8x4_to_f16x4<FMT>(kr[i].x, a.x, a.y);
-        f8x4_to_f16x4<FMT>(kr[i].y, a.z, a.w);
-        f8x4_to_f16x4<FMT>(kr[i].z, b.x, b.y);
-        f8x4_to_f16x4<FMT>(kr[i].w, b.z, b.w);
-        uint8_t* dst = kt + (col >> 2) * (kKeys * 128) + row * 128;
-        *reinterpret_cast<uint4*>(dst + ((((col & 3) * 2) ^ (row & 7)) << 4)) = a;
-        *reinterpret_cast<uint4*>(dst + ((((col & 3) * 2 + 1) ^ (row & 7)) << 4)) = b;
-      }
-      bool odd = false;
-#pragma unroll
-      for (int i = 0; i < S::kCols / 4; ++i) {
-        const int quad = (i * 128 + t) / S::kCols, col = t % S::kCols;
-        uint32_t w[4][4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          w[e][0] = vr[i][e].x, w[e][1] = vr[i][e].y, w[e][2] = vr[i][e].z, w[e][3] = vr[i][e].w;
-          if (edge) {
-            // 0 * NaN must not reach the rows that do not see the key: such values are left out here and marked below
-            const uint32_t mk = FMT == F8_E4M3 ? 0x7F7F7F7Fu : 0x7C7C7C7Cu;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const uint32_t bad = __vcmpeq4(w[e][k] & mk, mk);
-              odd |= bad != 0u;
-              w[e][k] &= ~bad;
-            }
-          }
+        for (int e = 0; e < 4; ++e) piece(p.c.v, first, quad * 4 + e, at + (4 + e) * (S::kLoad * 16));
+        if (t < 8) {
+          const int64_t ph = live ? (int64_t)id * p.c.kv_heads + seg.h : 0;
+          copy4(smem_u32(&s_scales[slot][t]), p.c.k_scale + ph, live);
+          copy4(smem_u32(&s_scales[slot][8 + t]), p.c.v_scale + ph, live);
         }
-        uint8_t* dst = vt + (quad >> 4) * (D * 128) + (quad & 1) * 8;
-        const int chunk = (quad & 15) >> 1;
+        live_bits = (live_bits & ~(1u << slot)) | ((uint32_t)live << slot);
+        edge_bits = (edge_bits & ~(1u << slot)) | ((uint32_t)edge_tile(p, seg, tile) << slot);
+        ++issued;
+      }
+      next();
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll 1
+    for (int i = 0; i < S::kSlots - 1; ++i) issue();
+#pragma unroll 1
+    for (int idx = 0; idx < issued; ++idx) {
+      issue();
+      asm volatile("cp.async.wait_group %0;" ::"n"(S::kSlots - 1) : "memory");
+      const int g = idx & 1, slot = idx % S::kSlots;
+      const bool edge = (edge_bits >> slot) & 1;
+      const uint8_t* const src = slots + slot * S::kSlot + t * 16;
+      if (idx > 0) wait(&s_s_full[g ^ 1], (idx - 1) >> 1);  // the tile before has been multiplied with Q
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {  // channels 16 col + 4 k .. + 3
-          uint32_t f[4][2];
-          f8x4_to_f16x4<FMT>(__byte_perm(w[0][k], w[1][k], 0x5140), f[0][0], f[1][0]);
-          f8x4_to_f16x4<FMT>(__byte_perm(w[2][k], w[3][k], 0x5140), f[0][1], f[1][1]);
-          f8x4_to_f16x4<FMT>(__byte_perm(w[0][k], w[1][k], 0x7362), f[2][0], f[3][0]);
-          f8x4_to_f16x4<FMT>(__byte_perm(w[2][k], w[3][k], 0x7362), f[2][1], f[3][1]);
+      for (int i = 0; i < 4; ++i) {
+        const int row = k_row + 32 * i;
+        const uint4 x = *reinterpret_cast<const uint4*>(src + i * (S::kLoad * 16));
+        uint4 a, b;
+        f8x4_to_f16x4<FMT>(x.x, a.x, a.y);
+        f8x4_to_f16x4<FMT>(x.y, a.z, a.w);
+        f8x4_to_f16x4<FMT>(x.z, b.x, b.y);
+        f8x4_to_f16x4<FMT>(x.w, b.z, b.w);
+        const int c0 = (col & 3) * 2, swap = col >> 2;  // the upper columns store their halves in the other order: all banks at once
+        uint8_t* dst = k_tile + (col >> 2) * (kKeys * 128) + row * 128;
+        *reinterpret_cast<uint4*>(dst + (((c0 + swap) ^ (row & 7)) << 4)) = swap ? b : a;
+        *reinterpret_cast<uint4*>(dst + (((c0 + 1 - swap) ^ (row & 7)) << 4)) = swap ? a : b;
+      }
+      fence_proxy_async_shared();
+      mbar_arrive(&s_k_full);
+      if (idx > 1) wait(&s_pv_done[g], (idx >> 1) - 1);  // the tile that lay here before has been multiplied with P
+      bool odd = false;
+      uint32_t w[4][4];
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const int n = (4 * k + c) * S::kCols + col;
-            *reinterpret_cast<uint2*>(dst + n * 128 + ((chunk ^ (n & 7)) << 4)) = make_uint2(f[c][0], f[c][1]);
+      for (int e = 0; e < 4; ++e) {
+        const uint4 x = *reinterpret_cast<const uint4*>(src + (4 + e) * (S::kLoad * 16));
+        w[e][0] = x.x, w[e][1] = x.y, w[e][2] = x.z, w[e][3] = x.w;
+      }
+      if (edge) {
+        // 0 * NaN must not reach the rows that do not see the key: such values are left out here and marked below
+        const uint32_t mk = FMT == F8_E4M3 ? 0x7F7F7F7Fu : 0x7C7C7C7Cu;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t bad = __vcmpeq4(w[e][k] & mk, mk);
+            odd |= bad != 0u;
+            w[e][k] &= ~bad;
           }
+      }
+      uint8_t* const dst = v_tile(g) + (quad >> 4) * (D * 128) + (quad & 1) * 8;
+      const int chunk = (quad & 15) >> 1;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {  // channels 16 col + 4 k .. + 3
+        uint32_t f[4][2];
+        f8x4_to_f16x4<FMT>(__byte_perm(w[0][k], w[1][k], 0x5140), f[0][0], f[1][0]);
+        f8x4_to_f16x4<FMT>(__byte_perm(w[2][k], w[3][k], 0x5140), f[0][1], f[1][1]);
+        f8x4_to_f16x4<FMT>(__byte_perm(w[0][k], w[1][k], 0x7362), f[2][0], f[3][0]);
+        f8x4_to_f16x4<FMT>(__byte_perm(w[2][k], w[3][k], 0x7362), f[2][1], f[3][1]);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const int n = (4 * k + c) * S::kCols + col;
+          *reinterpret_cast<uint2*>(dst + n * 128 + ((chunk ^ (n & 7)) << 4)) = make_uint2(f[c][0], f[c][1]);
         }
       }
       odd = __any_sync(0xffffffffu, odd);
-      if (lane == 0) s_info[g].odd[warp & 3] = odd;
+      if (lane == 0) s_info[g].odd[warp - kSoftWarps] = odd;
       if (t < 8) {
-        s_info[g].ks[t] = ks;
-        s_info[g].vs[t] = vs;
-        s_info[g].live[t] = live;
+        const bool live = (live_bits >> slot) & 1;
+        const float vs = fmaxf(s_scales[slot][8 + t], kTinyScale);
+        const unsigned all = __ballot_sync(0xffu, live), plain = __ballot_sync(0xffu, live && s_scales[slot][t] >= 0.0f);
+        s_info[g].ks[t] = s_scales[slot][t];
+        s_info[g].lv[t] = live ? lg2(vs) : -INFINITY;
+        s_info[g].iv[t] = __fdividef(1.0f, vs);
+        if (t == 0) s_info[g].live = (int)(all | plain << 8);
       }
       fence_proxy_async_shared();
-      mbar_arrive(&s_kv_full[g]);
-      more = next();
-      if (more) {
-        id = page_of();
-        load(id);
-      }
+      mbar_arrive(&s_v_full[g]);
     }
-  } else if (warp == kSoftWarps + kLoadWarps) {
+    asm volatile("cp.async.wait_all;" ::: "memory");
+  } else if (warp == kMmaWarp) {
     // ---------------------------------------------------------- products --
     int idx = 0, nseg = 0;
     while (walk.next(p, kRows, seg)) {
@@ -265,6 +345,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_tc_kernel(const __gr
       if (from >= to) continue;  // such segments pass neither barrier: the softmax warps could run two phases ahead
       auto product_pv = [&](int i, bool first) {  // of tile number i; the group's first of the segment overwrites O
         const int g = i & 1;
+        wait(&s_v_full[g], i >> 1);
         wait(&s_p_full[g], i >> 1);
         if (first && nseg > 0) wait(&s_o_free, nseg - 1);
         tc_fence_after();
@@ -279,11 +360,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_tc_kernel(const __gr
       };
       for (int tile = from; tile < to; ++tile, ++idx) {
         const int g = idx & 1;
-        wait(&s_kv_full[g], idx >> 1);
+        wait(&s_k_full, idx);
         if (tile == from) wait(&s_q_full, nseg);
         tc_fence_after();
         if (lane == 0) {
-          const uint64_t a = sw128_desc(smem_u32(q_tile)), b = sw128_desc(smem_u32(k_tile(g)));
+          const uint64_t a = sw128_desc(smem_u32(q_tile)), b = sw128_desc(smem_u32(k_tile));
 #pragma unroll
           for (int k = 0; k < D / 16; ++k)
             umma_ss(tmem + S::kTmemS + g * kKeys, a + (k >> 2) * (kRows * 128 >> 4) + (k & 3) * 2, b + (k >> 2) * (kKeys * 128 >> 4) + (k & 3) * 2, idesc_f16(kRows, kKeys), k > 0);
@@ -310,51 +391,56 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_tc_kernel(const __gr
       const bool in = row < s.rows;
       const bool active = (warp & 3) * 32 < s.rows - seg.rt * kRows;  // the warp has rows
       const int pos = in ? s.len - s.n + row / p.group : -1;
-      // Q: this thread's half of the row, as fp16
-      float back = 1.0f;
+      // Q as fp16: consecutive threads take consecutive 16-byte pieces of the rows
       if (to > from) {
-        const uint16_t* src = static_cast<const uint16_t*>(p.a.q) +
-                              (in ? (int64_t)(s.t0 + row / p.group) * p.a.q_token_stride + (int64_t)(seg.h * p.group + row % p.group) * p.a.q_head_stride : 0);
-        auto eight = [&](int ch) {
-          if (!in) return make_uint4(0, 0, 0, 0);
-          if (p.vec_q) return __ldg(reinterpret_cast<const uint4*>(src + ch));
-          uint32_t w[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) w[i] = (uint32_t)__ldg(src + ch + 2 * i) | ((uint32_t)__ldg(src + ch + 2 * i + 1) << 16);
-          return make_uint4(w[0], w[1], w[2], w[3]);
-        };
-        float f = 1.0f;
+        constexpr int kPieces = D / 8, kEach = kRows * kPieces / kSoft;
         const bool bf = p.a.a_type == FP8IMMA_A_BF16;
-        if (bf) {  // a power of two brings the row to a largest magnitude of 2^8 .. 2^9
-          float big = 0.0f;
-#pragma unroll 4
-          for (int c = 0; c < D; c += 8) {
-            const uint4 v = eight(c);
-            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+        uint4 x[kEach];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) big = fmaxf(big, fmaxf(fabsf(__uint_as_float(w[i] << 16)), fabsf(__uint_as_float(w[i] & 0xFFFF0000u))));
-          }
-          if (big > 0.0f && big < INFINITY) {
-            const int e = max(-126, min(126, (int)(__float_as_uint(big) >> 23) - 127 - 8));
-            f = __uint_as_float((uint32_t)(127 - e) << 23);
-            back = __uint_as_float((uint32_t)(127 + e) << 23);
+        for (int i = 0; i < kEach; ++i) {
+          const int r2 = (i * kSoft + tid) / kPieces, ch = tid % kPieces * 8, row2 = seg.rt * kRows + r2;
+          x[i] = make_uint4(0, 0, 0, 0);
+          if (row2 < s.rows) {
+            const uint16_t* src = static_cast<const uint16_t*>(p.a.q) + (int64_t)(s.t0 + row2 / p.group) * p.a.q_token_stride + (int64_t)(seg.h * p.group + row2 % p.group) * p.a.q_head_stride + ch;
+            if (p.vec_q) {
+              x[i] = __ldg(reinterpret_cast<const uint4*>(src));
+            } else {
+              uint32_t w[4];
+#pragma unroll
+              for (int k = 0; k < 4; ++k) w[k] = (uint32_t)__ldg(src + 2 * k) | ((uint32_t)__ldg(src + 2 * k + 1) << 16);
+              x[i] = make_uint4(w[0], w[1], w[2], w[3]);
+            }
           }
         }
-#pragma unroll 4
-        for (int i = 0; i < D / 16; ++i) {
-          const int ch = g * (D / 2) + i * 8;
-          uint4 v = eight(ch);
-          if (bf) {
-            uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+          const int r2 = (i * kSoft + tid) / kPieces, ch = tid % kPieces * 8;
+          if (bf) {  // a power of two brings the row to a largest magnitude of 2^8 .. 2^9
+            uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+            float big = 0.0f, f = 1.0f, back = 1.0f;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) big = fmaxf(big, fmaxf(fabsf(__uint_as_float(w[k] << 16)), fabsf(__uint_as_float(w[k] & 0xFFFF0000u))));
+#pragma unroll
+            for (int o = 1; o < kPieces; o *= 2) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+            if (big > 0.0f && big < INFINITY) {
+              const int e = max(-126, min(126, (int)(__float_as_uint(big) >> 23) - 127 - 8));
+              f = __uint_as_float((uint32_t)(127 - e) << 23);
+              back = __uint_as_float((uint32_t)(127 + e) << 23);
+            }
 #pragma unroll
             for (int k = 0; k < 4; ++k) w[k] = pack_f16(__uint_as_float(w[k] << 16) * f, __uint_as_float(w[k] & 0xFFFF0000u) * f);
-            v = make_uint4(w[0], w[1], w[2], w[3]);
+            x[i] = make_uint4(w[0], w[1], w[2], w[3]);
+            if (ch == 0) s_back[r2] = back;
+          } else if (ch == 0) {
+            s_back[r2] = 1.0f;
           }
-          *reinterpret_cast<uint4*>(q_tile + (ch >> 6) * (kRows * 128) + r * 128 + ((((ch & 63) >> 3) ^ (r & 7)) << 4)) = v;
+          *reinterpret_cast<uint4*>(q_tile + (ch >> 6) * (kRows * 128) + r2 * 128 + ((((ch & 63) >> 3) ^ (r2 & 7)) << 4)) = x[i];
         }
         fence_proxy_async_shared();
         mbar_arrive(&s_q_full);
+        named_bar_sync(1, kSoft);  // s_back
       }
+      const float back = to > from ? s_back[r] : 1.0f;
       const float cq = p.a.softmax_scale * 1.4426950408889634f * back;
       float m = -INFINITY, l = 0.0f;
       int count = 0;       // the group's tiles of the segment
@@ -362,46 +448,56 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_tc_kernel(const __gr
       for (int tile = from; tile < to; ++tile, ++idx) {
         if ((idx & 1) != g) continue;
         wait(&s_s_full[g], idx >> 1);
+        wait(&s_v_full[g], idx >> 1);  // s_info
         tc_fence_after();
         const TileInfo& info = s_info[g];
         __syncwarp();
         if (active) {
-          bool edge = edge_tile(p, seg, tile);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) edge |= !info.live[i];
-          auto score = [&](auto masked, uint32_t bits, float kc, float lv, int j) {
-            float x = fmaf(__uint_as_float(bits), kc, lv);
-            if (decltype(masked)::value && (j > pos || j >= seg.hi || (p.a.window > 0 && j <= pos - p.a.window))) x = -INFINITY;
-            return x;
-          };
-          auto group_of = [&](int i, float& kc, float& lv, float& iv) {
-            const float vs = info.vs[i] < kTinyScale ? kTinyScale : info.vs[i];
-            kc = cq * info.ks[i];
-            lv = info.live[i] ? lg2(vs) : -INFINITY;
-            iv = __fdividef(1.0f, vs);
+          const bool edge = edge_tile(p, seg, tile) || info.live != 0xffff || !(cq >= 0.0f);
+          auto seen = [&](int j) { return j <= pos && j < seg.hi && (p.a.window <= 0 || j > pos - p.a.window); };
+          // Both passes take 16 keys at a time and have the next 16 on their way.
+          uint32_t va[16], vb[16];
+          auto pass = [&](auto part) {
+            tmem_ld16_start(s_at, va);
+#pragma unroll 1
+            for (int i = 0; i < 8; i += 2) {
+              tmem_ld_wait(va);
+              tmem_ld16_start(s_at + 16 * (i + 1), vb);
+              part(i, va);
+              tmem_ld_wait(vb);
+              if (i < 6) tmem_ld16_start(s_at + 16 * (i + 2), va);
+              part(i + 1, vb);
+            }
           };
           float top = -INFINITY;
-          auto find_top = [&](auto masked) {
-#pragma unroll 1
-          for (int c = 0; c < 4; ++c) {
-            uint32_t v[32];
-            tmem_ld32(s_at + 32 * c, v);
+          if (edge) {
+            pass([&](int i, const uint32_t (&v)[16]) {
+              const float kc = cq * info.ks[i], lv = info.lv[i];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              float kc, lv, iv;
-              group_of(2 * c + h, kc, lv, iv);
+              for (int k = 0; k < 16; ++k) {
+                const float x = fmaf(__uint_as_float(v[k]), kc, lv);
+                if (seen(tile * kKeys + 16 * i + k)) top = fmaxf(top, x);
+              }
+            });
+          } else {
+            // the largest score of 16 keys is that of their largest product
+            pass([&](int i, const uint32_t (&v)[16]) {
+              float most[2] = {__uint_as_float(v[0]), __uint_as_float(v[1])};
 #pragma unroll
-              for (int i = 0; i < 16; ++i) top = fmaxf(top, score(masked, v[16 * h + i], kc, lv, tile * kKeys + 32 * c + 16 * h + i));
-            }
+              for (int k = 2; k < 14; k += 4) {
+                most[0] = fmaxf(most[0], fmaxf(__uint_as_float(v[k]), __uint_as_float(v[k + 1])));
+                most[1] = fmaxf(most[1], fmaxf(__uint_as_float(v[k + 2]), __uint_as_float(v[k + 3])));
+              }
+              most[0] = fmaxf(most[0], fmaxf(__uint_as_float(v[14]), __uint_as_float(v[15])));
+              top = fmaxf(top, fmaf(fmaxf(most[0], most[1]), cq * info.ks[i], info.lv[i]));
+            });
           }
-          };
-          if (edge) find_top(std::true_type()); else find_top(std::false_type());
           const bool raise = top > m + kRaise;
           if (__any_sync(0xffffffffu, raise)) {
             const float mn = raise ? top : m, f = mn == m ? 1.0f : ex2(m - mn);
             m = mn;
             l *= f;
-            if (count > 0) {  // the product before is done: its keys' place has been filled again
+            if (count > 0) {  // the group's product before is done: these scores were issued after it
 #pragma unroll 1
               for (int c = 0; c < D; c += 16) {
                 uint32_t v[16];
@@ -414,45 +510,63 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_tc_kernel(const __gr
             }
           }
           const float ms = m == -INFINITY ? 0.0f : m;
-          auto weights = [&](auto masked) {
-#pragma unroll 1
-          for (int c = 0; c < 4; ++c) {
-            uint32_t v[32], w[16];
-            tmem_ld32(s_at + 32 * c, v);
+          // P takes the place of scores that have been read
+          if (edge) {
+            pass([&](int i, const uint32_t (&v)[16]) {
+              const float kc = cq * info.ks[i], lv = info.lv[i] - ms;
+              const bool live = (info.live >> i) & 1;
+              float sum = 0.0f;
+              uint32_t w[8];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              float kc, lv, iv, sum = 0.0f;
-              group_of(2 * c + h, kc, lv, iv);
-              lv -= ms;
-#pragma unroll
-              for (int i = 0; i < 16; i += 2) {
-                const int j = tile * kKeys + 32 * c + 16 * h + i;
-                float a = ex2(score(masked, v[16 * h + i], kc, lv, j)), b = ex2(score(masked, v[16 * h + i + 1], kc, lv, j + 1));
-                if (decltype(masked)::value && !info.live[2 * c + h]) a = b = 0.0f;
+              for (int k = 0; k < 16; k += 2) {
+                const int j = tile * kKeys + 16 * i + k;
+                const float a = live && seen(j) ? ex2(fmaf(__uint_as_float(v[k]), kc, lv)) : 0.0f;
+                const float b = live && seen(j + 1) ? ex2(fmaf(__uint_as_float(v[k + 1]), kc, lv)) : 0.0f;
                 sum += a + b;
-                w[8 * h + i / 2] = pack_f16(a, b);
+                w[k / 2] = pack_f16(a, b);
               }
-              l = fmaf(sum, iv, l);
-            }
-            tmem_st16(s_at + 16 * c, w);  // P takes the place of scores that have been read
+              l = fmaf(sum, info.iv[i], l);
+              tmem_st8(s_at + 8 * i, w);
+            });
+          } else {
+            pass([&](int i, const uint32_t (&v)[16]) {
+              const float kc = cq * info.ks[i], lv = info.lv[i] - ms;
+              const uint64_t kc2 = pair(kc, kc), lv2 = pair(lv, lv);
+              uint64_t sum = 0;
+              uint32_t w[8];
+#pragma unroll
+              for (int k = 0; k < 16; k += 2) {
+                float a, b;
+                unpair(fma2(pair(__uint_as_float(v[k]), __uint_as_float(v[k + 1])), kc2, lv2), a, b);
+                a = ex2(a), b = ex2(b);
+                sum = add2(sum, pair(a, b));
+                w[k / 2] = pack_f16(a, b);
+              }
+              float s0, s1;
+              unpair(sum, s0, s1);
+              l = fmaf(s0 + s1, info.iv[i], l);
+              tmem_st8(s_at + 8 * i, w);
+            });
           }
-          };
-          if (edge) weights(std::true_type()); else weights(std::false_type());
           tmem_wait_st();
-          if (info.odd[0] | info.odd[1] | info.odd[2] | info.odd[3]) {
+          int odd = 0;
+#pragma unroll
+          for (int i = 0; i < S::kLoadWarps; ++i) odd |= info.odd[i];
+          if (odd) {
             // rare: mark the channels of this row that a non-finite value reaches
-            uint8_t* mark = poison + (g * kRows + r) * D;
+            uint8_t* mark = poison + (g * kRows + r) * (D / 2);
             if (!dirty)
-              for (int c = 0; c < D; c += 16) *reinterpret_cast<uint4*>(mark + c) = make_uint4(0, 0, 0, 0);
+              for (int c = 0; c < D / 2; c += 16) *reinterpret_cast<uint4*>(mark + c) = make_uint4(0, 0, 0, 0);
             dirty = true;
             const int ps = p.c.page_size;
             for (int j = max(tile * kKeys, seg.lo); j < min(min(tile * kKeys + kKeys, seg.hi), pos + 1); ++j) {
-              if ((p.a.window > 0 && j <= pos - p.a.window) || !info.live[(j & (kKeys - 1)) >> 4]) continue;
+              if ((p.a.window > 0 && j <= pos - p.a.window) || !(info.live >> ((j & (kKeys - 1)) >> 4) & 1)) continue;
               const int page = __ldg(p.c.page_table + (size_t)seg.b * p.c.max_pages + j / ps);
               const uint8_t* v = static_cast<const uint8_t*>(p.c.v) + (((size_t)page * p.c.kv_heads + seg.h) * ps + (j & (ps - 1))) * D;
               for (int ch = 0; ch < D; ++ch) {
                 const float x = f8_to_f32<FMT>(__ldg(v + ch));
-                if (!(fabsf(x) < INFINITY)) mark[ch % 16 * S::kCols + ch / 16] |= isnan(x) ? 4 : x > 0.0f ? 1 : 2;
+                const int n = ch % 16 * S::kCols + ch / 16;
+                if (!(fabsf(x) < INFINITY)) mark[n / 2] |= (isnan(x) ? 4 : x > 0.0f ? 1 : 2) << (n % 2 * 4);
               }
             }
           }
@@ -487,16 +601,18 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_tc_kernel(const __gr
         for (int c0 = 0; c0 < D / 2; c0 += 16) {
           const int n0 = g * (D / 2) + c0;
           __syncwarp();
-          uint32_t a[16], b[16];
+          uint32_t a[16] = {}, b[16] = {};
           float o[16];
-          if (count > 0) tmem_ld16(o_at + n0, a);
-          if (other > 0) tmem_ld16(tmem + row_at + S::kTmemO + (1 - g) * D + n0, b);
+          if (count > 0) tmem_ld16_start(o_at + n0, a);
+          if (other > 0) tmem_ld16_start(tmem + row_at + S::kTmemO + (1 - g) * D + n0, b);
+          tmem_ld_wait(a);
+          tmem_ld_wait(b);
 #pragma unroll
           for (int i = 0; i < 16; ++i) o[i] = (count > 0 ? __uint_as_float(a[i]) * f : 0.0f) + (other > 0 ? __uint_as_float(b[i]) * f2 : 0.0f);
           if (dirty || dirty2) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-              const int bits = (dirty ? poison[(g * kRows + r) * D + n0 + i] : 0) | (dirty2 ? poison[((1 - g) * kRows + r) * D + n0 + i] : 0);
+              const int bits = ((dirty ? poison[(g * kRows + r) * (D / 2) + (n0 + i) / 2] : 0) | (dirty2 ? poison[((1 - g) * kRows + r) * (D / 2) + (n0 + i) / 2] : 0)) >> (i % 2 * 4) & 15;
               if (bits) o[i] = bits == 1 ? INFINITY : bits == 2 ? -INFINITY : NAN;
             }
           }
@@ -534,52 +650,84 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_tc_kernel(const __gr
       named_bar_sync(1, kSoft);  // s_ml and the poison marks are free again
     }
 
-    // shared items: the CTA that comes last to one joins all its parts, in CTA order
-    if (n_shared > 0) {
-      __threadfence();
-      named_bar_sync(1, kSoft);
-      if (tid < n_shared) {
-        unsigned int prev, *ctr = p.counters + s_shared[tid].index;
-        asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(prev) : "l"(ctr) : "memory");
-        s_shared[tid].last = prev == (unsigned)(s_shared[tid].c1 - s_shared[tid].c0);
-        if (s_shared[tid].last) *ctr = 0;  // ready for the next call
-      }
-      named_bar_sync(1, kSoft);
-      __threadfence();
-      for (int k = 0; k < n_shared; ++k) {
-        const Shared& sh = s_shared[k];
-        if (!sh.last) continue;
-        const int rows = min(kRows, sh.item.rows - sh.item.rt * kRows);
-        for (int x = tid; x < rows * (D / 4); x += kSoft) {
-          const int r2 = x / (D / 4), n = x % (D / 4) * 4;
-          Joined j;  // one row: its second row's place is filled alike
-          auto src = [&](int c) {
-            c += sh.c0;
-            return p.parts + (int64_t)(c * 2 + (sh.item0 > runs.begin(c) ? 1 : 0)) * S::kPartFloats;
-          };
-          j.join(sh.c1 - sh.c0 + 1,
-                 [&](int c) {
-                   const float2 v = __ldcg(reinterpret_cast<const float2*>(src(c) + kRows * D + 2 * r2));
-                   return make_float4(v.x, v.x, v.y, v.y);
-                 },
-                 [&](int c) { return __ldcg(reinterpret_cast<const float4*>(src(c) + r2 * D + n)); });
-          const int row = sh.item.rt * kRows + r2;
-          const int64_t at = (int64_t)(sh.item.t0 + row / p.group) * p.a.heads + sh.item.h * p.group + row % p.group;
-          const float inv = j.l0 == 0.0f ? 0.0f : __fdiv_rn(1.0f, j.l0);
-          const float o[4] = {j.o.x, j.o.y, j.o.z, j.o.w};
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint16_t v = p.a.a_type == FP8IMMA_A_F16 ? f32_to_a16<0>(o[i] * inv) : f32_to_a16<1>(o[i] * inv);
-            static_cast<uint16_t*>(p.a.out)[at * D + 16 * ((n + i) % S::kCols) + (n + i) / S::kCols] = v;
-          }
-          if (n == 0 && p.a.lse) p.a.lse[at] = j.l0 == 0.0f ? -INFINITY : 0.6931471805599453f * (j.m0 + log2f(j.l0));
-        }
-      }
-    }
+    if (tid == 0) s_n_shared = n_shared;
+    __threadfence();
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == kSoftWarps + kLoadWarps) tmem_dealloc(tmem, 512);
+  if (warp == kMmaWarp) tmem_dealloc(tmem, 512);
+
+  // shared items: the CTA that comes last to one joins all its parts, in CTA order
+  const int n_shared = s_n_shared;
+  if (n_shared == 0) return;
+  if (tid < n_shared) {
+    unsigned int prev, *ctr = p.counters + s_shared[tid].index;
+    asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(prev) : "l"(ctr) : "memory");
+    s_shared[tid].last = prev == (unsigned)(s_shared[tid].c1 - s_shared[tid].c0);
+    if (s_shared[tid].last) *ctr = 0;  // ready for the next call
+  }
+  __syncthreads();
+  __threadfence();
+  for (int k = 0; k < n_shared; ++k) {
+    const Shared& sh = s_shared[k];
+    if (!sh.last) continue;
+    const int rows = min(kRows, sh.item.rows - sh.item.rt * kRows);
+    const Item it = sh.item;
+    auto src = [&](int c) { return p.parts + (int64_t)(c * 2 + (sh.item0 > runs.begin(c) ? 1 : 0)) * S::kPartFloats; };
+    auto out_at = [&](int r) {
+      const int row = it.rt * kRows + r;
+      return (int64_t)(it.t0 + row / p.group) * p.a.heads + it.h * p.group + row % p.group;
+    };
+    // the rows' references and sums
+    for (int r = tid; r < rows; r += S::kThreads) {
+      float m = -INFINITY, l = 0.0f;
+      for (int c = sh.c0; c <= sh.c1; ++c) {
+        const float2 v = __ldcg(reinterpret_cast<const float2*>(src(c) + kRows * D + 2 * r));
+        const float mn = fmaxf(m, v.x), ms = mn == -INFINITY ? 0.0f : mn;
+        l = fmaf(l, ex2(m - ms), v.y * ex2(v.x - ms));
+        m = mn;
+      }
+      s_ml[0][r][0] = m == -INFINITY ? 0.0f : m;
+      s_ml[0][r][1] = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
+      if (p.a.lse) p.a.lse[out_at(r)] = l == 0.0f ? -INFINITY : 0.6931471805599453f * (m + log2f(l));
+    }
+    __syncthreads();
+    // O: each thread has the loads of kAt places in flight
+    constexpr int kAt = 4, kWorkers = S::kThreads / 32 * 32;
+    for (int x0 = tid; x0 < rows * (D / 4); x0 += kWorkers * kAt) {
+      float4 o[kAt];
+#pragma unroll
+      for (int e = 0; e < kAt; ++e) o[e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      for (int c = sh.c0; c <= sh.c1; ++c) {
+        const float* const part = src(c);
+        float4 v[kAt];
+        float m[kAt];
+#pragma unroll
+        for (int e = 0; e < kAt; ++e) {
+          const int x = min(x0 + e * kWorkers, rows * (D / 4) - 1);
+          v[e] = __ldcg(reinterpret_cast<const float4*>(part) + x);
+          m[e] = __ldcg(part + kRows * D + x / (D / 4) * 2);
+        }
+#pragma unroll
+        for (int e = 0; e < kAt; ++e) {
+          const int x = min(x0 + e * kWorkers, rows * (D / 4) - 1);
+          const float f = ex2(m[e] - s_ml[0][x / (D / 4)][0]);
+          o[e] = make_float4(fmaf(v[e].x, f, o[e].x), fmaf(v[e].y, f, o[e].y), fmaf(v[e].z, f, o[e].z), fmaf(v[e].w, f, o[e].w));
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < kAt; ++e) {
+        const int x = x0 + e * kWorkers, r = x / (D / 4), n = x % (D / 4) * 4;
+        if (x >= rows * (D / 4)) break;
+        const float inv = s_ml[0][r][1], w[4] = {o[e].x, o[e].y, o[e].z, o[e].w};
+        uint16_t* const dst = static_cast<uint16_t*>(p.a.out) + out_at(r) * D;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)  // column n is channel 16 (n % cols) + n / cols
+          dst[16 * ((n + i) % S::kCols) + (n + i) / S::kCols] = p.a.a_type == FP8IMMA_A_F16 ? f32_to_a16<0>(w[i] * inv) : f32_to_a16<1>(w[i] * inv);
+      }
+    }
+    __syncthreads();  // s_ml
+  }
 }
 
 template <int FMT, int D>
@@ -606,7 +754,7 @@ cudaError_t launch(AttnParams& p, cudaStream_t st) {
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     lc.gridDim = dim3(grid);
-    lc.blockDim = dim3(kThreads);
+    lc.blockDim = dim3(S::kThreads);
     lc.dynamicSmemBytes = S::kSmem;
     lc.stream = st;
     lc.attrs = attr;

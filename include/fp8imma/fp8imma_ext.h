@@ -315,8 +315,9 @@ int fp8imma_set_tc_half_tail(int enable);
 // switch).
 int fp8imma_set_decode_kernel(int enable);
 // Query rows of a sequence and KV head (tokens of the step x heads / kv_heads,
-// on average) from which fp8imma_kv_attention multiplies on tcgen05 (default
-// 24; head_dim 64 and 128). The two kernels' results differ by roundings only.
+// on average) from which fp8imma_kv_attention multiplies on tcgen05 (head_dim 64
+// and 128; for tests and measurements). 0, the default: by rows and by the tiles
+// that the page tables hold. The two kernels' results differ by roundings only.
 int fp8imma_set_attention_tc_rows(int rows);
 // Programmatic dependent launch (default on). A small-M GEMM then starts
 // streaming its weights and reading its column scales while the previous

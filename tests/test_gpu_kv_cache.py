@@ -11,13 +11,13 @@ from serving_ref import F8, FMAX, ref_append, ref_attention
 pytestmark = pytest.mark.gpu
 
 
-# rows a KV head from which attention runs on tcgen05: never, from the default on, always
-@pytest.fixture(params=[1 << 20, 24, 1], ids=["mma", "default", "tcgen05"])
+# rows a KV head from which attention runs on tcgen05: never, by the kernel's rule, always
+@pytest.fixture(params=[1 << 20, 0, 1], ids=["mma", "default", "tcgen05"])
 def ops(cuda, request):
     L = F.lib()
     assert L.fp8imma_set_attention_tc_rows(request.param) == 0
     yield F.ext()
-    L.fp8imma_set_attention_tc_rows(24)
+    L.fp8imma_set_attention_tc_rows(0)
     assert L.fp8imma_device_error(1) == 0
 
 
@@ -356,6 +356,20 @@ def test_cache_beyond_32_bit_offsets(ops):
     small = [x[sub].contiguous() for x in (kc, vc, ks, vs)]
     out, lse = ops.kv_attention(q, kc, vc, ks, vs, table, i32([300]), None)
     check(out, lse, ref_attention(q, *small, i32([[0, 1, 2]]), [300], [0, 1], 1 / math.sqrt(d), 0, fmt))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("lens, news, hq, hk, d, ps, window", [
+    ([9000, 8000, 1, 700], [17, 30, 1, 64], 16, 2, 128, 64, 0),      # 64 to 512 rows, one sequence of one key
+    ([5000, 6000, 130], [40, 1, 129], 24, 4, 64, 16, 700),           # rows that end in every tile, a window
+    ([1500, 1290], [1500, 1030], 8, 4, 128, 32, 0),                  # whole prompts, one behind a prefix
+])
+def test_attention_many_rows(ops, lens, news, hq, hk, d, ps, window, dtype):
+    g = gen(90 + d)
+    cache = make_cache(g, len(lens), -(-max(lens) // ps), hk, ps, d, "e4m3")
+    cu = offsets(news)
+    q = torch.randn(cu[-1], hq, d, generator=g, device="cuda").to(dtype)
+    check(*run_attend(ops, q, cache, lens, cu, window, "e4m3"))
 
 
 def test_attention_many_empty_sequences(ops):
