@@ -133,6 +133,14 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   return r;
 }
 
+// two fp16 values times a power of two
+__device__ __forceinline__ uint32_t mul_f16x2(uint32_t x, float f) {
+  const uint32_t f2 = pack_f16(f, f);
+  uint32_t r;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(f2));
+  return r;
+}
+
 struct TileInfo {
   float ks[8], lv[8], iv[8];  // by groups of 16 keys: K's scale, log2 of V's (-infinity: no page), 1 / V's
   int live;                   // a bit a group, and eight more: live, with a K scale that is not negative
@@ -155,9 +163,9 @@ template <int FMT, int D>
 __global__ void __launch_bounds__(Shape<D>::kThreads, 1) kv_attention_tc_kernel(const __grid_constant__ AttnParams p) {
   using S = Shape<D>;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ uint64_t s_k_full, s_v_full[2], s_s_full[2], s_p_full[2], s_pv_done[2], s_q_full, s_o_free;
+  __shared__ uint64_t s_k_full[2], s_v_full[2], s_s_full[2], s_p_full[2], s_pv_done[2], s_q_full, s_o_free;
   __shared__ float s_scales[S::kSlots][16];
-  __shared__ TileInfo s_info[2];
+  __shared__ TileInfo s_info[4];       // by tile number: a tile's is read until its weights are done, and four tiles on they are
   __shared__ Shared s_shared[2];
   __shared__ float s_ml[2][kRows][3];  // reference, sum, whether the group's poison marks count
   __shared__ float s_back[kRows];      // what a bf16 row of Q was divided by
@@ -174,12 +182,12 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) kv_attention_tc_kernel(
 
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_k_full[i], S::kLoad);
       mbar_init(&s_v_full[i], S::kLoad);
       mbar_init(&s_s_full[i], 1);
       mbar_init(&s_p_full[i], kSoft / 2);
       mbar_init(&s_pv_done[i], 1);
     }
-    mbar_init(&s_k_full, S::kLoad);
     mbar_init(&s_q_full, kSoft);
     mbar_init(&s_o_free, kSoft);
     fence_barrier_init();
@@ -240,7 +248,8 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) kv_attention_tc_kernel(
       const int begin = live ? ((id * p.c.kv_heads + seg.h) << ps_log) + ((tile * kKeys + lane * 16) & (ps - 1)) : -1;
       auto piece = [&](const void* pool, int first, int row, uint32_t dst) {  // 16 codes of a key
         const int j = tile * kKeys + row;
-        copy16(dst, static_cast<const uint8_t*>(pool) + ((int64_t)(first + (row & 15)) * D + col * 16), first >= 0 && j < seg.hi && j >= seg.lo);
+        const bool on = first >= 0 && j < seg.hi && j >= seg.lo;
+        copy16(dst, static_cast<const uint8_t*>(pool) + ((int64_t)(on ? first + (row & 15) : 0) * D + col * 16), on);
       };
       if (more) {
 #pragma unroll
@@ -273,19 +282,28 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) kv_attention_tc_kernel(
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int row = k_row + 32 * i;
-        const uint4 x = *reinterpret_cast<const uint4*>(src + i * (S::kLoad * 16));
-        uint4 a, b;
-        f8x4_to_f16x4<FMT>(x.x, a.x, a.y);
-        f8x4_to_f16x4<FMT>(x.y, a.z, a.w);
-        f8x4_to_f16x4<FMT>(x.z, b.x, b.y);
-        f8x4_to_f16x4<FMT>(x.w, b.z, b.w);
-        const int c0 = (col & 3) * 2, swap = col >> 2;  // the upper columns store their halves in the other order: all banks at once
         uint8_t* dst = k_tile + (col >> 2) * (kKeys * 128) + row * 128;
-        *reinterpret_cast<uint4*>(dst + (((c0 + swap) ^ (row & 7)) << 4)) = swap ? b : a;
-        *reinterpret_cast<uint4*>(dst + (((c0 + 1 - swap) ^ (row & 7)) << 4)) = swap ? a : b;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {  // the upper columns begin with their second half, so that the stores fall on all banks
+          const int half = h ^ (col >> 2);
+          const uint2 x = *reinterpret_cast<const uint2*>(src + i * (S::kLoad * 16) + half * 8);
+          uint4 y;
+          f8x4_to_f16x4<FMT>(x.x, y.x, y.y);
+          f8x4_to_f16x4<FMT>(x.y, y.z, y.w);
+          *reinterpret_cast<uint4*>(dst + ((((col & 3) * 2 + half) ^ (row & 7)) << 4)) = y;
+        }
+      }
+      if (t < 8) {
+        const bool live = (live_bits >> slot) & 1;
+        const float vs = fmaxf(s_scales[slot][8 + t], kTinyScale);
+        const unsigned all = __ballot_sync(0xffu, live), plain = __ballot_sync(0xffu, live && s_scales[slot][t] >= 0.0f);
+        s_info[idx & 3].ks[t] = s_scales[slot][t];
+        s_info[idx & 3].lv[t] = live ? lg2(vs) : -INFINITY;
+        s_info[idx & 3].iv[t] = __fdividef(1.0f, vs);
+        if (t == 0) s_info[idx & 3].live = (int)(all | plain << 8);
       }
       fence_proxy_async_shared();
-      mbar_arrive(&s_k_full);
+      mbar_arrive(&s_k_full[g]);
       if (idx > 1) wait(&s_pv_done[g], (idx >> 1) - 1);  // the tile that lay here before has been multiplied with P
       bool odd = false;
       uint32_t w[4][4];
@@ -322,16 +340,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) kv_attention_tc_kernel(
         }
       }
       odd = __any_sync(0xffffffffu, odd);
-      if (lane == 0) s_info[g].odd[warp - kSoftWarps] = odd;
-      if (t < 8) {
-        const bool live = (live_bits >> slot) & 1;
-        const float vs = fmaxf(s_scales[slot][8 + t], kTinyScale);
-        const unsigned all = __ballot_sync(0xffu, live), plain = __ballot_sync(0xffu, live && s_scales[slot][t] >= 0.0f);
-        s_info[g].ks[t] = s_scales[slot][t];
-        s_info[g].lv[t] = live ? lg2(vs) : -INFINITY;
-        s_info[g].iv[t] = __fdividef(1.0f, vs);
-        if (t == 0) s_info[g].live = (int)(all | plain << 8);
-      }
+      if (lane == 0) s_info[idx & 3].odd[warp - kSoftWarps] = odd;
       fence_proxy_async_shared();
       mbar_arrive(&s_v_full[g]);
     }
@@ -360,7 +369,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) kv_attention_tc_kernel(
       };
       for (int tile = from; tile < to; ++tile, ++idx) {
         const int g = idx & 1;
-        wait(&s_k_full, idx);
+        wait(&s_k_full[g], idx >> 1);
         if (tile == from) wait(&s_q_full, nseg);
         tc_fence_after();
         if (lane == 0) {
@@ -448,56 +457,33 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) kv_attention_tc_kernel(
       for (int tile = from; tile < to; ++tile, ++idx) {
         if ((idx & 1) != g) continue;
         wait(&s_s_full[g], idx >> 1);
-        wait(&s_v_full[g], idx >> 1);  // s_info
+        wait(&s_k_full[g], idx >> 1);  // s_info
         tc_fence_after();
-        const TileInfo& info = s_info[g];
+        const TileInfo& info = s_info[idx & 3];
         __syncwarp();
         if (active) {
           const bool edge = edge_tile(p, seg, tile) || info.live != 0xffff || !(cq >= 0.0f);
-          auto seen = [&](int j) { return j <= pos && j < seg.hi && (p.a.window <= 0 || j > pos - p.a.window); };
-          // Both passes take 16 keys at a time and have the next 16 on their way.
-          uint32_t va[16], vb[16];
-          auto pass = [&](auto part) {
-            tmem_ld16_start(s_at, va);
-#pragma unroll 1
-            for (int i = 0; i < 8; i += 2) {
-              tmem_ld_wait(va);
-              tmem_ld16_start(s_at + 16 * (i + 1), vb);
-              part(i, va);
-              tmem_ld_wait(vb);
-              if (i < 6) tmem_ld16_start(s_at + 16 * (i + 2), va);
-              part(i + 1, vb);
-            }
-          };
-          float top = -INFINITY;
-          if (edge) {
-            pass([&](int i, const uint32_t (&v)[16]) {
-              const float kc = cq * info.ks[i], lv = info.lv[i];
-#pragma unroll
-              for (int k = 0; k < 16; ++k) {
-                const float x = fmaf(__uint_as_float(v[k]), kc, lv);
-                if (seen(tile * kKeys + 16 * i + k)) top = fmaxf(top, x);
-              }
-            });
-          } else {
-            // the largest score of 16 keys is that of their largest product
-            pass([&](int i, const uint32_t (&v)[16]) {
-              float most[2] = {__uint_as_float(v[0]), __uint_as_float(v[1])};
-#pragma unroll
-              for (int k = 2; k < 14; k += 4) {
-                most[0] = fmaxf(most[0], fmaxf(__uint_as_float(v[k]), __uint_as_float(v[k + 1])));
-                most[1] = fmaxf(most[1], fmaxf(__uint_as_float(v[k + 2]), __uint_as_float(v[k + 3])));
-              }
-              most[0] = fmaxf(most[0], fmaxf(__uint_as_float(v[14]), __uint_as_float(v[15])));
-              top = fmaxf(top, fmaf(fmaxf(most[0], most[1]), cq * info.ks[i], info.lv[i]));
-            });
-          }
-          const bool raise = top > m + kRaise;
-          if (__any_sync(0xffffffffu, raise)) {
-            const float mn = raise ? top : m, f = mn == m ? 1.0f : ex2(m - mn);
+          // the row sees keys v0 <= j < v0 + nv
+          const int v0 = p.a.window > 0 ? max(0, pos - p.a.window + 1) : 0, nv = max(0, min(pos + 1, seg.hi) - v0);
+          // A score above m by more than kRaise moves m, in whole steps: what has
+          // been summed and the weights of the tile so far shrink by a power of two.
+          auto raise = [&](int done, float top) {  // 32 done keys have their weights
+            const bool up = top > m + kRaise;
+            const float mn = !up ? m : m == -INFINITY ? top : m + ceilf(top - m), f = up ? ex2(m - mn) : 1.0f;
+            // fp16's smallest number is 2^-24, so P takes the factor in halves
+            const float half = f > 0.0f && up ? floorf(0.5f * (m - mn)) : 0.0f, f0 = ex2(half), f1 = f > 0.0f && up ? ex2(m - mn - half) : f;
             m = mn;
             l *= f;
-            if (count > 0) {  // the group's product before is done: these scores were issued after it
+            tmem_wait_st();
+#pragma unroll 1
+            for (int c = 0; c < done; ++c) {
+              uint32_t v[16];
+              tmem_ld16(s_at + 16 * c, v);
+#pragma unroll
+              for (int i = 0; i < 16; ++i) v[i] = mul_f16x2(mul_f16x2(v[i], f0), f1);
+              tmem_st16(s_at + 16 * c, v);
+            }
+            if (count > 0) {  // O: the group's product before is done, these scores were issued after it
 #pragma unroll 1
               for (int c = 0; c < D; c += 16) {
                 uint32_t v[16];
@@ -506,49 +492,80 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) kv_attention_tc_kernel(
                 for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * f);
                 tmem_st16(o_at + c, v);
               }
-              tmem_wait_st();
             }
-          }
-          const float ms = m == -INFINITY ? 0.0f : m;
-          // P takes the place of scores that have been read
-          if (edge) {
-            pass([&](int i, const uint32_t (&v)[16]) {
-              const float kc = cq * info.ks[i], lv = info.lv[i] - ms;
-              const bool live = (info.live >> i) & 1;
-              float sum = 0.0f;
-              uint32_t w[8];
+            tmem_wait_st();
+          };
+          // 32 keys at a time; P takes the place of scores that have been read
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            uint32_t v[32], w[16];
+            tmem_ld32(s_at + 32 * c, v);
+            float sum[2];
+            if (edge) {
+              float x[32], top = -INFINITY;
 #pragma unroll
-              for (int k = 0; k < 16; k += 2) {
-                const int j = tile * kKeys + 16 * i + k;
-                const float a = live && seen(j) ? ex2(fmaf(__uint_as_float(v[k]), kc, lv)) : 0.0f;
-                const float b = live && seen(j + 1) ? ex2(fmaf(__uint_as_float(v[k + 1]), kc, lv)) : 0.0f;
-                sum += a + b;
-                w[k / 2] = pack_f16(a, b);
+              for (int k = 0; k < 32; ++k) {
+                const int i = 2 * c + k / 16;
+                x[k] = fmaf(__uint_as_float(v[k]), cq * info.ks[i], info.lv[i]);
+                if (!((info.live >> i) & 1) || (unsigned)(tile * kKeys + 32 * c + k - v0) >= (unsigned)nv) x[k] = -INFINITY;
+                top = fmaxf(top, x[k]);
               }
-              l = fmaf(sum, info.iv[i], l);
-              tmem_st8(s_at + 8 * i, w);
-            });
-          } else {
-            pass([&](int i, const uint32_t (&v)[16]) {
-              const float kc = cq * info.ks[i], lv = info.lv[i] - ms;
-              const uint64_t kc2 = pair(kc, kc), lv2 = pair(lv, lv);
-              uint64_t sum = 0;
-              uint32_t w[8];
+              if (__any_sync(0xffffffffu, top > m + kRaise)) raise(c, top);
+              const float ms = m == -INFINITY ? 0.0f : m;
 #pragma unroll
-              for (int k = 0; k < 16; k += 2) {
-                float a, b;
-                unpair(fma2(pair(__uint_as_float(v[k]), __uint_as_float(v[k + 1])), kc2, lv2), a, b);
-                a = ex2(a), b = ex2(b);
-                sum = add2(sum, pair(a, b));
-                w[k / 2] = pack_f16(a, b);
+              for (int h = 0; h < 2; ++h) {
+                sum[h] = 0.0f;
+#pragma unroll
+                for (int k = 16 * h; k < 16 * h + 16; k += 2) {
+                  const float a = ex2(x[k] - ms), b = ex2(x[k + 1] - ms);
+                  sum[h] += a + b;
+                  w[k / 2] = pack_f16(a, b);
+                }
               }
-              float s0, s1;
-              unpair(sum, s0, s1);
-              l = fmaf(s0 + s1, info.iv[i], l);
-              tmem_st8(s_at + 8 * i, w);
-            });
+            } else {
+              // the largest score of 16 keys is that of their largest product
+              float kc[2], top[2];
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                float most[2] = {__uint_as_float(v[16 * h]), __uint_as_float(v[16 * h + 1])};
+#pragma unroll
+                for (int k = 16 * h + 2; k < 16 * h + 14; k += 4) {
+                  most[0] = fmaxf(most[0], fmaxf(__uint_as_float(v[k]), __uint_as_float(v[k + 1])));
+                  most[1] = fmaxf(most[1], fmaxf(__uint_as_float(v[k + 2]), __uint_as_float(v[k + 3])));
+                }
+                most[0] = fmaxf(most[0], fmaxf(__uint_as_float(v[16 * h + 14]), __uint_as_float(v[16 * h + 15])));
+                kc[h] = cq * info.ks[2 * c + h];
+                top[h] = fmaf(fmaxf(most[0], most[1]), kc[h], info.lv[2 * c + h]);
+              }
+              const float most = fmaxf(top[0], top[1]);
+              if (__any_sync(0xffffffffu, most > m + kRaise)) raise(c, most);
+              const float ms = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const float lv = info.lv[2 * c + h] - ms;
+                const uint64_t kc2 = pair(kc[h], kc[h]), lv2 = pair(lv, lv);
+                uint64_t two = 0;
+#pragma unroll
+                for (int k = 16 * h; k < 16 * h + 16; k += 2) {
+                  float a, b;
+                  unpair(fma2(pair(__uint_as_float(v[k]), __uint_as_float(v[k + 1])), kc2, lv2), a, b);
+                  a = ex2(a), b = ex2(b);
+                  two = add2(two, pair(a, b));
+                  w[k / 2] = pack_f16(a, b);
+                }
+                float s0, s1;
+                unpair(two, s0, s1);
+                sum[h] = s0 + s1;
+              }
+            }
+            l = fmaf(sum[1], info.iv[2 * c + 1], fmaf(sum[0], info.iv[2 * c], l));
+            tmem_st16(s_at + 16 * c, w);
           }
           tmem_wait_st();
+        }
+        wait(&s_v_full[g], idx >> 1);  // the rest of s_info
+        __syncwarp();
+        if (active) {
           int odd = 0;
 #pragma unroll
           for (int i = 0; i < S::kLoadWarps; ++i) odd |= info.odd[i];

@@ -13,7 +13,13 @@
 // A team of 1 .. 8 warps owns one (page, head, K or V), so scales and codes of
 // a page have one writer and no atomics are needed. A CTA's teams share a page:
 // finding it (a scan of the sequences' lengths) is what a small append spends
-// its time on.
+// its time on. Rows are read twice, once for the scale and once for the codes;
+// the first pieces stay in registers between the two.
+//
+// Measured: 64 sequences of one token, 8 heads of 128: 4.6 us (6.0 with a page
+// lookup a warp), a chain of latencies: lengths, page id, row and scale, store.
+// Prompts of 9200 tokens: 25 us, 2.3 TB/s of the 57 MB read and written (39 us
+// with a page lookup a warp).
 #include "fp8_mma.cuh"
 #include "fp8imma/fp8imma_ext.h"
 #include "fp8imma_kernels.h"

@@ -32,6 +32,11 @@
 // of 4 KB reach 6.6 TB/s, copies of 2 KB 3.8 TB/s, 16-byte asynchronous copies
 // of 64-byte row pieces 5.6 TB/s. A team's sums meet in shared memory in a
 // fixed order; nothing depends on timing.
+//
+// Measured: 64 tokens, 4 of 32 experts, 4096 x 2048: 194 us (4.2 TB/s of the
+// 806 MB); 8 tokens, 2 of 8 experts, 4096 x 11008: 190 us (5.1 TB/s of 0.97 GB,
+// 79% of a copy); one token, 6 of 64 experts, 2048 x 1408: 28 us, of which the
+// bytes are 8: the router's chain and three grid barriers come on top.
 #include "fp8_mma.cuh"
 #include "fp8imma/fp8imma_ext.h"
 #include "fp8imma_kernels.h"

@@ -257,6 +257,17 @@ def test_attention_peaked_rows(ops):
         check(*run_attend(ops, q, cache, lens, [0, 1], 0, fmt, scale=scale))
 
 
+@pytest.mark.parametrize("d", [64, 128])
+def test_attention_rising_scores(ops, d):
+    """Scores that grow along the sequence: the running reference moves again and again, within tiles and between."""
+    g = gen(45)
+    table, kc, vc, ks, vs = make_cache(g, 1, 60, 2, 32, d, "e4m3")
+    for i in range(60):
+        ks[table[0, i].long()] *= 2.0 ** (i // 12)
+    q = torch.randn(9, 16, d, generator=g, device="cuda").half()
+    check(*run_attend(ops, q, (table, kc, vc, ks, vs), [1900], [0, 9], 0, "e4m3", scale=0.5))
+
+
 @pytest.mark.parametrize("mult", [2.0 ** -30, 2.0 ** 40])
 def test_attention_bf16_queries_outside_fp16(ops, mult):
     g = gen(44)
