@@ -23,14 +23,13 @@
 // as soon as its scores are made.
 //
 // Measured (e4m3, fp16): 16 sequences of 8000 keys, 64 heads over 8, 128
-// channels, 32 rows a KV head 123 us (2.1 TB/s), 128 rows 136 us (496 us in the
+// channels, 32 rows a KV head 121 us (2.2 TB/s), 128 rows 134 us (496 us in the
 // few-row kernel); prompts of 4 x 1000 tokens, 32 heads over 8, 214 us (577);
-// one of 8192 tokens 1.77 ms (7.58; 310 TFLOP/s of the causal half). What bounds
-// it is instruction issue and its latencies (4 warps a scheduler, 0.45
-// instructions a cycle): conversion of a tile some 2200 cycles in the load warps,
-// weights of 2 x 128 x 128 scores some 2000 in the softmax warps, 1024 of them
-// the exponentials' unit. Loads through registers instead of shared memory
-// waited for each other: 221 us where this takes 122.
+// one of 8192 tokens 1.72 ms (7.58; 320 TFLOP/s of the causal half). What bounds
+// it are the latencies of instruction issue (4 warps a scheduler, 0.44
+// instructions a cycle): a tile takes some 3500 cycles, of which its products
+// and its exponentials need about 1000 each. Loads through registers instead of
+// shared memory waited for each other: 221 us where this takes 121.
 #include "kv_attention.cuh"
 #include "sm100_umma.cuh"
 #include <type_traits>
@@ -165,7 +164,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) kv_attention_tc_kernel(
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t s_k_full[2], s_v_full[2], s_s_full[2], s_p_full[2], s_pv_done[2], s_q_full, s_o_free;
   __shared__ float s_scales[S::kSlots][16];
-  __shared__ TileInfo s_info[4];       // by tile number: a tile's is read until its weights are done, and four tiles on they are
+  __shared__ TileInfo s_info[4];       // by tile number mod 4: when a place is filled again, its last tile has been multiplied
   __shared__ Shared s_shared[2];
   __shared__ float s_ml[2][kRows][3];  // reference, sum, whether the group's poison marks count
   __shared__ float s_back[kRows];      // what a bf16 row of Q was divided by
