@@ -13,13 +13,13 @@
 // A team of 1 .. 8 warps owns one (page, head, K or V), so scales and codes of
 // a page have one writer and no atomics are needed. A CTA's teams share a page:
 // finding it (a scan of the sequences' lengths) is what a small append spends
-// its time on. Rows are read twice, once for the scale and once for the codes;
-// the first pieces stay in registers between the two.
+// its time on. Rows stay in registers between the pass for the scale and the one
+// for the codes, as far as kKeep pieces a thread go.
 //
 // Measured: 64 sequences of one token, 8 heads of 128: 4.6 us (6.0 with a page
 // lookup a warp), a chain of latencies: lengths, page id, row and scale, store.
-// Prompts of 9200 tokens: 25 us, 2.3 TB/s of the 57 MB read and written (39 us
-// with a page lookup a warp).
+// Prompts of 9200 tokens, rows from HBM: 21.7 us, 2.6 TB/s of the 57 MB read and
+// written (24.6 with two CTAs a SM, 39 us with a page lookup a warp as well).
 #include "fp8_mma.cuh"
 #include "fp8imma/fp8imma_ext.h"
 #include "fp8imma_kernels.h"
@@ -103,8 +103,8 @@ __device__ __forceinline__ int touched(const AppendParams& p, int b, int& first)
   return (n > 0 && len > start) ? min((len - 1) / p.c.page_size, p.c.max_pages - 1) - first + 1 : 0;
 }
 
-template <int AT, int FMT>
-__global__ void __launch_bounds__(kThreads) kv_append_kernel(const __grid_constant__ AppendParams p) {
+template <int AT, int FMT, int CTAS>
+__global__ void __launch_bounds__(kThreads, CTAS) kv_append_kernel(const __grid_constant__ AppendParams p) {
   __shared__ int s_pick[3];
   __shared__ int s_scan[kWarps];
   __shared__ float s_max[kWarps];
@@ -176,19 +176,20 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(const __grid_consta
   float* scale = (which ? p.c.v_scale : p.c.k_scale) + ph;
   const float s_old = on && slot0 > 0 ? *scale : 0.0f;
 
-  const int vr = D >> 3, nv = on ? rows * vr : 0;  // 8-element vectors of a row, of the page's new rows
+  const int vr = __ffs(D) - 4, nv = on ? rows << vr : 0;  // 8-element vectors of a row (log2), of the page's new rows
+  auto vec_at = [&](int v) { return src + (int64_t)(v >> vr) * p.ts[which] + (v & ((1 << vr) - 1)) * 8; };
   uint4 keep[kKeep];
   float amax = 0.0f;
 #pragma unroll
   for (int i = 0; i < kKeep; ++i) {
     const int v = tid + i * step;
-    if (v < nv) keep[i] = load_row8<AT>(src + (int64_t)(v / vr) * p.ts[which] + (v % vr) * 8, p.vec);
+    if (v < nv) keep[i] = load_row8<AT>(vec_at(v), p.vec);
   }
 #pragma unroll
   for (int i = 0; i < kKeep; ++i)
     if (tid + i * step < nv) amax = fmaxf(amax, absmax8<AT>(keep[i]));
   for (int v = tid + kKeep * step; v < nv; v += step)
-    amax = fmaxf(amax, absmax8<AT>(load_row8<AT>(src + (int64_t)(v / vr) * p.ts[which] + (v % vr) * 8, p.vec)));
+    amax = fmaxf(amax, absmax8<AT>(load_row8<AT>(vec_at(v), p.vec)));
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
   if (lane == 0) s_max[warp] = amax;
@@ -225,11 +226,16 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(const __grid_consta
     if (v < nv) out[v] = to_codes<AT, FMT>(keep[i], s_new, inv);
   }
   for (int v = tid + kKeep * step; v < nv; v += step)
-    out[v] = to_codes<AT, FMT>(load_row8<AT>(src + (int64_t)(v / vr) * p.ts[which] + (v % vr) * 8, p.vec), s_new, inv);
+    out[v] = to_codes<AT, FMT>(load_row8<AT>(vec_at(v), p.vec), s_new, inv);
   if (tid == 0) *scale = s_new;
 }
 
-template <int AT>
+// CTAS: CTAs a SM that registers have to leave room for. Two (86 registers) have
+// all loads of a page in flight at once; more than two a SM at hand, and four
+// take the waves faster. Measured with 1 and 4 in the bounds: 16 prompts of 200
+// tokens, 4 heads of 64, 6.2 / 8.2 us; 64 single tokens, 8 heads of 128, 3.9 /
+// 5.1; 256 single tokens 7.7 / 6.1; 6 prompts of 1536 tokens 24.3 / 18.0.
+template <int AT, int CTAS>
 cudaError_t launch_append(const AppendParams& p, dim3 grid, cudaStream_t st) {
   cudaLaunchConfig_t lc = {};
   cudaLaunchAttribute attr[1];
@@ -240,8 +246,8 @@ cudaError_t launch_append(const AppendParams& p, dim3 grid, cudaStream_t st) {
   lc.stream = st;
   lc.attrs = attr;
   lc.numAttrs = api_pdl() ? 1 : 0;
-  return p.c.format == FP8IMMA_B_E4M3 ? cudaLaunchKernelEx(&lc, kv_append_kernel<AT, F8_E4M3>, p)
-                                      : cudaLaunchKernelEx(&lc, kv_append_kernel<AT, F8_E5M2>, p);
+  return p.c.format == FP8IMMA_B_E4M3 ? cudaLaunchKernelEx(&lc, kv_append_kernel<AT, F8_E4M3, CTAS>, p)
+                                      : cudaLaunchKernelEx(&lc, kv_append_kernel<AT, F8_E5M2, CTAS>, p);
 }
 
 }  // namespace
@@ -299,5 +305,7 @@ extern "C" int fp8imma_kv_append(const fp8imma_kv_cache* c, const fp8imma_kv_app
   if (units > 0x7fffffffll || rows_y > 65535) return (int)cudaErrorInvalidValue;
   const dim3 grid((unsigned)units, (unsigned)rows_y);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return (int)(a->a_type == FP8IMMA_A_F16 ? launch_append<0>(p, grid, st) : launch_append<1>(p, grid, st));
+  if (units * rows_y > 2ll * num_sms_current())
+    return (int)(a->a_type == FP8IMMA_A_F16 ? launch_append<0, 4>(p, grid, st) : launch_append<1, 4>(p, grid, st));
+  return (int)(a->a_type == FP8IMMA_A_F16 ? launch_append<0, 1>(p, grid, st) : launch_append<1, 1>(p, grid, st));
 }
