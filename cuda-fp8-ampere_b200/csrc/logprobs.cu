@@ -17,10 +17,11 @@
 // GPU (one row of 32000 bf16 logits: latency; thousands of rows: bandwidth);
 // the last CTA to finish a row joins its parts in order.
 //
-// Measured: 4096 rows of 32000 bf16 logits 84 us (3.1 TB/s; instruction issue:
-// an exponential, two sums and a comparison a logit); one row of 32000 with 8
-// alternatives 9.6 us, latency: launch, part, join; 16 column-major rows of
-// 128000 with 20 alternatives 30 us, the sorting of short parts' candidates.
+// Measured: 4096 rows of 32001 bf16 logits 59 us without alternatives (4.5 TB/s;
+// instruction issue: an exponential and two sums a logit), 84 us with five of
+// them; one row of 32000 with 8 alternatives 9.4 us, latency: launch, part, join;
+// 16 column-major rows of 128000 with 20 alternatives 32 us, the sorting of short
+// parts' candidates.
 #include "fp8_mma.cuh"
 #include "fp8imma/fp8imma_ext.h"
 #include "fp8imma_kernels.h"
