@@ -162,7 +162,12 @@ template <int FMT, int D>
 __global__ void __launch_bounds__(Shape<D>::kThreads, 1) kv_attention_tc_kernel(const __grid_constant__ AttnParams p) {
   using S = Shape<D>;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ uint64_t s_k_full[2], s_v_full[2], s_s_full[2], s_p_full[2], s_pv_done[2], s_q_full, s_o_free;
+  // Tiles take their barriers in turn: K's (which s_info follows) by tile number
+  // mod 4, the others mod 2. A phase of a barrier ends only after all that wait
+  // for the one before it have passed: for V, S, P and O through the tile's
+  // product with P, two tiles back; for K, whose place is free as soon as its
+  // scores are made, through that product four tiles back.
+  __shared__ uint64_t s_k_full[4], s_v_full[2], s_s_full[2], s_p_full[2], s_pv_done[2], s_q_full, s_o_free;
   __shared__ float s_scales[S::kSlots][16];
   __shared__ TileInfo s_info[4];       // by tile number mod 4: when a place is filled again, its last tile has been multiplied
   __shared__ Shared s_shared[2];
@@ -180,8 +185,8 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) kv_attention_tc_kernel(
   constexpr int kMmaWarp = kSoftWarps + S::kLoadWarps;
 
   if (tid == 0) {
+    for (int i = 0; i < 4; ++i) mbar_init(&s_k_full[i], S::kLoad);
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&s_k_full[i], S::kLoad);
       mbar_init(&s_v_full[i], S::kLoad);
       mbar_init(&s_s_full[i], 1);
       mbar_init(&s_p_full[i], kSoft / 2);
@@ -302,7 +307,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) kv_attention_tc_kernel(
         if (t == 0) s_info[idx & 3].live = (int)(all | plain << 8);
       }
       fence_proxy_async_shared();
-      mbar_arrive(&s_k_full[g]);
+      mbar_arrive(&s_k_full[idx & 3]);
       if (idx > 1) wait(&s_pv_done[g], (idx >> 1) - 1);  // the tile that lay here before has been multiplied with P
       bool odd = false;
       uint32_t w[4][4];
@@ -368,7 +373,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) kv_attention_tc_kernel(
       };
       for (int tile = from; tile < to; ++tile, ++idx) {
         const int g = idx & 1;
-        wait(&s_k_full[g], idx >> 1);
+        wait(&s_k_full[idx & 3], idx >> 2);
         if (tile == from) wait(&s_q_full, nseg);
         tc_fence_after();
         if (lane == 0) {
@@ -456,7 +461,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) kv_attention_tc_kernel(
       for (int tile = from; tile < to; ++tile, ++idx) {
         if ((idx & 1) != g) continue;
         wait(&s_s_full[g], idx >> 1);
-        wait(&s_k_full[g], idx >> 1);  // s_info
+        wait(&s_k_full[idx & 3], idx >> 2);  // s_info
         tc_fence_after();
         const TileInfo& info = s_info[idx & 3];
         __syncwarp();
