@@ -50,14 +50,14 @@ namespace {
 
 using namespace fp8imma_dev;
 
-constexpr int kRouterDone = 64, kScaleMax = 128, kSyncWords = kScaleMax + 2 * FP8IMMA_MOE_MAX_EXPERTS;
+constexpr int kLeft = 3, kRouterDone = 64, kScaleMax = 128, kSyncWords = kScaleMax + 2 * FP8IMMA_MOE_MAX_EXPERTS;
 constexpr int kMaxSlots = FP8IMMA_MOE_MAX_TOKENS * FP8IMMA_MOE_MAX_TOP_K;
 
 struct MoeParams {
   fp8imma_moe_args a;
-  // kept zero between calls: three barrier counters, finished router units of
-  // each group of tokens (from kRouterDone on), the experts' largest gate / up
-  // scales as bits (from kScaleMax on, [experts, 2])
+  // kept zero between calls: three barrier counters, CTAs that have left (kLeft),
+  // finished router units of each group of tokens (from kRouterDone on), the
+  // experts' largest gate / up scales as bits (from kScaleMax on, [experts, 2])
   unsigned int* sync;
   float* logits;       // [tokens, experts]
   uint16_t* xf;        // [tokens, hidden padded to 128] fp16, operand order
@@ -131,6 +131,17 @@ __device__ __forceinline__ bool grid_barrier(unsigned int* ctr) {
   }
   __syncthreads();
   return s_ok != 0;
+}
+
+// A warp's report that its CTA has read and written the sync words for the last
+// time in this call. Every CTA makes it once, whichever of its waits ran out, so
+// the last one leaves them zero for the next call also after a failed barrier.
+__device__ __forceinline__ void leave(unsigned int* sync, int experts, int lane) {
+  unsigned int before = 0;
+  if (lane == 0) asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(before) : "l"(sync + kLeft) : "memory");
+  before = __shfl_sync(0xffffffffu, before, 0);
+  if (before != gridDim.x - 1) return;
+  for (int i = lane; i < kScaleMax + 2 * experts; i += 32) sync[i] = 0u;
 }
 
 struct Runs {  // CTA c's run of the units: they differ by one in length at most
@@ -265,7 +276,6 @@ __device__ __forceinline__ void router(const MoeParams& p, int wid, int nw, int 
     done = __shfl_sync(0xffffffffu, done, 0);
     __syncwarp();
     if (done == (unsigned)(eu - 1)) {
-      if (lane == 0) *ctr = 0u;
 #pragma unroll 1
       for (int t = t0; t < min(t0 + TX, p.a.tokens); ++t) {
         const int at = t * p.a.top_k;
@@ -423,8 +433,10 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
     scale_maxima(p, ((warp + WARPS / 2) % WARPS) * gridDim.x + blockIdx.x, nw, lane);  // from the middle warps on: the first have router units
   }
   for (int e = tid; e < E; e += kThreads) L.tokens[e] = 0ull;
-  if (!grid_barrier(p.sync)) return;
-  if (blockIdx.x == 0 && tid == 0) p.sync[2] = 0u;  // all CTAs of the call before have left its last barrier
+  if (!grid_barrier(p.sync)) {
+    if (warp == 0) leave(p.sync, E, lane);
+    return;
+  }
 
   // ---------------------------------------------------------------- lists --
   if (tid < T) L.xback[tid] = __ldcg(p.xback + 2 * tid);
@@ -702,12 +714,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
   if (p.ipad > I)
     for (int x = blockIdx.x * kThreads + tid; x < T * K * (p.ipad - I); x += gridDim.x * kThreads)
       p.h[(size_t)(x / (p.ipad - I)) * p.ipad + place(I + x % (p.ipad - I))] = 0;
-  const bool met = grid_barrier(p.sync + 1);
-  if (met && blockIdx.x == 0) {  // every CTA has read them
-    if (tid == 0) p.sync[0] = 0u;
-    for (int e = tid; e < 2 * E; e += kThreads) p.sync[kScaleMax + e] = 0u;
-  }
-  if (!met) {
+  if (!grid_barrier(p.sync + 1)) {
+    if (warp == 0) leave(p.sync, E, lane);
     drain();
     return;
   }
@@ -748,8 +756,9 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
     }
   }
   if (!ok) drain();
-  if (!grid_barrier(p.sync + 2)) return;
-  if (blockIdx.x == 0 && tid == 0) p.sync[1] = 0u;
+  const bool met = grid_barrier(p.sync + 2);
+  if (warp == WARPS - 1) leave(p.sync, E, lane);  // the others' loads of phase 3 are under way meanwhile
+  if (!met) return;
 
   // --------------------------------------------------- 3: a token's slots --
   for (int x = blockIdx.x * kThreads + tid; x < T * (H >> 1); x += gridDim.x * kThreads) {
