@@ -7,10 +7,18 @@
 // FP8 codes are multiplied as fp16 (exact); sums are fp32, scales are applied
 // to the sums. x enters as it is when it is fp16; a bf16 row is brought into
 // fp16's range by a power of two (exact within 2^22 of the row's largest). h
-// is rounded to fp16, 2^-11, after a power of two of its slot that keeps it
-// below 2^15: |act(g) u| <= |g| |u|, and a gate or up sum is at most
-// max_i s_i * fmax * sum |x|. Typical h lie some 2^16 below that bound, well
-// inside fp16's normal range, and no largest value has to be agreed on first.
+// is rounded to fp16 (2^-11; 16 bits are what the tensor cores take) as 16
+// columns at a time come out of a unit, after a power of two that brings their
+// largest magnitude to 2^-1 .. 2^15, where nothing is lost that matters beside
+// it (2^-24 of it). These powers lie 16 octaves apart, counted from the one that
+// a slot's columns are expected to take: |act(g) u| <= |g| |u|, a gate or up sum
+// is at most max_i s_i * fmax * sum |x|, and the largest h of well-spread
+// weights lie some 2^16 below that. So the columns of a row nearly always share
+// one, and the down product takes them as they are; a unit with a row whose
+// columns do not brings them to the row's largest as it reads them. Doing so in
+// every unit, with powers one octave apart, took 222 us instead of 197 for 64
+// tokens; one power a row, taken from the bound alone, loses small rows beside
+// scales that no weight uses.
 //
 // Bound: a few tokens use each weight byte a few times, so the layer costs the
 // bytes of the chosen experts. One cooperative grid, one CTA per SM, keeps
@@ -33,10 +41,11 @@
 // of 64-byte row pieces 5.6 TB/s. A team's sums meet in shared memory in a
 // fixed order; nothing depends on timing.
 //
-// Measured: 64 tokens, 4 of 32 experts, 4096 x 2048: 194 us (4.2 TB/s of the
-// 806 MB); 8 tokens, 2 of 8 experts, 4096 x 11008: 190 us (5.1 TB/s of 0.97 GB,
-// 79% of a copy); one token, 6 of 64 experts, 2048 x 1408: 28 us, of which the
-// bytes are 8: the router's chain and three grid barriers come on top.
+// Measured: 64 tokens, 4 of 32 experts, 4096 x 2048: 202 us (4.0 TB/s of the
+// 806 MB); 8 tokens, 2 of 8 experts, 4096 x 11008: 172 to 198 us by the board and
+// the run (4.9 to 5.6 TB/s of 0.97 GB, 75 to 87% of a copy); one token, 6 of 64
+// experts, 2048 x 1408: 29 us, of which the bytes are 8: the router's chain and
+// three grid barriers come on top.
 #include "fp8_mma.cuh"
 #include "fp8imma/fp8imma_ext.h"
 #include "fp8imma_kernels.h"
@@ -44,20 +53,24 @@
 #include "sm100_async.cuh"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace fp8imma_b200 {
 namespace {
 
 using namespace fp8imma_dev;
 
-constexpr int kLeft = 3, kRouterDone = 64, kScaleMax = 128, kSyncWords = kScaleMax + 2 * FP8IMMA_MOE_MAX_EXPERTS;
 constexpr int kMaxSlots = FP8IMMA_MOE_MAX_TOKENS * FP8IMMA_MOE_MAX_TOP_K;
+constexpr int kLeft = 3, kRouterDone = 64, kSteps = 128, kScaleMax = kSteps + 2 * kMaxSlots, kSyncWords = kScaleMax + 2 * FP8IMMA_MOE_MAX_EXPERTS;
+constexpr int kBias = 64;  // above the magnitude of every step of h's powers
 
 struct MoeParams {
   fp8imma_moe_args a;
   // kept zero between calls: three barrier counters, CTAs that have left (kLeft),
-  // finished router units of each group of tokens (from kRouterDone on), the
-  // experts' largest gate / up scales as bits (from kScaleMax on, [experts, 2])
+  // finished router units of each group of tokens (from kRouterDone on), kBias +
+  // the highest and kBias - the lowest step of each slot's columns that are not
+  // zero (from kSteps on, [slots, 2]), the experts' largest gate / up scales as
+  // bits (from kScaleMax on, [experts, 2])
   unsigned int* sync;
   float* logits;       // [tokens, experts]
   uint16_t* xf;        // [tokens, hidden padded to 128] fp16, operand order
@@ -65,6 +78,7 @@ struct MoeParams {
   int* ids;            // [slots] the choice
   float* weights;      // [slots]
   uint16_t* h;         // [slots, inter padded to 128] fp16, operand order
+  signed char* step;   // [slots, a 16th of that] of 16 columns of h: value = h * 2^(base + 16 step - 14), base by slot
   float* part;         // [slots, hidden]
   int hpad, ipad;
 };
@@ -81,6 +95,14 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
+__device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }  // e: -126 .. 127
+// v * 2^e for e of -252 .. 254, in two products
+__device__ __forceinline__ float times_pow2(float v, int e) { return v * pow2(e >> 1) * pow2(e - (e >> 1)); }
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -136,12 +158,13 @@ __device__ __forceinline__ bool grid_barrier(unsigned int* ctr) {
 // A warp's report that its CTA has read and written the sync words for the last
 // time in this call. Every CTA makes it once, whichever of its waits ran out, so
 // the last one leaves them zero for the next call also after a failed barrier.
-__device__ __forceinline__ void leave(unsigned int* sync, int experts, int lane) {
+__device__ __forceinline__ void leave(unsigned int* sync, int experts, int slots, int lane) {
   unsigned int before = 0;
   if (lane == 0) asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(before) : "l"(sync + kLeft) : "memory");
   before = __shfl_sync(0xffffffffu, before, 0);
   if (before != gridDim.x - 1) return;
-  for (int i = lane; i < kScaleMax + 2 * experts; i += 32) sync[i] = 0u;
+  for (int i = lane; i < kSteps + 2 * slots; i += 32) sync[i] = 0u;
+  for (int i = lane; i < 2 * experts; i += 32) sync[kScaleMax + i] = 0u;
 }
 
 struct Runs {  // CTA c's run of the units: they differ by one in length at most
@@ -163,6 +186,7 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, u
 // DEPTH: blocks of a warp's ring.
 template <int NT, int RU, int WARPS, int DEPTH>
 struct Shape {
+  static_assert(RU % 2 == 0, "a unit's gate rows are whole groups of 16 columns of h");
   static constexpr int kThreads = WARPS * 32;
   static constexpr int kBlockBytes = 2048 * RU;
   static constexpr int kRing = DEPTH * kBlockBytes;    // of a warp
@@ -382,7 +406,9 @@ struct Lists {
   short token[kMaxSlots];                              // and their tokens
   short id[kMaxSlots];                                 // expert of a slot
   float weight[kMaxSlots];                             // p of a slot
-  float scale[kMaxSlots];                              // factor that brings a slot's h into fp16's range
+  short base[kMaxSlots];                               // exponent that a slot's columns of h are expected to take
+  short power[kMaxSlots];                              // the one that its row enters the down product with
+  unsigned char mixed[kMaxSlots];                      // its columns do not share it
   float xback[FP8IMMA_MOE_MAX_TOKENS];
   int entries;
   int scan[16];
@@ -434,7 +460,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
   }
   for (int e = tid; e < E; e += kThreads) L.tokens[e] = 0ull;
   if (!grid_barrier(p.sync)) {
-    if (warp == 0) leave(p.sync, E, lane);
+    if (warp == 0) leave(p.sync, E, T * K, lane);
     return;
   }
 
@@ -442,16 +468,15 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
   if (tid < T) L.xback[tid] = __ldcg(p.xback + 2 * tid);
   for (int s = tid; s < T * K; s += kThreads) {
     const int t = s / K, e = __ldcg(p.ids + s);
-    const float l1 = __ldcg(p.xback + 2 * t + 1), w = __ldcg(p.weights + s);
+    const float l1 = __ldcg(p.xback + 2 * t + 1);
+    L.weight[s] = __ldcg(p.weights + s);
     L.id[s] = (short)e;
     atomicOr(&L.tokens[e], 1ull << t);
-    // the slot's power of two: gate sums are below 2^(eg + 1), up sums below 2^(eu + 1)
+    // gate sums are below 2^(eg + 1), up sums below 2^(eu + 1), h is expected 2^16 below their product
     const float fmax_v = FMT == F8_E4M3 ? 448.0f : 57344.0f;
     const uint2 m = __ldcg(reinterpret_cast<const uint2*>(p.sync + kScaleMax) + e);
     const int eg = (int)(__float_as_uint(__uint_as_float(m.x) * fmax_v * l1) >> 23) - 127, eu = (int)(__float_as_uint(__uint_as_float(m.y) * fmax_v * l1) >> 23) - 127;
-    const int k = max(-126, min(126, eg + eu - 13));
-    L.scale[s] = __uint_as_float((uint32_t)(127 - k) << 23);
-    L.weight[s] = w * __uint_as_float((uint32_t)(127 + k) << 23);  // a slot's result is multiplied by its weight and by what undoes the factor
+    L.base[s] = (short)max(-120, min(120, eg + eu - 7));
   }
   __syncthreads();
   {
@@ -620,15 +645,35 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
     named_bar_sync(1 + warp / ks, ks * 32);
     return true;
   };
-  // One block's products: fp16 rows xr (8 NT of them, operand order) times the ring's next block.
+  // One block's products: fp16 rows xr (8 NT of them, operand order) times the
+  // ring's next block. Mixed rows of h come to their row's power as they are read:
+  // half of a lane's places are 16 columns.
   const uint16_t* xr[NT];
-  auto multiply = [&](int kb, int tiles) {
+  int slot_of[NT];
+  auto multiply = [&](int kb, int tiles, auto mixed) {
+    char2 st[NT];
+    if (mixed)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+        st[nt] = xr[nt] ? *reinterpret_cast<const char2*>(p.step + (size_t)slot_of[nt] * (p.ipad >> 4) + kb * 8 + t4 * 2) : make_char2(0, 0);
+    auto to_row = [&](uint4 (&v)[2], int nt, int j) {
+      if (!mixed || !xr[nt]) return;
+      const int top = (L.power[slot_of[nt]] - L.base[slot_of[nt]]) >> 4;
+      // columns three steps below the row's are zero beside it
+      const float f = pow2(8 * max((j ? st[nt].y : st[nt].x) - top, -3));
+      const uint32_t ff = pack_f16(f, f);
+      auto scaled = [&](uint32_t w) { return mul_f16x2(mul_f16x2(w, ff), ff); };  // twice: 2^-32 is below fp16's range, the product need not be
+#pragma unroll
+      for (int i = 0; i < 2; ++i) v[i] = make_uint4(scaled(v[i].x), scaled(v[i].y), scaled(v[i].z), scaled(v[i].w));
+    };
     uint4 x[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int i = 0; i < 2; ++i) x[nt][i] = xr[nt] ? *reinterpret_cast<const uint4*>(xr[nt] + kb * 128 + i * 32) : make_uint4(0, 0, 0, 0);
     const uint8_t* w = next_block();
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) to_row(x[nt], nt, 0);
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       uint4 g[RU], b[RU], y[NT][2];
@@ -662,9 +707,11 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
       }
       if (j == 0) {
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
           for (int i = 0; i < 2; ++i) x[nt][i] = y[nt][i];
+          to_row(x[nt], nt, 1);
+        }
       }
     }
     __syncwarp();
@@ -688,7 +735,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
     for (int nt = 0; nt < NT; ++nt) xr[nt] = nt * 8 + q4 < cnt ? p.xf + (size_t)L.token[s0 + nt * 8 + q4] * p.hpad + t4 * 8 : nullptr;
     clear();
 #pragma unroll 1
-    for (int kb = warp % ks1; kb < nb1; kb += ks1) multiply(kb, tiles);
+    for (int kb = warp % ks1; kb < nb1; kb += ks1) multiply(kb, tiles, std::false_type());
     if (!gather(ks1)) continue;
     // gate and up of a row lie in one lane
 #pragma unroll
@@ -699,26 +746,58 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
         const int n = nt * 8 + 2 * t4 + c;
         const bool in = n < cnt;
         const int s = in ? L.slot[s0 + n] : 0;
-        if (!in) continue;
-        const float xb = L.xback[L.token[s0 + n]], f = L.scale[s];
+        const float xb = in ? L.xback[L.token[s0 + n]] : 0.0f;
+        const int e0 = L.base[s];
+        unsigned high = 0, low = 0;
 #pragma unroll
-        for (int r = 0; r < RU; ++r) {
-          const int i = i0 + r * 8 + q4;
-          const float hv = gate_act(acc[0][r][nt][c] * xb * sg[r], p.a.act) * (acc[0][r][nt][c + 2] * xb * su[r]);
-          if (i < I) p.h[(size_t)s * p.ipad + place(i)] = __half_as_ushort(__float2half_rn(hv * f));
+        for (int m = 0; m < RU / 2; ++m) {  // 16 columns: two of the lane's rows, those of the eight lanes with this token
+          const int i = i0 + m * 16 + q4;   // and i + 8; inter is a multiple of 16
+          float hv[2];
+#pragma unroll
+          for (int k = 0; k < 2; ++k) hv[k] = gate_act(acc[0][2 * m + k][nt][c] * xb * sg[2 * m + k], p.a.act) * (acc[0][2 * m + k][nt][c + 2] * xb * su[2 * m + k]);
+          float big = fmaxf(fabsf(hv[0]), fabsf(hv[1]));
+          big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 4));
+          big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 8));
+          big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 16));
+          const int e = (int)(__float_as_uint(big) >> 23) - 127, step = (e - e0 + 15) >> 4;  // big * 2^(14 - e0 - 16 step) lies in 2^-1 .. 2^15
+          if (in && i < I) {
+            const int up = 14 - e0 - 16 * step;
+            p.h[(size_t)s * p.ipad + place(i)] = __half_as_ushort(__float2half_rn(times_pow2(hv[0], up)));
+            p.h[(size_t)s * p.ipad + place(i + 8)] = __half_as_ushort(__float2half_rn(times_pow2(hv[1], up)));
+            if (q4 == 0) p.step[(size_t)s * (p.ipad >> 4) + (i >> 4)] = (signed char)step;
+            if (big > 0.0f) {
+              high = max(high, (unsigned)(kBias + step));
+              low = max(low, (unsigned)(kBias - step));
+            }
+          }
+        }
+        if (high && q4 == 0) {
+          atomicMax(p.sync + kSteps + 2 * s, high);
+          atomicMax(p.sync + kSteps + 2 * s + 1, low);
         }
       }
     }
   }
   // the columns from inter to the padded width are zero
   if (p.ipad > I)
-    for (int x = blockIdx.x * kThreads + tid; x < T * K * (p.ipad - I); x += gridDim.x * kThreads)
-      p.h[(size_t)(x / (p.ipad - I)) * p.ipad + place(I + x % (p.ipad - I))] = 0;
+    for (int x = blockIdx.x * kThreads + tid; x < T * K * (p.ipad - I); x += gridDim.x * kThreads) {
+      const int s = x / (p.ipad - I), i = I + x % (p.ipad - I);
+      p.h[(size_t)s * p.ipad + place(i)] = 0;
+      if ((i & 15) == 0) p.step[(size_t)s * (p.ipad >> 4) + (i >> 4)] = -kBias;
+    }
   if (!grid_barrier(p.sync + 1)) {
-    if (warp == 0) leave(p.sync, E, lane);
+    if (warp == 0) leave(p.sync, E, T * K, lane);
     drain();
     return;
   }
+
+  // the powers of the rows of h, and which have columns of others
+  for (int s = tid; s < T * K; s += kThreads) {
+    const uint2 m = __ldcg(reinterpret_cast<const uint2*>(p.sync + kSteps) + s);
+    L.power[s] = (short)(L.base[s] + (m.x ? 16 * ((int)m.x - kBias) : 0));  // a row of zeros: any
+    L.mixed[s] = m.x && m.x + m.y != 2u * kBias;
+  }
+  __syncthreads();
 
   // -------------------------------------------------------------- 2: down --
 #pragma unroll 1
@@ -726,15 +805,26 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
     const int a = (u2 + u) / per2, r0 = (u2 + u - a * per2) * (16 * RU);
     const int s0 = L.start[a], cnt = min(L.start[a + 1] - s0, 8 * NT), tiles = (cnt + 7) >> 3;
     float sd[2][RU];
+    bool mixed = false;
 #pragma unroll
     for (int k = 0; k < 2; ++k)
 #pragma unroll
       for (int r = 0; r < RU; ++r) sd[k][r] = __ldg(p.a.s_down + (size_t)L.expert[a] * H + min(r0 + k * 8 * RU + r * 8 + q4, H - 1));
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) xr[nt] = nt * 8 + q4 < cnt ? p.h + (size_t)L.slot[s0 + nt * 8 + q4] * p.ipad + t4 * 8 : nullptr;
+    for (int nt = 0; nt < NT; ++nt) {
+      const bool in = nt * 8 + q4 < cnt;
+      slot_of[nt] = in ? L.slot[s0 + nt * 8 + q4] : 0;
+      xr[nt] = in ? p.h + (size_t)slot_of[nt] * p.ipad + t4 * 8 : nullptr;
+      mixed |= in && L.mixed[slot_of[nt]];
+    }
     clear();
+    if (!__any_sync(0xffffffffu, mixed)) {
 #pragma unroll 1
-    for (int kb = warp % ks2; kb < nb2; kb += ks2) multiply(kb, tiles);
+      for (int kb = warp % ks2; kb < nb2; kb += ks2) multiply(kb, tiles, std::false_type());
+    } else {
+#pragma unroll 1
+      for (int kb = warp % ks2; kb < nb2; kb += ks2) multiply(kb, tiles, std::true_type());
+    }
     if (!gather(ks2)) continue;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -744,20 +834,21 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
         const int n = nt * 8 + 2 * t4 + c;
         if (n >= cnt) continue;
         const int s = L.slot[s0 + n];
-        const float wt = L.weight[s];
+        const int e = L.power[s] - 14;
+        const float wt = L.weight[s] * pow2(e >> 1), back = pow2(e - (e >> 1));
 #pragma unroll
         for (int k = 0; k < 2; ++k)
 #pragma unroll
           for (int r = 0; r < RU; ++r) {
             const int row = r0 + k * 8 * RU + r * 8 + q4;
-            if (row < H) p.part[(size_t)s * H + row] = acc[0][r][nt][c + 2 * k] * sd[k][r] * wt;
+            if (row < H) p.part[(size_t)s * H + row] = acc[0][r][nt][c + 2 * k] * sd[k][r] * wt * back;
           }
       }
     }
   }
   if (!ok) drain();
   const bool met = grid_barrier(p.sync + 2);
-  if (warp == WARPS - 1) leave(p.sync, E, lane);  // the others' loads of phase 3 are under way meanwhile
+  if (warp == WARPS - 1) leave(p.sync, E, T * K, lane);  // the others' loads of phase 3 are under way meanwhile
   if (!met) return;
 
   // --------------------------------------------------- 3: a token's slots --
@@ -801,7 +892,7 @@ cudaError_t launch(const fp8imma_moe_args& a, cudaStream_t st) {
     return was;
   };
   const size_t o_logits = take((size_t)a.tokens * a.experts * 4), o_xf = take((size_t)a.tokens * p.hpad * 2), o_back = take((size_t)a.tokens * 8),
-               o_ids = take(slots * 4), o_wts = take(slots * 4), o_h = take(slots * p.ipad * 2), o_part = take(slots * a.hidden * 4);
+               o_ids = take(slots * 4), o_wts = take(slots * 4), o_h = take(slots * p.ipad * 2), o_step = take(slots * (p.ipad >> 4)), o_part = take(slots * a.hidden * 4);
   ScopedScratch sync, work;
   e = sync.get(kSyncWords * 4, st, kScratchMoeSync);
   if (e == cudaSuccess && sync.owned) e = cudaMemsetAsync(sync.ptr, 0, kSyncWords * 4, st);
@@ -815,6 +906,7 @@ cudaError_t launch(const fp8imma_moe_args& a, cudaStream_t st) {
     p.ids = reinterpret_cast<int*>(base + o_ids);
     p.weights = reinterpret_cast<float*>(base + o_wts);
     p.h = reinterpret_cast<uint16_t*>(base + o_h);
+    p.step = reinterpret_cast<signed char*>(base + o_step);
     p.part = reinterpret_cast<float*>(base + o_part);
     cudaLaunchConfig_t lc = {};
     cudaLaunchAttribute attr[1];

@@ -229,7 +229,8 @@ int fp8imma_kv_attention(const fp8imma_kv_cache* cache, const fp8imma_kv_attenti
 //   out = sum_{e in S} p_e (act(x Wg_e^T) * (x Wu_e^T)) Wd_e^T
 // with FP8 expert weights as fp8imma_quantize_weights makes them (one fp32
 // scale per weight row). Sums are fp32; the product act(g) * u is rounded to
-// fp16 within its row's range before the second product.
+// fp16 before the second product, after a power of two taken from its own
+// values: to 2^-11, or to 2^-24 of the row's largest where that is more.
 #define FP8IMMA_MOE_MAX_TOKENS 64
 #define FP8IMMA_MOE_MAX_TOP_K 16
 #define FP8IMMA_MOE_MAX_EXPERTS 1024
