@@ -1,11 +1,16 @@
 // Log probabilities of given tokens, entropy and top alternatives of logits
 // (fp8imma_token_logprobs).
 //
-// Mathematics, z = x / temperature, in base 2 (u = z log2 e), one pass with a
-// running reference M per lane:
-//   l = sum 2^(u - M),  s = sum 2^(u - M) (u - M)
-//   lse = ln2 (M + log2 l),  entropy = ln2 (log2 l - s / l),  lp(t) = z_t - lse
-// and parts join as l = sum l_i 2^(M_i - M), s = sum 2^(M_i - M) (s_i + (M_i - M) l_i).
+// Mathematics, z = x / temperature, in base 2 (c = log2 e / temperature), one
+// pass with a running reference M per lane, which is a logit:
+//   d = (x - M) c,  l = sum 2^d,  s = sum 2^d d
+//   entropy = ln2 (log2 l - s / l),  lp(t) = (x_t - M) / temperature - ln2 log2 l
+// and parts join as l = sum l_i 2^d_i, s = sum 2^d_i (s_i + d_i l_i), d_i = (M_i - M) c.
+// Differences are taken before the product with c, so that equal logits give
+// exactly 1 however large they are: a lane may see nothing but logits masked by
+// -1e9, and c x - c M would be off by more than fp32's exponent can hold then. A
+// side whose 2^d_i is zero takes no part (d_i l_i may be infinite). A pair of
+// logits costs a sum more than with c M: 4096 rows of 32001 bf16 59.5 us instead of 58.8.
 // The top logits are a warp's list of 32, one a lane in descending order. The
 // pass compares a lane's largest of eight logits with what the list would take;
 // those that reach it go to a buffer in shared memory, and 32 of them at a time
@@ -17,9 +22,10 @@
 // GPU (one row of 32000 bf16 logits: latency; thousands of rows: bandwidth);
 // the last CTA to finish a row joins its parts in order.
 //
-// Measured: 4096 rows of 32001 bf16 logits 59 us without alternatives (4.5 TB/s;
-// instruction issue: an exponential and two sums a logit), 84 us with five of
-// them; one row of 32000 with 8 alternatives 9.4 us, latency: launch, part, join;
+// Measured: 4096 rows of 32001 bf16 logits 60 us without alternatives (4.4 TB/s;
+// instruction issue: an exponential and two sums a logit), 86 us with five of
+// them; 16 rows of 128000 with 20, half of the logits masked, 17 us whether by
+// -inf or by -1e30; one row of 32000 with 8 alternatives 9.4 us, latency: launch, part, join;
 // 16 column-major rows of 128000 with 20 alternatives 32 us, the sorting of short
 // parts' candidates.
 #include "fp8_mma.cuh"
@@ -81,34 +87,43 @@ __device__ __forceinline__ float ex2(float x) {
   return r;
 }
 
-constexpr float kLowest = -1e38f;  // reference before any logit was seen
-constexpr float kRaise = 8.0f;     // the reference follows the maximum when it lies this far above
+constexpr float kLowest = -3.4028234663852886e38f;  // reference before any logit was seen: the lowest number
+constexpr float kRaise = 8.0f;                      // the reference follows the maximum when it lies this far above
 
-// Running sums of a lane or of joined parts.
+// Running sums of a lane or of joined parts; c: log2(e) / temperature.
 struct Sums {
   float m = kLowest, l = 0.0f, s = 0.0f;
-  __device__ __forceinline__ void join(float m2, float l2, float s2) {
-    const float mn = fmaxf(m, m2), da = m - mn, db = m2 - mn, a = ex2(da), b = ex2(db);
-    s = a * fmaf(da, l, s) + b * fmaf(db, l2, s2);
-    l = a * l + b * l2;
+  // (l, s) against a reference that lies -d higher
+  static __device__ __forceinline__ void shift(float d, float& l, float& s) {
+    const float f = ex2(d);
+    s = f == 0.0f ? 0.0f : f * fmaf(d, l, s);
+    l *= f;
+  }
+  __device__ __forceinline__ void join(float m2, float l2, float s2, float c) {
+    const float mn = fmaxf(m, m2);
+    shift((m - mn) * c, l, s);
+    shift((m2 - mn) * c, l2, s2);
+    l += l2;
+    s += s2;
     m = mn;
   }
-  __device__ __forceinline__ void raise(float to) {
-    const float d = m - to, f = ex2(d);
-    s = f * fmaf(d, l, s);
-    l *= f;
-    m = to;
+  // to the largest of the next logits, when it lies far above
+  __device__ __forceinline__ void follow(float big, float c) {
+    if ((big - m) * c > kRaise) {
+      shift((m - big) * c, l, s);
+      m = big;
+    }
   }
   __device__ __forceinline__ void add(float x, float c) {
-    const float d = fmaf(x, c, -m), e = ex2(d);
+    const float d = (x - m) * c, e = ex2(d);
     l += e;
     s = fmaf(e, fmaxf(d, -1000.0f), s);  // a logit of -inf: 0 * -1000
   }
-  __device__ __forceinline__ void warp_join() {
+  __device__ __forceinline__ void warp_join(float c) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
       const float m2 = __shfl_xor_sync(0xffffffffu, m, o), l2 = __shfl_xor_sync(0xffffffffu, l, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
-      join(m2, l2, s2);
+      join(m2, l2, s2, c);
     }
   }
 };
@@ -122,6 +137,16 @@ struct Pair {
     return r;
   }
   static __device__ __forceinline__ void to(unsigned long long x, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x)); }
+  static __device__ __forceinline__ unsigned long long sum(unsigned long long a, unsigned long long b) {
+    unsigned long long r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+  }
+  static __device__ __forceinline__ unsigned long long product(unsigned long long a, unsigned long long b) {
+    unsigned long long r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+  }
   static __device__ __forceinline__ unsigned long long fma(unsigned long long a, unsigned long long b, unsigned long long c) {
     unsigned long long r;
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
@@ -130,9 +155,9 @@ struct Pair {
   __device__ __forceinline__ Pair(const Sums& z, float to_log2) : c(of(to_log2, to_log2)), m(of(-z.m, -z.m)), l(of(z.l, 0.0f)), s(of(z.s, 0.0f)) {}
   __device__ __forceinline__ void add(float x, float y) {
     float d0, d1;
-    to(fma(of(x, y), c, m), d0, d1);
+    to(product(sum(of(x, y), m), c), d0, d1);
     const unsigned long long e = of(ex2(d0), ex2(d1));
-    asm("add.rn.f32x2 %0, %0, %1;" : "+l"(l) : "l"(e));
+    l = sum(l, e);
     s = fma(e, of(fmaxf(d0, -1000.0f), fmaxf(d1, -1000.0f)), s);  // a logit of -inf: 0 * -1000
   }
   __device__ __forceinline__ void fold(Sums& z) const {
@@ -227,8 +252,8 @@ struct Norm {
   unsigned long long mine;  // the lane's entry of the list
 };
 
-// Rows that the pass cannot do: no logit within (-1e38, 1e38) log2 units, NaN,
-// infinities. One warp, two passes over the row, differences before scaling.
+// Rows that the pass cannot do: those that hold NaN or +inf or only -inf. One
+// warp, two passes over the row.
 template <int LT, class Load>
 __device__ __noinline__ Norm careful(int vocab, int n_top, float to_log2, float inv_temp, Load load, int lane) {
   float m = -INFINITY;
@@ -277,8 +302,8 @@ __device__ __forceinline__ void finish(const LpParams& p, int t, Sums z, const T
   const int id = __ldg(p.a.token_ids + t);
   const bool known = (unsigned)id < (unsigned)p.a.vocab;
   const float x = known ? load(id) : NAN;
-  Norm n = {0.0f, p.inv_temp, 0.6931471805599453f * (z.m + log2f(z.l)), 0.6931471805599453f * (log2f(z.l) - z.s / z.l), top.mine};
-  if (!(z.l > 0.0f && z.l < INFINITY && fabsf(z.m) < -kLowest)) n = careful<LT>(p.a.vocab, p.a.top, p.to_log2, p.inv_temp, load, lane);
+  Norm n = {z.m, p.inv_temp, 0.6931471805599453f * log2f(z.l), 0.6931471805599453f * (log2f(z.l) - z.s / z.l), top.mine};
+  if (!(z.l > 0.0f && z.l < INFINITY)) n = careful<LT>(p.a.vocab, p.a.top, p.to_log2, p.inv_temp, load, lane);
   if (lane == 0) {
     p.a.logprobs[t] = fmaf(x - n.at, n.inv, -n.ln_l);
     p.a.entropy[t] = n.entropy;
@@ -317,9 +342,9 @@ __device__ __forceinline__ Sums get_sums(const LpParams& p, int first, int strid
   Sums z;
   for (int k = first + lane * stride; k < p.parts; k += 32 * stride) {
     const float4 v = __ldcg(reinterpret_cast<const float4*>(p.sums + ((int64_t)k * p.a.tokens + t) * 4));
-    z.join(v.x, v.y, v.z);
+    z.join(v.x, v.y, v.z, p.to_log2);
   }
-  z.warp_join();
+  z.warp_join(p.to_log2);
   return z;
 }
 // Their lists merged, the next one under way.
@@ -431,7 +456,7 @@ __device__ __noinline__ void gather(Quad v, float bar, unsigned long long* buf, 
 // A CTA's sums and lists (one a warp) joined in the first warp, the sums in its
 // lane 0: pairs of warps in a fixed order.
 template <int kWarps>
-__device__ __forceinline__ void join_warps(Sums& z, Top& list, float (*sums)[3], unsigned long long (*lists)[32], bool top, int warp, int lane) {
+__device__ __forceinline__ void join_warps(Sums& z, Top& list, float (*sums)[3], unsigned long long (*lists)[32], float c, bool top, int warp, int lane) {
   if (lane == 0) {
     sums[warp][0] = z.m;
     sums[warp][1] = z.l;
@@ -459,7 +484,7 @@ __device__ __forceinline__ void join_warps(Sums& z, Top& list, float (*sums)[3],
 #pragma unroll
     for (int o = kWarps / 2; o > 0; o >>= 1) {
       const float m2 = __shfl_xor_sync(0xffffffffu, z.m, o), l2 = __shfl_xor_sync(0xffffffffu, z.l, o), s2 = __shfl_xor_sync(0xffffffffu, z.s, o);
-      z.join(m2, l2, s2);
+      z.join(m2, l2, s2, c);
     }
   }
 }
@@ -500,7 +525,7 @@ __global__ void __launch_bounds__(kWarps * 32, 32 / kWarps) logprobs_row_kernel(
     auto end = [&](int j) {  // one logit a lane from an end of the row (j < 0: none)
       float x = -INFINITY;
       if (j >= 0) x = LT == FP8IMMA_L_F32 ? __ldg(reinterpret_cast<const float*>(row) + j) : to_f32<LT>(__ldg(reinterpret_cast<const unsigned short*>(row) + j));
-      if (x * c > z.m + kRaise) z.raise(x * c);
+      z.follow(x, c);
       z.add(x, c);
       if (top) n = put(x, j >= 0 && x >= bar, buf, n, j, lane);
     };
@@ -525,7 +550,7 @@ __global__ void __launch_bounds__(kWarps * 32, 32 / kWarps) logprobs_row_kernel(
         else if (kWarps > 1) bar = fmaxf(bar, enters_at(Top(), *(volatile unsigned int*)&s_floor));
         fresh = false;
       }
-      if (big * c > z.m + kRaise) z.raise(big * c);
+      z.follow(big, c);
       Pair two(z, c);
 #pragma unroll
       for (int k = 0; k < kAhead; ++k)
@@ -568,8 +593,8 @@ __global__ void __launch_bounds__(kWarps * 32, 32 / kWarps) logprobs_row_kernel(
       end(j < V ? j : -1);
     }
     if (top) list = flush(list, buf, n, top, lane);
-    z.warp_join();
-    join_warps<kWarps>(z, list, s_sums, s_list, top > 0, warp, lane);
+    z.warp_join(c);
+    join_warps<kWarps>(z, list, s_sums, s_list, c, top > 0, warp, lane);
     if (threadIdx.x == 0) s_floor = 0u;
     if (warp == 0) {
       if (p.parts == 1) finish<LT>(p, t, z, list, lane);
@@ -579,7 +604,7 @@ __global__ void __launch_bounds__(kWarps * 32, 32 / kWarps) logprobs_row_kernel(
       Sums all = get_sums(p, warp, kWarps, t, lane);
       Top l;
       if (top) l = get_lists(p, warp, kWarps, t, lane);
-      join_warps<kWarps>(all, l, s_sums, s_list, top > 0, warp, lane);
+      join_warps<kWarps>(all, l, s_sums, s_list, c, top > 0, warp, lane);
       if (warp == 0) finish<LT>(p, t, all, l, lane);
     }
     __syncthreads();  // shared memory is free for the next row
@@ -658,7 +683,7 @@ __global__ void __launch_bounds__(kColWarps * 32, 4) logprobs_col_kernel(const _
         float big = x[0];
 #pragma unroll
         for (int i = 1; i < kEach; ++i) big = fmaxf(big, x[i]);
-        if (big * c > z[k].m + kRaise) z[k].raise(big * c);
+        z[k].follow(big, c);
 #pragma unroll
         for (int i = 0; i < kEach; ++i) z[k].add(x[i], c);
         if (top) {
@@ -677,7 +702,7 @@ __global__ void __launch_bounds__(kColWarps * 32, 4) logprobs_col_kernel(const _
     for (int k = 0; k < 2; ++k) {
       const int t = warp + k * kWarps;
       if (t >= n) break;
-      z[k].warp_join();
+      z[k].warp_join(c);
       if (p.parts == 1) finish<LT>(p, t0 + t, z[k], list[k], lane);
       else put_part(p, part, t0 + t, z[k], list[k], lane);
     }
