@@ -496,7 +496,7 @@ int fp8imma_set_pdl(int enable) {
 
 unsigned int fp8imma_device_error(int clear) {
   return gemv_device_error(clear != 0) | decode_device_error(clear != 0) | tc_device_error(clear != 0) |
-         peer_device_error(clear != 0) | attn_device_error(clear != 0) |
+         peer_device_error(clear != 0) | kv_append_device_error(clear != 0) | attn_device_error(clear != 0) |
          attn_tc_device_error(clear != 0) | moe_device_error(clear != 0);
 }
 

@@ -182,6 +182,7 @@ cudaError_t launch_row_scales(const void* A, int a_type, int M, int K, uint16_t*
                               float* g, cudaStream_t stream);
 
 // Checks of a paged KV cache shared by its append and its attention.
+unsigned int kv_append_device_error(bool clear);
 unsigned int attn_device_error(bool clear);
 unsigned int moe_device_error(bool clear);
 cudaError_t attn_set_wait_limit(unsigned long long ns);

@@ -26,7 +26,6 @@ struct AttnParams {
   int group;     // query heads per KV head
   int vec_q;     // query rows are 16-byte aligned
   int copy;      // pages are copied by lanes instead of TMA
-  int max_items; // items of the step at most (counters)
   unsigned int* counters;  // per item: finished parts; zero between calls
   float* parts;            // per (CTA, first / last segment, row warp): M, L, O of a shared item
 };
@@ -158,7 +157,9 @@ struct Runs {
 };
 
 // This CTA's run of units, by a scan of the sequences' units and items; all
-// threads of the CTA take part. False: it has none.
+// threads of the CTA take part. False: it has none, or the offsets of the step's
+// tokens do not ascend (two sequences could own a row, and their items would be
+// more than the counters that the host has made room for).
 template <int THREADS>
 __device__ __forceinline__ bool find_run(const AttnParams& p, int rows_per_tile, Walk& walk, int& units, int& ctas) {
   __shared__ int s_scan[2][THREADS / 32];
@@ -166,10 +167,12 @@ __device__ __forceinline__ bool find_run(const AttnParams& p, int rows_per_tile,
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   units = 0;
   int items = 0, n = 0, ni = 0, at = 0, at_i = 0;
+  bool bad = false;
   auto scan = [&](int b0) {  // of sequences b0 .. b0 + THREADS: this thread's start, the running totals
     n = ni = 0;
     if (b0 + tid < p.c.batch) {
       const Seq s = load_seq(p, b0 + tid, rows_per_tile);
+      bad |= p.per_seq == 0 && __ldg(p.c.cu_new + b0 + tid + 1) < __ldg(p.c.cu_new + b0 + tid);
       ni = s.row_tiles * p.c.kv_heads;
       n = ni * s.tiles;
     }
@@ -187,7 +190,7 @@ __device__ __forceinline__ bool find_run(const AttnParams& p, int rows_per_tile,
       s_scan[0][warp] = x;
       s_scan[1][warp] = xi;
     }
-    __syncthreads();
+    bad = __syncthreads_or(bad);
     at = units + x - n;
     at_i = items + xi - ni;
 #pragma unroll
@@ -201,11 +204,11 @@ __device__ __forceinline__ bool find_run(const AttnParams& p, int rows_per_tile,
     }
   };
   for (int b0 = 0; b0 < p.c.batch; b0 += THREADS) scan(b0);
-  if (units == 0) return false;
-  if (items > p.max_items) {  // offsets that do not ascend: more rows than tokens
+  if (bad) {
     if (tid == 0) atomicCAS(&g_fp8imma_device_error, 0u, (unsigned int)ERR_BAD_OFFSETS);
     return false;
   }
+  if (units == 0) return false;
   ctas = min((int)gridDim.x, units);
   if ((int)blockIdx.x >= ctas) return false;
   const Runs runs(units, ctas);

@@ -761,7 +761,6 @@ cudaError_t launch(AttnParams& p, cudaStream_t st) {
   const int64_t tiles = ((int64_t)p.c.max_pages * p.c.page_size + kKeys - 1) / kKeys;
   if (items * tiles > 0x7fffffffll) return cudaErrorInvalidValue;  // units are counted in 31 bits
   const int grid = (int)std::min<int64_t>(num_sms_current(), std::max<int64_t>(1, items * tiles));
-  p.max_items = (int)items;
   const size_t ctr_bytes = (size_t)items * 4, part_bytes = (size_t)grid * 2 * S::kPartFloats * 4;
   ScopedScratch ctr, part;
   e = ctr.get(ctr_bytes, st, kScratchAttn);

@@ -16,10 +16,11 @@
 // its time on. Rows stay in registers between the pass for the scale and the one
 // for the codes, as far as kKeep pieces a thread go.
 //
-// Measured: 64 sequences of one token, 8 heads of 128: 4.6 us (6.0 with a page
+// Measured: 64 sequences of one token, 8 heads of 128: 4.8 us (6.0 with a page
 // lookup a warp), a chain of latencies: lengths, page id, row and scale, store.
-// Prompts of 9200 tokens, rows from HBM: 21.7 us, 2.6 TB/s of the 57 MB read and
-// written (24.6 with two CTAs a SM, 39 us with a page lookup a warp as well).
+// Prompts of 9200 tokens, rows from HBM: 22.6 us, 2.5 TB/s of the 57 MB read and
+// written (24.6 with two CTAs a SM, 39 us with a page lookup a warp as well); the
+// look at all offsets is 0.8 of them.
 #include "fp8_mma.cuh"
 #include "fp8imma/fp8imma_ext.h"
 #include "fp8imma_kernels.h"
@@ -106,7 +107,7 @@ __device__ __forceinline__ int touched(const AppendParams& p, int b, int& first)
 template <int AT, int FMT, int CTAS>
 __global__ void __launch_bounds__(kThreads, CTAS) kv_append_kernel(const __grid_constant__ AppendParams p) {
   __shared__ int s_pick[3];
-  __shared__ int s_scan[kWarps];
+  __shared__ int s_scan[2][kWarps];
   __shared__ float s_max[kWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   pdl_launch_dependents();
@@ -119,7 +120,8 @@ __global__ void __launch_bounds__(kThreads, CTAS) kv_append_kernel(const __grid_
   } else {
     // unit blockIdx.x of the sequences' touched pages laid end to end
     if (threadIdx.x == 0) s_pick[0] = -1;
-    int base = 0;
+    int base = 0, turn = 0;
+    bool bad = false;
     for (int b0 = 0; b0 < p.c.batch; b0 += kThreads) {
       const int mine = b0 + (int)threadIdx.x;
       int f = 0;
@@ -130,15 +132,22 @@ __global__ void __launch_bounds__(kThreads, CTAS) kv_append_kernel(const __grid_
         const int y = __shfl_up_sync(0xffffffffu, x, o);
         if (lane >= o) x += y;
       }
-      __syncthreads();
-      if (lane == 31) s_scan[warp] = x;
-      __syncthreads();
+      if (lane == 31) s_scan[turn][warp] = x;
+      // Offsets that do not ascend would give a token to two sequences. Every CTA
+      // looks at all of them first, so that none of them stores anything.
+      if (b0 == 0)
+        for (int i = mine; i < p.c.batch; i += kThreads) bad |= __ldg(p.c.cu_new + i + 1) < __ldg(p.c.cu_new + i);
+      if (__syncthreads_or(bad)) {
+        if (threadIdx.x == 0) atomicCAS(&g_fp8imma_device_error, 0u, (unsigned int)ERR_BAD_OFFSETS);
+        return;
+      }
       int before = base;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        if (w < warp) before += s_scan[w];
-        base += s_scan[w];
+        if (w < warp) before += s_scan[turn][w];
+        base += s_scan[turn][w];
       }
+      turn ^= 1;  // the other one has been read by all: they have met since
       const int lo = before + x - n;
       if ((int)blockIdx.x >= lo && (int)blockIdx.x < lo + n) {
         s_pick[0] = mine;
@@ -251,6 +260,8 @@ cudaError_t launch_append(const AppendParams& p, dim3 grid, cudaStream_t st) {
 }
 
 }  // namespace
+
+unsigned int kv_append_device_error(bool clear) { return fp8imma_dev::tu_device_error(clear); }
 
 cudaError_t kv_cache_check(const fp8imma_kv_cache* c) {
   if (!c) return cudaErrorInvalidValue;

@@ -175,7 +175,9 @@ int fp8imma_set_fused_gather(int enable);
 // read a page through several tables (shared prefixes). A page id outside
 // [0, num_pages) is a hole: nothing is stored there and attention skips it.
 // Tokens past max_pages * page_size have no place: they are neither stored nor
-// read. Scales are not negative.
+// read. Scales are not negative. A cu_new that descends anywhere sets the error
+// word (fp8imma_device_error(): 7) and nothing is written; rows of the packed
+// axis that no sequence owns are not read, and not written.
 typedef struct fp8imma_kv_cache {
   void* k;                    // [num_pages, kv_heads, page_size, head_dim] FP8 bytes, 16-byte aligned
   void* v;
