@@ -505,7 +505,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                   }
                 }
                 if (__any_sync(0xffffffffu, odd)) {
-                  // rare: take the non-finite codes out of the product and add them to the rows that see them
+                  // rare: take the non-finite codes out of the product and add them to the rows that see their keys,
+                  // whatever the weight (one below fp32's range is still a weight)
 #pragma unroll
                   for (int e = 0; e < 4; ++e)
 #pragma unroll
@@ -515,15 +516,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
 #pragma unroll 1
                   for (int e = 0; e < 16; ++e) {
-                    const int fr = D == 64 ? ((e >> 2) * 2 + (e & 1) + (e & 2) * 4) : e;  // fragment row of key e
-                    float pv[NT][2];
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                      for (int c = 0; c < 2; ++c) {
-                        const float lo = __shfl_sync(0xffffffffu, sa[k][nt][c], (fr & 7) * 4 + t4), hi = __shfl_sync(0xffffffffu, sa[k][nt][c + 2], (fr & 7) * 4 + t4);
-                        pv[nt][c] = fr < 8 ? lo : hi;
-                      }
                     const int r = (g0 + k) * 16 + e, j = tile * kKeys + r;
                     if (j >= g.hi || j < g.lo) continue;
 #pragma unroll
@@ -539,7 +531,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                             for (int c = 0; c < 2; ++c)
-                              if (pv[nt][c] != 0.0f) o[hf * 2 * W + i][nt][c + 2 * f] += pv[nt][c] * val;
+                              if (j <= pos[nt][c] && (p.a.window == 0 || j > pos[nt][c] - p.a.window)) o[hf * 2 * W + i][nt][c + 2 * f] += val;
                         }
                       }
                   }
