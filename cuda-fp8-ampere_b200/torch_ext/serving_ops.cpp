@@ -36,6 +36,13 @@ bool is_bytes(const torch::Tensor& x) {
   return t == at::kByte || t == at::kFloat8_e4m3fn || t == at::kFloat8_e5m2;
 }
 
+// bytes of any dtype that does not name the other format
+void check_format(const torch::Tensor& x, int format, const char* name) {
+  const auto t = x.scalar_type();
+  TORCH_CHECK(t == at::kByte || t == (format == FP8IMMA_B_E4M3 ? at::kFloat8_e4m3fn : at::kFloat8_e5m2), name, " is ", t,
+              ", but the format asked for is ", format == FP8IMMA_B_E4M3 ? "'e4m3'" : "'e5m2'");
+}
+
 void check_on(const torch::Tensor& x, const torch::Tensor& like, const char* name) {
   TORCH_CHECK(x.is_cuda(), name, " must be a CUDA tensor");
   TORCH_CHECK(x.device() == like.device(), name, " must be on ", like.device());
@@ -57,10 +64,12 @@ fp8imma_kv_cache cache_args(const torch::Tensor& rows, const torch::Tensor& k_ca
                             const torch::Tensor& seq_lens, const c10::optional<torch::Tensor>& cu_seqlens,
                             const std::string& fmt) {
   fp8imma_kv_cache c = {};
+  c.format = byte_format(fmt, "fmt");
   for (const auto* x : {&k_cache, &v_cache}) {
     check_on(*x, rows, "k_cache / v_cache");
     TORCH_CHECK(is_bytes(*x) && x->dim() == 4 && x->is_contiguous(),
                 "k_cache / v_cache must be contiguous uint8 [num_pages, kv_heads, page_size, head_dim]");
+    check_format(*x, c.format, "k_cache / v_cache");
   }
   TORCH_CHECK(k_cache.sizes() == v_cache.sizes(), "k_cache and v_cache must have the same shape");
   for (const auto* x : {&k_scale, &v_scale}) {
@@ -78,7 +87,6 @@ fp8imma_kv_cache cache_args(const torch::Tensor& rows, const torch::Tensor& k_ca
   c.v_scale = v_scale.data_ptr<float>();
   c.page_table = page_table.data_ptr<int>();
   c.seq_lens = seq_lens.data_ptr<int>();
-  c.format = byte_format(fmt, "fmt");
   c.num_pages = to_int(k_cache.size(0), "num_pages");
   c.kv_heads = to_int(k_cache.size(1), "kv_heads");
   c.page_size = to_int(k_cache.size(2), "page_size");
@@ -172,9 +180,11 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> moe_forward(
   check_packed(router, x, x.scalar_type(), "router");
   TORCH_CHECK(router.dim() == 2 && router.size(1) == x.size(1), "router must have shape [experts, hidden]");
   const int64_t T = x.size(0), H = x.size(1), E = router.size(0);
+  a.format = byte_format(b_format, "b_format");
   for (const auto* w : {&w_gate_up, &w_down}) {
     check_on(*w, x, "w_gate_up / w_down");
     TORCH_CHECK(is_bytes(*w) && w->dim() == 3 && w->is_contiguous(), "w_gate_up / w_down must be contiguous 3-D uint8");
+    check_format(*w, a.format, "w_gate_up / w_down");
   }
   const int64_t I = w_down.size(2);
   TORCH_CHECK(w_gate_up.size(0) == E && w_gate_up.size(1) == 2 * I && w_gate_up.size(2) == H,
@@ -192,7 +202,6 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> moe_forward(
   if (act == "silu") a.act = 3;
   else if (act == "gelu") a.act = 2;
   else TORCH_CHECK(false, "act must be 'silu' or 'gelu'");
-  a.format = byte_format(b_format, "b_format");
   const c10::cuda::CUDAGuard guard(x.device());
   torch::Tensor o;
   if (out.has_value()) {
