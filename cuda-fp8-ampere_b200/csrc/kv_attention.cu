@@ -683,25 +683,35 @@ cudaError_t launch(AttnParams& p, cudaStream_t st) {
   return e != cudaSuccess ? e : e1 != cudaSuccess ? e1 : e2;
 }
 
-// Whether many rows and enough tiles are there for the tcgen05 kernel
-// (kv_attention_tc.cu). A tile costs it about 2 us at head_dim 128, 1.6 at 64,
-// whatever the rows, and a call some 12 us more than here (TMEM, a deeper
-// pipeline); a tile costs this file's kernel 3.2 us with 32 rows of 128 channels,
-// 4.7 with 64, 9 with 128, and half of that at 64 channels, where up to 32 rows
-// stay here. Measured, this kernel against that one, in us: 16 sequences of 8000
-// keys, 64 heads over 8: 32 rows 181/121, 64 rows 263/124, 128 rows 495/134; 24
-// of 6000, 28 heads over 4 of 64: 28 rows 59/69, 35 rows 100/69; few tiles: 8 of
-// 2000, 32 heads over 8, 16 rows 30/39; 4 of 300 18 against 16. Tiles are
-// counted by what the page tables can hold, since lengths lie on the device.
+// Whether rows and tiles are enough for the tcgen05 kernel (kv_attention_tc.cu).
+// Its tile of up to 128 rows costs much the same whatever the rows (1.7 us a tile
+// and SM at 128 channels, 1.3 at 64) and a call about 10 us more than here (TMEM, a
+// deeper pipeline); here a tile costs by the rows that launch_d() rounds them up to:
+// 128 channels 2.3 us with 32 rows, 4.4 with 64, as much again for each further 64;
+// about half of that at 64 channels. With up to 16 rows (32 of 64 channels) it never
+// pays, with up to twice as many from 16 (8) tiles an SM on, with more from 1.5 on.
+// Measured, this kernel against that one, in us, tiles an SM in brackets:
+//   128 channels, 16 rows: [28] 53/76, [221] 308/468
+//     24 rows: [7] 36/42, [14] 52/53, [17] 62/60, [28] 84/78, [221] 541/472
+//     40 rows: [0.9] 32/31, [1.7] 29/27, [7] 61/42, [28] 154/79, [221] 1033/477
+//     128 rows: [0.9] 35/41, [1.7] 49/33, [14] 146/70;  512 rows: [14] 169/78
+//   64 channels, 28 rows: [14] 37/46, [111] 186/207
+//     35 rows: [3.5] 29/31, [7] 40/39, [9] 45/40, [111] 332/207
+//     112 rows: [1.3] 26/30, [1.7] 31/28, [9] 70/44
+// Tiles are counted by what the page tables can hold, since lengths lie on the
+// device: under a table for 131072 keys, 24 rows of 8 sequences of 300 take 30 us
+// there where they would take 24 here, of 32 sequences of 1000 64 for 56.
 bool tc_pays(const AttnParams& p, int64_t rows) {
-  if (p.c.head_dim == 256) return false;
+  const int D = p.c.head_dim;
+  if (D == 256) return false;
   const int forced = g_tc_rows.load();
   if (forced > 0) return rows >= forced;
-  if (rows < (p.c.head_dim == 64 ? 33 : 16)) return false;
+  const int none = D == 64 ? 32 : 16;
+  if (rows <= none) return false;
   int64_t keys = (int64_t)p.c.max_pages * p.c.page_size;
   if (p.a.window > 0) keys = std::min<int64_t>(keys, (int64_t)p.a.window + rows / p.group + kKeys);
   const int64_t tiles = (keys + kKeys - 1) / kKeys * ((rows + 127) / 128) * p.c.batch * p.c.kv_heads;
-  return tiles * std::min<int64_t>(rows, 128) >= 320ll * num_sms_current();
+  return 2 * tiles >= (rows <= 2 * none ? (D == 64 ? 16 : 32) : 3) * (int64_t)num_sms_current();
 }
 
 // Query rows a CTA works on at once: the rows of a sequence and KV head
