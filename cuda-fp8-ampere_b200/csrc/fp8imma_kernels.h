@@ -181,7 +181,7 @@ cudaError_t launch_generic_s8(const GemvParams& p, int a_type, int fmt, cudaStre
 cudaError_t launch_row_scales(const void* A, int a_type, int M, int K, uint16_t* a_inv_h,
                               float* g, cudaStream_t stream);
 
-// Checks of a paged KV cache shared by its append and its attention.
+// The same of the decode-step operators.
 unsigned int kv_append_device_error(bool clear);
 unsigned int attn_device_error(bool clear);
 unsigned int moe_device_error(bool clear);
@@ -191,6 +191,7 @@ cudaError_t attn_tc_set_wait_limit(unsigned long long ns);
 // query rows of a sequence and KV head from which the cache attention runs on tcgen05 (0: by its own rule)
 void attn_set_tc_rows(int rows);
 cudaError_t moe_set_wait_limit(unsigned long long ns);
+// Checks of a paged KV cache shared by its append and its attention.
 cudaError_t kv_cache_check(const ::fp8imma_kv_cache* cache);
 
 }  // namespace fp8imma_b200

@@ -23,13 +23,13 @@
 // as soon as its scores are made.
 //
 // Measured (e4m3, fp16): 16 sequences of 8000 keys, 64 heads over 8, 128
-// channels, 32 rows a KV head 121 us (2.2 TB/s), 128 rows 134 us (496 us in the
-// few-row kernel); prompts of 4 x 1000 tokens, 32 heads over 8, 214 us (577);
-// one of 8192 tokens 1.72 ms (7.58; 320 TFLOP/s of the causal half). What bounds
-// it are the latencies of instruction issue (4 warps a scheduler, 0.44
-// instructions a cycle): a tile takes some 3500 cycles, of which its products
-// and its exponentials need about 1000 each. Loads through registers instead of
-// shared memory waited for each other: 221 us where this takes 121.
+// channels, 32 rows a KV head 125 us (2.1 TB/s), 128 rows 137 us (493 us in the
+// few-row kernel); prompts of 4 x 1000 tokens, 32 heads over 8, 220 us (576);
+// one of 8192 tokens 1.73 ms (7.26; 318 TFLOP/s of the causal half). What bounds
+// it are the latencies of instruction issue (4.2 warps a scheduler, 0.43
+// instructions a cycle, the tensor pipe 21% of the time): a tile takes some 4000
+// cycles, of which its products need about 900. Loads through registers instead
+// of shared memory waited for each other: 221 us where this took 121.
 #include "kv_attention.cuh"
 #include "sm100_umma.cuh"
 #include <type_traits>

@@ -926,7 +926,10 @@ cudaError_t launch(const fp8imma_moe_args& a, cudaStream_t st) {
 
 // Token tiles by the number of tokens, which an expert may all be given; with
 // many tokens a unit has more rows, so that the tokens' operands, read again
-// for each unit, cost less beside the weights.
+// for each unit, cost less beside the weights. Measured with 1, 2 and 4 tiles:
+// one token, 6 of 64, 2048 x 1408 25 / 27 / 31 us; 8 tokens, 2 of 8, 4096 x 11008
+// 197 / 214 / 221; 16 tokens 223 / 245 with 2 and 4; 12 and 16 tokens, 4 of 32,
+// 4096 x 2048 141 / 157 and 149 / 162.
 template <int FMT>
 cudaError_t launch_nt(const fp8imma_moe_args& a, cudaStream_t st) {
   if (a.tokens <= 8) return launch<FMT, 1, 2, 16, 2>(a, st);

@@ -298,6 +298,7 @@ void register_serving_ops(pybind11::module_& m) {
         "Mixture-of-experts layer with FP8 weights for 1..64 tokens (fp8imma_moe_forward)\n"
         "x: [tokens, hidden] fp16/bf16; router: [experts, hidden]; w_gate_up: [experts, 2 * inter, hidden] uint8 (gate rows, then up rows)\n"
         "w_down: [experts, hidden, inter] uint8; s_gate_up, s_down: one fp32 scale per weight row (quantize_weights)\n"
+        "act: 'silu' or 'gelu' (tanh form)\n"
         "Returns (out [tokens, hidden], ids [tokens, top_k] int32, weights [tokens, top_k] fp32)",
         py::arg("x"), py::arg("router"), py::arg("w_gate_up"), py::arg("s_gate_up"), py::arg("w_down"),
         py::arg("s_down"), py::arg("top_k"), py::arg("renormalize") = true, py::arg("act") = "silu",
