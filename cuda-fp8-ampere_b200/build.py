@@ -31,7 +31,7 @@ NVCC_FLAGS = ["-DFP8IMMA_NVTX", "-O3", "-std=c++17", "-lineinfo", "-Xcompiler", 
               "--expt-relaxed-constexpr", "-I" + INCLUDE, "-I" + CSRC]
 
 CU_SOURCES = ["api.cu", "gemv_splitk.cu", "decode.cu", "generic.cu", "fp8wgt.cu", "host_util.cu", "gemm_tc.cu", "noalloc.cu", "peer.cu", "quantize.cu",
-              "kv_cache.cu", "kv_attention.cu", "kv_attention_tc.cu", "moe.cu", "logprobs.cu"]
+              "kv_cache.cu", "kv_attention.cu", "kv_attention_tc.cu", "moe.cu", "logprobs.cu", "residual_norm.cu", "lora.cu", "kv_rope.cu", "kv_attention_tree.cu", "kv_attention_tree_tc.cu"]
 
 
 def _run(cmd: list[str]) -> None:
@@ -90,14 +90,18 @@ def _torch_ext(name: str, sources: list[str], force: bool = False) -> str:
     suffix = sysconfig.get_config_var("EXT_SUFFIX") or ".so"
     out = os.path.join(HERE, name + suffix)
     srcs = [os.path.join(HERE, "torch_ext", s) for s in sources]
-    if not force and _newer(out, srcs + [LIB, os.path.join(INCLUDE, "fp8imma", "imma_fp8.h")]):
+    hdrs = [os.path.join(HERE, "torch_ext", "serving_checks.h"), os.path.join(INCLUDE, "fp8imma", "imma_fp8.h")]
+    if not force and _newer(out, srcs + hdrs + [LIB]):
         return out
     inc = ce.include_paths() + [os.path.join(CUDA_HOME, "include"), INCLUDE, sysconfig.get_paths()["include"]]
     libdirs = ce.library_paths() + [HERE]
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
-    cmd = ["g++", "-O3", "-shared", "-fPIC", "-std=c++17", "-DTORCH_EXTENSION_NAME=" + name,
-           "-DTORCH_API_INCLUDE_EXTENSION_H", "-D_GLIBCXX_USE_CXX11_ABI=%d" % abi]
-    cmd += ["-I" + p for p in inc] + srcs + ["-o", out]
+    flags = ["-O3", "-fPIC", "-std=c++17", "-DTORCH_EXTENSION_NAME=" + name, "-DTORCH_API_INCLUDE_EXTENSION_H", "-D_GLIBCXX_USE_CXX11_ABI=%d" % abi]
+    objs = [os.path.join(OBJ, s.replace(".cpp", ".o")) for s in sources]
+    jobs = [["g++"] + flags + ["-I" + p for p in inc] + ["-c", s, "-o", o] for s, o in zip(srcs, objs)]
+    with cf.ThreadPoolExecutor(max_workers=len(jobs)) as ex:
+        list(ex.map(_run, jobs))
+    cmd = ["g++", "-shared"] + objs + ["-o", out]
     cmd += ["-L" + p for p in libdirs]
     cmd += ["-lfp8imma", "-lc10", "-ltorch", "-ltorch_cpu", "-ltorch_python", "-lc10_cuda", "-ltorch_cuda",
             "-L" + os.path.join(CUDA_HOME, "lib64"), "-lcudart"]
@@ -109,7 +113,7 @@ def _torch_ext(name: str, sources: list[str], force: bool = False) -> str:
 def build_all(force: bool = False) -> None:
     build_lib(force=force)
     with cf.ThreadPoolExecutor(max_workers=2) as ex:
-        futs = [ex.submit(_torch_ext, "fp8imma_ext", ["fp8imma_ext.cpp", "serving_ops.cpp"], force),
+        futs = [ex.submit(_torch_ext, "fp8imma_ext", ["fp8imma_ext.cpp", "serving_ops.cpp", "layer_ops.cpp"], force),
                 ex.submit(_torch_ext, "fp8wgt_ext", ["fp8wgt_ext.cpp"], force)]
         for f in futs:
             f.result()

@@ -82,8 +82,17 @@ void* stream_scratch(cudaStream_t stream, size_t bytes, int tag, bool* fresh = n
 struct ScopedScratch {
   void* ptr = nullptr;
   bool owned = false;
+  bool own = false;
+  // A captured call takes memory of its own, so that graphs captured on one
+  // stream may be replayed at once on several.
+  cudaError_t own_if_captured(cudaStream_t st) {
+    cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
+    const cudaError_t e = cudaStreamIsCapturing(st, &cs);
+    own = cs != cudaStreamCaptureStatusNone;
+    return e;
+  }
   cudaError_t get(size_t bytes, cudaStream_t st, int tag) {
-    ptr = stream_scratch(st, bytes, tag);
+    if (!own) ptr = stream_scratch(st, bytes, tag);
     if (ptr) return cudaSuccess;
     owned = true;
     return cudaMallocAsync(&ptr, bytes, st);
@@ -191,6 +200,11 @@ cudaError_t attn_tc_set_wait_limit(unsigned long long ns);
 // query rows of a sequence and KV head from which the cache attention runs on tcgen05 (0: by its own rule)
 void attn_set_tc_rows(int rows);
 cudaError_t moe_set_wait_limit(unsigned long long ns);
+unsigned int kv_rope_device_error(bool clear);
+unsigned int attn_tree_device_error(bool clear);
+unsigned int attn_tree_tc_device_error(bool clear);
+cudaError_t attn_tree_set_wait_limit(unsigned long long ns);
+cudaError_t attn_tree_tc_set_wait_limit(unsigned long long ns);
 // Checks of a paged KV cache shared by its append and its attention.
 cudaError_t kv_cache_check(const ::fp8imma_kv_cache* cache);
 

@@ -1,5 +1,5 @@
-// What the two kernels of the cache attention share (kv_attention.cu: few query
-// rows a KV head; kv_attention_tc.cu: many): the cut of the work into equal
+// What the two kernels of the cache attention share (kv_attention_few.cuh: few
+// query rows a KV head; kv_attention_tc.cuh: many): the cut of the work into equal
 // runs of 128-key tiles, and the join of parts.
 #pragma once
 
@@ -19,6 +19,14 @@ constexpr int kKeys = 128;                  // keys of a tile
 constexpr float kTinyScale = 7.888609e-31f; // 2^-100: value scales below count as this (values below 2^-91)
 constexpr float kRaise = 8.0f;              // M follows the maximum when it lies this far above
 
+// What kv_attention_tree adds; the kernels' TREE variants read it.
+struct TreeParams {
+  const uint32_t* mask;      // null: the step is causal
+  const int32_t* positions;  // null: a token's place
+  int words;
+  float cap;                 // 0: scores as they are
+};
+
 struct AttnParams {
   fp8imma_kv_cache c;
   fp8imma_kv_attention_args a;
@@ -28,6 +36,7 @@ struct AttnParams {
   int copy;      // pages are copied by lanes instead of TMA
   unsigned int* counters;  // per item: finished parts; zero between calls
   float* parts;            // per (CTA, first / last segment, row warp): M, L, O of a shared item
+  TreeParams t;
 };
 
 // ---------------------------------------------------------------- helpers --
@@ -56,6 +65,12 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   uint32_t r;
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
+}
+// cap tanh(s / cap) in base 2, from x = s log2 e: cap2 = cap log2 e, icap = 2 / cap.
+// tanh y = 1 - 2 / (1 + e^2y) is off by some 2^-23 wherever y lies, so the score is
+// by cap 2^-23: 2^-17 of a weight at a cap of 50.
+__device__ __forceinline__ float cap_score(float x, float cap2, float icap) {
+  return fmaf(-2.0f * cap2, __fdividef(1.0f, 1.0f + ex2(x * icap)), cap2);
 }
 // 16 bytes global -> shared, asynchronously
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
@@ -118,6 +133,7 @@ struct Walk {
   int u, end, base, item_base;  // base: first unit of sequence b, item_base: its first item
   int b;
   Seq s;
+  template <bool TREE = false>
   __device__ __forceinline__ bool next(const AttnParams& p, int rows_per_tile, Segment& g) {
     if (u >= end) return false;
     int items = s.row_tiles * p.c.kv_heads;
@@ -140,8 +156,60 @@ struct Walk {
     g.pos_max = s.len - s.n + r1 / p.group;
     g.lo = p.a.window > 0 ? (int)max((int64_t)0, (int64_t)g.pos_min - p.a.window + 1) : 0;
     g.hi = min(s.cap, g.pos_max + 1);
+    if (TREE && p.t.mask) {
+      // any of the step's keys may be seen by any row; all rows see the keys before it, up to the window
+      g.pos_min = s.len - s.n - 1;
+      g.pos_max = s.len - 1;
+      g.lo = p.a.window > 0 ? (int)max((int64_t)0, (int64_t)s.len - s.n - p.a.window + 1) : 0;
+      g.hi = s.cap;
+    }
     u += g.count;
     return true;
+  }
+};
+
+// A row's token as the mask sees it.
+template <bool TREE>
+struct Sight {
+  int pos;                // its place, for the window (below all places: no row)
+  int start;              // the step's first place
+  const uint32_t* mask;   // its mask row, null: causal
+  __device__ __forceinline__ void set(const AttnParams& p, const Seq& s, int row) {
+    const bool in = row < s.rows;
+    const int tok = row / p.group;
+    pos = in ? s.len - s.n + tok : TREE ? -(1 << 30) : -1;  // with a mask places below 0 have rows too
+    if (TREE) {
+      start = s.len - s.n;
+      mask = nullptr;
+      if (p.t.mask) {
+        mask = p.t.mask + (in ? (int64_t)(s.t0 + tok) * p.t.words : 0);
+        if (in && p.t.positions) pos = min(max(__ldg(p.t.positions + s.t0 + tok), start), s.len - 1);
+      }
+    }
+  }
+  // key j < cap
+  __device__ __forceinline__ bool sees(const AttnParams& p, int j) const {
+    if (TREE && p.t.mask) {
+      const int k = j - start;
+      if (k >= 0) return pos >= start && (k >> 5) < p.t.words && ((__ldg(mask + (k >> 5)) >> (k & 31)) & 1u);
+      return pos >= start && (p.a.window == 0 || j > pos - p.a.window);
+    }
+    return j <= pos && (p.a.window == 0 || j > pos - p.a.window);
+  }
+  // keys j0 .. j0 + 31 as bits, without regard to the cache's end
+  __device__ __forceinline__ uint32_t sees32(const AttnParams& p, int j0) const {
+    const bool tree = TREE && p.t.mask;
+    // before the step (or all of them): first <= j < last
+    const int first = p.a.window > 0 ? max(0, pos - p.a.window + 1) : 0, last = tree ? (pos >= start ? start : 0) : pos + 1;
+    const int a = min(max(first - j0, 0), 32), b = min(max(last - j0, 0), 32);
+    uint32_t bits = b > a ? (b == 32 ? 0xffffffffu : (1u << b) - 1u) & ~((1u << a) - 1u) : 0u;
+    if (tree && pos >= start && j0 + 31 >= start) {
+      const int k = j0 - start, w = k >> 5;  // bit k of the mask row is key j0's
+      const uint32_t lo = w >= 0 && w < p.t.words ? __ldg(mask + w) : 0u;
+      const uint32_t hi = w + 1 < p.t.words ? __ldg(mask + w + 1) : 0u;
+      bits |= __funnelshift_r(lo, hi, k & 31);
+    }
+    return bits;
   }
 };
 
@@ -291,7 +359,10 @@ struct Joined {
 
 }  // namespace attn
 
-// Many query rows a KV head: products by tcgen05 (kv_attention_tc.cu).
+// Many query rows a KV head: products by tcgen05 (kv_attention_tc.cu, kv_attention_tree_tc.cu).
 cudaError_t launch_attention_tc(attn::AttnParams& p, cudaStream_t st);
+cudaError_t launch_attention_tree_tc(attn::AttnParams& p, cudaStream_t st);
+// Whether they take `rows` query rows of a sequence and KV head (kv_attention.cu).
+bool attention_tc_pays(const attn::AttnParams& p, int64_t rows);
 
 }  // namespace fp8imma_b200

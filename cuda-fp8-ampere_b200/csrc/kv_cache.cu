@@ -24,6 +24,7 @@
 #include "fp8_mma.cuh"
 #include "fp8imma/fp8imma_ext.h"
 #include "fp8imma_kernels.h"
+#include "kv_cache.cuh"
 #include "nvtx_range.h"
 #include "sm100_async.cuh"
 
@@ -34,6 +35,7 @@ namespace fp8imma_b200 {
 namespace {
 
 using namespace fp8imma_dev;
+using namespace kv;
 
 constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kKeep = 8;  // 16-byte vectors of a page that a thread keeps between the two passes
@@ -48,57 +50,10 @@ struct AppendParams {
   int team;        // warps of a (page, head, K or V)
 };
 
-template <int AT>
-__device__ __forceinline__ uint4 load_row8(const uint16_t* p, bool vec) {
-  if (vec) return __ldg(reinterpret_cast<const uint4*>(p));
-  uint32_t w[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) w[i] = (uint32_t)__ldg(p + 2 * i) | ((uint32_t)__ldg(p + 2 * i + 1) << 16);
-  return make_uint4(w[0], w[1], w[2], w[3]);
-}
-
-template <int AT>
-__device__ __forceinline__ float absmax8(uint4 v) {
-  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-  float m = 0.0f;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float a = fabsf(a16_to_f32<AT>((uint16_t)(w[i] & 0xFFFFu))), b = fabsf(a16_to_f32<AT>((uint16_t)(w[i] >> 16)));
-    m = fmaxf(m, a < INFINITY ? a : 0.0f);
-    m = fmaxf(m, b < INFINITY ? b : 0.0f);
-  }
-  return m;
-}
-
-template <int AT, int FMT>
-__device__ __forceinline__ uint2 to_codes(uint4 v, float s, float inv) {
-  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-  // a page's scale that the caller set to something else than a power of two takes the division
-  const bool pow2 = (__float_as_uint(s) & 0x7FFFFFu) == 0u;
-  uint32_t o[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float a = a16_to_f32<AT>((uint16_t)(w[i] & 0xFFFFu)), b = a16_to_f32<AT>((uint16_t)(w[i] >> 16));
-    o[i] = pow2 ? f32x2_to_f8x2<FMT>(a * inv, b * inv) : f32x2_to_f8x2<FMT>(__fdiv_rn(a, s), __fdiv_rn(b, s));
-  }
-  return make_uint2(o[0] | (o[1] << 16), o[2] | (o[3] << 16));
-}
-
-// sequence b's packed token range, clamped to the packed axis
-__device__ __forceinline__ void token_range(const AppendParams& p, int b, int& t0, int& n) {
-  if (p.per_seq > 0) {
-    t0 = b * p.per_seq;
-    n = p.per_seq;
-  } else {
-    t0 = max(0, __ldg(p.c.cu_new + b));
-    n = max(0, min(__ldg(p.c.cu_new + b + 1), p.c.tokens) - t0);
-  }
-}
-
 // pages that sequence b's new tokens touch: first page index and count
 __device__ __forceinline__ int touched(const AppendParams& p, int b, int& first) {
   int t0, n;
-  token_range(p, b, t0, n);
+  token_range(p.c, p.per_seq, b, t0, n);
   const int len = __ldg(p.c.seq_lens + b), start = max(0, len - n);
   first = start / p.c.page_size;
   return (n > 0 && len > start) ? min((len - 1) / p.c.page_size, p.c.max_pages - 1) - first + 1 : 0;
@@ -106,69 +61,19 @@ __device__ __forceinline__ int touched(const AppendParams& p, int b, int& first)
 
 template <int AT, int FMT, int CTAS>
 __global__ void __launch_bounds__(kThreads, CTAS) kv_append_kernel(const __grid_constant__ AppendParams p) {
-  __shared__ int s_pick[3];
-  __shared__ int s_scan[2][kWarps];
   __shared__ float s_max[kWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   pdl_launch_dependents();
   pdl_wait();
   int b = 0, first = 0, pi = 0;
-  if (p.per_seq > 0) {
-    b = blockIdx.x / p.pages_seq;
-    pi = blockIdx.x % p.pages_seq;
-    if (pi >= touched(p, b, first)) return;
-  } else {
-    // unit blockIdx.x of the sequences' touched pages laid end to end
-    if (threadIdx.x == 0) s_pick[0] = -1;
-    int base = 0, turn = 0;
-    bool bad = false;
-    for (int b0 = 0; b0 < p.c.batch; b0 += kThreads) {
-      const int mine = b0 + (int)threadIdx.x;
-      int f = 0;
-      const int n = mine < p.c.batch ? max(0, touched(p, mine, f)) : 0;
-      int x = n;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, x, o);
-        if (lane >= o) x += y;
-      }
-      if (lane == 31) s_scan[turn][warp] = x;
-      // Offsets that do not ascend would give a token to two sequences. Every CTA
-      // looks at all of them first, so that none of them stores anything.
-      if (b0 == 0)
-        for (int i = mine; i < p.c.batch; i += kThreads) bad |= __ldg(p.c.cu_new + i + 1) < __ldg(p.c.cu_new + i);
-      if (__syncthreads_or(bad)) {
-        if (threadIdx.x == 0) atomicCAS(&g_fp8imma_device_error, 0u, (unsigned int)ERR_BAD_OFFSETS);
-        return;
-      }
-      int before = base;
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        if (w < warp) before += s_scan[turn][w];
-        base += s_scan[turn][w];
-      }
-      turn ^= 1;  // the other one has been read by all: they have met since
-      const int lo = before + x - n;
-      if ((int)blockIdx.x >= lo && (int)blockIdx.x < lo + n) {
-        s_pick[0] = mine;
-        s_pick[1] = f;
-        s_pick[2] = (int)blockIdx.x - lo;
-      }
-      if ((int)blockIdx.x < base) break;
-    }
-    __syncthreads();
-    b = s_pick[0];
-    if (b < 0) return;
-    first = s_pick[1];
-    pi = s_pick[2];
-  }
+  if (!find_page<kThreads>(p.c, p.per_seq, p.pages_seq, [&](int i, int& f) { return touched(p, i, f); }, b, first, pi)) return;
   const int ps = p.c.page_size, D = p.c.head_dim;
   pi += first;
   if (pi >= p.c.max_pages) return;
   const int page = __ldg(p.c.page_table + (size_t)b * p.c.max_pages + pi);
   if ((unsigned)page >= (unsigned)p.c.num_pages) return;
   int t0, n;
-  token_range(p, b, t0, n);
+  token_range(p.c, p.per_seq, b, t0, n);
   const int len = __ldg(p.c.seq_lens + b);
   const int start = len - n;  // position of token t0 (may be negative: those tokens have no place)
   const int lo = max(max(start, 0), pi * ps), hi = min(len, (pi + 1) * ps);
@@ -206,26 +111,13 @@ __global__ void __launch_bounds__(kThreads, CTAS) kv_append_kernel(const __grid_
   if (!on) return;
   for (int w = 0; w < p.team; ++w) amax = fmaxf(amax, s_max[warp / p.team * p.team + w]);
 
-  // amax = 1.m * 2^e <= 1.75 * 2^(8|15) * 2^k  <=>  k >= e - (8|15), one more when 1.m > 1.75
-  const uint32_t bits = __float_as_uint(amax);
-  const int e = (int)(bits >> 23) - 127 - (FMT == F8_E4M3 ? 8 : 15) + ((bits & 0x7FFFFFu) > 0x600000u ? 1 : 0);
-  const float need = __uint_as_float((uint32_t)(max(e, -126) + 127) << 23);
-  const float s_new = fmaxf(s_old, need);
+  const float s_new = fmaxf(s_old, needed_scale<FMT>(amax));
   const float inv = __fdiv_rn(1.0f, s_new);
   if (slot0 > 0 && s_new != s_old) {  // uniform: the page's earlier codes move to the larger scale
     const float ratio = __fdiv_rn(s_old, s_new);
     for (int v = tid; v < slot0 * (D >> 4); v += step) {
-      uint4 c = reinterpret_cast<uint4*>(dst)[v];
-      uint32_t w[4] = {c.x, c.y, c.z, c.w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        uint32_t a, bb;
-        f8x4_to_f16x4<FMT>(w[i], a, bb);
-        const float2 fa = __half22float2(*reinterpret_cast<__half2*>(&a)), fb = __half22float2(*reinterpret_cast<__half2*>(&bb));
-        w[i] = (uint32_t)f32x2_to_f8x2<FMT>(fa.x * ratio, fa.y * ratio) |
-               ((uint32_t)f32x2_to_f8x2<FMT>(fb.x * ratio, fb.y * ratio) << 16);
-      }
-      reinterpret_cast<uint4*>(dst)[v] = make_uint4(w[0], w[1], w[2], w[3]);
+      uint4* at = reinterpret_cast<uint4*>(dst) + v;
+      *at = moved_codes<FMT>(*at, ratio);
     }
   }
   uint2* out = reinterpret_cast<uint2*>(dst + (size_t)slot0 * D);

@@ -47,6 +47,10 @@ EXT_SYMBOLS = [
     "fp8imma_kv_attention",
     "fp8imma_moe_forward",
     "fp8imma_token_logprobs",
+    "fp8imma_residual_norm",
+    "fp8imma_lora_add",
+    "fp8imma_kv_append_rope",
+    "fp8imma_kv_attention_tree",
     "fp8imma_set_splitk",
     "fp8imma_set_stream_k",
     "fp8imma_set_small_m_max",
@@ -101,6 +105,22 @@ FP8ImmaMoeArgs = _struct(
 FP8ImmaLogprobsArgs = _struct(
     "FP8ImmaLogprobsArgs", "fp8imma_logprobs_args", i0="l_type tokens vocab top", f1="temperature", p2="logits",
     l3="token_stride vocab_stride", p4="token_ids logprobs entropy top_ids top_logprobs")
+FP8ImmaResidualNormArgs = _struct(
+    "FP8ImmaResidualNormArgs", "fp8imma_residual_norm_args", i0="a_type r_type w_type g_type tokens hidden",
+    f1="alpha eps weight_offset", p2="y", l3="y_stride", p4="residual", l5="residual_stride", p6="gate", l7="gate_stride",
+    p8="post_weight pre_weight residual_out out")
+FP8ImmaLoraArgs = _struct(
+    "FP8ImmaLoraArgs", "fp8imma_lora_args", i0="a_type d_type tokens in_features out_features rank adapters", p1="x",
+    l2="x_stride", p3="lora_a lora_b adapter_ids scales base", l4="base_token_stride base_feature_stride", p5="out",
+    l6="out_token_stride out_feature_stride")
+FP8ImmaKvAppendRopeArgs = _struct(
+    "FP8ImmaKvAppendRopeArgs", "fp8imma_kv_append_rope_args", i0="a_type heads rotary interleaved", f1="rope_scale",
+    p2="inv_freq positions q k v",
+    l3="q_token_stride q_head_stride k_token_stride k_head_stride v_token_stride v_head_stride", p4="q_out",
+    l5="q_out_token_stride q_out_head_stride")
+FP8ImmaKvAttentionTreeArgs = _struct(
+    "FP8ImmaKvAttentionTreeArgs", "fp8imma_kv_attention_tree_args", i0="a_type heads window mask_words",
+    f1="softmax_scale softcap", p2="q", l3="q_token_stride q_head_stride", p4="tree_mask positions out lse")
 
 
 def lib() -> ctypes.CDLL:
@@ -144,6 +164,14 @@ def lib() -> ctypes.CDLL:
     L.fp8imma_moe_forward.argtypes = [ctypes.POINTER(FP8ImmaMoeArgs), P]
     L.fp8imma_token_logprobs.restype = I
     L.fp8imma_token_logprobs.argtypes = [ctypes.POINTER(FP8ImmaLogprobsArgs), P]
+    L.fp8imma_residual_norm.restype = I
+    L.fp8imma_residual_norm.argtypes = [ctypes.POINTER(FP8ImmaResidualNormArgs), P]
+    L.fp8imma_lora_add.restype = I
+    L.fp8imma_lora_add.argtypes = [ctypes.POINTER(FP8ImmaLoraArgs), P]
+    L.fp8imma_kv_append_rope.restype = I
+    L.fp8imma_kv_append_rope.argtypes = [ctypes.POINTER(FP8ImmaKvCache), ctypes.POINTER(FP8ImmaKvAppendRopeArgs), P]
+    L.fp8imma_kv_attention_tree.restype = I
+    L.fp8imma_kv_attention_tree.argtypes = [ctypes.POINTER(FP8ImmaKvCache), ctypes.POINTER(FP8ImmaKvAttentionTreeArgs), P]
     L.fp8imma_fp8wgt_linear_forward.restype = I
     L.fp8imma_fp8wgt_linear_forward.argtypes = [P, P, F, P, I, I, I, P]
     L.fp8imma_set_splitk.restype = I

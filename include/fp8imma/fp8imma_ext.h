@@ -281,6 +281,112 @@ typedef struct fp8imma_logprobs_args {
 } fp8imma_logprobs_args;
 int fp8imma_token_logprobs(const fp8imma_logprobs_args* args, void* stream);
 
+// ------------------------------------- operators between the products ----
+// The rest of a layer of a decode or verify step. Same conventions as above.
+
+// The residual connection with the norms on both sides of it, o = weight_offset:
+//   b = rms(y) (post_weight + o), or y without post_weight
+//   r' = residual + alpha * gate * b      (no residual: 0, no gate: 1)
+//   h = rms(r') (pre_weight + o),         rms(x) = x / sqrt(mean(x^2) + eps)
+// in fp32, r' (residual_out) and h (out) rounded once each; h is made from the
+// unrounded r'. residual_out may be residual, out may be y, where strides agree.
+#define FP8IMMA_NORM_MAX_HIDDEN 32768
+typedef struct fp8imma_residual_norm_args {
+  int a_type;                 // of y and out
+  int r_type;                 // fp8imma_l_type of residual and residual_out
+  int w_type;                 // fp8imma_l_type of the weights
+  int g_type;                 // fp8imma_l_type of the gate
+  int tokens, hidden;         // hidden 1 .. FP8IMMA_NORM_MAX_HIDDEN
+  float alpha, eps, weight_offset;
+  const void* y;              // [tokens, hidden], last dimension contiguous
+  int64_t y_stride;
+  const void* residual;       // optional [tokens, hidden], last dimension contiguous
+  int64_t residual_stride;
+  const void* gate;           // optional [tokens, hidden], or [hidden] with gate_stride 0
+  int64_t gate_stride;
+  const void* post_weight;    // optional [hidden]
+  const void* pre_weight;     // optional [hidden]
+  void* residual_out;         // [tokens, hidden] contiguous (optional with pre_weight)
+  void* out;                  // [tokens, hidden] contiguous, with pre_weight only
+} fp8imma_residual_norm_args;
+int fp8imma_residual_norm(const fp8imma_residual_norm_args* args, void* stream);
+
+// Low-rank adapters of many requests beside a projection:
+//   out[t,n] = base[t,n] + scales[e] sum_r lora_b[e,n,r] sum_k lora_a[e,r,k] x[t,k],
+// e = adapter_ids[t]; an id outside [0, adapters) leaves the token without an
+// adapter (out = base). base is the projection's result in either layout (the
+// GEMM's default is column-major). Neighbouring tokens of one adapter share its
+// weights' way to the SM, so requests are best laid one after another. Sums are
+// fp32; the inner sums enter the second product as two 16-bit numbers each.
+#define FP8IMMA_LORA_MAX_RANK 128
+typedef struct fp8imma_lora_args {
+  int a_type;                 // of x, lora_a and lora_b
+  int d_type;                 // fp8imma_out_type of base and out
+  int tokens, in_features, out_features, rank, adapters;  // in_features and rank multiples of 8, rank <= FP8IMMA_LORA_MAX_RANK
+  const void* x;              // [tokens, in_features], last dimension contiguous, rows 16-byte aligned
+  int64_t x_stride;
+  const void* lora_a;         // [adapters, rank, in_features], 16-byte aligned
+  const void* lora_b;         // [adapters, out_features, rank], 16-byte aligned
+  const int32_t* adapter_ids; // [tokens]
+  const float* scales;        // optional [adapters]
+  const void* base;           // one of the two strides is 1
+  int64_t base_token_stride, base_feature_stride;
+  void* out;                  // laid out along the same dimension; may be base
+  int64_t out_token_stride, out_feature_stride;
+} fp8imma_lora_args;
+int fp8imma_lora_add(const fp8imma_lora_args* args, void* stream);
+
+// fp8imma_kv_append with the position rotation of queries and keys on the way.
+// Channels (i, i + rotary / 2) of the first `rotary` of a head (interleaved:
+// (2i, 2i + 1)) turn by the angle position * inv_freq[i], taken modulo a turn in
+// 64 bits, and are multiplied by rope_scale; the other channels stay. Keys enter
+// the cache from fp32, queries are rounded to their type. Queries of every
+// token that a sequence owns are written, whether its key has a place or not.
+typedef struct fp8imma_kv_append_rope_args {
+  int a_type;
+  int heads;                  // query heads (0: no queries)
+  int rotary;                 // a multiple of 16, at most head_dim
+  int interleaved;
+  float rope_scale;
+  const float* inv_freq;      // [rotary / 2]
+  const int32_t* positions;   // optional [tokens]; without: the token's place in its sequence
+  const void* q;              // [tokens, heads, head_dim], last dimension contiguous, as k and v
+  const void* k;              // [tokens, kv_heads, head_dim]
+  const void* v;
+  int64_t q_token_stride, q_head_stride;
+  int64_t k_token_stride, k_head_stride;
+  int64_t v_token_stride, v_head_stride;
+  void* q_out;                // [tokens, heads, head_dim], last dimension contiguous; may be q
+  int64_t q_out_token_stride, q_out_head_stride;
+} fp8imma_kv_append_rope_args;
+int fp8imma_kv_append_rope(const fp8imma_kv_cache* cache, const fp8imma_kv_append_rope_args* args, void* stream);
+
+// fp8imma_kv_attention for the nodes of drafted trees, with capped scores.
+// Keys before the step are seen by all of the step's tokens; of the step's own,
+// token i (counted within its sequence) sees token j where bit j % 32 of
+// tree_mask[t][j / 32] is set, t being i's packed place (tokens past the mask's
+// words are not seen). That is a tree when each node's bits are its ancestors
+// and itself, and any other mask within the step as well. Without tree_mask the
+// step is causal. A window holds back keys before the step only:
+// j > position(t) - window, the positions (a node's depth counts from the
+// step's first place) taken between the step's first and last place; without
+// them a token's place counts. softcap > 0: scores are
+// softcap * tanh(s / softcap), s = softmax_scale <q, K_j>.
+typedef struct fp8imma_kv_attention_tree_args {
+  int a_type;                 // of q and out
+  int heads;                  // query heads, a multiple of kv_heads
+  int window;                 // 0: no window
+  int mask_words;             // words of a mask row
+  float softmax_scale, softcap;
+  const void* q;              // [tokens, heads, head_dim], last dimension contiguous
+  int64_t q_token_stride, q_head_stride;
+  const uint32_t* tree_mask;  // optional [tokens, mask_words]
+  const int32_t* positions;   // optional [tokens], with tree_mask only
+  void* out;                  // [tokens, heads, head_dim] contiguous
+  float* lse;                 // optional [tokens, heads]
+} fp8imma_kv_attention_tree_args;
+int fp8imma_kv_attention_tree(const fp8imma_kv_cache* cache, const fp8imma_kv_attention_tree_args* args, void* stream);
+
 // Tuning / introspection (no reference counterpart).
 // Force the K split of the small-M kernel (0 = automatic; 1, 2, 4 or 8).
 int fp8imma_set_splitk(int splits);
