@@ -58,6 +58,17 @@ __device__ __forceinline__ int touched(const RopeParams& p, int b, int& first) {
   return n > 0 ? ((len - 1) >> pl) - first + 1 : 0;
 }
 
+// position * inv_freq / 2 pi without its whole turns, in -0.5 .. 0.5. 1 / 2 pi and the
+// products are held as two 64-bit numbers: one alone would leave 2^-21 of an angle at
+// a position of 2^31.
+__device__ __forceinline__ float turn_fraction(int position, float inv_freq) {
+  constexpr double kHi = 0.15915494309189535, kLo = -9.839338337591243e-18;  // 1 / 2 pi
+  const double f = inv_freq, at = position;
+  const double hi = f * kHi, lo = fma(f, kHi, -hi) + f * kLo;
+  const double t = at * hi, rest = fma(at, hi, -t) + at * lo;
+  return (float)((t - rint(t)) + rest);
+}
+
 template <int AT>
 __device__ __forceinline__ void unpack8(uint4 v, float (&x)[8]) {
   const uint32_t w[4] = {v.x, v.y, v.z, v.w};
@@ -149,9 +160,8 @@ __global__ void __launch_bounds__(kThreads, 2) kv_append_rope_kernel(const __gri
   for (int e = threadIdx.x; e < rows * half; e += kThreads) {
     const int r = e / half, i = e - r * half;
     const int at = p.a.positions ? __ldg(p.a.positions + tok + r) : lo + r;
-    const double turns = (double)at * ((double)__ldg(p.a.inv_freq + i) * 0.15915494309189533577);
     float sn, cs;
-    sincospif((float)(2.0 * (turns - rint(turns))), &sn, &cs);
+    sincospif(2.0f * turn_fraction(at, __ldg(p.a.inv_freq + i)), &sn, &cs);
     table[e] = cs * p.a.rope_scale;
     sines[e] = sn * p.a.rope_scale;
   }
