@@ -497,7 +497,7 @@ int fp8imma_set_pdl(int enable) {
 unsigned int fp8imma_device_error(int clear) {
   return gemv_device_error(clear != 0) | decode_device_error(clear != 0) | tc_device_error(clear != 0) |
          peer_device_error(clear != 0) | kv_append_device_error(clear != 0) | attn_device_error(clear != 0) |
-         attn_tc_device_error(clear != 0) | moe_device_error(clear != 0) | kv_rope_device_error(clear != 0) |
+         attn_tc_device_error(clear != 0) | moe_device_error(clear != 0) | kv_rope_device_error(clear != 0) | norm_device_error(clear != 0) |
          attn_tree_device_error(clear != 0) | attn_tree_tc_device_error(clear != 0);
 }
 
@@ -510,6 +510,7 @@ int fp8imma_set_wait_limit_ns(unsigned long long ns) {
   if (e == cudaSuccess) e = attn_set_wait_limit(ns);
   if (e == cudaSuccess) e = attn_tc_set_wait_limit(ns);
   if (e == cudaSuccess) e = moe_set_wait_limit(ns);
+  if (e == cudaSuccess) e = norm_set_wait_limit(ns);
   if (e == cudaSuccess) e = attn_tree_set_wait_limit(ns);
   if (e == cudaSuccess) e = attn_tree_tc_set_wait_limit(ns);
   return (int)e;

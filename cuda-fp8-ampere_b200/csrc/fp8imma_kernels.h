@@ -201,6 +201,8 @@ cudaError_t attn_tc_set_wait_limit(unsigned long long ns);
 void attn_set_tc_rows(int rows);
 cudaError_t moe_set_wait_limit(unsigned long long ns);
 unsigned int kv_rope_device_error(bool clear);
+unsigned int norm_device_error(bool clear);
+cudaError_t norm_set_wait_limit(unsigned long long ns);
 unsigned int attn_tree_device_error(bool clear);
 unsigned int attn_tree_tc_device_error(bool clear);
 cudaError_t attn_tree_set_wait_limit(unsigned long long ns);

@@ -305,7 +305,7 @@ template <int AT, int FMT>
 cudaError_t launch_rope(const RopeParams& p, dim3 grid, cudaStream_t st) {
   const auto kern = kv_append_rope_kernel<AT, FMT>;
   const int smem = p.table_rows * p.a.rotary * 4;
-  const cudaError_t e = ensure_smem_attr(reinterpret_cast<const void*>(kern), smem);
+  const cudaError_t e = ensure_smem_attr(reinterpret_cast<const void*>(kern), smem + 1024);  // static shared memory counts too
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t lc = {};
   cudaLaunchAttribute attr[1];

@@ -8,6 +8,7 @@
 #include <torch/extension.h>
 
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 
 #include <cmath>
@@ -20,6 +21,12 @@ namespace {
 
 using namespace fp8imma_torch;
 using OptTensor = c10::optional<torch::Tensor>;
+
+// A result, straight from the allocator: on the smallest calls the dispatcher's
+// way to it costs as much as the kernel (1 us each).
+torch::Tensor fresh(const torch::Tensor& like, c10::IntArrayRef sizes, at::ScalarType dt) {
+  return at::detail::empty_cuda(sizes, dt, like.device(), c10::nullopt);
+}
 
 int real_type(const torch::Tensor& x, const char* name) {
   if (x.scalar_type() == at::kHalf) return FP8IMMA_L_F16;
@@ -89,7 +96,7 @@ std::tuple<torch::Tensor, OptTensor> residual_norm(const torch::Tensor& y, const
     TORCH_CHECK(real_type(r, "residual_out") == a.r_type, "residual_out must have residual's dtype");
     TORCH_CHECK(r.sizes() == y.sizes() && r.is_contiguous(), "residual_out must be contiguous and shaped like y");
   } else {
-    r = torch::empty(y.sizes(), y.options().dtype(a.r_type == FP8IMMA_L_F32 ? at::kFloat : y.scalar_type()));
+    r = fresh(y, y.sizes(), a.r_type == FP8IMMA_L_F32 ? at::kFloat : y.scalar_type());
   }
   OptTensor h;
   if (pre_weight.has_value()) {
@@ -98,7 +105,7 @@ std::tuple<torch::Tensor, OptTensor> residual_norm(const torch::Tensor& y, const
       check_packed(*h, y, y.scalar_type(), "out");
       TORCH_CHECK(h->sizes() == y.sizes(), "out must be shaped like y");
     } else {
-      h = torch::empty(y.sizes(), y.options());
+      h = fresh(y, y.sizes(), y.scalar_type());
     }
   }
   const char* across = "residual_out and out must be the inputs themselves or lie apart from them";
@@ -170,9 +177,9 @@ torch::Tensor lora_add(const torch::Tensor& base, const torch::Tensor& x, const 
     check_apart(o, base, across);
     for (const auto* t : {&x, &lora_a, &lora_b}) check_apart(o, *t, across, false);
   } else if (row) {
-    o = torch::empty({T, N}, base.options());
+    o = fresh(base, {T, N}, base.scalar_type());
   } else {
-    o = torch::empty({N, T}, base.options()).t();
+    o = at::detail::empty_strided_cuda({T, N}, {1, T}, base.scalar_type(), base.device());
   }
   if (T == 0) return o;
   a.tokens = to_int(T, "tokens");
@@ -250,7 +257,7 @@ OptTensor kv_append_rope(const OptTensor& q, const torch::Tensor& k, const torch
         check_apart(*o, v, across, false);
       }
     } else {
-      o = torch::empty(q->sizes(), q->options());
+      o = fresh(*q, q->sizes(), q->scalar_type());
     }
   }
   if (c.tokens == 0) return o;
@@ -314,9 +321,9 @@ std::tuple<torch::Tensor, torch::Tensor> kv_attention_tree(
     TORCH_CHECK(o.sizes() == q.sizes(), "out must be shaped like q");
     check_apart(o, q, "out must lie apart from q", false);
   } else {
-    o = torch::empty(q.sizes(), q.options());
+    o = fresh(q, q.sizes(), q.scalar_type());
   }
-  torch::Tensor lse = torch::empty({q.size(0), q.size(1)}, q.options().dtype(at::kFloat));
+  torch::Tensor lse = fresh(q, {q.size(0), q.size(1)}, at::kFloat);
   if (c.tokens == 0) return {o, lse};
   a.q = q.data_ptr();
   a.q_token_stride = q.stride(0);

@@ -69,6 +69,19 @@ def test_fp32_weights_and_residual_without_one(ops):
     assert bool(((out.double() - want[0]).abs() <= bound[0]).all())
 
 
+@pytest.mark.parametrize("t, h", [(9601, 64), (20000, 8), (5000, 1000), (1301, 4096), (701, 8192), (450, 16384)])
+@pytest.mark.parametrize("dt, res, gate, pad", [(B, B, "token", 8), (H, S, "channel", 0), (B, None, None, 0), (H, H, "f32", 16)])
+def test_many_rows(ops, t, h, dt, res, gate, pad):
+    """Several rounds of rows for each CTA, copied ahead."""
+    x = inputs(t, t, h, dt, res=res, gate=gate, pad=pad)
+    got = ops.residual_norm(**x)
+    check(got, x)
+    if res is not None:  # and in place
+        r2, _ = ops.residual_norm(**x, residual_out=x["residual"])
+        assert torch.equal(r2, got[0])
+    assert F.lib().fp8imma_device_error(1) == 0
+
+
 @pytest.mark.parametrize("h", [512, 515])
 def test_in_place_is_the_same(ops, h):
     x = inputs(3, 50, h, H, res=H, gate="channel")
