@@ -61,4 +61,15 @@ __device__ __forceinline__ uint16_t f32_to_a16(float v) {
   return AT == 0 ? __half_as_ushort(__float2half_rn(v)) : __bfloat16_as_ushort(__float2bfloat16_rn(v));
 }
 
+// two fp32 values -> two 16-bit activations, lo in the low half
+template <int AT>
+__device__ __forceinline__ uint32_t f32x2_to_a16x2(float lo, float hi) {
+  uint32_t r;
+  if (AT == 0)
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  else
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
 }  // namespace fp8imma_dev

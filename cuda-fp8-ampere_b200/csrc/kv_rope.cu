@@ -24,6 +24,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cuda_runtime.h>
+#include <type_traits>
 
 namespace fp8imma_b200 {
 namespace {
@@ -32,8 +33,8 @@ using namespace fp8imma_dev;
 using namespace kv;
 
 constexpr int kThreads = 256, kWarps = kThreads / 32;
-constexpr int kKeep = 4;  // pairs of pieces of a page that a thread keeps between the two passes
-constexpr int kQ = 4;     // pairs of query pieces that a thread has in flight
+constexpr int kKeep = 2;  // pairs of pieces of a page that a thread keeps (as fp32) between the two passes
+constexpr int kQ = 4;     // heads whose pair a thread has in flight
 
 struct RopeParams {
   fp8imma_kv_cache c;
@@ -61,13 +62,18 @@ __device__ __forceinline__ int touched(const RopeParams& p, int b, int& first) {
 // position * inv_freq / 2 pi without its whole turns, in -0.5 .. 0.5. 1 / 2 pi and the
 // products are held as two 64-bit numbers: one alone would leave 2^-21 of an angle at
 // a position of 2^31.
-__device__ __forceinline__ float turn_fraction(int position, float inv_freq) {
-  constexpr double kHi = 0.15915494309189535, kLo = -9.839338337591243e-18;  // 1 / 2 pi
-  const double f = inv_freq, at = position;
-  const double hi = f * kHi, lo = fma(f, kHi, -hi) + f * kLo;
-  const double t = at * hi, rest = fma(at, hi, -t) + at * lo;
-  return (float)((t - rint(t)) + rest);
-}
+struct Frequency {
+  double hi, lo;  // inv_freq / 2 pi
+  __device__ __forceinline__ explicit Frequency(float inv_freq) {
+    constexpr double kHi = 0.15915494309189535, kLo = -9.839338337591243e-18;  // 1 / 2 pi
+    hi = inv_freq * kHi;
+    lo = fma((double)inv_freq, kHi, -hi) + inv_freq * kLo;
+  }
+  __device__ __forceinline__ float turns(int position) const {
+    const double at = position, t = at * hi;
+    return (float)((t - rint(t)) + fma(at, lo, fma(at, hi, -t)));
+  }
+};
 
 template <int AT>
 __device__ __forceinline__ void unpack8(uint4 v, float (&x)[8]) {
@@ -89,7 +95,13 @@ __device__ __forceinline__ uint2 codes8(const float (&x)[8], float s, float inv)
   return make_uint2(o[0] | (o[1] << 16), o[2] | (o[3] << 16));
 }
 
+// NaN is left out by fmaxf; an infinity shows in the result, which is then made anew without any.
 __device__ __forceinline__ float absmax8(const float (&x)[8], float m) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(x[i]));
+  return m;
+}
+__device__ __forceinline__ float absmax8_finite(const float (&x)[8], float m) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(x[i]) < INFINITY ? fabsf(x[i]) : 0.0f);
   return m;
@@ -105,41 +117,44 @@ struct PairAt {
   }
 };
 
-// Turns pair j (j < turning); cos and sin: the row's.
-__device__ __forceinline__ void turn(float (&x)[8], float (&y)[8], int j, int turning, bool interleaved, const float* cs, const float* sn) {
-  if (!interleaved) {
-    const float4* c4 = reinterpret_cast<const float4*>(cs + 8 * j);
-    const float4* s4 = reinterpret_cast<const float4*>(sn + 8 * j);
-    const float4 c0 = c4[0], c1 = c4[1], s0 = s4[0], s1 = s4[1];
-    const float c[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w}, s[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
+// The eight cosines and sines of pair j (j < turning) of a row.
+struct Turn {
+  float c[8], s[8];
+  __device__ __forceinline__ void load(int j, int turning, bool interleaved, const float* cs, const float* sn) {
+    // interleaved: four of the first piece, four of the second
+    const int at0 = interleaved ? j : 2 * j, at1 = interleaved ? j + turning : 2 * j + 1;
+    const float4 c0 = reinterpret_cast<const float4*>(cs)[at0], c1 = reinterpret_cast<const float4*>(cs)[at1];
+    const float4 s0 = reinterpret_cast<const float4*>(sn)[at0], s1 = reinterpret_cast<const float4*>(sn)[at1];
+    c[0] = c0.x, c[1] = c0.y, c[2] = c0.z, c[3] = c0.w, c[4] = c1.x, c[5] = c1.y, c[6] = c1.z, c[7] = c1.w;
+    s[0] = s0.x, s[1] = s0.y, s[2] = s0.z, s[3] = s0.w, s[4] = s1.x, s[5] = s1.y, s[6] = s1.z, s[7] = s1.w;
+  }
+  __device__ __forceinline__ void apply(float (&x)[8], float (&y)[8], bool interleaved) const {
+    if (!interleaved) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float u = x[i], v = y[i];
-      x[i] = fmaf(u, c[i], -(v * s[i]));
-      y[i] = fmaf(v, c[i], u * s[i]);
-    }
-  } else {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      float(&z)[8] = h ? y : x;
-      const float4 c4 = *reinterpret_cast<const float4*>(cs + 4 * (j + h * turning));
-      const float4 s4 = *reinterpret_cast<const float4*>(sn + 4 * (j + h * turning));
-      const float c[4] = {c4.x, c4.y, c4.z, c4.w}, s[4] = {s4.x, s4.y, s4.z, s4.w};
+      for (int i = 0; i < 8; ++i) one(x[i], y[i], i);
+    } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float u = z[2 * i], v = z[2 * i + 1];
-        z[2 * i] = fmaf(u, c[i], -(v * s[i]));
-        z[2 * i + 1] = fmaf(v, c[i], u * s[i]);
+        one(x[2 * i], x[2 * i + 1], i);
+        one(y[2 * i], y[2 * i + 1], 4 + i);
       }
     }
   }
-}
+  __device__ __forceinline__ void one(float& u, float& v, int i) const {
+    const float a = u, b = v;
+    u = fmaf(a, c[i], -(b * s[i]));
+    v = fmaf(b, c[i], a * s[i]);
+  }
+};
 
-template <int AT, int FMT>
+// PLAIN: half-split pairs and aligned rows, which are most calls; less code for the
+// instruction cache.
+template <int AT, int FMT, bool PLAIN>
 __global__ void __launch_bounds__(kThreads, 2) kv_append_rope_kernel(const __grid_constant__ RopeParams p) {
   extern __shared__ __align__(16) float table[];  // cosines [rows][rotary / 2], then sines
   __shared__ float s_max[2][kWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const bool interleaved = !PLAIN && p.a.interleaved, vec = PLAIN || p.vec, vec_q = PLAIN || p.vec_q;
   pdl_launch_dependents();
   pdl_wait();
   int b = 0, first = 0, pi = 0;
@@ -157,13 +172,16 @@ __global__ void __launch_bounds__(kThreads, 2) kv_append_rope_kernel(const __gri
 
   const int half = p.a.rotary >> 1, turning = half >> 3;
   float* const sines = table + p.table_rows * half;
-  for (int e = threadIdx.x; e < rows * half; e += kThreads) {
-    const int r = e / half, i = e - r * half;
-    const int at = p.a.positions ? __ldg(p.a.positions + tok + r) : lo + r;
-    float sn, cs;
-    sincospif(2.0f * turn_fraction(at, __ldg(p.a.inv_freq + i)), &sn, &cs);
-    table[e] = cs * p.a.rope_scale;
-    sines[e] = sn * p.a.rope_scale;
+  {
+    // a thread keeps to one frequency
+    const int per = kThreads / half, i = threadIdx.x % half;
+    const Frequency f(__ldg(p.a.inv_freq + i));
+    for (int r = threadIdx.x / half; r < rows && (int)threadIdx.x < per * half; r += per) {
+      float sn, cs;
+      sincospif(2.0f * f.turns(p.a.positions ? __ldg(p.a.positions + tok + r) : lo + r), &sn, &cs);
+      table[r * half + i] = cs * p.a.rope_scale;
+      sines[r * half + i] = sn * p.a.rope_scale;
+    }
   }
   __syncthreads();
 
@@ -189,31 +207,50 @@ __global__ void __launch_bounds__(kThreads, 2) kv_append_rope_kernel(const __gri
       auto load = [&](int v, uint4& x, uint4& y) {
         const PairAt at(v & (pairs - 1), turning);
         const uint16_t* row = src + (int64_t)(v >> pl) * ts;
-        x = load_row8<AT>(row + at.a * 8, p.vec);
-        y = load_row8<AT>(row + at.b * 8, p.vec);
+        x = load_row8<AT>(row + at.a * 8, vec);
+        y = load_row8<AT>(row + at.b * 8, vec);
       };
       auto values = [&](int v, uint4 a, uint4 c, float (&x)[8], float (&y)[8]) {
         unpack8<AT>(a, x);
         unpack8<AT>(c, y);
         const int j = v & (pairs - 1);
-        if (key && j < turning) turn(x, y, j, turning, p.a.interleaved, table + (v >> pl) * half, sines + (v >> pl) * half);
-      };
-      uint4 keep[kKeep][2];
-      float amax = 0.0f, x[8], y[8];
-#pragma unroll
-      for (int i = 0; i < kKeep; ++i)
-        if (tid + i * step < nv) load(tid + i * step, keep[i][0], keep[i][1]);
-#pragma unroll
-      for (int i = 0; i < kKeep; ++i)
-        if (tid + i * step < nv) {
-          values(tid + i * step, keep[i][0], keep[i][1], x, y);
-          amax = absmax8(y, absmax8(x, amax));
+        if (key && j < turning) {
+          Turn t;
+          t.load(j, turning, interleaved, table + (v >> pl) * half, sines + (v >> pl) * half);
+          t.apply(x, y, interleaved);
         }
+      };
+      float keep[kKeep][2][8], amax = 0.0f;
+      {
+        uint4 raw[kKeep][2];
+#pragma unroll
+        for (int i = 0; i < kKeep; ++i)
+          if (tid + i * step < nv) load(tid + i * step, raw[i][0], raw[i][1]);
+#pragma unroll
+        for (int i = 0; i < kKeep; ++i)
+          if (tid + i * step < nv) {
+            values(tid + i * step, raw[i][0], raw[i][1], keep[i][0], keep[i][1]);
+            amax = absmax8(keep[i][1], absmax8(keep[i][0], amax));
+          }
+      }
+#pragma unroll 1
       for (int v = tid + kKeep * step; v < nv; v += step) {
         uint4 a, c;
+        float x[8], y[8];
         load(v, a, c);
         values(v, a, c, x, y);
         amax = absmax8(y, absmax8(x, amax));
+      }
+      if (__any_sync(0xffffffffu, amax == INFINITY)) {
+        amax = 0.0f;
+#pragma unroll 1
+        for (int v = tid; v < nv; v += step) {
+          uint4 a, c;
+          float x[8], y[8];
+          load(v, a, c);
+          values(v, a, c, x, y);
+          amax = absmax8_finite(y, absmax8_finite(x, amax));
+        }
       }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
@@ -232,8 +269,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv_append_rope_kernel(const __gri
           *at = moved_codes<FMT>(*at, ratio);
         }
       }
-      auto put = [&](int v, uint4 a, uint4 c) {
-        values(v, a, c, x, y);
+      auto put = [&](int v, const float(&x)[8], const float(&y)[8]) {
         const PairAt at(v & (pairs - 1), turning);
         uint8_t* row = dst + (size_t)(slot0 + (v >> pl)) * D;
         *reinterpret_cast<uint2*>(row + at.a * 8) = codes8<FMT>(x, s_new, inv);
@@ -242,68 +278,83 @@ __global__ void __launch_bounds__(kThreads, 2) kv_append_rope_kernel(const __gri
 #pragma unroll
       for (int i = 0; i < kKeep; ++i)
         if (tid + i * step < nv) put(tid + i * step, keep[i][0], keep[i][1]);
+#pragma unroll 1
       for (int v = tid + kKeep * step; v < nv; v += step) {
         uint4 a, c;
+        float x[8], y[8];
         load(v, a, c);
-        put(v, a, c);
+        values(v, a, c, x, y);
+        put(v, x, y);
       }
       if (tid == 0) *scale = s_new;
     }
   }
 
-  // queries: the page's rows, all heads, pair after pair
-  const int row_pairs = p.a.heads << pl, all = rows * row_pairs, stride = gridDim.y * kThreads;
-  for (int e0 = blockIdx.y * kThreads + threadIdx.x; e0 < all; e0 += kQ * stride) {
-    uint4 raw[kQ][2];
-    int row[kQ], hp[kQ];
+  // queries: a thread keeps to one pair of one row, its cosines and sines in
+  // registers, and goes through the heads (every `groups`-th of them)
+  const int places = rows << pl, threads = gridDim.y * kThreads, id = blockIdx.y * kThreads + threadIdx.x;
+  const int groups = max(1, threads / places);
+  for (int at = id; at < groups * places; at += threads) {
+    const int group = at / places, place = at - group * places, row = place >> pl, j = place & (pairs - 1);
+    const PairAt piece(j, turning);
+    const uint16_t* const src = static_cast<const uint16_t*>(p.a.q) + (int64_t)(tok + row) * p.a.q_token_stride;
+    uint16_t* const dst = static_cast<uint16_t*>(p.a.q_out) + (int64_t)(tok + row) * p.a.q_out_token_stride;
+    Turn t;
+    if (j < turning) t.load(j, turning, interleaved, table + row * half, sines + row * half);
+    for (int h0 = group; h0 < p.a.heads; h0 += kQ * groups) {
+      uint4 raw[kQ][2];
 #pragma unroll
-    for (int k = 0; k < kQ; ++k) {
-      const int e = e0 + k * stride;
-      if (e >= all) continue;
-      row[k] = e / row_pairs;
-      hp[k] = e - row[k] * row_pairs;
-      const PairAt at(hp[k] & (pairs - 1), turning);
-      const uint16_t* src = static_cast<const uint16_t*>(p.a.q) + (int64_t)(tok + row[k]) * p.a.q_token_stride + (int64_t)(hp[k] >> pl) * p.a.q_head_stride;
+      for (int k = 0; k < kQ; ++k) {
+        const int h = h0 + k * groups;
+        if (h >= p.a.heads) break;
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const uint16_t* s = src + (c ? at.b : at.a) * 8;  // q may be q_out: no read-only loads
-        if (p.vec_q) raw[k][c] = *reinterpret_cast<const uint4*>(s);
-        else
-          raw[k][c] = make_uint4(s[0] | (uint32_t)s[1] << 16, s[2] | (uint32_t)s[3] << 16, s[4] | (uint32_t)s[5] << 16, s[6] | (uint32_t)s[7] << 16);
-      }
-    }
-#pragma unroll
-    for (int k = 0; k < kQ; ++k) {
-      if (e0 + k * stride >= all) continue;
-      const int j = hp[k] & (pairs - 1);
-      const PairAt at(j, turning);
-      uint16_t* dst = static_cast<uint16_t*>(p.a.q_out) + (int64_t)(tok + row[k]) * p.a.q_out_token_stride + (int64_t)(hp[k] >> pl) * p.a.q_out_head_stride;
-      float x[8], y[8];
-      unpack8<AT>(raw[k][0], x);
-      unpack8<AT>(raw[k][1], y);
-      if (j < turning) {
-        turn(x, y, j, turning, p.a.interleaved, table + row[k] * half, sines + row[k] * half);
+        for (int c = 0; c < 2; ++c) {
+          const uint16_t* s = src + (int64_t)h * p.a.q_head_stride + (c ? piece.b : piece.a) * 8;  // q may be q_out: no read-only loads
+          if (vec_q) raw[k][c] = *reinterpret_cast<const uint4*>(s);
+          else
+            raw[k][c] = make_uint4(s[0] | (uint32_t)s[1] << 16, s[2] | (uint32_t)s[3] << 16, s[4] | (uint32_t)s[5] << 16, s[6] | (uint32_t)s[7] << 16);
+        }
       }
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const float(&z)[8] = c ? y : x;
-        uint32_t w[4];
+      for (int k = 0; k < kQ; ++k) {
+        const int h = h0 + k * groups;
+        if (h >= p.a.heads) break;
+        uint4 out[2] = {raw[k][0], raw[k][1]};  // pieces that stay are copied
+        if (j < turning) {
+          float x[8], y[8];
+          unpack8<AT>(raw[k][0], x);
+          unpack8<AT>(raw[k][1], y);
+          t.apply(x, y, interleaved);
+          out[0] = make_uint4(f32x2_to_a16x2<AT>(x[0], x[1]), f32x2_to_a16x2<AT>(x[2], x[3]), f32x2_to_a16x2<AT>(x[4], x[5]), f32x2_to_a16x2<AT>(x[6], x[7]));
+          out[1] = make_uint4(f32x2_to_a16x2<AT>(y[0], y[1]), f32x2_to_a16x2<AT>(y[2], y[3]), f32x2_to_a16x2<AT>(y[4], y[5]), f32x2_to_a16x2<AT>(y[6], y[7]));
+        }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = (uint32_t)f32_to_a16<AT>(z[2 * i]) | (uint32_t)f32_to_a16<AT>(z[2 * i + 1]) << 16;
-        uint16_t* d = dst + (c ? at.b : at.a) * 8;
-        if (p.vec_q) *reinterpret_cast<uint4*>(d) = make_uint4(w[0], w[1], w[2], w[3]);
-        else {
+        for (int c = 0; c < 2; ++c) {
+          uint16_t* d = dst + (int64_t)h * p.a.q_out_head_stride + (c ? piece.b : piece.a) * 8;
+          if (vec_q) *reinterpret_cast<uint4*>(d) = out[c];
+          else {
+            const uint32_t w[4] = {out[c].x, out[c].y, out[c].z, out[c].w};
 #pragma unroll
-          for (int i = 0; i < 4; ++i) d[2 * i] = (uint16_t)w[i], d[2 * i + 1] = (uint16_t)(w[i] >> 16);
+            for (int i = 0; i < 4; ++i) d[2 * i] = (uint16_t)w[i], d[2 * i + 1] = (uint16_t)(w[i] >> 16);
+          }
         }
       }
     }
   }
 }
 
-template <int AT, int FMT>
-cudaError_t launch_rope(const RopeParams& p, dim3 grid, cudaStream_t st) {
-  const auto kern = kv_append_rope_kernel<AT, FMT>;
+template <int AT, int FMT, bool PLAIN>
+cudaError_t launch_rope(RopeParams& p, int64_t units, int64_t rows, cudaStream_t st) {
+  // a team keeps its rows in registers: kKeep pairs a lane
+  const int64_t pairs = p.c.head_dim / 16;
+  p.team = 1;
+  while (p.team < kWarps && rows * pairs > (int64_t)p.team * 32 * kKeep) p.team *= 2;
+  // shares of a page: as many as keep its CTAs' threads busy, as long as the
+  // whole grid has few CTAs (prompts of 9200 tokens: 63 us with one share, 60 with
+  // two; a kernel for the queries of its own, with twice the warps: 73)
+  const int64_t cache = (2ll * p.c.kv_heads * p.team + kWarps - 1) / kWarps, queries = (rows * p.a.heads * pairs + kThreads - 1) / kThreads;
+  const int64_t shares = std::max<int64_t>(1, std::min<int64_t>(std::max(cache, queries), 12ll * num_sms_current() / units));
+  const auto kern = kv_append_rope_kernel<AT, FMT, PLAIN>;
   const int smem = p.table_rows * p.a.rotary * 4;
   const cudaError_t e = ensure_smem_attr(reinterpret_cast<const void*>(kern), smem + 1024);  // static shared memory counts too
   if (e != cudaSuccess) return e;
@@ -311,7 +362,7 @@ cudaError_t launch_rope(const RopeParams& p, dim3 grid, cudaStream_t st) {
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
-  lc.gridDim = grid;
+  lc.gridDim = dim3((unsigned)units, (unsigned)std::min<int64_t>(shares, 65535));
   lc.blockDim = dim3(kThreads);
   lc.dynamicSmemBytes = (size_t)smem;
   lc.stream = st;
@@ -355,17 +406,17 @@ extern "C" int fp8imma_kv_append_rope(const fp8imma_kv_cache* c, const fp8imma_k
   }
   if (units > 0x7fffffffll) return (int)cudaErrorInvalidValue;
   p.table_rows = std::min(c->page_size, c->cu_new ? c->tokens : p.per_seq);
-  // a team keeps its rows in registers: kKeep pairs a lane
   const int64_t rows = std::min<int64_t>(c->page_size, ((int64_t)c->tokens + c->batch - 1) / c->batch);
-  p.team = 1;
-  while (p.team < kWarps && rows * (c->head_dim / 16) > (int64_t)p.team * 32 * kKeep) p.team *= 2;
-  // shares of a page: as many as keep its CTAs' threads busy, as long as the
-  // whole grid has few CTAs
-  const int64_t most = std::max<int64_t>((2ll * c->kv_heads * p.team + kWarps - 1) / kWarps, (rows * a->heads * (c->head_dim / 16) + kThreads - 1) / kThreads);
-  const int64_t shares = std::min<int64_t>({most, std::max<int64_t>(1, 8ll * num_sms_current() / units), 65535});
-  const dim3 grid((unsigned)units, (unsigned)shares);
+  const bool plain = !a->interleaved && p.vec && p.vec_q;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const bool e4 = c->format == FP8IMMA_B_E4M3;
-  if (a->a_type == FP8IMMA_A_F16) return (int)(e4 ? launch_rope<0, F8_E4M3>(p, grid, st) : launch_rope<0, F8_E5M2>(p, grid, st));
-  return (int)(e4 ? launch_rope<1, F8_E4M3>(p, grid, st) : launch_rope<1, F8_E5M2>(p, grid, st));
+  auto run = [&](auto at, auto fmt) {
+    constexpr int AT = decltype(at)::value, FMT = decltype(fmt)::value;
+    return (int)(plain ? launch_rope<AT, FMT, true>(p, units, rows, st) : launch_rope<AT, FMT, false>(p, units, rows, st));
+  };
+  using F16 = std::integral_constant<int, 0>;
+  using BF16 = std::integral_constant<int, 1>;
+  using E4M3 = std::integral_constant<int, F8_E4M3>;
+  using E5M2 = std::integral_constant<int, F8_E5M2>;
+  if (a->a_type == FP8IMMA_A_F16) return c->format == FP8IMMA_B_E4M3 ? run(F16(), E4M3()) : run(F16(), E5M2());
+  return c->format == FP8IMMA_B_E4M3 ? run(BF16(), E4M3()) : run(BF16(), E5M2());
 }

@@ -140,7 +140,7 @@ template <int AT>
 __device__ __forceinline__ uint4 pack8(const float (&v)[8]) {
   uint32_t w[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) w[i] = (uint32_t)f32_to_a16<AT>(v[2 * i]) | (uint32_t)f32_to_a16<AT>(v[2 * i + 1]) << 16;
+  for (int i = 0; i < 4; ++i) w[i] = f32x2_to_a16x2<AT>(v[2 * i], v[2 * i + 1]);
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
