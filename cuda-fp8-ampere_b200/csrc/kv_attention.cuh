@@ -9,6 +9,7 @@
 #include "sm100_async.cuh"
 
 #include <algorithm>
+#include <cstring>
 
 namespace fp8imma_b200 {
 namespace attn {
@@ -25,7 +26,25 @@ struct TreeParams {
   const int32_t* positions;  // null: a token's place
   int words;
   float cap;                 // 0: scores as they are
+  unsigned long long poly[7];  // coefficients of capped(), twice each
 };
+// cap tanh(s / cap) = x P((x / cap2)^2) for |x| <= cap2 (x = s log2 e, cap2 = cap log2 e):
+// tanh(sqrt w) / sqrt w on 0 <= w <= 1, a minimax fit of degree 6, to 2^-24 relative. The
+// powers of 1 / cap2 go into the coefficients, which stand as pairs for fma.f32x2.
+inline void set_cap(TreeParams& t, float cap) {
+  static const double c[7] = {0.9999999403953552, -0.33332839608192444, 0.13325203955173492, -0.05345702916383743,
+                              0.020289979875087738, -0.006203379016369581, 0.0010410225950181484};
+  t.cap = cap;
+  const double by = cap > 0.0f ? 1.0 / ((double)cap * 1.4426950408889634) : 0.0;
+  double f = 1.0;
+  for (int i = 0; i < 7; ++i, f *= by * by) {
+    const float d = (float)(c[i] * f);
+    unsigned int bits;
+    static_assert(sizeof(bits) == sizeof(d), "");
+    std::memcpy(&bits, &d, sizeof(bits));
+    t.poly[i] = (unsigned long long)bits << 32 | bits;
+  }
+}
 
 struct AttnParams {
   fp8imma_kv_cache c;

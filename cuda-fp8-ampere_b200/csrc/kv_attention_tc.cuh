@@ -128,9 +128,25 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
   return r;
 }
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
 __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   uint64_t r;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ float min3(float a, float b, float c) {
+  float r;
+  asm("min.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
 
@@ -511,7 +527,58 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) kv_attention_tc_kernel(
             uint32_t v[32], w[16];
             tmem_ld32(s_at + 32 * c, v);
             float sum[2];
-            if (edge || capped) {
+            if (TREE && capped && !edge) {
+              // the largest score of 16 keys is the capped one of their largest product
+              float kc[2], top[2], most_abs = 0.0f;
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                float hi = -INFINITY, lo = INFINITY;
+#pragma unroll
+                for (int k = 16 * h; k < 16 * h + 16; k += 2) {
+                  hi = max3(hi, __uint_as_float(v[k]), __uint_as_float(v[k + 1]));
+                  lo = min3(lo, __uint_as_float(v[k]), __uint_as_float(v[k + 1]));
+                }
+                kc[h] = cq * info.ks[2 * c + h];
+                most_abs = fmaxf(most_abs, kc[h] * fmaxf(hi, -lo));
+                top[h] = cap_score(hi * kc[h], cap2, icap) + info.lv[2 * c + h];
+              }
+              const float most = fmaxf(top[0], top[1]);
+              if (__any_sync(0xffffffffu, most > m + kRaise)) raise(c, most);
+              const float ms = m == -INFINITY ? 0.0f : m;
+              // a NaN hides from the maxima; it passes through either form
+              const bool near = !__any_sync(0xffffffffu, most_abs > cap2);
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const float lv = info.lv[2 * c + h] - ms;
+                const uint64_t kc2 = pair(kc[h], kc[h]), lv2 = pair(lv, lv);
+                uint64_t two = 0;
+                if (near) {
+#pragma unroll
+                  for (int k = 16 * h; k < 16 * h + 16; k += 2) {
+                    const uint64_t x = mul2(pair(__uint_as_float(v[k]), __uint_as_float(v[k + 1])), kc2), u = mul2(x, x);
+                    uint64_t q = fma2(u, p.t.poly[6], p.t.poly[5]);
+#pragma unroll
+                    for (int i = 4; i >= 0; --i) q = fma2(u, q, p.t.poly[i]);
+                    float a, b;
+                    unpair(fma2(x, q, lv2), a, b);
+                    a = ex2(a), b = ex2(b);
+                    two = add2(two, pair(a, b));
+                    w[k / 2] = pack_f16(a, b);
+                  }
+                } else {
+#pragma unroll
+                  for (int k = 16 * h; k < 16 * h + 16; k += 2) {
+                    const float a = ex2(cap_score(__uint_as_float(v[k]) * kc[h], cap2, icap) + lv);
+                    const float b = ex2(cap_score(__uint_as_float(v[k + 1]) * kc[h], cap2, icap) + lv);
+                    two = add2(two, pair(a, b));
+                    w[k / 2] = pack_f16(a, b);
+                  }
+                }
+                float s0, s1;
+                unpair(two, s0, s1);
+                sum[h] = s0 + s1;
+              }
+            } else if (edge) {
               float x[32], top = -INFINITY;
               uint32_t vis = 0xffffffffu;  // keys that the row sees
               if (TREE && edge) {

@@ -43,7 +43,7 @@ extern "C" int fp8imma_kv_attention_tree(const fp8imma_kv_cache* c, const fp8imm
   p.t.mask = a->tree_mask;
   p.t.positions = a->positions;
   p.t.words = a->mask_words;
-  p.t.cap = a->softcap;
+  attn::set_cap(p.t, a->softcap);
   p.per_seq = c->cu_new ? 0 : c->tokens / c->batch;
   p.group = a->heads / c->kv_heads;
   p.vec_q = ((reinterpret_cast<uintptr_t>(a->q) | (uintptr_t)((a->q_token_stride | a->q_head_stride) * 2)) & 15u) == 0;
