@@ -36,7 +36,7 @@ constexpr int kMaxTokens = kThreads * 64;  // tokens of a launch: a thread marks
 struct LoraParams {
   fp8imma_lora_args a;
   int cluster;  // CTAs of a cluster
-  int split;    // clusters that share a unit's outputs (each makes the inner sums)
+  int split;    // clusters that may share a unit's outputs at most (each makes the inner sums)
   int vec;      // base and out are 16-byte aligned along their contiguous dimension, their other stride a multiple of 16 bytes
   int col;      // tokens are contiguous
 };
@@ -172,16 +172,33 @@ struct Units {
 
 // ------------------------------------------------------------- few tokens --
 // Units of up to 8 tokens. Warps deal out 32-element blocks of the CTA's slice of
-// k, then 16-row strips of its outputs; the first strip's weights and base are
-// asked for before the cluster meets.
-template <int AT, int STRIPS>
-__global__ void __launch_bounds__(kThreads, STRIPS >= 8 ? 2 : STRIPS >= 4 ? 3 : 4) lora_few_kernel(const __grid_constant__ LoraParams p) {
-  constexpr int kBlocks = (STRIPS + 1) / 2;  // 32-element blocks of the rank
-  constexpr int kSums = STRIPS * 16 * 8;     // [token][rank row] inner sums of a unit
-  constexpr int kRow = STRIPS * 16;
-  __shared__ __align__(16) float s_red[kWarps][kSums];
-  __shared__ __align__(16) float s_part[kSums], s_u[8 * (kBlocks * 32 + 4)];
+// k, then blocks of kOuts of its outputs, whose weights are copied one block ahead;
+// the first of them are under way before the inner sums are begun. Sums go through
+// shared memory, so that a lane adds and stores neighbouring outputs of a token.
+template <int STRIPS>
+struct Few {
+  static constexpr int kBlocks = (STRIPS + 1) / 2;      // 32-element blocks of the rank
+  static constexpr int kRow = STRIPS * 16;
+  static constexpr int kSums = kRow * 8;                // [token][rank row] inner sums of a unit
+  static constexpr int kURow = kBlocks * 32 + 4;
+  static constexpr int kOuts = 64 / kBlocks;            // outputs of a warp's block: 4 KB of weights
+  static constexpr int kStage = 256;                    // uint4 of a block's weights
+  static constexpr int kLine = kOuts + 2;               // floats of a token's sums
+  static constexpr int kRed = kWarps * kSums * 4;       // the warps' parts of the inner sums, then the outputs' sums
+  static constexpr int kOutBytes = kWarps * 8 * kLine * 4;
+  static constexpr int kSmem = kWarps * 2 * kStage * 16 + (kRed > kOutBytes ? kRed : kOutBytes) + kSums * 4 + 8 * kURow * 4;
+};
+
+template <int AT, int STRIPS, bool COL>
+__global__ void __launch_bounds__(kThreads, STRIPS >= 8 ? 2 : 3) lora_few_kernel(const __grid_constant__ LoraParams p) {
+  using F = Few<STRIPS>;
+  constexpr int kBlocks = F::kBlocks, kRow = F::kRow, kSums = F::kSums, kOuts = F::kOuts;
+  extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int s_find[kWarps + 1];
+  uint4* const s_ring = reinterpret_cast<uint4*>(smem);
+  float* const s_red = reinterpret_cast<float*>(smem + kWarps * 2 * F::kStage * 16);
+  float* const s_part = reinterpret_cast<float*>(smem + F::kSmem) - kSums - 8 * F::kURow;
+  float* const s_u = s_part + kSums;
   pdl_launch_dependents();
   pdl_wait();
   const fp8imma_lora_args& a = p.a;
@@ -191,43 +208,36 @@ __global__ void __launch_bounds__(kThreads, STRIPS >= 8 ? 2 : STRIPS >= 4 ? 3 : 
   units.scan(a, s_find);
   const int R = a.rank, K = a.in_features, N = a.out_features;
   const int kb = (K + 31) / 32, kb0 = (int)((int64_t)kb * c / S), kb1 = (int)((int64_t)kb * (c + 1) / S);
-  for (int item = cid; item < units.total * p.split; item += clusters) {
+  uint4* const ring = s_ring + warp * (2 * F::kStage) + lane;
+  float* const outs = s_red + warp * (8 * F::kLine);
+  // few units share the clusters that the others would have taken
+  const int split = max(1, min(p.split, clusters / max(1, units.total)));
+  for (int item = cid; item < units.total * split; item += clusters) {
     int t0, t1;
-    units.find(a, item / p.split, s_find, t0, t1);
+    units.find(a, item / split, s_find, t0, t1);
     const int tb = t0 & ~7;  // tokens keep their place within 8
     const int e = __ldg(a.adapter_ids + t0);
     const bool held = (unsigned)e < (unsigned)a.adapters;
-    const int share = item % p.split * S + c, shares = p.split * S, strips = (N + 15) / 16;
-    const int ns0 = (int)((int64_t)strips * share / shares), ns1 = (int)((int64_t)strips * (share + 1) / shares);
     if (!held && a.out == a.base) continue;
+    const int share = item % split * S + c, shares = split * S, groups = (N + kOuts - 1) / kOuts;
+    const int g0 = (int)((int64_t)groups * share / shares), g1 = (int)((int64_t)groups * (share + 1) / shares);
+    // a lane copies the pieces that it multiplies itself: rows q4 + 8 i of a block of outputs
+    auto fetch = [&](int g, int slot) {
+      if (held && g < g1) {
+        const uint16_t* src = static_cast<const uint16_t*>(a.lora_b) + ((int64_t)e * N + g * kOuts + q4) * R + t4 * 8;
+#pragma unroll
+        for (int i = 0; i < kOuts / 8; ++i)
+#pragma unroll
+          for (int b = 0; b < kBlocks; ++b) {
+            const bool on = g * kOuts + i * 8 + q4 < N && b * 32 + t4 * 8 < R;
+            copy16(ring + slot * F::kStage + (i * kBlocks + b) * 32, on ? src + i * 8 * R + b * 32 : static_cast<const uint16_t*>(a.lora_b), on);
+          }
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    fetch(g0 + warp, 0);
     uint4 hi[kBlocks], lo[kBlocks];
     float f[2] = {0.0f, 0.0f};  // of tokens 2 t4 and 2 t4 + 1
-
-    // a strip's weights and base
-    uint4 w[kBlocks][2];
-    uint16_t have[4];
-    auto at = [&](const void*, int64_t ts, int64_t fs, int ns, int k) {
-      return (int64_t)(tb + 2 * t4 + (k & 1)) * ts + (int64_t)(ns * 16 + q4 + (k >> 1) * 8) * fs;
-    };
-    auto inside = [&](int ns, int k) {
-      const int t = tb + 2 * t4 + (k & 1);
-      return ns < ns1 && t >= t0 && t < t1 && ns * 16 + q4 + (k >> 1) * 8 < N;
-    };
-    auto fetch = [&](int ns) {
-#pragma unroll
-      for (int b = 0; b < kBlocks; ++b)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int n = ns * 16 + q4 + h * 8, r = b * 32 + t4 * 8;
-          w[b][h] = make_uint4(0, 0, 0, 0);
-          if (held && ns < ns1 && n < N && r < R)
-            w[b][h] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.lora_b) + ((int64_t)e * N + n) * R + r));
-        }
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        have[k] = inside(ns, k) ? static_cast<const uint16_t*>(a.base)[at(a.base, a.base_token_stride, a.base_feature_stride, ns, k)] : (uint16_t)0;
-    };
-
     if (held) {
       float acc[STRIPS][4];
 #pragma unroll
@@ -236,7 +246,7 @@ __global__ void __launch_bounds__(kThreads, STRIPS >= 8 ? 2 : STRIPS >= 4 ? 3 : 
         for (int k = 0; k < 4; ++k) acc[s][k] = 0.0f;
       const bool live = tb + q4 >= t0 && tb + q4 < t1;
       const uint16_t* xr = static_cast<const uint16_t*>(a.x) + (int64_t)(tb + q4) * a.x_stride;
-      const uint16_t* ar = static_cast<const uint16_t*>(a.lora_a) + (int64_t)e * R * K;
+      const uint16_t* ar = static_cast<const uint16_t*>(a.lora_a) + ((int64_t)e * R + q4) * K;
 #pragma unroll 2
       for (int blk = kb0 + warp; blk < kb1; blk += kWarps) {
         const int k = blk * 32 + t4 * 8;
@@ -246,9 +256,8 @@ __global__ void __launch_bounds__(kThreads, STRIPS >= 8 ? 2 : STRIPS >= 4 ? 3 : 
         for (int s = 0; s < STRIPS; ++s)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const int r = s * 16 + q4 + h * 8;
             m[s][h] = make_uint4(0, 0, 0, 0);
-            if (r < R && k < K) m[s][h] = __ldg(reinterpret_cast<const uint4*>(ar + (int64_t)r * K + k));
+            if (s * 16 + h * 8 + q4 < R && k < K) m[s][h] = __ldg(reinterpret_cast<const uint4*>(ar + (int64_t)(s * 16 + h * 8) * K + k));
           }
 #pragma unroll
         for (int s = 0; s < STRIPS; ++s) mma32<AT>(acc[s], m[s][0], m[s][1], x);
@@ -256,26 +265,24 @@ __global__ void __launch_bounds__(kThreads, STRIPS >= 8 ? 2 : STRIPS >= 4 ? 3 : 
 #pragma unroll
       for (int s = 0; s < STRIPS; ++s)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) s_red[warp][(2 * t4 + (k & 1)) * kRow + s * 16 + q4 + (k >> 1) * 8] = acc[s][k];
-    }
-    fetch(ns0 + warp);
-    if (held) {
+        for (int k = 0; k < 4; ++k) s_red[warp * kSums + (2 * t4 + (k & 1)) * kRow + s * 16 + q4 + (k >> 1) * 8] = acc[s][k];
       __syncthreads();
       for (int i = threadIdx.x; i < kSums; i += kThreads) {
         float s = 0.0f;
 #pragma unroll
-        for (int k = 0; k < kWarps; ++k) s += s_red[k][i];
+        for (int k = 0; k < kWarps; ++k) s += s_red[k * kSums + i];
         s_part[i] = s;
       }
       cluster_arrive();
       cluster_wait();
       for (int i = threadIdx.x; i < kSums / 4; i += kThreads) {
         float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
         for (int k = 0; k < S; ++k) {
           const float4 v = peer_load(peer_addr(s_part + i * 4, k));
           s = make_float4(s.x + v.x, s.y + v.y, s.z + v.z, s.w + v.w);
         }
-        *reinterpret_cast<float4*>(s_u + i * 4 / kRow * (kBlocks * 32 + 4) + i * 4 % kRow) = s;
+        *reinterpret_cast<float4*>(s_u + i * 4 / kRow * F::kURow + i * 4 % kRow) = s;
       }
       cluster_arrive();  // the parts may be written again once all have read them
       __syncthreads();
@@ -285,7 +292,7 @@ __global__ void __launch_bounds__(kThreads, STRIPS >= 8 ? 2 : STRIPS >= 4 ? 3 : 
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const int r = b * 32 + t4 * 8 + i;
-          u[b][i] = r < kRow ? s_u[q4 * (kBlocks * 32 + 4) + r] : 0.0f;
+          u[b][i] = r < kRow ? s_u[q4 * F::kURow + r] : 0.0f;
           big = fmaxf(big, fabsf(u[b][i]));
         }
       big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
@@ -298,25 +305,98 @@ __global__ void __launch_bounds__(kThreads, STRIPS >= 8 ? 2 : STRIPS >= 4 ? 3 : 
 #pragma unroll
       for (int k = 0; k < 2; ++k) f[k] = scale * __shfl_sync(0xffffffffu, back, (2 * t4 + k) * 4);
     }
-    for (int ns = ns0 + warp; ns < ns1; ns += kWarps) {
-      float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-      uint16_t was[4];
-      if (held) {
+    int slot = 0;
+    const bool wide = COL && p.vec && tb + 8 <= a.tokens, all8 = wide && t1 - t0 == 8;
+    for (int g = g0 + warp; g < g1; g += kWarps, slot ^= 1) {
+      // This lane's outputs: n0 + lane and n0 + lane + 32, of all tokens at once where
+      // tokens are contiguous, or two neighbours, token after token, where outputs are.
+      constexpr int kEach = kOuts / 32 > 0 ? kOuts / 32 : 1;
+      const int n0 = g * kOuts, at0 = COL || kEach == 1 ? lane : 2 * lane;
+      auto out_at = [&](int i) { return at0 + (COL ? 32 * i : i); };
+      auto there = [&](int i) { return out_at(i) < kOuts && n0 + out_at(i) < N; };
+      uint16_t was[kEach];
+      uint4 was8[kEach];
+      auto load = [&](int t) {
+        const uint16_t* src = static_cast<const uint16_t*>(a.base) + (int64_t)t * a.base_token_stride;
 #pragma unroll
-        for (int b = 0; b < kBlocks; ++b) {
-          mma32<AT>(acc, w[b][0], w[b][1], lo[b]);
-          mma32<AT>(acc, w[b][0], w[b][1], hi[b]);
+        for (int i = 0; i < kEach; ++i)
+          if (there(i)) was[i] = src[(int64_t)(n0 + out_at(i)) * a.base_feature_stride];
+      };
+      if (COL) {
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+          if (!there(i)) continue;
+          const uint16_t* src = static_cast<const uint16_t*>(a.base) + tb + (int64_t)(n0 + out_at(i)) * a.base_feature_stride;
+          if (wide) was8[i] = *reinterpret_cast<const uint4*>(src);  // the other tokens' values are not used
+          else {
+            uint32_t x[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = tb + j >= t0 && tb + j < t1 ? src[j] : 0u;
+            was8[i] = make_uint4(x[0] | x[1] << 16, x[2] | x[3] << 16, x[4] | x[5] << 16, x[6] | x[7] << 16);
+          }
+        }
+      } else {
+        load(t0);
+      }
+      fetch(g + kWarps, slot ^ 1);
+      if (held) {
+        asm volatile("cp.async.wait_group 1;" ::: "memory");
+        float acc[kOuts / 16][4];
+#pragma unroll
+        for (int s = 0; s < kOuts / 16; ++s) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) acc[s][k] = 0.0f;
+#pragma unroll
+          for (int b = 0; b < kBlocks; ++b) {
+            const uint4 w0 = ring[slot * F::kStage + (2 * s * kBlocks + b) * 32], w1 = ring[slot * F::kStage + ((2 * s + 1) * kBlocks + b) * 32];
+            mma32<AT>(acc[s], w0, w1, lo[b]);
+            mma32<AT>(acc[s], w0, w1, hi[b]);
+          }
+        }
+        __syncwarp();  // the sums of the block before have been read
+#pragma unroll
+        for (int s = 0; s < kOuts / 16; ++s)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) outs[(2 * t4 + (k & 1)) * F::kLine + s * 16 + q4 + (k >> 1) * 8] = f[k & 1] * acc[s][k];
+        __syncwarp();
+      }
+      if (COL) {
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+          if (!there(i)) continue;
+          uint16_t* const dst = static_cast<uint16_t*>(a.out) + tb + (int64_t)(n0 + out_at(i)) * a.out_feature_stride;
+          uint32_t w[4] = {was8[i].x, was8[i].y, was8[i].z, was8[i].w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            if (tb + 2 * j + 1 < t0 || tb + 2 * j >= t1) continue;
+            if (held) {
+              const float x = d_to_f32((uint16_t)w[j], a.d_type) + outs[2 * j * F::kLine + out_at(i)];
+              const float y = d_to_f32((uint16_t)(w[j] >> 16), a.d_type) + outs[(2 * j + 1) * F::kLine + out_at(i)];
+              w[j] = a.d_type == FP8IMMA_OUT_F16 ? f32x2_to_a16x2<0>(x, y) : f32x2_to_a16x2<1>(x, y);
+            }
+            if (!all8) {
+              if (tb + 2 * j >= t0 && tb + 2 * j < t1) dst[2 * j] = (uint16_t)w[j];
+              if (tb + 2 * j + 1 >= t0 && tb + 2 * j + 1 < t1) dst[2 * j + 1] = (uint16_t)(w[j] >> 16);
+            }
+          }
+          if (all8) *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+      } else {
+        for (int t = t0; t < t1; ++t) {
+          uint16_t* const dst = static_cast<uint16_t*>(a.out) + (int64_t)t * a.out_token_stride;
+          uint16_t old[kEach];
+#pragma unroll
+          for (int i = 0; i < kEach; ++i) old[i] = was[i];
+          if (t + 1 < t1) load(t + 1);
+#pragma unroll
+          for (int i = 0; i < kEach; ++i)
+            if (there(i))
+              dst[(int64_t)(n0 + out_at(i)) * a.out_feature_stride] =
+                  held ? f32_to_d(d_to_f32(old[i], a.d_type) + outs[(t & 7) * F::kLine + out_at(i)], a.d_type) : old[i];
         }
       }
-#pragma unroll
-      for (int k = 0; k < 4; ++k) was[k] = have[k];
-      fetch(ns + kWarps);
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (inside(ns, k))
-          static_cast<uint16_t*>(a.out)[at(a.out, a.out_token_stride, a.out_feature_stride, ns, k)] =
-              held ? f32_to_d(fmaf(f[k & 1], acc[k], d_to_f32(was[k], a.d_type)), a.d_type) : was[k];
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
     if (held) cluster_wait();
   }
 }
@@ -324,35 +404,36 @@ __global__ void __launch_bounds__(kThreads, STRIPS >= 8 ? 2 : STRIPS >= 4 ? 3 : 
 // ------------------------------------------------------------ many tokens --
 // Units of up to 64 tokens. x and the adapter's slice of A stream through shared
 // memory 128 elements of k at a time (asynchronous copies, kStages deep); a warp
-// multiplies 32 tokens with a quarter of those. The second product goes 32 outputs x 32
-// tokens a warp, results pass through shared memory so that base and out are read
-// and written along their contiguous dimension.
-constexpr int kTile = 64, kStep = 128, kStages = 3;
+// multiplies 32 tokens with a quarter of those. The second product goes 64 tokens x
+// 64 outputs a step, B's rows and the base under way kAhead steps before: a warp
+// keeps the inner sums of 16 tokens in registers and makes 32 outputs of each. It adds
+// them to the base in shared memory, two neighbours along the contiguous dimension a
+// lane (COL: tokens, so they are the 8-column operand; else outputs), and stores 16
+// bytes a lane.
+constexpr int kTile = 64, kStep = 128, kStages = 3, kAhead = 4;
 
 template <int STRIPS>
 struct Many {
   static constexpr int kRow = STRIPS * 16;                          // rank rows, rounded up
   static constexpr int kBlocks = (STRIPS + 1) / 2;                  // 32-element blocks of the rank
   static constexpr int kStageBytes = (kTile + kRow) * kStep * 2;
-  static constexpr int kURow = kBlocks > 1 ? kBlocks * 32 + 32 : 32;  // 16-bit elements of a token's hi (or lo): an odd number of 64 bytes
   static constexpr int kRing = kStages * kStageBytes;               // used again for the 4 parts of the sums,
   static constexpr int kParts = 4 * kTile * kRow * 4;               // and then for
-  static constexpr int kOut = kWarps * 32 * 40 * 4;                 // outputs and
-  static constexpr int kU = 2 * kTile * kURow * 2;                  // hi and lo
-  static constexpr int kPool = kRing > kParts ? (kRing > kOut + kU ? kRing : kOut + kU) : (kParts > kOut + kU ? kParts : kOut + kU);
+  static constexpr int kLine = kTile * 2 + 16;                      // lines of the base: 16 bytes apart modulo 128
+  static constexpr int kBytesB = kTile * kBlocks * 64;              // steps of B and
+  static constexpr int kOutBytes = kBytesB + kTile * kLine;         // the base
+  static constexpr int kPool0 = kRing > kParts ? kRing : kParts;
+  static constexpr int kPool = kPool0 > kAhead * kOutBytes ? kPool0 : kAhead * kOutBytes;
   static constexpr int kSmem = kPool + kTile * kRow * 4;            // and the unit's sums
 };
 
-template <int AT, int STRIPS>
+template <int AT, int STRIPS, bool COL>
 __global__ void __launch_bounds__(kThreads, STRIPS >= 8 ? 1 : 2) lora_many_kernel(const __grid_constant__ LoraParams p) {
   using M = Many<STRIPS>;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int s_find[kWarps + 1];
-  __shared__ float s_f[kTile];
   float* const parts = reinterpret_cast<float*>(smem);
   float* const s_sum = reinterpret_cast<float*>(smem + M::kPool);
-  uint16_t* const s_hi = reinterpret_cast<uint16_t*>(smem + M::kOut);
-  uint16_t* const s_lo = s_hi + kTile * M::kURow;
   pdl_launch_dependents();
   pdl_wait();
   const fp8imma_lora_args& a = p.a;
@@ -362,15 +443,17 @@ __global__ void __launch_bounds__(kThreads, STRIPS >= 8 ? 1 : 2) lora_many_kerne
   units.scan(a, s_find);
   const int R = a.rank, K = a.in_features, N = a.out_features;
   const int ks = (K + kStep - 1) / kStep, ks0 = (int)((int64_t)ks * c / S), ks1 = (int)((int64_t)ks * (c + 1) / S);
-  const int tg = warp & 1, kg = warp >> 1;  // 32 tokens, and a quarter of k (or of the outputs)
-  for (int item = cid; item < units.total * p.split; item += clusters) {
+  const int split = max(1, min(p.split, clusters / max(1, units.total)));
+  for (int item = cid; item < units.total * split; item += clusters) {
     int t0, t1;
-    units.find(a, item / p.split, s_find, t0, t1);
+    units.find(a, item / split, s_find, t0, t1);
     const int tb = t0 & ~(kTile - 1);  // tokens keep their place within 64
     const int i0 = t0 - tb, i1 = t1 - tb;
     const int e = __ldg(a.adapter_ids + t0);
     const bool held = (unsigned)e < (unsigned)a.adapters;
     if (!held && a.out == a.base) continue;
+    const int share = item % split * S + c, shares = split * S, groups = (N + kTile - 1) / kTile;
+    const int g0 = (int)((int64_t)groups * share / shares), g1 = (int)((int64_t)groups * (share + 1) / shares);
     if (held) {
       const uint16_t* xb = static_cast<const uint16_t*>(a.x);
       const uint16_t* ab = static_cast<const uint16_t*>(a.lora_a) + (int64_t)e * R * K;
@@ -389,6 +472,7 @@ __global__ void __launch_bounds__(kThreads, STRIPS >= 8 ? 1 : 2) lora_many_kerne
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
       };
+      const int tg = warp & 1, kg = warp >> 1;  // 32 tokens, and a quarter of k
       float acc[STRIPS][4][4];
 #pragma unroll
       for (int s = 0; s < STRIPS; ++s)
@@ -448,10 +532,53 @@ __global__ void __launch_bounds__(kThreads, STRIPS >= 8 ? 1 : 2) lora_many_kerne
         for (int k = 0; k < S; ++k) peer_store(peer_addr(s_sum + v * 4, k), s);
       }
       cluster_arrive();
-      cluster_wait();
-      {
-        // a warp takes 8 tokens, four lanes a token
-        const int i = warp * 8 + q4;
+      cluster_wait();  // the sums are here, and the parts have been read
+    }
+
+    // where line l, element 8 j of a step lies: token (within the 64) and output
+    auto place = [&](int g, int l, int j, int& i, int& n) {
+      i = COL ? 8 * j : l;
+      n = g * kTile + (COL ? l : 8 * j);
+    };
+    auto whole = [&](int i, int n) {
+      return p.vec && (COL ? i >= i0 && i + 8 <= i1 && n < N : i >= i0 && i < i1 && n + 8 <= N);
+    };
+    auto load = [&](int g) {
+      if (g < g1) {
+        uint8_t* const dst = smem + (g - g0) % kAhead * M::kOutBytes;
+        if (held) {
+          const uint16_t* bb = static_cast<const uint16_t*>(a.lora_b) + (int64_t)e * N * R;
+          for (int v = threadIdx.x; v < kTile * M::kBlocks * 4; v += kThreads) {
+            const int row = v / (M::kBlocks * 4), ch = v % (M::kBlocks * 4), n = g * kTile + row;
+            const bool on = n < N && ch * 8 < R;
+            copy16(dst + row * (M::kBlocks * 64) + ((M::kBlocks == 1 ? ch : ch ^ ((row & 1) << 2)) << 4), on ? bb + (int64_t)n * R + ch * 8 : bb, on);
+          }
+        }
+#pragma unroll
+        for (int v = threadIdx.x; v < kTile * 8; v += kThreads) {
+          int i, n;
+          place(g, v >> 3, v & 7, i, n);
+          const uint16_t* src = static_cast<const uint16_t*>(a.base) + (int64_t)(tb + i) * a.base_token_stride + (int64_t)n * a.base_feature_stride;
+          uint16_t* line = reinterpret_cast<uint16_t*>(dst + M::kBytesB + (v >> 3) * M::kLine + (v & 7) * 16);
+          if (whole(i, n)) copy16(line, src, true);
+          else
+            for (int k = 0; k < 8; ++k) {
+              const int ii = i + (COL ? k : 0), nn = n + (COL ? 0 : k);
+              if (ii >= i0 && ii < i1 && nn < N) line[k] = src[k];
+            }
+        }
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    // inner sums of the warp's 16 tokens
+    const int tok = (warp & 3) * 16, half = (warp >> 2) * 32;  // and the outputs of a step
+    uint4 hi[2][M::kBlocks], lo[2][M::kBlocks];
+    float f[4];  // COL: of tokens 2 t4, 2 t4 + 1 of both eights; else of q4 of both
+    if (held) {
+      const float scale = a.scales ? __ldg(a.scales + e) : 1.0f;
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const int i = tok + t * 8 + q4;
         const bool live = i >= i0 && i < i1;
         float u[M::kBlocks][8], big = 0.0f;
 #pragma unroll
@@ -466,122 +593,84 @@ __global__ void __launch_bounds__(kThreads, STRIPS >= 8 ? 1 : 2) lora_many_kerne
         big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
         float g, back;
         range_of<AT>(big, g, back);
+        back *= scale;
 #pragma unroll
-        for (int b = 0; b < M::kBlocks; ++b) {
-          uint4 hi, lo;
-          split8<AT>(u[b], g, hi, lo);
-          *reinterpret_cast<uint4*>(s_hi + i * M::kURow + b * 32 + t4 * 8) = hi;
-          *reinterpret_cast<uint4*>(s_lo + i * M::kURow + b * 32 + t4 * 8) = lo;
-        }
-        if (t4 == 0) s_f[i] = back * (a.scales ? __ldg(a.scales + e) : 1.0f);
-      }
-      __syncthreads();
-    }
-
-    const int share = item % p.split * S + c, shares = p.split * S, groups = (N + 31) / 32;
-    const int g0 = (int)((int64_t)groups * share / shares), g1 = (int)((int64_t)groups * (share + 1) / shares);
-    float* const stage = reinterpret_cast<float*>(smem) + warp * (32 * 40);
-    const bool any = tg * 32 < i1 && tg * 32 + 32 > i0;  // the warp's 32 tokens hold some of the unit
-    for (int g = g0 + kg; any && g < g1; g += 4) {
-      const int n0 = g * 32;
-      // what this lane reads and writes: four runs of 8 elements along the contiguous dimension
-      auto run = [&](int j, int& i, int& n) {  // first token (within the 64) and output of run j
-        const int line = j * 8 + (lane >> 2), at = (lane & 3) * 8;
-        i = tg * 32 + (p.col ? at : line);
-        n = n0 + (p.col ? line : at);
-      };
-      auto whole = [&](int i, int n) {
-        return p.vec && (p.col ? i >= i0 && i + 8 <= i1 && n < N : i >= i0 && i < i1 && n + 8 <= N);
-      };
-      uint4 was[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        int i, n;
-        run(j, i, n);
-        if (whole(i, n)) was[j] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.base) + (int64_t)(tb + i) * a.base_token_stride + (int64_t)n * a.base_feature_stride);
-      }
-      if (held) {
-        float acc[2][4][4];
-#pragma unroll
-        for (int s = 0; s < 2; ++s)
-#pragma unroll
-          for (int t = 0; t < 4; ++t)
-#pragma unroll
-            for (int k = 0; k < 4; ++k) acc[s][t][k] = 0.0f;
-#pragma unroll
-        for (int b = 0; b < M::kBlocks; ++b) {
-          uint4 w[2][2];
-#pragma unroll
-          for (int s = 0; s < 2; ++s)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const int n = n0 + s * 16 + h * 8 + q4, r = b * 32 + t4 * 8;
-              w[s][h] = make_uint4(0, 0, 0, 0);
-              if (n < N && r < R) w[s][h] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.lora_b) + ((int64_t)e * N + n) * R + r));
-            }
-#pragma unroll
-          for (int t = 0; t < 4; ++t) {
-            const int i = tg * 32 + t * 8 + q4;
-            const uint4 hi = *reinterpret_cast<const uint4*>(s_hi + i * M::kURow + b * 32 + t4 * 8);
-            const uint4 lo = *reinterpret_cast<const uint4*>(s_lo + i * M::kURow + b * 32 + t4 * 8);
-#pragma unroll
-            for (int s = 0; s < 2; ++s) {
-              mma32<AT>(acc[s][t], w[s][0], w[s][1], lo);
-              mma32<AT>(acc[s][t], w[s][0], w[s][1], hi);
-            }
-          }
-        }
-        __syncwarp();
-        // row stride 36 (outputs contiguous) or 40 (tokens contiguous): stores fall on all banks
-#pragma unroll
-        for (int s = 0; s < 2; ++s)
-#pragma unroll
-          for (int t = 0; t < 4; ++t)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const int n = s * 16 + h * 8 + q4, i = t * 8 + 2 * t4;
-              const float x = acc[s][t][2 * h] * s_f[tg * 32 + i], y = acc[s][t][2 * h + 1] * s_f[tg * 32 + i + 1];
-              if (p.col) *reinterpret_cast<float2*>(stage + n * 40 + i) = make_float2(x, y);
-              else stage[i * 36 + n] = x, stage[(i + 1) * 36 + n] = y;
-            }
-        __syncwarp();
-      }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        int i, n;
-        run(j, i, n);
-        float v[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = 0.0f;
-        if (held) {
-          const float4* s = reinterpret_cast<const float4*>(stage + (j * 8 + (lane >> 2)) * (p.col ? 40 : 36) + (lane & 3) * 8);
-          const float4 x = s[0], y = s[1];
-          v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w, v[4] = y.x, v[5] = y.y, v[6] = y.z, v[7] = y.w;
-        }
-        uint16_t* const dst = static_cast<uint16_t*>(a.out) + (int64_t)(tb + i) * a.out_token_stride + (int64_t)n * a.out_feature_stride;
-        if (whole(i, n)) {
-          uint32_t w[4] = {was[j].x, was[j].y, was[j].z, was[j].w};
-          if (held) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              w[k] = (uint32_t)f32_to_d(d_to_f32((uint16_t)w[k], a.d_type) + v[2 * k], a.d_type) |
-                     (uint32_t)f32_to_d(d_to_f32((uint16_t)(w[k] >> 16), a.d_type) + v[2 * k + 1], a.d_type) << 16;
-          }
-          *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+        for (int b = 0; b < M::kBlocks; ++b) split8<AT>(u[b], g, hi[t][b], lo[t][b]);
+        if (COL) {
+          f[2 * t] = __shfl_sync(0xffffffffu, back, 2 * t4 * 4);
+          f[2 * t + 1] = __shfl_sync(0xffffffffu, back, (2 * t4 + 1) * 4);
         } else {
-          const uint16_t* src = static_cast<const uint16_t*>(a.base) + (int64_t)(tb + i) * a.base_token_stride + (int64_t)n * a.base_feature_stride;
-#pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const int ii = i + (p.col ? k : 0), nn = n + (p.col ? 0 : k);
-            if (ii >= i0 && ii < i1 && nn < N) {
-              const uint16_t b = src[k];
-              dst[k] = held ? f32_to_d(d_to_f32(b, a.d_type) + v[k], a.d_type) : b;
-            }
-          }
+          f[2 * t] = f[2 * t + 1] = back;
         }
       }
     }
-    __syncthreads();  // outputs' places are the next unit's ring
+    const bool any = tok < i1 && tok + 16 > i0;  // the warp has tokens of the unit
+    for (int i = 0; i < kAhead - 1; ++i) load(g0 + i);
+    for (int g = g0; g < g1; ++g) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 2) : "memory");
+      __syncthreads();  // the step is there, and the one to be filled has been stored
+      load(g + kAhead - 1);
+      if (!any) continue;
+      uint8_t* const step = smem + (g - g0) % kAhead * M::kOutBytes;
+      uint8_t* const lines = step + M::kBytesB;
+      if (held) {
+        // COL: [strip of 16 outputs][eight of tokens]; else [eight of outputs] x 16 tokens
+        float acc[4][4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[k][j] = 0.0f;
+        auto piece = [&](int row, int b) {
+          return *reinterpret_cast<const uint4*>(step + row * (M::kBlocks * 64) + ((M::kBlocks == 1 ? t4 : (b * 4 + t4) ^ ((row & 1) << 2)) << 4));
+        };
+#pragma unroll
+        for (int b = 0; b < M::kBlocks; ++b) {
+          uint4 w[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) w[k] = piece(half + k * 8 + q4, b);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            if (COL) {  // k: strip k / 2, eight of tokens k % 2
+              mma32<AT>(acc[k], w[k / 2 * 2], w[k / 2 * 2 + 1], lo[k & 1][b]);
+              mma32<AT>(acc[k], w[k / 2 * 2], w[k / 2 * 2 + 1], hi[k & 1][b]);
+            } else {
+              mma32<AT>(acc[k], lo[0][b], lo[1][b], w[k]);
+              mma32<AT>(acc[k], hi[0][b], hi[1][b], w[k]);
+            }
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            // rows q4 and q4 + 8 of the 16-row operand, columns 2 t4 and 2 t4 + 1 of the other
+            const int line = COL ? half + k / 2 * 16 + h * 8 + q4 : tok + h * 8 + q4, at = COL ? tok + (k & 1) * 8 + 2 * t4 : half + k * 8 + 2 * t4;
+            uint32_t* const two = reinterpret_cast<uint32_t*>(lines + line * M::kLine + at * 2);
+            const uint32_t was = *two;
+            const float f0 = COL ? f[2 * (k & 1)] : f[2 * h], f1 = COL ? f[2 * (k & 1) + 1] : f[2 * h];
+            const float x = fmaf(f0, acc[k][2 * h], d_to_f32((uint16_t)was, a.d_type)), y = fmaf(f1, acc[k][2 * h + 1], d_to_f32((uint16_t)(was >> 16), a.d_type));
+            *two = a.d_type == FP8IMMA_OUT_F16 ? f32x2_to_a16x2<0>(x, y) : f32x2_to_a16x2<1>(x, y);
+          }
+        __syncwarp();
+      }
+      // the warp's 16 x 32 (COL: 32 x 16) elements, 16 bytes a lane
+#pragma unroll
+      for (int v = lane; v < 64; v += 32) {
+        const int l = COL ? half + (v >> 1) : tok + (v >> 2), j = COL ? tok / 8 + (v & 1) : half / 8 + (v & 3);
+        int i, n;
+        place(g, l, j, i, n);
+        uint16_t* const dst = static_cast<uint16_t*>(a.out) + (int64_t)(tb + i) * a.out_token_stride + (int64_t)n * a.out_feature_stride;
+        const uint16_t* const line = reinterpret_cast<const uint16_t*>(lines + l * M::kLine + j * 16);
+        if (whole(i, n)) *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(line);
+        else
+          for (int k = 0; k < 8; ++k) {
+            const int ii = i + (COL ? k : 0), nn = n + (COL ? 0 : k);
+            if (ii >= i0 && ii < i1 && nn < N) dst[k] = line[k];
+          }
+      }
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();  // the steps' places are the next unit's ring
   }
   // no CTA leaves while another may still write its sums: each has passed the last
   // barrier after those writes, so nothing is left to wait for
@@ -589,7 +678,7 @@ __global__ void __launch_bounds__(kThreads, STRIPS >= 8 ? 1 : 2) lora_many_kerne
 
 template <class Kern>
 cudaError_t launch_clusters(Kern kern, const LoraParams& p, int clusters, int smem, cudaStream_t st) {
-  cudaError_t e = ensure_smem_attr(reinterpret_cast<const void*>(kern), smem);
+  cudaError_t e = ensure_smem_attr(reinterpret_cast<const void*>(kern), smem + 1024);  // static shared memory counts too
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t lc = {};
   cudaLaunchAttribute attr[2];
@@ -612,14 +701,25 @@ cudaError_t launch(LoraParams& p, cudaStream_t st) {
   const int sms = num_sms_current(), T = p.a.tokens;
   p.cluster = 8;
   if (T <= 128) {
-    // a unit of its own for each token at most: as many clusters share a unit's
-    // outputs as the SMs have room for, each with a strip a warp or so
-    const int strips = (p.a.out_features + 15) / 16;
-    p.split = std::max(1, std::min(sms / (T * p.cluster), (strips + p.cluster * kWarps - 1) / (p.cluster * kWarps)));
-    return launch_clusters(lora_few_kernel<AT, STRIPS>, p, T * p.split, 0, st);
+    // a unit of its own for each token at most: clusters small enough to run all at
+    // once, and more of them where there are few tokens, each with a block a warp or so
+    using F = Few<STRIPS>;
+    while (p.cluster > 4 && T * p.cluster > 3 * sms) p.cluster /= 2;
+    const int groups = (p.a.out_features + F::kOuts - 1) / F::kOuts;
+    p.split = std::max(1, (groups + p.cluster * kWarps - 1) / (p.cluster * kWarps));
+    const int clusters = std::max(T, std::min(T * p.split, sms / p.cluster));
+    return p.col ? launch_clusters(lora_few_kernel<AT, STRIPS, true>, p, clusters, F::kSmem, st)
+                 : launch_clusters(lora_few_kernel<AT, STRIPS, false>, p, clusters, F::kSmem, st);
   }
-  p.split = 1;
-  return launch_clusters(lora_many_kernel<AT, STRIPS>, p, std::min(T, 2 * sms / p.cluster), Many<STRIPS>::kSmem, st);
+  // As large a cluster as lets about T / 64 units run at once, so that a unit's
+  // weights cross few SMs' links.
+  const int room = sms * (STRIPS >= 8 ? 1 : 2), units = (T + kTile - 1) / kTile;
+  while (p.cluster > 1 && units * p.cluster > room) p.cluster /= 2;
+  const int groups = (p.a.out_features + kTile - 1) / kTile;
+  p.split = std::max(1, groups / (2 * p.cluster));
+  const int clusters = (int)std::min<int64_t>((int64_t)T * p.split, room / p.cluster);
+  return p.col ? launch_clusters(lora_many_kernel<AT, STRIPS, true>, p, clusters, Many<STRIPS>::kSmem, st)
+               : launch_clusters(lora_many_kernel<AT, STRIPS, false>, p, clusters, Many<STRIPS>::kSmem, st);
 }
 
 }  // namespace
