@@ -24,6 +24,7 @@
 #include "sm100_async.cuh"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace fp8imma_b200 {
 namespace {
@@ -452,24 +453,47 @@ __global__ void __launch_bounds__(kThreads, STRIPS >= 8 ? 1 : 2) lora_many_kerne
     const int e = __ldg(a.adapter_ids + t0);
     const bool held = (unsigned)e < (unsigned)a.adapters;
     if (!held && a.out == a.base) continue;
+    // of an eight that begins at token i (within the 64), output n: whether it is whole and aligned, and else its elements
+    auto whole = [&](int i, int n) {
+      return p.vec && (COL ? i >= i0 && i + 8 <= i1 && n < N : i >= i0 && i < i1 && n + 8 <= N);
+    };
+    auto part = [&](int i, int n, auto each) {
+      if (i >= i1 || i + (COL ? 8 : 1) <= i0 || n >= N) return;
+#pragma unroll 1
+      for (int k = 0; k < 8; ++k) {
+        const int ii = i + (COL ? k : 0), nn = n + (COL ? 0 : k);
+        if (ii >= i0 && ii < i1 && nn < N) each(k);
+      }
+    };
     const int share = item % split * S + c, shares = split * S, groups = (N + kTile - 1) / kTile;
-    const int g0 = (int)((int64_t)groups * share / shares), g1 = (int)((int64_t)groups * (share + 1) / shares);
+    // the steps of a cluster's CTAs lie side by side, so that they read and write whole pages of memory together
     if (held) {
-      const uint16_t* xb = static_cast<const uint16_t*>(a.x);
-      const uint16_t* ab = static_cast<const uint16_t*>(a.lora_a) + (int64_t)e * R * K;
-      auto load = [&](int i) {
+      // 16-byte pieces of 256-byte rows: a thread copies piece ch of rows row0 + 16 i, of
+      // the tokens first. A piece's place takes the row's lowest bit, so that two rows'
+      // fall on all banks.
+      const int row0 = threadIdx.x >> 4, ch0 = threadIdx.x & 15;
+      const uint16_t* xp = static_cast<const uint16_t*>(a.x) + (int64_t)(tb + row0) * a.x_stride + (int64_t)ks0 * kStep + ch0 * 8;
+      const uint16_t* ap = static_cast<const uint16_t*>(a.lora_a) + ((int64_t)e * R + row0) * K + (int64_t)ks0 * kStep + ch0 * 8;
+      const int64_t x_rows = 16 * a.x_stride, a_rows = 16ll * K;
+      int k_left = K - ks0 * kStep - ch0 * 8;  // elements from the piece to the row's end
+      uint8_t* const dst0 = smem + row0 * (kStep * 2) + ((ch0 ^ ((row0 & 1) << 2)) << 4);
+      auto load = [&](int i, int stage) {
         if (i < ks1) {
-          uint8_t* dst = smem + (i - ks0) % kStages * M::kStageBytes;
-          // 16-byte pieces of 256-byte rows; a piece's place takes the row's lowest bit, so that two rows' fall on all banks
-          for (int v = threadIdx.x; v < (kTile + M::kRow) * 16; v += kThreads) {
-            const int row = v >> 4, ch = v & 15, k = i * kStep + ch * 8;
-            const bool tok = row < kTile;
-            const int r = row - kTile;
-            const bool on = k < K && (tok ? row >= i0 && row < i1 : r < R);
-            const uint16_t* src = !on ? xb + (int64_t)t0 * a.x_stride : tok ? xb + (int64_t)(tb + row) * a.x_stride + k : ab + (int64_t)r * K + k;
-            copy16(dst + row * (kStep * 2) + ((ch ^ ((row & 1) << 2)) << 4), src, on);
+          uint8_t* const dst = dst0 + stage * M::kStageBytes;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const bool on = k_left > 0 && row0 + 16 * r >= i0 && row0 + 16 * r < i1;
+            copy16(dst + r * (16 * kStep * 2), on ? xp + r * x_rows : static_cast<const uint16_t*>(a.x), on);
+          }
+#pragma unroll
+          for (int r = 0; r < STRIPS; ++r) {
+            const bool on = k_left > 0 && row0 + 16 * r < R;
+            copy16(dst + (4 + r) * (16 * kStep * 2), on ? ap + r * a_rows : static_cast<const uint16_t*>(a.lora_a), on);
           }
         }
+        xp += kStep;
+        ap += kStep;
+        k_left -= kStep;
         asm volatile("cp.async.commit_group;" ::: "memory");
       };
       const int tg = warp & 1, kg = warp >> 1;  // 32 tokens, and a quarter of k
@@ -480,12 +504,12 @@ __global__ void __launch_bounds__(kThreads, STRIPS >= 8 ? 1 : 2) lora_many_kerne
         for (int t = 0; t < 4; ++t)
 #pragma unroll
           for (int k = 0; k < 4; ++k) acc[s][t][k] = 0.0f;
-      for (int i = 0; i < kStages - 1; ++i) load(ks0 + i);
-      for (int i = ks0; i < ks1; ++i) {
+      for (int i = 0; i < kStages - 1; ++i) load(ks0 + i, i);
+      for (int i = ks0, stage = 0; i < ks1; ++i, stage = stage == kStages - 1 ? 0 : stage + 1) {
         asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
         __syncthreads();  // the stage is there, and the one to be filled has been read
-        load(i + kStages - 1);
-        const uint8_t* st = smem + (i - ks0) % kStages * M::kStageBytes;
+        load(i + kStages - 1, stage == 0 ? kStages - 1 : stage - 1);
+        const uint8_t* st = smem + stage * M::kStageBytes;
         const int ch = kg * 4 + t4;
         auto piece = [&](int row) { return *reinterpret_cast<const uint4*>(st + row * (kStep * 2) + ((ch ^ ((row & 1) << 2)) << 4)); };
         uint4 x[4];
@@ -535,37 +559,33 @@ __global__ void __launch_bounds__(kThreads, STRIPS >= 8 ? 1 : 2) lora_many_kerne
       cluster_wait();  // the sums are here, and the parts have been read
     }
 
-    // where line l, element 8 j of a step lies: token (within the 64) and output
-    auto place = [&](int g, int l, int j, int& i, int& n) {
-      i = COL ? 8 * j : l;
-      n = g * kTile + (COL ? l : 8 * j);
-    };
-    auto whole = [&](int i, int n) {
-      return p.vec && (COL ? i >= i0 && i + 8 <= i1 && n < N : i >= i0 && i < i1 && n + 8 <= N);
-    };
-    auto load = [&](int g) {
-      if (g < g1) {
-        uint8_t* const dst = smem + (g - g0) % kAhead * M::kOutBytes;
+    // Lines of a step's base: tokens (COL: outputs), 64 elements each in eights. A
+    // thread copies eight j of lines l and l + 32; in which of its tokens the unit
+    // lies and which outputs there are is settled line by line.
+    auto load = [&](int g, int stage) {
+      if (g < groups) {
+        uint8_t* const dst = smem + stage * M::kOutBytes;
         if (held) {
-          const uint16_t* bb = static_cast<const uint16_t*>(a.lora_b) + (int64_t)e * N * R;
-          for (int v = threadIdx.x; v < kTile * M::kBlocks * 4; v += kThreads) {
-            const int row = v / (M::kBlocks * 4), ch = v % (M::kBlocks * 4), n = g * kTile + row;
-            const bool on = n < N && ch * 8 < R;
-            copy16(dst + row * (M::kBlocks * 64) + ((M::kBlocks == 1 ? ch : ch ^ ((row & 1) << 2)) << 4), on ? bb + (int64_t)n * R + ch * 8 : bb, on);
+          constexpr int kChunks = M::kBlocks * 4, kRows = kThreads / kChunks;
+          const int row = threadIdx.x / kChunks, ch = threadIdx.x % kChunks;
+          const uint16_t* src = static_cast<const uint16_t*>(a.lora_b) + ((int64_t)e * N + g * kTile + row) * R + ch * 8;
+#pragma unroll
+          for (int i = 0; i < kTile / kRows; ++i) {
+            const bool on = g * kTile + row + i * kRows < N && ch * 8 < R;
+            const int r = row + i * kRows;
+            copy16(dst + r * (M::kBlocks * 64) + ((M::kBlocks == 1 ? ch : ch ^ ((r & 1) << 2)) << 4), on ? src + i * kRows * R : static_cast<const uint16_t*>(a.lora_b), on);
           }
         }
+        const int l = threadIdx.x >> 3, j = threadIdx.x & 7;
+        const uint16_t* src = static_cast<const uint16_t*>(a.base) + (int64_t)(tb + (COL ? 8 * j : l)) * a.base_token_stride +
+                              (int64_t)(g * kTile + (COL ? l : 8 * j)) * a.base_feature_stride;
+        const int64_t lines = 32 * (COL ? a.base_feature_stride : a.base_token_stride);
+        uint8_t* line = dst + M::kBytesB + l * M::kLine + j * 16;
 #pragma unroll
-        for (int v = threadIdx.x; v < kTile * 8; v += kThreads) {
-          int i, n;
-          place(g, v >> 3, v & 7, i, n);
-          const uint16_t* src = static_cast<const uint16_t*>(a.base) + (int64_t)(tb + i) * a.base_token_stride + (int64_t)n * a.base_feature_stride;
-          uint16_t* line = reinterpret_cast<uint16_t*>(dst + M::kBytesB + (v >> 3) * M::kLine + (v & 7) * 16);
-          if (whole(i, n)) copy16(line, src, true);
-          else
-            for (int k = 0; k < 8; ++k) {
-              const int ii = i + (COL ? k : 0), nn = n + (COL ? 0 : k);
-              if (ii >= i0 && ii < i1 && nn < N) line[k] = src[k];
-            }
+        for (int h = 0; h < 2; ++h) {
+          const int i = COL ? 8 * j : l + 32 * h, n = g * kTile + (COL ? l + 32 * h : 8 * j);
+          if (whole(i, n)) copy16(line + h * 32 * M::kLine, src + h * lines, true);
+          else part(i, n, [&](int k) { reinterpret_cast<uint16_t*>(line + h * 32 * M::kLine)[k] = src[h * lines + k]; });
         }
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
@@ -605,15 +625,23 @@ __global__ void __launch_bounds__(kThreads, STRIPS >= 8 ? 1 : 2) lora_many_kerne
       }
     }
     const bool any = tok < i1 && tok + 16 > i0;  // the warp has tokens of the unit
-    for (int i = 0; i < kAhead - 1; ++i) load(g0 + i);
-    for (int g = g0; g < g1; ++g) {
+    for (int i = 0; i < kAhead - 1; ++i) load(share + i * shares, i);
+    for (int g = share, stage = 0; g < groups; g += shares, stage = stage == kAhead - 1 ? 0 : stage + 1) {
       asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 2) : "memory");
       __syncthreads();  // the step is there, and the one to be filled has been stored
-      load(g + kAhead - 1);
+      load(g + (kAhead - 1) * shares, stage == 0 ? kAhead - 1 : stage - 1);
       if (!any) continue;
-      uint8_t* const step = smem + (g - g0) % kAhead * M::kOutBytes;
+      uint8_t* const step = smem + stage * M::kOutBytes;
       uint8_t* const lines = step + M::kBytesB;
       if (held) {
+        // rows q4 and q4 + 8 of the 16-row operand, columns 2 t4 and 2 t4 + 1 of the other
+        uint8_t* const mine = lines + (COL ? half + q4 : tok + q4) * M::kLine + ((COL ? tok : half) + 2 * t4) * 2;
+        auto two = [&](int k, int h) { return reinterpret_cast<uint32_t*>(mine + (COL ? k / 2 * 16 + h * 8 : h * 8) * M::kLine + (COL ? (k & 1) * 8 : k * 8) * 2); };
+        uint32_t was[4][2];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) was[k][h] = *two(k, h);
         // COL: [strip of 16 outputs][eight of tokens]; else [eight of outputs] x 16 tokens
         float acc[4][4];
 #pragma unroll
@@ -629,44 +657,41 @@ __global__ void __launch_bounds__(kThreads, STRIPS >= 8 ? 1 : 2) lora_many_kerne
 #pragma unroll
           for (int k = 0; k < 4; ++k) w[k] = piece(half + k * 8 + q4, b);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            if (COL) {  // k: strip k / 2, eight of tokens k % 2
-              mma32<AT>(acc[k], w[k / 2 * 2], w[k / 2 * 2 + 1], lo[k & 1][b]);
-              mma32<AT>(acc[k], w[k / 2 * 2], w[k / 2 * 2 + 1], hi[k & 1][b]);
-            } else {
-              mma32<AT>(acc[k], lo[0][b], lo[1][b], w[k]);
-              mma32<AT>(acc[k], hi[0][b], hi[1][b], w[k]);
+          for (int p = 0; p < 2; ++p)  // the small parts first
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              if (COL) mma32<AT>(acc[k], w[k / 2 * 2], w[k / 2 * 2 + 1], (p ? hi : lo)[k & 1][b]);  // strip k / 2, eight of tokens k % 2
+              else mma32<AT>(acc[k], (p ? hi : lo)[0][b], (p ? hi : lo)[1][b], w[k]);
             }
-          }
         }
+        auto add = [&](auto type) {
+          constexpr int DT = decltype(type)::value;
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
+          for (int k = 0; k < 4; ++k)
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            // rows q4 and q4 + 8 of the 16-row operand, columns 2 t4 and 2 t4 + 1 of the other
-            const int line = COL ? half + k / 2 * 16 + h * 8 + q4 : tok + h * 8 + q4, at = COL ? tok + (k & 1) * 8 + 2 * t4 : half + k * 8 + 2 * t4;
-            uint32_t* const two = reinterpret_cast<uint32_t*>(lines + line * M::kLine + at * 2);
-            const uint32_t was = *two;
-            const float f0 = COL ? f[2 * (k & 1)] : f[2 * h], f1 = COL ? f[2 * (k & 1) + 1] : f[2 * h];
-            const float x = fmaf(f0, acc[k][2 * h], d_to_f32((uint16_t)was, a.d_type)), y = fmaf(f1, acc[k][2 * h + 1], d_to_f32((uint16_t)(was >> 16), a.d_type));
-            *two = a.d_type == FP8IMMA_OUT_F16 ? f32x2_to_a16x2<0>(x, y) : f32x2_to_a16x2<1>(x, y);
-          }
+            for (int h = 0; h < 2; ++h) {
+              const float f0 = COL ? f[2 * (k & 1)] : f[2 * h], f1 = COL ? f[2 * (k & 1) + 1] : f[2 * h];
+              const uint32_t b = was[k][h];
+              const float b0 = a16_to_f32<DT>((uint16_t)b), b1 = DT == 0 ? a16_to_f32<0>((uint16_t)(b >> 16)) : __uint_as_float(b & 0xFFFF0000u);
+              *two(k, h) = f32x2_to_a16x2<DT>(fmaf(f0, acc[k][2 * h], b0), fmaf(f1, acc[k][2 * h + 1], b1));
+            }
+        };
+        if (a.d_type == FP8IMMA_OUT_F16) add(std::integral_constant<int, 0>());
+        else add(std::integral_constant<int, 1>());
         __syncwarp();
       }
       // the warp's 16 x 32 (COL: 32 x 16) elements, 16 bytes a lane
+      const int l = COL ? half + (lane >> 1) : tok + (lane >> 2), j = COL ? tok / 8 + (lane & 1) : half / 8 + (lane & 3);
+      constexpr int kNext = COL ? 16 : 8;  // lines to the lane's second eight
+      uint16_t* const dst = static_cast<uint16_t*>(a.out) + (int64_t)(tb + (COL ? 8 * j : l)) * a.out_token_stride +
+                            (int64_t)(g * kTile + (COL ? l : 8 * j)) * a.out_feature_stride;
+      const int64_t next = kNext * (COL ? a.out_feature_stride : a.out_token_stride);
+      const uint8_t* const line = lines + l * M::kLine + j * 16;
 #pragma unroll
-      for (int v = lane; v < 64; v += 32) {
-        const int l = COL ? half + (v >> 1) : tok + (v >> 2), j = COL ? tok / 8 + (v & 1) : half / 8 + (v & 3);
-        int i, n;
-        place(g, l, j, i, n);
-        uint16_t* const dst = static_cast<uint16_t*>(a.out) + (int64_t)(tb + i) * a.out_token_stride + (int64_t)n * a.out_feature_stride;
-        const uint16_t* const line = reinterpret_cast<const uint16_t*>(lines + l * M::kLine + j * 16);
-        if (whole(i, n)) *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(line);
-        else
-          for (int k = 0; k < 8; ++k) {
-            const int ii = i + (COL ? k : 0), nn = n + (COL ? 0 : k);
-            if (ii >= i0 && ii < i1 && nn < N) dst[k] = line[k];
-          }
+      for (int h = 0; h < 2; ++h) {
+        const int i = COL ? 8 * j : l + kNext * h, n = g * kTile + (COL ? l + kNext * h : 8 * j);
+        if (whole(i, n)) *reinterpret_cast<uint4*>(dst + h * next) = *reinterpret_cast<const uint4*>(line + h * kNext * M::kLine);
+        else part(i, n, [&](int k) { dst[h * next + k] = reinterpret_cast<const uint16_t*>(line + h * kNext * M::kLine)[k]; });
       }
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
@@ -713,7 +738,7 @@ cudaError_t launch(LoraParams& p, cudaStream_t st) {
   }
   // As large a cluster as lets about T / 64 units run at once, so that a unit's
   // weights cross few SMs' links.
-  const int room = sms * (STRIPS >= 8 ? 1 : 2), units = (T + kTile - 1) / kTile;
+  const int room = sms * (STRIPS >= 8 ? 95 : 190) / 100, units = (T + kTile - 1) / kTile;  // clusters leave some SMs out
   while (p.cluster > 1 && units * p.cluster > room) p.cluster /= 2;
   const int groups = (p.a.out_features + kTile - 1) / kTile;
   p.split = std::max(1, groups / (2 * p.cluster));
