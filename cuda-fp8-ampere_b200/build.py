@@ -33,6 +33,9 @@ NVCC_FLAGS = ["-DFP8IMMA_NVTX", "-O3", "-std=c++17", "-lineinfo", "-Xcompiler", 
 CU_SOURCES = ["api.cu", "gemv_splitk.cu", "decode.cu", "generic.cu", "fp8wgt.cu", "host_util.cu", "gemm_tc.cu", "noalloc.cu", "peer.cu", "quantize.cu",
               "kv_cache.cu", "kv_attention.cu", "kv_attention_tc.cu", "moe.cu", "logprobs.cu", "residual_norm.cu", "lora.cu", "kv_rope.cu", "kv_attention_tree.cu", "kv_attention_tree_tc.cu"]
 
+# sources that include another one (variants of its kernel)
+INCLUDES = {"kv_attention_tree_tc.cu": "kv_attention_tc.cu"}
+
 
 def _run(cmd: list[str]) -> None:
     r = subprocess.run(cmd, capture_output=True, text=True)
@@ -69,7 +72,8 @@ def build_lib(force: bool = False, extra_flags: list[str] | None = None) -> str:
         s = os.path.join(CSRC, src)
         o = os.path.join(OBJ, src.replace(".cu", ".o"))
         objs.append(o)
-        if force or not _newer(o, [s] + hdrs):
+        deps = [s] + ([os.path.join(CSRC, INCLUDES[src])] if src in INCLUDES else [])
+        if force or not _newer(o, deps + hdrs):
             jobs.append([NVCC] + ARCH + NVCC_FLAGS + (extra_flags or []) + ["-c", s, "-o", o])
     with cf.ThreadPoolExecutor(max_workers=max(1, min(len(jobs), os.cpu_count() or 1))) as ex:
         list(ex.map(_run, jobs))

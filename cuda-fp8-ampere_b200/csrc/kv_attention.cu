@@ -1,5 +1,5 @@
 // The C entry of the cache attention (fp8imma_kv_attention) and the rule between
-// its two kernels (kv_attention_few.cuh, kv_attention_tc.cuh).
+// its two kernels (kv_attention_few.cuh, kv_attention_tc.cu).
 #include "kv_attention_few.cuh"
 #include "nvtx_range.h"
 

@@ -1,5 +1,5 @@
 // What the two kernels of the cache attention share (kv_attention_few.cuh: few
-// query rows a KV head; kv_attention_tc.cuh: many): the cut of the work into equal
+// query rows a KV head; kv_attention_tc.cu: many): the cut of the work into equal
 // runs of 128-key tiles, and the join of parts.
 #pragma once
 
@@ -220,7 +220,7 @@ struct Sight {
   __device__ __forceinline__ uint32_t sees32(const AttnParams& p, int j0) const {
     const bool tree = TREE && p.t.mask;
     // before the step (or all of them): first <= j < last
-    const int first = p.a.window > 0 ? max(0, pos - p.a.window + 1) : 0, last = tree ? (pos >= start ? start : 0) : pos + 1;
+    const int first = p.a.window > 0 ? (int)max((int64_t)0, (int64_t)pos - p.a.window + 1) : 0, last = tree ? (pos >= start ? start : 0) : pos + 1;
     const int a = min(max(first - j0, 0), 32), b = min(max(last - j0, 0), 32);
     uint32_t bits = b > a ? (b == 32 ? 0xffffffffu : (1u << b) - 1u) & ~((1u << a) - 1u) : 0u;
     if (tree && pos >= start && j0 + 31 >= start) {

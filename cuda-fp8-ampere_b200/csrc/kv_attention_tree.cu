@@ -1,6 +1,6 @@
 // Attention over the paged 8-bit cache for the nodes of drafted trees, with capped
 // scores (fp8imma_kv_attention_tree). The kernels are those of the causal attention
-// (kv_attention_few.cuh, kv_attention_tc.cuh) in variants of their own (TREE):
+// (kv_attention_few.cuh, kv_attention_tc.cu) in variants of their own (TREE):
 //   x_rj = cap tanh(s_rj / cap),  s_rj = softmax_scale <q_r, K_j>,
 // and in the tiles that hold keys of the step a row's mask bits decide what it
 // sees. All tiles before those are multiplied as in the causal attention.

@@ -768,10 +768,10 @@ extern "C" int fp8imma_lora_add(const fp8imma_lora_args* a, void* stream) {
   const uintptr_t bits = reinterpret_cast<uintptr_t>(a->base) | reinterpret_cast<uintptr_t>(a->out) | (uintptr_t)((row ? bt | ot : bf | of) * 2);
   if (bits & 1u) return (int)cudaErrorInvalidValue;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  for (int t = 0; t < a->tokens; t += kMaxTokens) {
+  for (int64_t t = 0; t < a->tokens; t += kMaxTokens) {
     LoraParams p = {};
     p.a = *a;
-    p.a.tokens = std::min(a->tokens - t, kMaxTokens);
+    p.a.tokens = (int)std::min<int64_t>(a->tokens - t, kMaxTokens);
     p.a.x = static_cast<const uint16_t*>(a->x) + t * a->x_stride;
     p.a.adapter_ids = a->adapter_ids + t;
     p.a.base = static_cast<const uint16_t*>(a->base) + t * bt;
