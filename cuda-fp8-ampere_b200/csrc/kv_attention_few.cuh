@@ -36,7 +36,7 @@
 // channels, one token each, 237 to 255 us by the board (4.8 to 5.1 TB/s: equal
 // runs end some 10% apart, for SMs do not get equal shares of the memory); one
 // sequence of 131000 keys 57 us (4.7 TB/s with start and join); one short
-// sequence 9.3 us, latency. With many rows see tc_pays().
+// sequence 9.3 us, latency. With many rows see attention_tc_pays().
 #pragma once
 
 #include "kv_attention.cuh"
