@@ -14,6 +14,12 @@
 //    rotation needs no exchange between threads;
 //  * a team of 1 .. 8 warps owns one (page, head, K or V) as in kv_cache.cu, its
 //    rows in registers between the pass for the scale and the one for the codes.
+//
+// Measured: 64 sequences of one token, 64/8 heads of 128, 4.4 us; 32 trees of up to 16
+// nodes, 28/4 heads of 64, 6.1 us; prompts of 9200 tokens, 32/8 heads of 128, 60 us,
+// 3.5 TB/s of the 208 MB read and written: with 124 registers 16 warps an SM go
+// through search, angles, keys and queries one after another, at 1.7 instructions a
+// cycle.
 #include "fp8_mma.cuh"
 #include "fp8imma/fp8imma_ext.h"
 #include "fp8imma_kernels.h"

@@ -2,7 +2,7 @@
 //   out_t = base_t + s_e B_e (A_e x_t),  e the adapter of token t.
 //
 // Both products are far below the tensor rate (2 r flops a byte of x and of out),
-// so every call is bound by its bytes: x, base, out, and the adapters' weights.
+// so a call's floor is its bytes: x, base, out, and the adapters' weights.
 //  * One launch, no scratch: a cluster of CTAs takes a unit, up to kTile
 //    neighbouring tokens of one adapter. Each CTA makes the inner sums of a slice
 //    of k, the cluster adds them up in distributed shared memory, and each CTA
@@ -17,6 +17,13 @@
 //    that they keep 16 (bf16) or 22 (fp16) bits: one rounding to the type would show
 //    in outputs whose base cancels the addend. fp16 has no range for u; a token's sums
 //    are first brought to a largest magnitude of 1 .. 2 by a power of two.
+//
+// Measured: one token, rank 16, 4096 -> 4096 5.2 us; 64 requests of one token, rank
+// 32, 4096 -> 11008 27 us on column-major results (their 2-byte pieces cost 10 of
+// them: 15 us row-major), one adapter for all of them 9.6 us; prompts of 4001
+// tokens, rank 64, 8192 -> 8192 78 us, 2.6 TB/s of the 205 MB (160 us with outputs
+// straight from memory), bound by the latency of a step's instructions: a CTA's chain
+// of 32 steps takes as long with one CTA an SM as with two.
 #include "fp8_mma.cuh"
 #include "fp8imma/fp8imma_ext.h"
 #include "fp8imma_kernels.h"
@@ -32,6 +39,7 @@ namespace {
 using namespace fp8imma_dev;
 
 constexpr int kThreads = 256, kWarps = 8;
+constexpr int kRunTokens = 4;  // runs of this mean length and more go through the kernel for many tokens
 constexpr int kMaxTokens = kThreads * 64;  // tokens of a launch: a thread marks where units begin in 64 bits
 
 struct LoraParams {
@@ -40,6 +48,7 @@ struct LoraParams {
   int split;    // clusters that may share a unit's outputs at most (each makes the inner sums)
   int vec;      // base and out are 16-byte aligned along their contiguous dimension, their other stride a multiple of 16 bytes
   int col;      // tokens are contiguous
+  int choose;   // both kernels are launched: the ids say which one works
 };
 
 template <int AT>
@@ -122,14 +131,26 @@ __device__ __forceinline__ void range_of(float big, float& f, float& back) {
 template <int TILE>
 struct Units {
   unsigned long long marks;
-  int first, mine, base, total;
+  int first, mine, base, total, runs;  // runs: of equal ids
   __device__ __forceinline__ static bool begins(const int32_t* ids, int t) { return t % TILE == 0 || __ldg(ids + t) != __ldg(ids + t - 1); }
-  __device__ __forceinline__ void scan(const fp8imma_lora_args& a, int* s) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, each = (a.tokens + kThreads - 1) / kThreads;
-    first = threadIdx.x * each;
-    marks = 0;
-    for (int i = 0; i < each; ++i)
-      if (first + i < a.tokens && begins(a.adapter_ids, first + i)) marks |= 1ull << i;
+  // s: kWarps words, words: one for each 32 tokens
+  __device__ __forceinline__ void scan(const fp8imma_lora_args& a, int* s, uint32_t* words) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int changes = 0;
+#pragma unroll 4
+    for (int t0 = 0; t0 < a.tokens; t0 += kThreads) {
+      const int t = t0 + (int)threadIdx.x;
+      const bool in = t < a.tokens;
+      const int id = in ? __ldg(a.adapter_ids + t) : 0, before = in && t > 0 ? __ldg(a.adapter_ids + t - 1) : 0;
+      const bool change = in && (t == 0 || id != before);
+      const uint32_t word = __ballot_sync(0xffffffffu, change || (in && t % TILE == 0));
+      changes += __popc(__ballot_sync(0xffffffffu, change));
+      if (lane == 0) words[t >> 5] = word;
+    }
+    __syncthreads();
+    const int end = (a.tokens + kThreads - 1) / kThreads * kThreads / 32;  // words written
+    first = threadIdx.x * 64;
+    marks = 2 * threadIdx.x < end ? words[2 * threadIdx.x] | (unsigned long long)words[2 * threadIdx.x + 1] << 32 : 0ull;
     mine = __popcll(marks);
     int x = mine;
 #pragma unroll
@@ -137,14 +158,15 @@ struct Units {
       const int y = __shfl_up_sync(0xffffffffu, x, o);
       if (lane >= o) x += y;
     }
-    if (lane == 31) s[warp] = x;
+    if (lane == 31) s[warp] = x | changes << 16;  // at most 2^14 of either
     __syncthreads();
     base = x - mine;
-    total = 0;
+    total = runs = 0;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      if (w < warp) base += s[w];
-      total += s[w];
+      if (w < warp) base += s[w] & 0xFFFF;
+      total += s[w] & 0xFFFF;
+      runs += s[w] >> 16;
     }
     __syncthreads();
   }
@@ -206,7 +228,8 @@ __global__ void __launch_bounds__(kThreads, STRIPS >= 8 ? 2 : 3) lora_few_kernel
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, q4 = lane >> 2, t4 = lane & 3;
   const int S = p.cluster, c = (int)cluster_rank(), cid = blockIdx.x / S, clusters = gridDim.x / S;
   Units<8> units;
-  units.scan(a, s_find);
+  units.scan(a, s_find, reinterpret_cast<uint32_t*>(smem));
+  if (p.choose && a.tokens >= kRunTokens * units.runs) return;
   const int R = a.rank, K = a.in_features, N = a.out_features;
   const int kb = (K + 31) / 32, kb0 = (int)((int64_t)kb * c / S), kb1 = (int)((int64_t)kb * (c + 1) / S);
   uint4* const ring = s_ring + warp * (2 * F::kStage) + lane;
@@ -441,7 +464,8 @@ __global__ void __launch_bounds__(kThreads, STRIPS >= 8 ? 1 : 2) lora_many_kerne
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, q4 = lane >> 2, t4 = lane & 3;
   const int S = p.cluster, c = (int)cluster_rank(), cid = blockIdx.x / S, clusters = gridDim.x / S;
   Units<kTile> units;
-  units.scan(a, s_find);
+  units.scan(a, s_find, reinterpret_cast<uint32_t*>(smem));
+  if (p.choose && a.tokens < kRunTokens * units.runs) return;
   const int R = a.rank, K = a.in_features, N = a.out_features;
   const int ks = (K + kStep - 1) / kStep, ks0 = (int)((int64_t)ks * c / S), ks1 = (int)((int64_t)ks * (c + 1) / S);
   const int split = max(1, min(p.split, clusters / max(1, units.total)));
@@ -559,7 +583,15 @@ __global__ void __launch_bounds__(kThreads, STRIPS >= 8 ? 1 : 2) lora_many_kerne
       cluster_wait();  // the sums are here, and the parts have been read
     }
 
-    // Lines of a step's base: tokens (COL: outputs), 64 elements each in eights. A
+    // Element v of a step's 64 lines: whether it is one of the unit's, and where it lies.
+    auto element = [&](int g, int v, auto* from, int64_t ts, int64_t fs, auto*& at) {
+      const int i = COL ? v & 63 : v >> 6, n = g * kTile + (COL ? v >> 6 : v & 63);
+      using E = std::remove_reference_t<decltype(*at)>;
+      at = static_cast<E*>(from) + (int64_t)(tb + i) * ts + (int64_t)n * fs;
+      return i >= i0 && i < i1 && n < N;
+    };
+    // Lines of a step's base: tokens (COL: outputs), 64 elements each in eights, or, where
+    // they are not aligned, neighbouring elements for neighbouring threads. A
     // thread copies eight j of lines l and l + 32; in which of its tokens the unit
     // lies and which outputs there are is settled line by line.
     auto load = [&](int g, int stage) {
@@ -575,6 +607,20 @@ __global__ void __launch_bounds__(kThreads, STRIPS >= 8 ? 1 : 2) lora_many_kerne
             const int r = row + i * kRows;
             copy16(dst + r * (M::kBlocks * 64) + ((M::kBlocks == 1 ? ch : ch ^ ((r & 1) << 2)) << 4), on ? src + i * kRows * R : static_cast<const uint16_t*>(a.lora_b), on);
           }
+        }
+        if (!p.vec) {
+          uint16_t x[16];
+          const uint16_t* src;
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (element(g, threadIdx.x + i * kThreads, a.base, a.base_token_stride, a.base_feature_stride, src)) x[i] = *src;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int v = threadIdx.x + i * kThreads;
+            *reinterpret_cast<uint16_t*>(dst + M::kBytesB + (v >> 6) * M::kLine + (v & 63) * 2) = x[i];
+          }
+          asm volatile("cp.async.commit_group;" ::: "memory");
+          return;
         }
         const int l = threadIdx.x >> 3, j = threadIdx.x & 7;
         const uint16_t* src = static_cast<const uint16_t*>(a.base) + (int64_t)(tb + (COL ? 8 * j : l)) * a.base_token_stride +
@@ -680,6 +726,16 @@ __global__ void __launch_bounds__(kThreads, STRIPS >= 8 ? 1 : 2) lora_many_kerne
         else add(std::integral_constant<int, 1>());
         __syncwarp();
       }
+      if (!p.vec) {
+        // the warp's elements, half a line's neighbours a time
+#pragma unroll 4
+        for (int i = 0; i < 16; ++i) {
+          const int l = COL ? half + 2 * i + (lane >> 4) : tok + i, at = COL ? tok + (lane & 15) : half + lane;
+          uint16_t* to;
+          if (element(g, l * kTile + at, a.out, a.out_token_stride, a.out_feature_stride, to)) *to = *reinterpret_cast<const uint16_t*>(lines + l * M::kLine + at * 2);
+        }
+        continue;
+      }
       // the warp's 16 x 32 (COL: 32 x 16) elements, 16 bytes a lane
       const int l = COL ? half + (lane >> 1) : tok + (lane >> 2), j = COL ? tok / 8 + (lane & 1) : half / 8 + (lane & 3);
       constexpr int kNext = COL ? 16 : 8;  // lines to the lane's second eight
@@ -721,24 +777,31 @@ cudaError_t launch_clusters(Kern kern, const LoraParams& p, int clusters, int sm
   return cudaLaunchKernelEx(&lc, kern, p);
 }
 
+// Up to 128 tokens take the kernel for few, more than 1024 the one for many. Between
+// them, where a decode batch as well as a prompt may lie, both are launched, and the
+// ids say which of them returns at once (5 to 10 us). Measured, rank 32, 4096 -> 11008,
+// column-major, 150 requests of one token: 56 us, 476 in the kernel for many alone.
 template <int AT, int STRIPS>
 cudaError_t launch(LoraParams& p, cudaStream_t st) {
   const int sms = num_sms_current(), T = p.a.tokens;
-  p.cluster = 8;
-  if (T <= 128) {
+  p.choose = T > 128 && T <= 1024;
+  if (T <= 1024) {
     // a unit of its own for each token at most: clusters small enough to run all at
     // once, and more of them where there are few tokens, each with a block a warp or so
     using F = Few<STRIPS>;
+    p.cluster = 8;
     while (p.cluster > 4 && T * p.cluster > 3 * sms) p.cluster /= 2;
     const int groups = (p.a.out_features + F::kOuts - 1) / F::kOuts;
     p.split = std::max(1, (groups + p.cluster * kWarps - 1) / (p.cluster * kWarps));
-    const int clusters = std::max(T, std::min(T * p.split, sms / p.cluster));
-    return p.col ? launch_clusters(lora_few_kernel<AT, STRIPS, true>, p, clusters, F::kSmem, st)
-                 : launch_clusters(lora_few_kernel<AT, STRIPS, false>, p, clusters, F::kSmem, st);
+    const int clusters = std::min(3 * sms / p.cluster, std::max(T, std::min(T * p.split, sms / p.cluster)));
+    const cudaError_t e = p.col ? launch_clusters(lora_few_kernel<AT, STRIPS, true>, p, clusters, F::kSmem, st)
+                                : launch_clusters(lora_few_kernel<AT, STRIPS, false>, p, clusters, F::kSmem, st);
+    if (e != cudaSuccess || !p.choose) return e;
   }
   // As large a cluster as lets about T / 64 units run at once, so that a unit's
   // weights cross few SMs' links.
   const int room = sms * (STRIPS >= 8 ? 95 : 190) / 100, units = (T + kTile - 1) / kTile;  // clusters leave some SMs out
+  p.cluster = 8;
   while (p.cluster > 1 && units * p.cluster > room) p.cluster /= 2;
   const int groups = (p.a.out_features + kTile - 1) / kTile;
   p.split = std::max(1, groups / (2 * p.cluster));
