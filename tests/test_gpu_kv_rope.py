@@ -112,6 +112,13 @@ def test_tree_nodes_share_a_position(ops):
     run(ops, 5, [50, 8], [7, 5], 4, 2, 128, 16, 128, False, B, "e4m3", i32([43, 44, 44, 45, 45, 46, 45, 3, 4, 4, 5, 5]))
 
 
+@pytest.mark.parametrize("d, rotary, ps", [(128, 96, 128), (256, 96, 128), (256, 48, 128), (64, 48, 64), (256, 256, 128), (128, 80, 32)])
+def test_parts_of_a_head_that_are_no_power_of_two(ops, d, rotary, ps):
+    """Any multiple of 16 turns; the tables of a full page's angles pass the sizes where shared memory changes its kind."""
+    run(ops, d + rotary, [ps + 40, 5], [ps + 30, 3], 3, 1, d, ps, rotary, False, H, "e4m3")
+    run(ops, d + rotary, [ps + 40, 5], [ps + 30, 3], 3, 1, d, ps, rotary, True, B, "e5m2")
+
+
 def test_unaligned_rows_and_keys_only(ops):
     g = gen(6)
     table, kc, vc, ks, vs = make_cache(g, 1, 2, 1, 16, 64, "e4m3")

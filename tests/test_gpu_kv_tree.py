@@ -263,6 +263,42 @@ def test_repeats_streams_and_graphs_at_once(ops):
         assert torch.equal(got[0], w[0]) and torch.equal(got[1], w[1])
 
 
+def test_sequences_longer_than_their_table(ops):
+    """Keys past the table are not read, the step's own among them."""
+    g = gen(11)
+    lens, news = [70, 64, 500], [10, 5, 7]  # the table holds 64 keys
+    cache = make_cache(g, 3, 4, 2, 16, 128, "e4m3")
+    cu = offsets(news)
+    q = queries(g, cu[-1], 4, 128, H)
+    mask, _ = trees(11, news)
+    for window in (0, 30):
+        a = dict(mask=mask, cap=10.0, window=window)
+        check(attend(ops, q, cache, lens, cu, "e4m3", **a), define(q, cache, lens, cu, "e4m3", **a))
+
+
+def test_two_streams_at_once(ops):
+    g = gen(12)
+    lens, news = [2600, 1300], [9, 16]
+    cache = make_cache(g, 2, 2600 // 64 + 1, 2, 64, 64, "e5m2")
+    cu = offsets(news)
+    mask, _ = trees(12, news)
+    q = [queries(g, cu[-1], 14, 64, B) for _ in range(2)]
+    lens_d, cu_d = i32(lens), i32(cu)
+    table, kc, vc, ks, vs = cache
+    call = lambda x: ops.kv_attention_tree(x, kc, vc, ks, vs, table, lens_d, mask, cu_d, softcap=30.0, fmt="e5m2")  # noqa: E731
+    want = [call(x) for x in q]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for _ in range(8):
+        for k in (0, 1):
+            with torch.cuda.stream(streams[k]):
+                got[k].append(call(q[k]))
+    torch.cuda.synchronize()
+    for k in (0, 1):
+        assert all(torch.equal(o, want[k][0]) and torch.equal(l, want[k][1]) for o, l in got[k])
+
+
 def test_descending_offsets_are_refused_on_the_device(ops):
     g = gen(8)
     cache = make_cache(g, 2, 4, 1, 16, 64, "e4m3")

@@ -59,6 +59,15 @@ def test_matches_definition(ops, name, k, n, r, dt, base_dt, col):
     check(ops.lora_add(**x), x)
 
 
+@pytest.mark.parametrize("t", [129, 600, 1024, 1025])
+@pytest.mark.parametrize("length", [1, 3, 4, 5, 90])
+@pytest.mark.parametrize("col", [False, True])
+def test_runs_of_any_length(ops, t, length, col):
+    """Whichever kernel the runs' length chooses, to the border of the range where the ids choose."""
+    x = inputs(t + length, [i // length % 4 - 1 for i in range(t)], 72, 90, 16, 3, B, H, col)
+    check(ops.lora_add(**x), x)
+
+
 @pytest.mark.parametrize("t", [1, 60, 128, 129, 200])
 @pytest.mark.parametrize("col", [False, True])
 def test_in_place_strided_base_and_tokens_without_adapter(ops, t, col):
