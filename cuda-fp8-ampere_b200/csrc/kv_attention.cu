@@ -44,6 +44,7 @@ bool attention_tc_pays(const AttnParams& p, int64_t rows) {
 }
 
 void attn_set_tc_rows(int rows) { g_tc_rows.store(rows); }
+int attention_tc_forced() { return g_tc_rows.load(); }
 unsigned int attn_device_error(bool clear) { return fp8imma_dev::tu_device_error(clear); }
 cudaError_t attn_set_wait_limit(unsigned long long ns) { return fp8imma_dev::tu_set_wait_limit(ns); }
 

@@ -384,5 +384,6 @@ cudaError_t launch_attention_tc(attn::AttnParams& p, cudaStream_t st);
 cudaError_t launch_attention_tree_tc(attn::AttnParams& p, cudaStream_t st);
 // Whether they take `rows` query rows of a sequence and KV head (kv_attention.cu).
 bool attention_tc_pays(const attn::AttnParams& p, int64_t rows);
+int attention_tc_forced();  // the number of rows set by fp8imma_set_attention_tc_rows, 0: none
 
 }  // namespace fp8imma_b200

@@ -695,6 +695,17 @@ cudaError_t launch(AttnParams& p, cudaStream_t st) {
 template <int FMT, bool TREE>
 cudaError_t launch_d(AttnParams& p, cudaStream_t st) {
   const int64_t rows = ((int64_t)p.c.tokens * p.group + p.c.batch - 1) / p.c.batch;
+  // Where tiles of 8 rows leave SMs free, each takes a CTA of its own, whose eight
+  // warps share the keys: a small tree over a short context is a chain of latencies
+  // (8 nodes of 32/8 heads over 700 keys: 16.2 us with 32 rows a CTA, 10.8 so). The
+  // causal operator keeps to its order of sums.
+  if (TREE && rows > 8 && attention_tc_forced() == 0) {
+    const int64_t tiles = ((int64_t)p.c.max_pages * p.c.page_size + kKeys - 1) / kKeys * p.c.batch * p.c.kv_heads;
+    if (tiles * ((rows + 7) / 8) <= 2ll * num_sms_current()) {
+      if (p.c.head_dim == 256) return launch<FMT, 256, 1, 1, TREE>(p, st);
+      return p.c.head_dim == 128 ? launch<FMT, 128, 1, 1, TREE>(p, st) : launch<FMT, 64, 1, 1, TREE>(p, st);
+    }
+  }
   if (attention_tc_pays(p, rows)) return TREE ? launch_attention_tree_tc(p, st) : launch_attention_tc(p, st);
   if (p.c.head_dim == 256) {
     if (rows <= 8) return launch<FMT, 256, 1, 1, TREE>(p, st);
