@@ -96,7 +96,9 @@ struct Eight {
   }
 };
 
-// Sum over the row's team: every thread gets it, in one order.
+// Sum over the row's team: every thread gets it, in one order. A caller in a loop takes
+// two places in turn: a warp may write its part of the next sum while others still read
+// this one's, and it is the next sum's barrier that tells that they have.
 __device__ __forceinline__ float team_sum(float x, float* s, int team, int warp) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
@@ -216,6 +218,7 @@ __global__ void __launch_bounds__(CTA, CTA == 256 ? (V == 4 ? 2 : 3) : 1) residu
   };
   int stage = 0;
   uint32_t phase = 0;
+  int turn = 0;  // of s_sum: sums alternate, whether a round has one or two
   bool ok = true;
   if (BULK && threadIdx.x == 0)
     for (int i = 0; i < p.stages; ++i) copy((int64_t)blockIdx.x * rows + i * step, i);
@@ -295,7 +298,8 @@ __global__ void __launch_bounds__(CTA, CTA == 256 ? (V == 4 ? 2 : 3) : 1) residu
       for (int v = 0; v < V; ++v)
 #pragma unroll
         for (int i = 0; i < 8; ++i) s = fmaf(x[v][i], x[v][i], s);
-      s = team_sum(s, s_sum[0], p.team, warp);
+      s = team_sum(s, s_sum[turn], p.team, warp);
+      turn ^= 1;
       const float f = rsqrtf(fmaf(s, by_n, a.eps));
 #pragma unroll
       for (int v = 0; v < V; ++v) {
@@ -329,7 +333,8 @@ __global__ void __launch_bounds__(CTA, CTA == 256 ? (V == 4 ? 2 : 3) : 1) residu
       }
     }
     if (!a.pre_weight) continue;
-    s = team_sum(s, s_sum[1], p.team, warp);
+    s = team_sum(s, s_sum[turn], p.team, warp);
+    turn ^= 1;
     const float f = rsqrtf(fmaf(s, by_n, a.eps));
 #pragma unroll
     for (int v = 0; v < V; ++v) {
