@@ -25,20 +25,25 @@ struct TreeParams {
   const uint32_t* mask;      // null: the step is causal
   const int32_t* positions;  // null: a token's place
   int words;
-  float cap;                 // 0: scores as they are
-  unsigned long long poly[7];  // coefficients of capped(), twice each
+  float cap2, by, twice;     // cap log2 e (0: scores as they are), 1 / cap2, 2 log2 e / cap2
+  unsigned long long poly[7];  // cap2 times the coefficients below, twice each: pairs for fma.f32x2
 };
-// cap tanh(s / cap) = x P((x / cap2)^2) for |x| <= cap2 (x = s log2 e, cap2 = cap log2 e):
-// tanh(sqrt w) / sqrt w on 0 <= w <= 1, a minimax fit of degree 6, to 2^-24 relative. The
-// powers of 1 / cap2 go into the coefficients, which stand as pairs for fma.f32x2.
+// Scores are capped in base 2: with x = s log2 e, y = x / cap2,
+//   cap tanh(s / cap) log2 e = cap2 tanh y = y cap2 P(y^2)  for |y| <= 1,
+// P(w) = tanh(sqrt w) / sqrt w on 0 <= w <= 1 by a minimax fit of degree 6, to 2^-24
+// relative (2^-21.8 as 32 bits evaluate it, scaling and all), whatever the cap: no power
+// of it enters but the first.
+// A cap counts as 2^-30 at least and 2^99 at most: below, all scores lie within 2^-29 of
+// one another, and above, tanh changes no score that lies below 2^87.
 inline void set_cap(TreeParams& t, float cap) {
   static const double c[7] = {0.9999999403953552, -0.33332839608192444, 0.13325203955173492, -0.05345702916383743,
                               0.020289979875087738, -0.006203379016369581, 0.0010410225950181484};
-  t.cap = cap;
-  const double by = cap > 0.0f ? 1.0 / ((double)cap * 1.4426950408889634) : 0.0;
-  double f = 1.0;
-  for (int i = 0; i < 7; ++i, f *= by * by) {
-    const float d = (float)(c[i] * f);
+  const double cap2 = cap > 0.0f ? std::min(std::max((double)cap, 0x1p-30), 0x1p99) * 1.4426950408889634 : 0.0;
+  t.cap2 = (float)cap2;
+  t.by = cap > 0.0f ? (float)(1.0 / cap2) : 0.0f;
+  t.twice = cap > 0.0f ? (float)(2.8853900817779268 / cap2) : 0.0f;
+  for (int i = 0; i < 7; ++i) {
+    const float d = (float)(c[i] * cap2);
     unsigned int bits;
     static_assert(sizeof(bits) == sizeof(d), "");
     std::memcpy(&bits, &d, sizeof(bits));
@@ -85,12 +90,24 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
-// cap tanh(s / cap) in base 2, from x = s log2 e: cap2 = cap log2 e, icap = 2 / cap.
-// tanh y = 1 - 2 / (1 + e^2y) is off by 2^-21 at most wherever y lies, so a score is
-// by cap 2^-21 and its weight by as much relative: 2^-15 at a cap of 50, against
-// the 2^-12 of a weight's rounding to fp16.
-__device__ __forceinline__ float cap_score(float x, float cap2, float icap) {
-  return fmaf(-2.0f * cap2, __fdividef(1.0f, 1.0f + ex2(x * icap)), cap2);
+// The capped score in base 2 of x = s log2 e beyond the polynomial's range, by
+// tanh y = 1 - 2 / (1 + e^2y). It is off by cap2 2^-22 wherever y lies, so what is
+// small beside the cap takes the polynomial.
+__device__ __forceinline__ float cap_far(const TreeParams& t, float x) {
+  return fmaf(-2.0f * t.cap2, __fdividef(1.0f, 1.0f + ex2(x * t.twice)), t.cap2);
+}
+// near where |y| <= 1; in asm, since the compiler makes a branch of it at which lanes part
+__device__ __forceinline__ float cap_pick(float y, float near, float far) {
+  float r;
+  asm("{\n\t.reg .pred p;\n\tsetp.le.f32 p, %1, 0f3F800000;\n\tselp.f32 %0, %2, %3, p;\n\t}" : "=f"(r) : "f"(fabsf(y)), "f"(near), "f"(far));
+  return r;
+}
+__device__ __forceinline__ float cap_score(const TreeParams& t, float x) {
+  const float y = x * t.by, u = y * y;
+  float q = __uint_as_float((uint32_t)t.poly[6]);
+#pragma unroll
+  for (int i = 5; i >= 0; --i) q = fmaf(u, q, __uint_as_float((uint32_t)t.poly[i]));
+  return cap_pick(y, y * q, cap_far(t, x));
 }
 // 16 bytes global -> shared, asynchronously
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src) {

@@ -282,8 +282,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   float cq[NT][2];
   Sight<TREE> sight[NT][2];
   const int walk_begin = walk.u;
-  const bool capped = TREE && p.t.cap > 0.0f;
-  const float cap2 = p.t.cap * 1.4426950408889634f, icap = capped ? __fdiv_rn(2.0f, p.t.cap) : 0.0f;
+  const bool capped = TREE && p.t.cap2 > 0.0f;
   int n_shared = 0;
   float o[S::kMT][NT][4], m[NT][2], l[NT][2];
 
@@ -431,7 +430,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
               for (int c = 0; c < 4; ++c) {
                 float x;
-                if (TREE && capped) x = cap_score((sa[k][nt][c] + sb[k][nt][c]) * (cq[nt][c & 1] * ks[k]), cap2, icap) + lvs[k];
+                if (TREE && capped) x = cap_score(p.t, (sa[k][nt][c] + sb[k][nt][c]) * (cq[nt][c & 1] * ks[k])) + lvs[k];
                 else x = fmaf(sa[k][nt][c] + sb[k][nt][c], cq[nt][c & 1] * ks[k], lvs[k]);
                 if (edge) {
                   const int j = tile * kKeys + (g0 + k) * 16 + (c < 2 ? key_lo : key_hi);

@@ -411,8 +411,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) kv_attention_tc_kernel(
     const uint32_t row_at = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t s_at = tmem + row_at + S::kTmemS + g * kKeys, o_at = tmem + row_at + S::kTmemO + g * D;
     const int walk_begin = walk.u;
-    const bool capped = TREE && p.t.cap > 0.0f;
-    const float cap2 = p.t.cap * 1.4426950408889634f, icap = capped ? __fdiv_rn(2.0f, p.t.cap) : 0.0f;
+    const bool capped = TREE && p.t.cap2 > 0.0f;
     int idx = 0, n_shared = 0;
     while (walk.next<TREE>(p, kRows, seg)) {
       const Seq& s = walk.s;
@@ -527,50 +526,76 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) kv_attention_tc_kernel(
             float sum[2];
             if (TREE && capped && !edge) {
               // the largest score of 16 keys is the capped one of their largest product
-              float kc[2], top[2], most_abs = 0.0f;
+              float ky[2], hi[2];  // scores as parts of the cap: factor, largest
+              bool near = true;    // all of them lie within the cap (a NaN hides here; it passes through either form)
 #pragma unroll
               for (int h = 0; h < 2; ++h) {
-                float hi = -INFINITY, lo = INFINITY;
+                float lo = INFINITY;
+                hi[h] = -INFINITY;
 #pragma unroll
                 for (int k = 16 * h; k < 16 * h + 16; k += 2) {
-                  hi = max3(hi, __uint_as_float(v[k]), __uint_as_float(v[k + 1]));
+                  hi[h] = max3(hi[h], __uint_as_float(v[k]), __uint_as_float(v[k + 1]));
                   lo = min3(lo, __uint_as_float(v[k]), __uint_as_float(v[k + 1]));
                 }
-                kc[h] = cq * info.ks[2 * c + h];
-                most_abs = fmaxf(most_abs, kc[h] * fmaxf(hi, -lo));
-                top[h] = cap_score(hi * kc[h], cap2, icap) + info.lv[2 * c + h];
+                ky[h] = cq * info.ks[2 * c + h] * p.t.by;
+                near &= ky[h] * fmaxf(hi[h], -lo) <= 1.0f;
               }
+              auto capped2 = [&](uint64_t y, uint64_t add) {  // cap2 tanh y + add, by the polynomial
+                const uint64_t u = mul2(y, y);
+                uint64_t q = fma2(u, p.t.poly[6], p.t.poly[5]);
+#pragma unroll
+                for (int i = 4; i >= 0; --i) q = fma2(u, q, p.t.poly[i]);
+                return fma2(y, q, add);
+              };
+              if (!__all_sync(0xffffffffu, near)) {
+                // Scores beyond the cap. This branch goes its own way to the end of the 32 keys, which
+                // costs the other one the fewest registers (joined before the sums: 513 us for 474).
+                float most = -INFINITY;
+#pragma unroll 1
+                for (int h = 0; h < 2; ++h) most = fmaxf(most, cap_score(p.t, (h ? hi[1] : hi[0]) * (cq * info.ks[2 * c + h])) + info.lv[2 * c + h]);
+                if (__any_sync(0xffffffffu, most > m + kRaise)) raise(c, most);
+                const float ms = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                  const float kc = cq * info.ks[2 * c + h], lv = info.lv[2 * c + h] - ms;
+                  const uint64_t ky2 = pair(kc * p.t.by, kc * p.t.by), lv2 = pair(lv, lv);
+                  uint64_t two = 0;
+#pragma unroll
+                  for (int k = 16 * h; k < 16 * h + 16; k += 2) {
+                    const float v0 = __uint_as_float(v[k]), v1 = __uint_as_float(v[k + 1]);
+                    const uint64_t y = mul2(pair(v0, v1), ky2);
+                    float y0, y1, n0, n1;
+                    unpair(y, y0, y1);
+                    unpair(capped2(y, lv2), n0, n1);
+                    n0 = ex2(cap_pick(y0, n0, cap_far(p.t, v0 * kc) + lv));
+                    n1 = ex2(cap_pick(y1, n1, cap_far(p.t, v1 * kc) + lv));
+                    two = add2(two, pair(n0, n1));
+                    w[k / 2] = pack_f16(n0, n1);
+                  }
+                  float s0, s1;
+                  unpair(two, s0, s1);
+                  l = fmaf(s0 + s1, info.iv[2 * c + h], l);
+                }
+                tmem_st16(s_at + 16 * c, w);
+                continue;
+              }
+              float top[2];
+              unpair(capped2(pair(hi[0] * ky[0], hi[1] * ky[1]), pair(info.lv[2 * c], info.lv[2 * c + 1])), top[0], top[1]);
               const float most = fmaxf(top[0], top[1]);
               if (__any_sync(0xffffffffu, most > m + kRaise)) raise(c, most);
               const float ms = m == -INFINITY ? 0.0f : m;
-              // a NaN hides from the maxima; it passes through either form
-              const bool near = !__any_sync(0xffffffffu, most_abs > cap2);
 #pragma unroll
               for (int h = 0; h < 2; ++h) {
                 const float lv = info.lv[2 * c + h] - ms;
-                const uint64_t kc2 = pair(kc[h], kc[h]), lv2 = pair(lv, lv);
+                const uint64_t ky2 = pair(ky[h], ky[h]), lv2 = pair(lv, lv);
                 uint64_t two = 0;
-                if (near) {
 #pragma unroll
-                  for (int k = 16 * h; k < 16 * h + 16; k += 2) {
-                    const uint64_t x = mul2(pair(__uint_as_float(v[k]), __uint_as_float(v[k + 1])), kc2), u = mul2(x, x);
-                    uint64_t q = fma2(u, p.t.poly[6], p.t.poly[5]);
-#pragma unroll
-                    for (int i = 4; i >= 0; --i) q = fma2(u, q, p.t.poly[i]);
-                    float a, b;
-                    unpair(fma2(x, q, lv2), a, b);
-                    a = ex2(a), b = ex2(b);
-                    two = add2(two, pair(a, b));
-                    w[k / 2] = pack_f16(a, b);
-                  }
-                } else {
-#pragma unroll
-                  for (int k = 16 * h; k < 16 * h + 16; k += 2) {
-                    const float a = ex2(cap_score(__uint_as_float(v[k]) * kc[h], cap2, icap) + lv);
-                    const float b = ex2(cap_score(__uint_as_float(v[k + 1]) * kc[h], cap2, icap) + lv);
-                    two = add2(two, pair(a, b));
-                    w[k / 2] = pack_f16(a, b);
-                  }
+                for (int k = 16 * h; k < 16 * h + 16; k += 2) {
+                  float a, b;
+                  unpair(capped2(mul2(pair(__uint_as_float(v[k]), __uint_as_float(v[k + 1])), ky2), lv2), a, b);
+                  a = ex2(a), b = ex2(b);
+                  two = add2(two, pair(a, b));
+                  w[k / 2] = pack_f16(a, b);
                 }
                 float s0, s1;
                 unpair(two, s0, s1);
@@ -586,7 +611,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) kv_attention_tc_kernel(
 #pragma unroll
               for (int k = 0; k < 32; ++k) {
                 const int i = 2 * c + k / 16;
-                if (capped) x[k] = cap_score(__uint_as_float(v[k]) * (cq * info.ks[i]), cap2, icap) + info.lv[i];
+                if (capped) x[k] = cap_score(p.t, __uint_as_float(v[k]) * (cq * info.ks[i])) + info.lv[i];
                 else x[k] = fmaf(__uint_as_float(v[k]), cq * info.ks[i], info.lv[i]);
                 if (!((info.live >> i) & 1) || (TREE ? !((vis >> k) & 1u) : (unsigned)(tile * kKeys + 32 * c + k - v0) >= (unsigned)nv)) x[k] = -INFINITY;
                 top = fmaxf(top, x[k]);

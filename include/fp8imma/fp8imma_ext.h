@@ -371,7 +371,8 @@ int fp8imma_kv_append_rope(const fp8imma_kv_cache* cache, const fp8imma_kv_appen
 // j > position(t) - window, the positions (a node's depth counts from the
 // step's first place) taken between the step's first and last place; without
 // them a token's place counts. softcap > 0: scores are
-// softcap * tanh(s / softcap), s = softmax_scale <q, K_j>.
+// softcap * tanh(s / softcap), s = softmax_scale <q, K_j>, off by 2^-21 relative
+// under any finite cap (one below 2^-30 counts as that, one above 2^99 too).
 typedef struct fp8imma_kv_attention_tree_args {
   int a_type;                 // of q and out
   int heads;                  // query heads, a multiple of kv_heads
