@@ -65,8 +65,8 @@ __device__ __forceinline__ int touched(const RopeParams& p, int b, int& first) {
   return n > 0 ? ((len - 1) >> pl) - first + 1 : 0;
 }
 
-// position * inv_freq / 2 pi without its whole turns, in -0.5 .. 0.5. 1 / 2 pi and the
-// products are held as two 64-bit numbers: one alone would leave 2^-21 of an angle at
+// An angle as position * inv_freq / 2 pi without its whole turns, in -0.5 .. 0.5. 1 / 2 pi
+// and the products are held as two 64-bit numbers: one alone would leave 2^-21 of an angle at
 // a position of 2^31.
 struct Frequency {
   double hi, lo;  // inv_freq / 2 pi
@@ -75,9 +75,16 @@ struct Frequency {
     hi = inv_freq * kHi;
     lo = fma((double)inv_freq, kHi, -hi) + inv_freq * kLo;
   }
-  __device__ __forceinline__ float turns(int position) const {
-    const double at = position, t = at * hi;
-    return (float)((t - rint(t)) + fma(at, lo, fma(at, hi, -t)));
+  // cosine and sine of the angle: of its fraction of a turn t as fp32, then a step of the
+  // first order by what that leaves (delta, up to 2^-23.3: cos (a + d) = cos a - d sin a
+  // to 2^-47), so that small cosines and sines keep their relative precision too
+  __device__ __forceinline__ void turn(int position, float& cs, float& sn) const {
+    const double at = position, whole = at * hi, t = (whole - rint(whole)) + fma(at, lo, fma(at, hi, -whole));
+    const float near = (float)t, delta = (float)((t - near) * 6.283185307179586);
+    float s, c;
+    sincospif(2.0f * near, &s, &c);
+    cs = fmaf(-delta, s, c);
+    sn = fmaf(delta, c, s);
   }
 };
 
@@ -184,7 +191,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv_append_rope_kernel(const __gri
     const Frequency f(__ldg(p.a.inv_freq + i));
     for (int r = threadIdx.x / half; r < rows && (int)threadIdx.x < per * half; r += per) {
       float sn, cs;
-      sincospif(2.0f * f.turns(p.a.positions ? __ldg(p.a.positions + tok + r) : lo + r), &sn, &cs);
+      f.turn(p.a.positions ? __ldg(p.a.positions + tok + r) : lo + r, cs, sn);
       table[r * half + i] = cs * p.a.rope_scale;
       sines[r * half + i] = sn * p.a.rope_scale;
     }
