@@ -5,6 +5,7 @@
 #include <cuda_runtime.h>
 #include <cstddef>
 #include <cstdint>
+#include <initializer_list>
 
 struct fp8imma_kv_cache;
 
@@ -207,6 +208,12 @@ unsigned int attn_tree_device_error(bool clear);
 unsigned int attn_tree_tc_device_error(bool clear);
 cudaError_t attn_tree_set_wait_limit(unsigned long long ns);
 cudaError_t attn_tree_tc_set_wait_limit(unsigned long long ns);
+// Whether all of the addresses (null ones too) are those of 32-bit elements.
+inline bool aligned4(std::initializer_list<const void*> at) {
+  for (const void* p : at)
+    if (reinterpret_cast<uintptr_t>(p) & 3u) return false;
+  return true;
+}
 // Checks of a paged KV cache shared by its append and its attention.
 cudaError_t kv_cache_check(const ::fp8imma_kv_cache* cache);
 

@@ -58,7 +58,7 @@ extern "C" int fp8imma_kv_attention(const fp8imma_kv_cache* c, const fp8imma_kv_
   if (e != cudaSuccess) return (int)e;
   if (!a || !a->q || !a->out || a->a_type < 0 || a->a_type > 1) return (int)cudaErrorInvalidValue;
   if (a->heads <= 0 || a->heads % c->kv_heads || a->heads > 65535 || a->window < 0) return (int)cudaErrorInvalidValue;
-  if (reinterpret_cast<uintptr_t>(a->q) & 1u) return (int)cudaErrorInvalidValue;
+  if ((reinterpret_cast<uintptr_t>(a->q) & 1u) || !aligned4({a->lse})) return (int)cudaErrorInvalidValue;
   if (reinterpret_cast<uintptr_t>(a->out) & 15u) return (int)cudaErrorInvalidValue;
   if ((int64_t)c->tokens * (a->heads / c->kv_heads) > 0x7fffffffll) return (int)cudaErrorInvalidValue;
   AttnParams p = {};

@@ -32,7 +32,7 @@ extern "C" int fp8imma_kv_attention_tree(const fp8imma_kv_cache* c, const fp8imm
   if (a->heads <= 0 || a->heads % c->kv_heads || a->heads > 65535 || a->window < 0) return (int)cudaErrorInvalidValue;
   if (!(a->softcap >= 0.0f) || !std::isfinite(a->softcap) || !std::isfinite(a->softmax_scale)) return (int)cudaErrorInvalidValue;
   if ((a->tree_mask && a->mask_words <= 0) || (a->positions && !a->tree_mask)) return (int)cudaErrorInvalidValue;
-  if (reinterpret_cast<uintptr_t>(a->q) & 1u) return (int)cudaErrorInvalidValue;
+  if ((reinterpret_cast<uintptr_t>(a->q) & 1u) || !aligned4({a->tree_mask, a->positions, a->lse})) return (int)cudaErrorInvalidValue;
   if (reinterpret_cast<uintptr_t>(a->out) & 15u) return (int)cudaErrorInvalidValue;
   if ((int64_t)c->tokens * (a->heads / c->kv_heads) > 0x7fffffffll) return (int)cudaErrorInvalidValue;
   AttnParams p = {};

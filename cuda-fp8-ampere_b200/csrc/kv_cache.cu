@@ -161,6 +161,7 @@ cudaError_t kv_cache_check(const fp8imma_kv_cache* c) {
     return cudaErrorInvalidConfiguration;
   if (!c->k || !c->v || !c->k_scale || !c->v_scale || !c->page_table || !c->seq_lens) return cudaErrorInvalidValue;
   if ((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v)) & 15u) return cudaErrorInvalidValue;
+  if (!aligned4({c->k_scale, c->v_scale, c->page_table, c->seq_lens, c->cu_new})) return cudaErrorInvalidValue;
   if (c->format < 0 || c->format > 1) return cudaErrorInvalidValue;
   if (c->page_size != 16 && c->page_size != 32 && c->page_size != 64 && c->page_size != 128) return cudaErrorInvalidValue;
   if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256) return cudaErrorInvalidValue;

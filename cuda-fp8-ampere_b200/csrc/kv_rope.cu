@@ -406,7 +406,7 @@ extern "C" int fp8imma_kv_append_rope(const fp8imma_kv_cache* c, const fp8imma_k
                        (uintptr_t)((a->k_token_stride | a->k_head_stride | a->v_token_stride | a->v_head_stride) * 2);
   const uintptr_t q = a->heads == 0 ? 0 : reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->q_out) |
                        (uintptr_t)((a->q_token_stride | a->q_head_stride | a->q_out_token_stride | a->q_out_head_stride) * 2);
-  if ((kv | q) & 1u) return (int)cudaErrorInvalidValue;
+  if (((kv | q) & 1u) || !aligned4({a->inv_freq, a->positions})) return (int)cudaErrorInvalidValue;
   p.vec = (kv & 15u) == 0;
   p.vec_q = (q & 15u) == 0;
   int64_t units;

@@ -804,6 +804,7 @@ extern "C" int fp8imma_token_logprobs(const fp8imma_logprobs_args* a, void* stre
   if (a->vocab_stride != 1 && a->token_stride != 1) return (int)cudaErrorInvalidValue;
   if (a->vocab > 0x7fffff00) return (int)cudaErrorInvalidValue;
   if (reinterpret_cast<uintptr_t>(a->logits) & (a->l_type == FP8IMMA_L_F32 ? 3u : 1u)) return (int)cudaErrorInvalidValue;
+  if (!aligned4({a->token_ids, a->logprobs, a->entropy}) || (a->top > 0 && !aligned4({a->top_ids, a->top_logprobs}))) return (int)cudaErrorInvalidValue;
   LpParams p = {};
   p.a = *a;
   p.inv_temp = 1.0f / a->temperature;

@@ -823,7 +823,7 @@ extern "C" int fp8imma_lora_add(const fp8imma_lora_args* a, void* stream) {
   if (a->rank > FP8IMMA_LORA_MAX_RANK || a->rank % 8 || a->in_features % 8) return (int)cudaErrorInvalidValue;
   if (!a->x || !a->lora_a || !a->lora_b || !a->adapter_ids || !a->base || !a->out) return (int)cudaErrorInvalidValue;
   if ((reinterpret_cast<uintptr_t>(a->x) | reinterpret_cast<uintptr_t>(a->lora_a) | reinterpret_cast<uintptr_t>(a->lora_b)) & 15u) return (int)cudaErrorInvalidValue;
-  if (a->x_stride < 0 || a->x_stride % 8) return (int)cudaErrorInvalidValue;
+  if (a->x_stride < 0 || a->x_stride % 8 || !aligned4({a->adapter_ids, a->scales})) return (int)cudaErrorInvalidValue;
   const int64_t bt = a->base_token_stride, bf = a->base_feature_stride, ot = a->out_token_stride, of = a->out_feature_stride;
   if (bt < 0 || bf < 0 || ot < 0 || of < 0) return (int)cudaErrorInvalidValue;
   const bool row = bf == 1 && of == 1, col = !row && bt == 1 && ot == 1;

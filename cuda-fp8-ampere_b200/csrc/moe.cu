@@ -961,7 +961,7 @@ extern "C" int fp8imma_moe_forward(const fp8imma_moe_args* a, void* stream) {
   if ((reinterpret_cast<uintptr_t>(a->w_gate_up) | reinterpret_cast<uintptr_t>(a->w_down)) & 15u)
     return (int)cudaErrorInvalidValue;
   if ((reinterpret_cast<uintptr_t>(a->x) | reinterpret_cast<uintptr_t>(a->router)) & 1u) return (int)cudaErrorInvalidValue;
-  if (reinterpret_cast<uintptr_t>(a->out) & 3u) return (int)cudaErrorInvalidValue;
+  if (!aligned4({a->out, a->s_gate_up, a->s_down, a->ids, a->weights})) return (int)cudaErrorInvalidValue;
   // weight rows are indexed with 31 bits
   if ((int64_t)a->experts * 2 * a->inter > 0x7fffffffll || (int64_t)a->experts * a->hidden > 0x7fffffffll)
     return (int)cudaErrorInvalidValue;

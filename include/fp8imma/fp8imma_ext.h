@@ -163,7 +163,8 @@ int fp8imma_set_fused_gather(int enable);
 // FP8IMMA_A_BF16); FP8 bytes are E4M3FN or E5M2 (FP8IMMA_B_E4M3 / _E5M2).
 // Forward only, like the GEMMs. Strides are in elements. Same errors as above:
 // cudaErrorInvalidConfiguration for an empty problem, cudaErrorInvalidValue
-// for a missing pointer or an argument outside its range.
+// for a missing pointer, one that is not aligned to its elements, or an
+// argument outside its range.
 
 // A paged KV cache in 8 bits with one fp32 scale per (page, KV head) for the
 // keys and one for the values: value = code * scale. Page p holds `page_size`
