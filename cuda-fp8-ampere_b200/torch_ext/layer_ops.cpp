@@ -11,7 +11,9 @@
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 
+#include <algorithm>
 #include <cmath>
+#include <cstdlib>
 #include <string>
 #include <tuple>
 
@@ -45,6 +47,35 @@ void check_apart(const torch::Tensor& out, const torch::Tensor& in, const char* 
     return static_cast<const char*>(x.data_ptr()) + n * x.element_size();
   };
   TORCH_CHECK(end(out) <= static_cast<const char*>(in.data_ptr()) || end(in) <= static_cast<const char*>(out.data_ptr()), what);
+}
+
+// Whether rows (t, h) of x and y, [tokens, heads, dim] of one type with contiguous last
+// dimensions, share an element; with `other` false a row does not meet itself. Slices of
+// one buffer may lie in turn with one another.
+bool rows_meet(const torch::Tensor& x, const torch::Tensor& y, bool other = true) {
+  const int64_t T = x.size(0), D = x.size(2), Hx = x.size(1), Hy = y.size(1);
+  if (!x.numel() || !y.numel()) return false;
+  const int64_t off = (static_cast<const char*>(x.data_ptr()) - static_cast<const char*>(y.data_ptr())) / (int64_t)x.element_size();
+  // a dimension of one element has no stride of its own
+  const int64_t hx = Hx == 1 ? 0 : x.stride(1), hy = Hy == 1 ? 0 : y.stride(1), sx = T == 1 ? 0 : x.stride(0), sy = T == 1 ? 0 : y.stride(0);
+  const int64_t lx = (Hx - 1) * hx + D, ly = (Hy - 1) * hy + D;  // a token's span
+  if (off + (T - 1) * sx + lx <= 0 || off >= (T - 1) * sy + ly) return false;
+  if (sx != sy) return true;  // not told apart
+  if (other && sx >= std::max(lx, ly)) {  // spans within the token stride: apart in the first tokens is apart in all
+    const int64_t r = ((off % sx) + sx) % sx;
+    if (r >= ly && r + lx <= sx) return false;
+  }
+  // heads within tokens, or tokens within heads
+  if (!other && ((T == 1 || sx >= lx) && (Hx == 1 || hx >= D))) return false;
+  if (!other && ((Hx == 1 || hx >= (T - 1) * sx + D) && (T == 1 || sx >= D))) return false;
+  for (int64_t i = 0; i < Hx; ++i)
+    for (int64_t j = 0; j < Hy; ++j) {
+      // rows i and j of tokens dt apart, where they come nearest
+      const int64_t at = off + i * hx - j * hy, dt0 = sx ? std::clamp(-at / sx, 1 - T, T - 1) : 0;
+      for (int64_t dt = std::max(dt0 - 1, 1 - T); dt <= std::min(dt0 + 1, T - 1); ++dt)
+        if (std::abs(at + dt * sx) < D && (other || i != j || dt != 0)) return true;
+    }
+  return false;
 }
 
 // a [tokens, hidden] tensor with contiguous rows; its row stride
@@ -255,6 +286,9 @@ OptTensor kv_append_rope(const OptTensor& q, const torch::Tensor& k, const torch
         check_apart(*o, *q, across);
         check_apart(*o, k, across, false);
         check_apart(*o, v, across, false);
+      } else {
+        TORCH_CHECK(!rows_meet(*o, *o, false), "rows of q must lie apart where q_out is q");
+        TORCH_CHECK(!rows_meet(*o, k) && !rows_meet(*o, v), "q must lie apart from k and v where q_out is q");
       }
     } else {
       o = fresh(*q, q->sizes(), q->scalar_type());

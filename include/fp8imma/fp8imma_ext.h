@@ -357,7 +357,8 @@ typedef struct fp8imma_kv_append_rope_args {
   int64_t q_token_stride, q_head_stride;
   int64_t k_token_stride, k_head_stride;
   int64_t v_token_stride, v_head_stride;
-  void* q_out;                // [tokens, heads, head_dim], last dimension contiguous; may be q
+  void* q_out;                // [tokens, heads, head_dim], last dimension contiguous; may be q, where q's rows lie
+                              // apart from one another and from those of k and v
   int64_t q_out_token_stride, q_out_head_stride;
 } fp8imma_kv_append_rope_args;
 int fp8imma_kv_append_rope(const fp8imma_kv_cache* cache, const fp8imma_kv_append_rope_args* args, void* stream);
