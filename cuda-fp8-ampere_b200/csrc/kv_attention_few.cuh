@@ -695,9 +695,13 @@ template <int FMT, bool TREE>
 cudaError_t launch_d(AttnParams& p, cudaStream_t st) {
   const int64_t rows = ((int64_t)p.c.tokens * p.group + p.c.batch - 1) / p.c.batch;
   // Where tiles of 8 rows leave SMs free, each takes a CTA of its own, whose eight
-  // warps share the keys: a small tree over a short context is a chain of latencies
-  // (8 nodes of 32/8 heads over 700 keys: 16.2 us with 32 rows a CTA, 10.8 so). The
-  // causal operator keeps to its order of sums.
+  // warps share the keys: a small tree over a short context is a chain of latencies.
+  // Up to the border it won at each of 102 shapes (16 to 512 rows, 200 to 8000 keys,
+  // 1 to 8 KV heads); this / as many rows a CTA as below / tcgen05 in us, tiles of 8
+  // rows in brackets: 64 channels, 256 rows, 200 keys, 4 heads [256] 10.3/19.8/20.4;
+  // 128 channels, 32 rows, 700 keys, 8 heads [192] 11.2/16.4/23.4, 32 rows, 8000
+  // keys, 1 head [252] 21.9/37.2/60.7; 256 channels, 128 rows, 2000 keys, 1 head [256]
+  // 15.1/54.8. The causal operator keeps to its order of sums.
   if (TREE && rows > 8 && attention_tc_forced() == 0) {
     const int64_t tiles = ((int64_t)p.c.max_pages * p.c.page_size + kKeys - 1) / kKeys * p.c.batch * p.c.kv_heads;
     if (tiles * ((rows + 7) / 8) <= 2ll * num_sms_current()) {

@@ -6,8 +6,8 @@
 // sees. All tiles before those are multiplied as in the causal attention.
 //
 // Measured (one B200): 32 sequences of up to 8192 keys, 64/8 heads of 128, up to 16
-// nodes, capped 282 to 314 us by the board; two documents of up to 100000 keys, 64 nodes
-// of 32/8 heads, capped 401. Two of 100000 each: 378 us without a cap, 476 with all
+// nodes, capped 275 to 314 us by the board; two documents of up to 100000 keys, 64 nodes
+// of 32/8 heads, capped 379 to 410. Two of 100000 each: 378 us without a cap, 476 with all
 // scores within it, 640 where every tile holds some beyond it. One sequence of 700
 // keys, 8 nodes of 32/8 heads 11 us.
 #include "kv_attention_few.cuh"

@@ -39,7 +39,7 @@ namespace {
 using namespace fp8imma_dev;
 
 constexpr int kThreads = 256, kWarps = 8;
-constexpr int kRunTokens = 4;  // runs of this mean length and more go through the kernel for many tokens
+constexpr int kRunTokens = 4;  // runs of this length in the mean of a call and more go through the kernel for many tokens
 constexpr int kMaxTokens = kThreads * 64;  // tokens of a launch: a thread marks where units begin in 64 bits
 
 struct LoraParams {
@@ -780,7 +780,10 @@ cudaError_t launch_clusters(Kern kern, const LoraParams& p, int clusters, int sm
 // Up to 128 tokens take the kernel for few, more than 1024 the one for many. Between
 // them, where a decode batch as well as a prompt may lie, both are launched, and the
 // ids say which of them returns at once (5 to 10 us). Measured, rank 32, 4096 -> 11008,
-// column-major, 150 requests of one token: 56 us, 476 in the kernel for many alone.
+// column-major, 150 requests of one token: 56 to 63 us, 476 in the kernel for many alone.
+// Where the mean of the runs belongs to none of them, and above 1024 tokens, short runs
+// pay for a tile of 64 tokens each: one prompt of 900 tokens beside 124 requests of one
+// 484 us, 1025 requests of one token 3350 (1024 of them 402, one prompt of 1024 36).
 template <int AT, int STRIPS>
 cudaError_t launch(LoraParams& p, cudaStream_t st) {
   const int sms = num_sms_current(), T = p.a.tokens;

@@ -9,10 +9,11 @@
 // so the two sums over the row cost no further pass. A team of 1 .. 32 warps owns
 // a row; a CTA holds as many teams as 256 threads make.
 //
-// Measured: 8192 rows of 4096 (bf16, both norms, a gate a token, residual) 56 to 60
-// us, 5.6 to 6.0 TB/s of the 336 MB; one row of 4096 2.0 us; 64 rows of 8192 with an
-// fp32 residual 4.5 us, the chain of two sums. Rows that are not whole, aligned
-// eights go an element a load: 8192 rows of 4097 288 us.
+// Measured: 8192 rows of 4096 (bf16, both norms, a gate a token, residual) 56 to 61
+// us, 5.5 to 6.0 TB/s of the 336 MB; one row of 4096 2.0 us; 64 rows of 8192 with an
+// fp32 residual 4.4 us, the chain of two sums. Without a gate, cold caches: both norms
+// 62 us, one 51; with fp32 weights, which rows copied ahead do not take, 83 and 64. Rows
+// that are not whole, aligned eights go an element a load: 8192 rows of 4097 288 us.
 #include "fp8_mma.cuh"
 #include "fp8imma/fp8imma_ext.h"
 #include "fp8imma_kernels.h"

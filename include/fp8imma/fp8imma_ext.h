@@ -290,7 +290,7 @@ int fp8imma_token_logprobs(const fp8imma_logprobs_args* args, void* stream);
 //   r' = residual + alpha * gate * b      (no residual: 0, no gate: 1)
 //   h = rms(r') (pre_weight + o),         rms(x) = x / sqrt(mean(x^2) + eps)
 // in fp32, r' (residual_out) and h (out) rounded once each; h is made from the
-// unrounded r'. residual_out may be residual, out may be y, where strides agree.
+// unrounded r'. A sum of squares past fp32's range counts as infinite (h = 0). residual_out may be residual, out may be y, where strides agree.
 #define FP8IMMA_NORM_MAX_HIDDEN 32768
 typedef struct fp8imma_residual_norm_args {
   int a_type;                 // of y and out
@@ -318,7 +318,8 @@ int fp8imma_residual_norm(const fp8imma_residual_norm_args* args, void* stream);
 // adapter (out = base). base is the projection's result in either layout (the
 // GEMM's default is column-major). Neighbouring tokens of one adapter share its
 // weights' way to the SM, so requests are best laid one after another. Sums are
-// fp32; the inner sums enter the second product as two 16-bit numbers each.
+// fp32; the inner sums enter the second product as two 16-bit numbers each, and
+// what an infinity in x or in an adapter reaches comes out infinite or NaN.
 #define FP8IMMA_LORA_MAX_RANK 128
 typedef struct fp8imma_lora_args {
   int a_type;                 // of x, lora_a and lora_b
