@@ -68,12 +68,10 @@ CAPS = [1e-38, 1e-4, 2e-3, 0.5, 50.0, 1100.0, 2000.0, 1e4, 1e6, 3e38]
 
 @pytest.mark.parametrize("dt, fmt", [(H, "e4m3"), (B, "e5m2")])
 @pytest.mark.parametrize("d", [64, 128, 256])
-@pytest.mark.parametrize("near", [False, True], ids=["ordinary", "at the cap"])
-@pytest.mark.parametrize("cap", CAPS)
+# scores beyond a cap of 3e38 are none
+@pytest.mark.parametrize("cap, near", [(c, near) for c in CAPS for near in (False, True) if not (near and c > 1e6)])
 def test_caps_of_any_size(ops, cap, near, d, dt, fmt):
     """Ordinary scores under any cap, and scores from far below the cap to four times it."""
-    if near and cap > 1e6:
-        pytest.skip("scores of that size are none")
     g = gen(d)
     lens, news = [400, 305, 140], [12, 3, 1]
     cache = make_cache(g, 3, 400 // 16 + 1, 2, 16, d, fmt)
